@@ -312,6 +312,88 @@ int tg_backward_b_strided_batched(int device, tg_dtype dtype, tg_layout layout,
 int tg_transpose(int device, tg_dtype dtype, const void* src, void* dst, int64_t batch,
                  int64_t rows, int64_t cols, void* stream);
 
+/* ---- 8-bit layer ---------------------------------------------------------
+ *
+ * What a linear layer in 8 bits needs beside the tropical products: rows of
+ * activations to 8-bit integers with one scale each (with or without a RMS
+ * norm before it), the product of such rows with the rows of an 8-bit weight
+ * matrix, and the gradients, which read the 8-bit operands as checkpoints of
+ * the forward pass.  No counterpart in the reference.
+ *
+ * Matrices are row-major; ld* is the distance of two rows in elements (at
+ * least the row's length; a row's elements are neighbours).  Rows may start
+ * at any address that suits an element; outputs are dense and overlap no
+ * input.  Sums, norms and scales are f32 (products of 8-bit integers: exact
+ * i32), and outputs are rounded once to the given type.  Calls are
+ * asynchronous on the stream, allocate nothing and launch kernels only, so
+ * they may be captured in a graph.  Workspaces are 256-byte aligned, of at
+ * least the bytes their size function gives; nothing in them needs clearing.
+ */
+
+/* Element type of activations, gradients and outputs. */
+typedef enum { TG_FLOAT32 = 0, TG_BF16 = 1, TG_F16 = 2 } tg_float;
+
+/* q[i, j] = rint(x[i, j] * 127 / top_i), scale[i] = top_i / 127 with
+ * top_i = max(max_j |x[i, j]|, 1e-30).  A row that holds a NaN gets a NaN
+ * scale; one that holds an infinity gets an infinite scale and zeros. */
+int tg_i8_quantize(int device, tg_float type, const void* x, int64_t ldx, int8_t* q, float* scale,
+                   int64_t rows, int64_t cols, void* stream);
+
+/* y[i, j] = q[i, j] * scale[i], rounded to type. */
+int tg_i8_dequantize(int device, tg_float type, const int8_t* q, int64_t ldq, const float* scale,
+                     void* y, int64_t rows, int64_t cols, void* stream);
+
+/* h = x + residual, rounded to type (residual and h NULL: h stands for x);
+ * y = h * (mean_j h^2 + eps)^-1/2 * weight, given as q and scale (q * scale is
+ * y to 8 bits of the row's maximum, as in tg_i8_quantize).  weight is of type
+ * or f32. */
+int tg_i8_rms_norm(int device, tg_float type, tg_float weight_type, const void* x, int64_t ldx,
+                   const void* residual, int64_t ldr, const void* weight, float eps, int8_t* q,
+                   float* scale, void* h, int64_t rows, int64_t cols, void* stream);
+
+/* Gradients of y above with respect to h and weight, for grad_y (the rounding
+ * to 8 bits passes them on unchanged):
+ *   xh = h * rstd, u = grad_y * weight, rstd = (mean_j h^2 + eps)^-1/2,
+ *   grad_x = rstd * (u - xh * mean_j(u * xh)) + grad_h,
+ *   grad_weight = sum_i grad_y * xh            (of weight_type).
+ * grad_h, the gradient that reaches h from elsewhere, may be NULL.  grad_x is
+ * the gradient of x and of residual.  Sums are made in a fixed order: equal
+ * calls give equal bits. */
+size_t tg_i8_rms_norm_backward_workspace_size(int64_t rows, int64_t cols);
+int tg_i8_rms_norm_backward(int device, tg_float type, tg_float weight_type, const void* grad_y,
+                            int64_t ldg, const void* h, int64_t ldh, const void* weight, float eps,
+                            const void* grad_h, int64_t ldgh, void* grad_x, void* grad_weight,
+                            int64_t rows, int64_t cols, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* c[i, j] = (sum_k a[i, k] * b[j, k]) * a_scale[i] * b_scale[j] + bias[j]:
+ * a is m x k, b is n x k (a weight matrix as it is stored: one row for each
+ * output), bias of type or NULL, c is m x n of type.  The sum is exact;
+ * k < 2^17.  k == 0 gives the bias (or zero). */
+size_t tg_i8_gemm_workspace_size(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb,
+                                 int64_t m, int64_t n, int64_t k);
+int tg_i8_gemm(int device, tg_float type, const int8_t* a, int64_t lda, const float* a_scale,
+               const int8_t* b, int64_t ldb, const float* b_scale, const void* bias, void* c,
+               int64_t m, int64_t n, int64_t k, void* workspace, size_t workspace_bytes,
+               void* stream);
+
+/* grad_a[i, k] = sum_j grad_c[i, j] * b_scale[j] * b[j, k]: the gradient of
+ * a[i, k] * a_scale[i].  grad_c is m x n and grad_a m x k, of type. */
+size_t tg_i8_backward_a_workspace_size(tg_float type, const void* grad_c, int64_t ldg, int64_t m,
+                                       int64_t n, int64_t k);
+int tg_i8_backward_a(int device, tg_float type, const void* grad_c, int64_t ldg, const int8_t* b,
+                     int64_t ldb, const float* b_scale, void* grad_a, int64_t m, int64_t n,
+                     int64_t k, void* workspace, size_t workspace_bytes, void* stream);
+
+/* grad_b[j, k] = sum_i grad_c[i, j] * a_scale[i] * a[i, k]: the gradient of
+ * b[j, k] * b_scale[j], from the forward pass's 8-bit activations.  grad_b is
+ * n x k of type. */
+size_t tg_i8_backward_b_workspace_size(tg_float type, const void* grad_c, int64_t ldg, int64_t m,
+                                       int64_t n, int64_t k);
+int tg_i8_backward_b(int device, tg_float type, const void* grad_c, int64_t ldg, const int8_t* a,
+                     int64_t lda, const float* a_scale, void* grad_b, int64_t m, int64_t n,
+                     int64_t k, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

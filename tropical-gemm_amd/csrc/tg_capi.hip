@@ -24,6 +24,7 @@
 #include "tg_gemm_kres8.hpp"
 #include "tg_gemm_kresw.hpp"
 #include "tg_gemm_shortk.hpp"
+#include "tg_host.hpp"
 #include "tg_kernels.hpp"
 #include "tg_kresg.hpp"
 #include "tg_small.hpp"
@@ -2024,6 +2025,14 @@ int backward_impl(int device, tg_dtype dt, tg_layout layout, bool want_a, const 
 // ============================================================================
 // Exported C ABI
 // ============================================================================
+
+namespace tg {
+
+int host_fail(int status, const std::string& msg) { return fail(status, msg); }
+int host_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
+int host_select_device(int device) { return select_device(device); }
+
+}  // namespace tg
 
 extern "C" {
 

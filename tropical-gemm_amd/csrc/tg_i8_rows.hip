@@ -1,0 +1,381 @@
+// tg_i8_rows.hip -- row operators of the 8-bit layer: RMS norm with the
+// residual's addition and 8-bit output, its backward pass, and rows packed to
+// 8 bits with a scale and restored.
+//
+// All of them are bound by HBM: every input element is read once, every
+// output written once, a row's values stay in registers between its reduction
+// and its output.
+#include "../../include/tropical_gemm_hip.h"
+#include "tg_i8.hpp"
+#include "tg_i8_types.hpp"
+
+namespace tg {
+namespace {
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// One row's threads: NT lanes of a workgroup, 256 / NT rows per workgroup
+// where NT is below 256.  A thread holds VPT groups of eight neighbouring
+// elements, group g of thread t starting at element (g * NT + t) * 8, so the
+// lanes of a wave read 1 KiB (of 16-bit elements) side by side.
+template <int NT>
+constexpr int kRowsPerBlock = NT < 256 ? 256 / NT : 1;
+template <int NT>
+constexpr int kBlock = NT < 256 ? 256 : NT;
+
+// Reduces (sum, top) over the NT threads of each row; every thread gets both.
+template <int NT>
+__device__ __forceinline__ void row_reduce(float& sum, float& top) {
+    sum = wave_sum(sum);
+    top = wave_max(top);
+    if constexpr (NT > 64) {
+        constexpr int W = NT / 64;
+        __shared__ float part[2][kRowsPerBlock<NT> * W];
+        const int wave = threadIdx.x / 64, first = wave / W * W;
+        if (threadIdx.x % 64 == 0) {
+            part[0][wave] = sum;
+            part[1][wave] = top;
+        }
+        __syncthreads();
+        sum = part[0][first];
+        top = part[1][first];
+#pragma unroll
+        for (int i = 1; i < W; ++i) {
+            sum += part[0][first + i];
+            top = max_nan(top, part[1][first + i]);
+        }
+    }
+}
+
+// h = round(x + residual); rstd = (mean h^2 + eps)^-1/2; v = h * w;
+// top = max(max |v|, tiny); q = rint(v * 127 / top); scale = top * rstd / 127.
+// rstd cancels in q, so q depends on no order of summation, and both
+// reductions of the row are made in one pass.  NORM false: v = x, rstd = 1.
+// A NaN or infinity makes the row's scale NaN or infinite with zeros in q, so
+// its values are NaN, as dividing by the row's maximum gives them.
+// VPT 0: rows of any length, read again (through L2) after the reduction.
+template <typename T, typename W, bool NORM, bool RES, int NT, int VPT>
+__global__ __launch_bounds__(kBlock<NT>) void tg_i8_rows(const T* __restrict__ x, int64_t ldx,
+                                                         const T* __restrict__ res, int64_t ldr,
+                                                         const W* __restrict__ w, float eps,
+                                                         int8_t* __restrict__ q,
+                                                         float* __restrict__ scale, T* __restrict__ h,
+                                                         int64_t rows, int64_t cols) {
+    const int t = threadIdx.x % NT;
+    const int64_t row = int64_t(blockIdx.x) * kRowsPerBlock<NT> + threadIdx.x / NT;
+    const bool live = row < rows;  // every thread reaches the reduction's barrier
+    const T* xr = x + row * ldx;
+    const T* rr = RES ? res + row * ldr : nullptr;
+    float sum = 0.0f, top = 0.0f;
+
+    // One group: the (rounded) stream and its weighted values.
+    auto take = [&](int64_t at, float(&v)[8], bool first) {
+        const int n = cols - at < 8 ? int(cols - at) : 8;
+        load_upto8(xr + at, n, v);
+        if constexpr (RES) {
+            float r[8];
+            load_upto8(rr + at, n, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_f32(static_cast<T>(v[i] + r[i]));
+            if (first) store_upto8(h + row * cols + at, n, v);
+        }
+        if constexpr (NORM) {
+            float g[8];
+            load_upto8(w + at, n, g);
+            if (first) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += v[i] * v[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= g[i];
+        }
+        if (first) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[i]));
+        }
+    };
+    auto give = [&](int64_t at, const float(&v)[8], float inv) {
+        int o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = __float2int_rn(v[i] * inv);
+            o[i] = r > 127 ? 127 : (r < -127 ? -127 : r);
+        }
+        store_i8_upto8(q + row * cols + at, cols - at < 8 ? int(cols - at) : 8, o);
+    };
+
+    constexpr int G = VPT > 0 ? VPT : 1;
+    float v[G][8];
+    if (live) {
+        if constexpr (VPT > 0) {
+#pragma unroll
+            for (int g = 0; g < VPT; ++g) {
+                const int64_t at = int64_t(g * NT + t) * 8;
+                if (at < cols) take(at, v[g], true);
+            }
+        } else {
+            for (int64_t at = int64_t(t) * 8; at < cols; at += NT * 8) take(at, v[0], true);
+        }
+    }
+    row_reduce<NT>(sum, top);
+    if (!live) return;
+    top = max_nan(top, kI8TinyTop);
+    const float inv = 127.0f / top;
+    if (t == 0) {
+        if constexpr (NORM) {
+            const float rstd = 1.0f / sqrtf(sum / float(cols > 0 ? cols : 1) + eps);
+            scale[row] = top * rstd / 127.0f;
+        } else {
+            scale[row] = top / 127.0f;
+        }
+    }
+    if constexpr (VPT > 0) {
+#pragma unroll
+        for (int g = 0; g < VPT; ++g) {
+            const int64_t at = int64_t(g * NT + t) * 8;
+            if (at < cols) give(at, v[g], inv);
+        }
+    } else {
+        for (int64_t at = int64_t(t) * 8; at < cols; at += NT * 8) {
+            take(at, v[0], false);
+            give(at, v[0], inv);
+        }
+    }
+}
+
+template <typename T, typename W, bool NORM, bool RES, int NT, int VPT>
+hipError_t launch_rows(const I8Norm& p, hipStream_t st) {
+    // A launch's thread count stays below 2^32.
+    constexpr int64_t kMost = int64_t(1) << 21;
+    for (int64_t r0 = 0; r0 < p.rows; r0 += kMost) {
+        const int64_t n = p.rows - r0 < kMost ? p.rows - r0 : kMost;
+        hipLaunchKernelGGL((tg_i8_rows<T, W, NORM, RES, NT, VPT>), dim3(unsigned(ceil_div(n, kRowsPerBlock<NT>))),
+                           dim3(kBlock<NT>), 0, st, static_cast<const T*>(p.x) + r0 * p.ldx, p.ldx,
+                           RES ? static_cast<const T*>(p.residual) + r0 * p.ldr : nullptr, p.ldr,
+                           static_cast<const W*>(p.weight), p.eps, p.q + r0 * p.cols, p.scale + r0,
+                           RES ? static_cast<T*>(p.h) + r0 * p.cols : nullptr, n, p.cols);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+template <typename T, typename W, bool NORM, bool RES>
+hipError_t rows_form(const I8Norm& p, hipStream_t st) {
+    const int64_t groups = ceil_div(p.cols, 8);
+    if (groups <= 64) return launch_rows<T, W, NORM, RES, 64, 1>(p, st);
+    if (groups <= 256) return launch_rows<T, W, NORM, RES, 256, 1>(p, st);
+    if (groups <= 1024) return launch_rows<T, W, NORM, RES, 256, 4>(p, st);
+    return launch_rows<T, W, NORM, RES, 1024, 0>(p, st);
+}
+
+template <typename T, typename W>
+hipError_t norm_typed(const I8Norm& p, hipStream_t st) {
+    return p.residual != nullptr ? rows_form<T, W, true, true>(p, st) : rows_form<T, W, true, false>(p, st);
+}
+
+// f(T()) for the element type.
+template <typename F>
+hipError_t by_type(int type, F&& f) {
+    switch (type) {
+        case TG_BF16: return f(bf16_t());
+        case TG_F16: return f(f16_t());
+        default: return f(float());
+    }
+}
+
+// y = round(q * scale), eight elements a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void tg_i8_restore(const int8_t* __restrict__ q, int64_t ldq,
+                                                     const float* __restrict__ scale, T* __restrict__ y,
+                                                     int64_t rows, int64_t cols, int64_t groups) {
+    const int64_t stride = int64_t(gridDim.x) * 256;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * groups; i += stride) {
+        const int64_t row = i / groups, at = (i - row * groups) * 8;
+        const int n = cols - at < 8 ? int(cols - at) : 8;
+        const float s = scale[row];
+        float v[8];
+        load_i8_upto8(q + row * ldq + at, n, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= s;
+        store_upto8(y + row * cols + at, n, v);
+    }
+}
+
+// Backward of the norm.  u = gy * w, rstd and c = rstd^2 * mean(u * h) of each
+// row, gx = rstd * (u - h * c) + gh; the workgroup adds gy * h * rstd of its
+// rows (blockIdx.x, + gridDim.x, ...) in that order in registers, and writes
+// that sum of each column to part[blockIdx.x].  The columns of a thread are as
+// in tg_i8_rows; blockIdx.y takes the next NT * VPT * 8 of them when COLS
+// does not hold the row (then every workgroup of a row reduces all of it).
+template <typename T, typename W, int NT, int VPT>
+__global__ __launch_bounds__(NT) void tg_i8_norm_backward(
+    const T* __restrict__ gy, int64_t ldg, const T* __restrict__ h, int64_t ldh, const W* __restrict__ w,
+    float eps, const T* __restrict__ gh, int64_t ldgh, T* __restrict__ gx, float* __restrict__ part,
+    int64_t rows, int64_t cols) {
+    constexpr int W64 = NT / 64;
+    __shared__ float red[2][2][W64];
+    const int t = threadIdx.x, wave = t / 64;
+    const int64_t base = int64_t(blockIdx.y) * (NT * VPT * 8);
+    float acc[VPT][8] = {};
+    int flip = 0;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, flip ^= 1) {
+        float g[VPT][8], hv[VPT][8];
+        float ss = 0.0f, dot = 0.0f;
+        auto add = [&](int64_t at, float(&gv)[8], float(&hh)[8]) {
+            const int n = cols - at < 8 ? int(cols - at) : 8;
+            float wv[8];
+            load_upto8(gy + row * ldg + at, n, gv);
+            load_upto8(h + row * ldh + at, n, hh);
+            load_upto8(w + at, n, wv);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                ss += hh[i] * hh[i];
+                dot += gv[i] * wv[i] * hh[i];
+            }
+        };
+        if (gridDim.y > 1) {  // the part of the row that other workgroups hold
+            float a[8], b[8];
+            for (int64_t at = int64_t(t) * 8; at < cols; at += NT * 8)
+                if (at < base || at >= base + NT * VPT * 8) add(at, a, b);
+        }
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int64_t at = base + int64_t(k * NT + t) * 8;
+            if (at < cols) add(at, g[k], hv[k]);
+        }
+        ss = wave_sum(ss);
+        dot = wave_sum(dot);
+        if (t % 64 == 0) {
+            red[flip][0][wave] = ss;
+            red[flip][1][wave] = dot;
+        }
+        __syncthreads();
+        ss = dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W64; ++i) {
+            ss += red[flip][0][i];
+            dot += red[flip][1][i];
+        }
+        const float inv_n = 1.0f / float(cols);
+        const float rstd = 1.0f / sqrtf(ss * inv_n + eps);
+        const float c = dot * inv_n * rstd * rstd;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int64_t at = base + int64_t(k * NT + t) * 8;
+            if (at >= cols) continue;
+            const int n = cols - at < 8 ? int(cols - at) : 8;
+            float wv[8], o[8];
+            load_upto8(w + at, n, wv);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                acc[k][i] += g[k][i] * (hv[k][i] * rstd);
+                o[i] = rstd * (g[k][i] * wv[i] - hv[k][i] * c);
+            }
+            if (gh != nullptr) {
+                float a[8];
+                load_upto8(gh + row * ldgh + at, n, a);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] += a[i];
+            }
+            store_upto8(gx + row * cols + at, n, o);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int64_t at = base + int64_t(k * NT + t) * 8;
+        if (at < cols) store_upto8(part + int64_t(blockIdx.x) * cols + at, cols - at < 8 ? int(cols - at) : 8, acc[k]);
+    }
+}
+
+// gw[j] = sum over the parts, in their order within each of the 16 slices and
+// then over the slices: the same bits in every run.
+template <typename W>
+__global__ __launch_bounds__(1024) void tg_i8_sum_parts(const float* __restrict__ part, int64_t parts,
+                                                        W* __restrict__ gw, int64_t cols) {
+    __shared__ float s[16][64];
+    const int c = threadIdx.x % 64, y = threadIdx.x / 64;
+    const int64_t col = int64_t(blockIdx.x) * 64 + c;
+    float a = 0.0f;
+    if (col < cols)
+        for (int64_t r = y; r < parts; r += 16) a += part[r * cols + col];
+    s[y][c] = a;
+    __syncthreads();
+    if (y == 0 && col < cols) {
+        for (int i = 1; i < 16; ++i) a += s[i][c];
+        gw[col] = static_cast<W>(a);
+    }
+}
+
+int64_t backward_parts(int64_t rows) { return rows < 512 ? rows : 512; }
+
+template <typename T, typename W, int NT, int VPT>
+hipError_t launch_norm_backward(const I8NormBackward& p, float* part, hipStream_t st) {
+    const int64_t parts = backward_parts(p.rows);
+    if (parts > 0) {
+        const dim3 grid(unsigned(parts), unsigned(ceil_div(p.cols, NT * VPT * 8)));
+        hipLaunchKernelGGL((tg_i8_norm_backward<T, W, NT, VPT>), grid, dim3(NT), 0, st,
+                           static_cast<const T*>(p.grad_y), p.ldg, static_cast<const T*>(p.h), p.ldh,
+                           static_cast<const W*>(p.weight), p.eps, static_cast<const T*>(p.grad_h), p.ldgh,
+                           static_cast<T*>(p.grad_x), part, p.rows, p.cols);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((tg_i8_sum_parts<W>), dim3(unsigned(ceil_div(p.cols, 64))), dim3(1024), 0, st, part,
+                       parts, static_cast<W*>(p.grad_weight), p.cols);
+    return hipGetLastError();
+}
+
+template <typename T, typename W>
+hipError_t norm_backward_typed(const I8NormBackward& p, float* part, hipStream_t st) {
+    const int64_t groups = ceil_div(p.cols, 8);
+    if (groups <= 64) return launch_norm_backward<T, W, 64, 1>(p, part, st);
+    if (groups <= 256) return launch_norm_backward<T, W, 256, 1>(p, part, st);
+    return launch_norm_backward<T, W, 512, 2>(p, part, st);
+}
+
+}  // namespace
+
+hipError_t i8_rms_norm(const I8Norm& p, hipStream_t st) {
+    if (p.rows == 0) return hipSuccess;
+    return by_type(p.type, [&](auto tag) {
+        using T = decltype(tag);
+        return p.weight_type == p.type ? norm_typed<T, T>(p, st) : norm_typed<T, float>(p, st);
+    });
+}
+
+hipError_t i8_quantize(const I8Norm& p, hipStream_t st) {
+    if (p.rows == 0) return hipSuccess;
+    return by_type(p.type, [&](auto tag) {
+        using T = decltype(tag);
+        return rows_form<T, T, false, false>(p, st);
+    });
+}
+
+hipError_t i8_dequantize(int type, const int8_t* q, int64_t ldq, const float* scale, void* y,
+                         int64_t rows, int64_t cols, hipStream_t st) {
+    if (rows == 0 || cols == 0) return hipSuccess;
+    const int64_t groups = ceil_div(cols, 8), blocks = ceil_div(rows * groups, 256);
+    return by_type(type, [&](auto tag) {
+        using T = decltype(tag);
+        hipLaunchKernelGGL((tg_i8_restore<T>), dim3(unsigned(blocks < 65536 ? blocks : 65536)), dim3(256), 0,
+                           st, q, ldq, scale, static_cast<T*>(y), rows, cols, groups);
+        return hipGetLastError();
+    });
+}
+
+size_t i8_rms_norm_backward_ws(int64_t rows, int64_t cols) {
+    return size_t(backward_parts(rows)) * size_t(cols) * sizeof(float);
+}
+
+hipError_t i8_rms_norm_backward(const I8NormBackward& p, void* ws, hipStream_t st) {
+    if (p.cols == 0) return hipSuccess;
+    float* part = static_cast<float*>(ws);
+    return by_type(p.type, [&](auto tag) {
+        using T = decltype(tag);
+        return p.weight_type == p.type ? norm_backward_typed<T, T>(p, part, st)
+                                       : norm_backward_typed<T, float>(p, part, st);
+    });
+}
+
+}  // namespace tg

@@ -29,12 +29,14 @@ TG_ERR_UNSUPPORTED = 7
 SEMIRING = {"maxplus": 0, "minplus": 1, "maxmul": 2}
 DTYPE = {"f32": 0, "f64": 1, "i32": 2, "i64": 3}
 LAYOUT = {"row": 0, "col": 1}
+FLOAT = {"f32": 0, "bf16": 1, "f16": 2}
 
 # Every symbol the header declares, with its ctypes signature.
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
+_f32 = ctypes.c_float
 SIGNATURES = {
     "tg_version": ([], _i32),
     "tg_status_string": ([_i32], ctypes.c_char_p),
@@ -80,6 +82,22 @@ SIGNATURES = {
     "tg_backward_b_strided_batched": ([_i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                        _i64, _i64, _i64, _i64, _vp], _i32),
     "tg_transpose": ([_i32, _i32, _vp, _vp, _i64, _i64, _i64, _vp], _i32),
+    "tg_i8_quantize": ([_i32, _i32, _vp, _i64, _vp, _vp, _i64, _i64, _vp], _i32),
+    "tg_i8_dequantize": ([_i32, _i32, _vp, _i64, _vp, _vp, _i64, _i64, _vp], _i32),
+    "tg_i8_rms_norm": ([_i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _f32, _vp, _vp, _vp, _i64, _i64,
+                        _vp], _i32),
+    "tg_i8_rms_norm_backward_workspace_size": ([_i64, _i64], _sz),
+    "tg_i8_rms_norm_backward": ([_i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _f32, _vp, _i64, _vp,
+                                 _vp, _i64, _i64, _vp, _sz, _vp], _i32),
+    "tg_i8_gemm_workspace_size": ([_vp, _i64, _vp, _i64, _i64, _i64, _i64], _sz),
+    "tg_i8_gemm": ([_i32, _i32, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _sz,
+                    _vp], _i32),
+    "tg_i8_backward_a_workspace_size": ([_i32, _vp, _i64, _i64, _i64, _i64], _sz),
+    "tg_i8_backward_a": ([_i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz,
+                          _vp], _i32),
+    "tg_i8_backward_b_workspace_size": ([_i32, _vp, _i64, _i64, _i64, _i64], _sz),
+    "tg_i8_backward_b": ([_i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz,
+                          _vp], _i32),
 }
 
 

@@ -1,0 +1,231 @@
+"""Linear layers in 8 bits: device tensors in, device tensors out.
+
+The operators a linear layer needs beside the tropical products, over the
+``tg_i8_*`` entry points of the C ABI.  No counterpart in the reference.
+
+* ``quantize`` / ``dequantize``: rows to 8-bit integers with one f32 scale each,
+  and back: a layer's activations kept for its backward pass in half the bytes.
+* ``rms_norm``: the residual's addition, the RMS norm and its 8-bit output in
+  one pass; ``rms_norm_backward`` its gradients.
+* ``matmul``: 8-bit rows times the rows of an 8-bit weight matrix, with a scale
+  for each token and each output channel.
+* ``backward_a`` / ``backward_b``: the gradients of that product, read from the
+  8-bit operands.
+
+``tropical_gemm.pytorch`` joins them to autograd functions.  Matrices are 2-D;
+rows may be strided (a slice of a wider matrix) and start anywhere, a row's
+elements must be neighbours.  Activations and gradients are bfloat16, float16
+or float32; sums and scales are f32 (i32 for 8-bit products).  Outputs and
+workspaces come from torch's allocator, launches go to torch's current stream
+of the inputs' device.  These functions do not record gradients themselves.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _native as nat
+from .ops import _ptr, _stream
+
+_FLOAT = {torch.float32: nat.FLOAT["f32"], torch.bfloat16: nat.FLOAT["bf16"],
+          torch.float16: nat.FLOAT["f16"]}
+
+
+def _rows(name: str, t: torch.Tensor, dtype=None) -> int:
+    """Checks a matrix on the GPU whose rows are neighbours; its row stride."""
+    if t.device.type != "cuda":
+        raise ValueError("tropical_gemm GPU entry points need device tensors "
+                         f"({name} is on {t.device.type}); move the tensors to the GPU first")
+    if t.dim() != 2:
+        raise ValueError(f"Expected a 2D tensor for {name}, got {t.dim()} dims")
+    if dtype is None:
+        if t.dtype not in _FLOAT:
+            raise ValueError(f"Unsupported dtype {t.dtype} of {name}: expected bfloat16, float16 or float32")
+    elif t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if rows <= 1 or cols == 0:
+        ld = cols
+    if (cols > 1 and step != 1) or ld < cols:
+        raise ValueError(f"The elements of a row of {name} must be neighbours and its rows apart, got strides "
+                         f"{tuple(t.stride())} (call .contiguous() on PyTorch tensors)")
+    return ld
+
+
+def _vector(name: str, t: torch.Tensor, n: int, dtypes) -> None:
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"Dimension mismatch: {name} has shape {tuple(t.shape)}, expected ({n},)")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if n > 1 and t.stride(0) != 1:
+        raise ValueError(f"{name} must be contiguous (call .contiguous() on PyTorch tensors)")
+
+
+def _same_device(*named) -> torch.device:
+    """The device of the first of (name, tensor) pairs, which all others that
+    are not None must share."""
+    first, dev = named[0][0], named[0][1].device
+    for name, t in named[1:]:
+        if t is not None and t.device != dev:
+            raise ValueError(f"Tensors must be on the same device: {first} is on {dev}, {name} is on {t.device}")
+    return dev
+
+
+def _same_shape(name: str, t: torch.Tensor, shape) -> None:
+    if t.shape != shape:
+        raise ValueError(f"Dimension mismatch: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _workspace(nbytes: int, dev: torch.device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def quantize(x: torch.Tensor):
+    """``(q, scale)`` of each row of ``x``: ``scale = max|x| / 127`` (f32) and
+    ``q = rint(x / scale)`` (int8), so that ``q * scale`` is x to half a step.
+    A row of zeros gives zeros; a row that holds a NaN or an infinity gives
+    values that are NaN."""
+    ld = _rows("x", x)
+    rows, cols = x.shape
+    dev = x.device
+    q = torch.empty((rows, cols), dtype=torch.int8, device=dev)
+    scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    nat.check(nat.load().tg_i8_quantize(dev.index or 0, _FLOAT[x.dtype], x.data_ptr(), ld, q.data_ptr(),
+                                        scale.data_ptr(), rows, cols, _stream(dev)))
+    return q, scale
+
+
+def dequantize(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``q * scale[:, None]`` rounded to ``dtype``."""
+    ld = _rows("q", q, torch.int8)
+    rows, cols = q.shape
+    _vector("scale", scale, rows, (torch.float32,))
+    dev = _same_device(("q", q), ("scale", scale))
+    _float_type(dtype)
+    y = torch.empty((rows, cols), dtype=dtype, device=dev)
+    nat.check(nat.load().tg_i8_dequantize(dev.index or 0, _FLOAT[dtype], q.data_ptr(), ld, scale.data_ptr(),
+                                          y.data_ptr(), rows, cols, _stream(dev)))
+    return y
+
+
+def _float_type(dtype: torch.dtype) -> int:
+    if dtype not in _FLOAT:
+        raise ValueError(f"Unsupported dtype {dtype}: expected bfloat16, float16 or float32")
+    return _FLOAT[dtype]
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6):
+    """``(q, scale, h)``: ``h = x + residual`` in x's type (x itself without a
+    residual), and ``h * rsqrt(mean(h^2) + eps) * weight`` as 8-bit rows with
+    scales.  ``weight`` is of x's type or float32."""
+    ldx = _rows("x", x)
+    rows, cols = x.shape
+    _vector("weight", weight, cols, (x.dtype, torch.float32))
+    dev = _same_device(("x", x), ("weight", weight), ("residual", residual))
+    ldr, h = 0, x
+    if residual is not None:
+        ldr = _rows("residual", residual, x.dtype)
+        _same_shape("residual", residual, x.shape)
+        h = torch.empty((rows, cols), dtype=x.dtype, device=dev)
+    q = torch.empty((rows, cols), dtype=torch.int8, device=dev)
+    scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    nat.check(nat.load().tg_i8_rms_norm(
+        dev.index or 0, _FLOAT[x.dtype], _FLOAT[weight.dtype], x.data_ptr(), ldx, _ptr(residual), ldr,
+        weight.data_ptr(), eps, q.data_ptr(), scale.data_ptr(), None if residual is None else h.data_ptr(), rows,
+        cols, _stream(dev)))
+    return q, scale, h
+
+
+def rms_norm_backward(grad_y: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+                      grad_h: torch.Tensor | None = None):
+    """``(grad_x, grad_weight)`` of ``rms_norm`` for the gradient of its
+    normalised output (the rounding to 8 bits passes it on unchanged), with
+    ``grad_h``, the gradient of the stream h from elsewhere, added to grad_x.
+    grad_x is the gradient of x and of the residual.  Equal calls give equal
+    bits."""
+    ldh = _rows("h", h)
+    rows, cols = h.shape
+    _same_shape("grad_y", grad_y, h.shape)
+    ldg = _rows("grad_y", grad_y, h.dtype)
+    _vector("weight", weight, cols, (h.dtype, torch.float32))
+    dev = _same_device(("h", h), ("grad_y", grad_y), ("weight", weight), ("grad_h", grad_h))
+    ldgh = 0
+    if grad_h is not None:
+        _same_shape("grad_h", grad_h, h.shape)
+        ldgh = _rows("grad_h", grad_h, h.dtype)
+    grad_x = torch.empty((rows, cols), dtype=h.dtype, device=dev)
+    grad_weight = torch.empty(cols, dtype=weight.dtype, device=dev)
+    lib = nat.load()
+    nbytes = lib.tg_i8_rms_norm_backward_workspace_size(rows, cols)
+    ws = _workspace(nbytes, dev)
+    nat.check(lib.tg_i8_rms_norm_backward(
+        dev.index or 0, _FLOAT[h.dtype], _FLOAT[weight.dtype], grad_y.data_ptr(), ldg, h.data_ptr(), ldh,
+        weight.data_ptr(), eps, _ptr(grad_h), ldgh, grad_x.data_ptr(), grad_weight.data_ptr(), rows, cols,
+        _ptr(ws), nbytes, _stream(dev)))
+    return grad_x, grad_weight
+
+
+def matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+           bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(a @ b.T) * a_scale[:, None] * b_scale + bias`` in ``dtype``: ``a`` (m, k)
+    int8 activations, ``b`` (n, k) an int8 weight matrix with one row for each
+    output, f32 scales, ``bias`` of ``dtype``.  The integer sum is exact
+    (k < 2**17)."""
+    lda = _rows("a", a, torch.int8)
+    ldb = _rows("b", b, torch.int8)
+    m, k = a.shape
+    n, k2 = b.shape
+    if k != k2:
+        raise ValueError(f"Dimension mismatch: a is {m}x{k}, b is {n}x{k2}")
+    _vector("a_scale", a_scale, m, (torch.float32,))
+    _vector("b_scale", b_scale, n, (torch.float32,))
+    kind = _float_type(dtype)
+    if bias is not None:
+        _vector("bias", bias, n, (dtype,))
+    dev = _same_device(("a", a), ("b", b), ("a_scale", a_scale), ("b_scale", b_scale), ("bias", bias))
+    c = torch.empty((m, n), dtype=dtype, device=dev)
+    lib = nat.load()
+    pa, pb = a.data_ptr(), b.data_ptr()
+    nbytes = lib.tg_i8_gemm_workspace_size(pa, lda, pb, ldb, m, n, k) if k < 1 << 17 else 0
+    ws = _workspace(nbytes, dev)
+    nat.check(lib.tg_i8_gemm(dev.index or 0, kind, pa, lda, a_scale.data_ptr(), pb, ldb, b_scale.data_ptr(),
+                             _ptr(bias), c.data_ptr(), m, n, k, _ptr(ws), nbytes, _stream(dev)))
+    return c
+
+
+def _backward(which: str, grad_c: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    ldg = _rows("grad_c", grad_c)
+    other = "b" if which == "a" else "a"
+    ldq = _rows(other, q, torch.int8)
+    m, n = grad_c.shape
+    depth, k = q.shape
+    if depth != (n if which == "a" else m):
+        raise ValueError(f"Dimension mismatch: grad_c is {m}x{n}, {other} is {depth}x{k}")
+    _vector(f"{other}_scale", scale, depth, (torch.float32,))
+    dev = _same_device(("grad_c", grad_c), (other, q), (f"{other}_scale", scale))
+    out = torch.empty((m if which == "a" else n, k), dtype=grad_c.dtype, device=dev)
+    lib = nat.load()
+    size, run = ((lib.tg_i8_backward_a_workspace_size, lib.tg_i8_backward_a) if which == "a" else
+                 (lib.tg_i8_backward_b_workspace_size, lib.tg_i8_backward_b))
+    kind = _FLOAT[grad_c.dtype]
+    nbytes = size(kind, grad_c.data_ptr(), ldg, m, n, k)
+    ws = _workspace(nbytes, dev)
+    nat.check(run(dev.index or 0, kind, grad_c.data_ptr(), ldg, q.data_ptr(), ldq, scale.data_ptr(),
+                  out.data_ptr(), m, n, k, _ptr(ws), nbytes, _stream(dev)))
+    return out
+
+
+def backward_a(grad_c: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor) -> torch.Tensor:
+    """``grad_c @ (b * b_scale[:, None])``: the gradient of matmul's activations
+    ``a * a_scale[:, None]``, in grad_c's type."""
+    return _backward("a", grad_c, b, b_scale)
+
+
+def backward_b(grad_c: torch.Tensor, a: torch.Tensor, a_scale: torch.Tensor) -> torch.Tensor:
+    """``grad_c.T @ (a * a_scale[:, None])``: the gradient of matmul's weights
+    ``b * b_scale[:, None]``, in grad_c's type, from the 8-bit activations that
+    the forward pass kept."""
+    return _backward("b", grad_c, a, a_scale)
+
+
+__all__ = ["quantize", "dequantize", "rms_norm", "rms_norm_backward", "matmul", "backward_a", "backward_b"]
