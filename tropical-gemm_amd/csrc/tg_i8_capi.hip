@@ -92,6 +92,9 @@ hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
 // an i32 sum.
 constexpr int64_t kMostK = (int64_t(1) << 17) - 1;
 
+// The operands laid out along the sum have row strides below 2^23 bytes.
+constexpr int64_t kMostDepth = int64_t(1) << 20;
+
 int check_gemm(const tg::I8Gemm& p) {
     TG_CHECK(check_type(p.type));
     TG_CHECK(check_dims({p.m, p.n, p.k}));
@@ -104,6 +107,7 @@ int check_gemm(const tg::I8Gemm& p) {
 int check_grad(const tg::I8Grad& p, const char* q_name) {
     TG_CHECK(check_type(p.type));
     TG_CHECK(check_dims({p.rows, p.cols, p.depth}));
+    if (p.depth > kMostDepth) return bad_size("the gradient's sum has " + std::to_string(p.depth) + " terms: at most 2^20 are supported");
     TG_CHECK(check_ld("grad_c", p.ldg, p.transposed ? p.rows : p.depth));
     return check_ld(q_name, p.ldq, p.cols);
 }

@@ -1,15 +1,19 @@
-// tg_i8_gemm.hip -- the 8-bit layer's products: rows times rows in 8-bit
-// integers with scales, and the two gradients, which read one 8-bit operand.
+// tg_i8_gemm.hip -- launches of the 8-bit layer's products: rows times rows in
+// 8-bit integers with scales, and the two gradients, which read one 8-bit
+// operand.
+#include <cstdio>
+
 #include "../../include/tropical_gemm_hip.h"
 #include "tg_i8.hpp"
-#include "tg_i8_types.hpp"
+#include "tg_i8_pack.hpp"
+#include "tg_i8_stream.hpp"
+#include "tg_i8_tiles.hpp"
 
 namespace tg {
 namespace {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
 template <typename F>
 hipError_t by_type(int type, F&& f) {
@@ -20,123 +24,347 @@ hipError_t by_type(int type, F&& f) {
     }
 }
 
-// C = (A B^T) * a_scale * b_scale + bias on 64 x 64 tiles, 64 k at a time; four
-// waves of 32 x 32.  v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k of
-// row l % 16 from k = (l / 16) * 16, and the outputs of column l % 16, rows
-// (l / 16) * 4 ... + 3.  Operands pass through LDS byte by byte, so any
-// strides, alignment and sizes are right.
-template <typename T>
-__global__ __launch_bounds__(256) void tg_i8_gemm_tiles(const int8_t* __restrict__ A, int64_t lda,
-                                                        const float* __restrict__ sa,
-                                                        const int8_t* __restrict__ B, int64_t ldb,
-                                                        const float* __restrict__ sb,
-                                                        const T* __restrict__ bias, T* __restrict__ C,
-                                                        int64_t M, int64_t N, int64_t K, int64_t tiles_n) {
-    __shared__ __align__(16) int8_t la[64][80], lb[64][80];
-    const int t = threadIdx.x, lane = t % 64, wave = t / 64;
-    const int64_t m0 = int64_t(blockIdx.x) / tiles_n * 64, n0 = int64_t(blockIdx.x) % tiles_n * 64;
-    const int wm = wave / 2 * 32, wn = wave % 2 * 32;
-    i32x4 acc[2][2] = {};
-    for (int64_t k0 = 0; k0 < K; k0 += 64) {
-        for (int i = t; i < 64 * 64; i += 256) {
-            const int r = i / 64, k = i % 64;
-            la[r][k] = m0 + r < M && k0 + k < K ? A[(m0 + r) * lda + k0 + k] : int8_t(0);
-            lb[r][k] = n0 + r < N && k0 + k < K ? B[(n0 + r) * ldb + k0 + k] : int8_t(0);
-        }
-        __syncthreads();
-        i32x4 fa[2], fb[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            fa[i] = *reinterpret_cast<const i32x4*>(&la[wm + i * 16 + lane % 16][lane / 16 * 16]);
-            fb[i] = *reinterpret_cast<const i32x4*>(&lb[wn + i * 16 + lane % 16][lane / 16 * 16]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[i], fb[j], acc[i][j], 0, 0, 0);
-        __syncthreads();
+// ---- choice of a tile ----------------------------------------------------
+
+// A tile's sizes, workgroups per CU, and its time in us: `start` + step for
+// each 128 bytes of the sum while every workgroup has a CU of its own,
+// otherwise rounds of `round` + full for each 128 bytes.  Measured on MI355X
+// over 135 products (M 32 ... 8192, N 512 ... 8192, K 512 ... 8192 bytes), 8-bit
+// and bf16 alike (the time goes by bytes): the tile with the least time so
+// reckoned is 0.5% slower than the best one in the mean, 13% at most.
+struct TileTime {
+    int bm, bn, threads, per_cu;
+    double start, step, round, full;
+};
+constexpr TileTime kTiles[] = {
+    {256, 256, 512, 1, 6.8, 1.05, 8.3, 1.46}, {128, 128, 512, 1, 3.4, 0.365, 2.5, 0.49},
+    {128, 128, 256, 2, 3.4, 0.40, 3.2, 0.894}, {64, 128, 512, 2, 2.8, 0.267, 2.0, 0.58},
+    {64, 64, 256, 3, 2.7, 0.19, 1.1, 0.55},    {32, 64, 256, 3, 2.6, 0.165, 1.0, 0.42},
+};
+constexpr int kTileForms = sizeof(kTiles) / sizeof(kTiles[0]);
+
+struct TilePlan {
+    int form, slices;
+    int64_t tiles_m, tiles_n, slice;
+};
+
+double tile_time(const TileTime& c, int64_t tiles, int64_t steps) {
+    if (tiles <= 256) {
+        // A CU's neighbours take bandwidth from a 256 x 256 tile's step.
+        const double crowd = c.bm == 256 && tiles > 128 ? 0.9 * (c.full - c.step) * double(tiles - 128) / 128 : 0;
+        return c.start + double(steps) * (c.step + crowd);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int64_t m = m0 + wm + i * 16 + lane / 16 * 4 + e, n = n0 + wn + j * 16 + lane % 16;
-                if (m >= M || n >= N) continue;
-                float v = float(acc[i][j][e]) * sa[m] * sb[n];
-                if (bias != nullptr) v += to_f32(bias[n]);
-                C[m * N + n] = static_cast<T>(v);
-            }
+    const int64_t slots = 256 * int64_t(c.per_cu), whole = tiles / slots;
+    double t = 3 + double(whole) * (c.round + double(steps) * c.full);
+    const double last = double(tiles - whole * slots) / double(slots), depth = last * c.per_cu;
+    if (last > 0 && c.per_cu > 1)
+        t += c.round + double(steps) * (depth <= 1 ? c.step : c.step + (c.full - c.step) * (depth - 1) / (c.per_cu - 1));
+    else if (last > 0)
+        t += c.round + double(steps) * c.full * (0.75 + 0.25 * last);
+    return t;
 }
 
-// out[i, j] = sum over r of G(i, r) * scale[r] * q[r, j] in f32: 64 x 64 tiles,
-// 16 r at a time, 4 x 4 outputs a thread.
-template <typename T, bool TRANS>
-__global__ __launch_bounds__(256) void tg_i8_grad_tiles(const T* __restrict__ G, int64_t ldg,
-                                                        const int8_t* __restrict__ Q, int64_t ldq,
-                                                        const float* __restrict__ scale, T* __restrict__ out,
-                                                        int64_t rows, int64_t cols, int64_t depth,
-                                                        int64_t tiles_n) {
-    __shared__ float lg[16][65], lq[16][65];
-    const int t = threadIdx.x, tx = t % 16, ty = t / 16;
-    const int64_t i0 = int64_t(blockIdx.x) / tiles_n * 64, j0 = int64_t(blockIdx.x) % tiles_n * 64;
-    float acc[4][4] = {};
-    for (int64_t r0 = 0; r0 < depth; r0 += 16) {
-        for (int e = t; e < 16 * 64; e += 256) {
-            const int r = TRANS ? e / 64 : e % 16, i = TRANS ? e % 64 : e / 16;
-            const bool in = i0 + i < rows && r0 + r < depth;
-            lg[r][i] = in ? to_f32(G[TRANS ? (r0 + r) * ldg + i0 + i : (i0 + i) * ldg + r0 + r]) : 0.0f;
-            const int rq = e / 64, j = e % 64;
-            lq[rq][j] = j0 + j < cols && r0 + rq < depth ? float(Q[(r0 + rq) * ldq + j0 + j]) * scale[r0 + rq] : 0.0f;
+// Tile and slices of the sum: slices where tiles are few, as long as the time
+// they save outweighs their partial sums' way through memory and the launch
+// that joins them (2.5 us and 4 TB/s).
+TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps) {
+    if (m <= 0 || n <= 0 || steps <= 0) return {0, 1, 0, 0, 1};
+    TilePlan best = {0, 1, ceil_div(m, 256), ceil_div(n, 256), steps};
+    double least = 1e30;
+    for (int f = 0; f < kTileForms; ++f) {
+        const TileTime& c = kTiles[f];
+        const int64_t tm = ceil_div(m, c.bm), tn = ceil_div(n, c.bn);
+        // A launch's thread count stays below 2^32.
+        if (tm * tn >= (int64_t(1) << 32) / c.threads) continue;
+        for (int s = 1; s <= 32; s *= 2) {
+            const int64_t slice = ceil_div(steps, s);
+            if (s > 1 && (tm * tn * s > 512 || slice < 4)) break;
+            double t = tile_time(c, tm * tn * s, slice);
+            if (s > 1) t += 2.5 + double(s + 1) * double(m) * double(n) * 4 / 4e6;
+            if (t < least) {
+                least = t;
+                best = {f, int(ceil_div(steps, slice)), tm, tn, slice};
+            }
         }
-        __syncthreads();
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] += lg[r][ty + 16 * i] * lq[r][tx + 16 * j];
-        __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = i0 + ty + 16 * i, n = j0 + tx + 16 * j;
-            if (m < rows && n < cols) out[m * cols + n] = static_cast<T>(acc[i][j]);
+    return best;
+}
+
+size_t part_bytes(const TilePlan& pl, int64_t m, int64_t n) {
+    return pl.slices > 1 ? size_t(pl.slices) * size_t(m) * size_t(round_up(n, 8)) * 4 : 0;
+}
+
+template <typename K>
+hipError_t allow_lds(K* kernel, int bytes) {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+unsigned stride_grid(int64_t items) {
+    const int64_t blocks = ceil_div(items, 256);
+    return unsigned(blocks < 65536 ? blocks : 65536);
+}
+
+template <typename V, typename T>
+hipError_t launch_join(const V* part, int slices, int64_t m, int64_t n, const TileStore<T>& out, hipStream_t st) {
+    const int64_t ld = round_up(n, 8);
+    hipLaunchKernelGGL((tg_i8_tiles_join<V, T>), dim3(stride_grid(m * ld / 8)), dim3(256), 0, st, part, ld, slices, m,
+                       n, out);
+    return hipGetLastError();
+}
+
+template <Mma KIND, int WM, int WN, int FM, int FN, int NS, int PER_CU, typename T>
+hipError_t launch_form(TileArgs p, const TilePlan& pl, const TileStore<T>& out, void* part, hipStream_t st) {
+    using Cfg = Tile<KIND, 16, WM, WN, FM, FN, NS>;
+    const dim3 grid(unsigned(pl.tiles_m * pl.tiles_n), unsigned(pl.slices));
+    if (pl.slices == 1) {
+        const auto kernel = &tg_i8_tiles<KIND, 16, WM, WN, FM, FN, NS, PER_CU, T>;
+        static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+        if (attr != hipSuccess) return attr;
+        hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, out);
+        return hipGetLastError();
+    }
+    const auto kernel = &tg_i8_tiles_slice<KIND, 16, WM, WN, FM, FN, NS, PER_CU>;
+    static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+    if (attr != hipSuccess) return attr;
+    auto* sums = static_cast<typename Cfg::Value*>(part);
+    hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, TilePartial<typename Cfg::Value>{sums, round_up(p.n, 8)});
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : launch_join(sums, pl.slices, p.m, p.n, out, st);
+}
+
+template <Mma KIND, typename T>
+hipError_t launch_tiles(TileArgs p, const TilePlan& pl, const TileStore<T>& out, void* part, hipStream_t st) {
+    p.tiles_m = int(pl.tiles_m);
+    p.tiles_n = int(pl.tiles_n);
+    p.slice = int(pl.slice);
+    switch (pl.form) {
+        case 0: return launch_form<KIND, 2, 4, 8, 4, 2, 1>(p, pl, out, part, st);
+        case 1: return launch_form<KIND, 2, 4, 4, 2, 4, 1>(p, pl, out, part, st);
+        case 2: return launch_form<KIND, 2, 2, 4, 4, 2, 2>(p, pl, out, part, st);
+        case 3: return launch_form<KIND, 2, 4, 2, 2, 3, 2>(p, pl, out, part, st);
+        case 4: return launch_form<KIND, 2, 2, 2, 2, 3, 3>(p, pl, out, part, st);
+        default: return launch_form<KIND, 2, 2, 1, 2, 4, 3>(p, pl, out, part, st);
+    }
+}
+
+// True when tg_i8_tiles can read rows of `bytes` bytes in place.
+bool in_place(const void* p, int64_t ld_bytes, int64_t bytes) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0 && ld_bytes < (int64_t(1) << 23) && bytes % 16 == 0;
+}
+
+// Carves 256-byte aligned parts out of a workspace.
+struct Carver {
+    char* at;
+    size_t used = 0;
+    void* take(size_t bytes) {
+        void* p = at == nullptr ? nullptr : at + used;
+        used += (bytes + 255) / 256 * 256;
+        return p;
+    }
+};
+
+// ---- the 8-bit product ---------------------------------------------------
+
+// Up to 16 rows of A take the kernel that streams B: M = 16 against a tile of
+// 32 x 64, N = K = 8192: 17 us against 18, and rows of any alignment.
+constexpr int64_t kStreamRows = 16;
+
+struct GemmPlan {
+    bool stream, pack_a, pack_b;
+    int64_t ld;  // of packed rows
+    TilePlan tiles;
+};
+
+GemmPlan plan_gemm(const I8Gemm& p) {
+    GemmPlan pl{};
+    pl.stream = p.m <= kStreamRows;
+    if (pl.stream) return pl;
+    pl.pack_a = !in_place(p.a, p.lda, p.k);
+    pl.pack_b = !in_place(p.b, p.ldb, p.k);
+    pl.ld = round_up(p.k, 128);
+    pl.tiles = plan_tiles(p.m, p.n, ceil_div(p.k, 128));
+    return pl;
+}
+
+struct GemmWs {
+    int8_t *a, *b;
+    void* part;
+    size_t bytes;
+};
+
+GemmWs carve_gemm(const I8Gemm& p, const GemmPlan& pl, void* ws) {
+    Carver c{static_cast<char*>(ws)};
+    GemmWs w{};
+    if (p.m == 0 || p.n == 0 || p.k == 0 || pl.stream) return w;
+    if (pl.pack_a) w.a = static_cast<int8_t*>(c.take(size_t(p.m) * size_t(pl.ld)));
+    if (pl.pack_b) w.b = static_cast<int8_t*>(c.take(size_t(p.n) * size_t(pl.ld)));
+    w.part = c.take(part_bytes(pl.tiles, p.m, p.n));
+    w.bytes = c.used;
+    return w;
+}
+
+hipError_t pack_bytes(const void* src, int64_t ld_src, int64_t rows, int64_t bytes, void* dst, int64_t ld,
+                      hipStream_t st) {
+    hipLaunchKernelGGL(tg_i8_pack_bytes, dim3(stride_grid(rows * ld / 16)), dim3(256), 0, st,
+                       static_cast<const int8_t*>(src), ld_src, rows, int(bytes), static_cast<int8_t*>(dst), ld);
+    return hipGetLastError();
+}
+
+template <int W, typename T>
+hipError_t launch_stream(const I8Gemm& p, const TileStore<T>& out, hipStream_t st) {
+    auto words = [](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 4 == 0 && ld % 4 == 0; };
+    const StreamArgs args{p.a, p.lda, p.b, p.ldb, int(p.m), int(p.n), int(p.k)};
+    const auto kernel = words(p.a, p.lda) && words(p.b, p.ldb) ? &tg_i8_stream<W, true, T> : &tg_i8_stream<W, false, T>;
+    hipLaunchKernelGGL(kernel, dim3(unsigned(ceil_div(p.n, 16))), dim3(W * 64), 0, st, args, out);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t gemm_typed(const I8Gemm& p, void* ws, hipStream_t st) {
+    const TileStore<T> out{p.a_scale, p.b_scale, nullptr, static_cast<const T*>(p.bias), static_cast<T*>(p.c), p.n};
+    if (p.k == 0) return launch_join<int32_t>(nullptr, 0, p.m, p.n, out, st);
+    const GemmPlan pl = plan_gemm(p);
+    if (pl.stream) {
+        // 16 waves a workgroup while the GPU holds all of them at once (M =
+        // 13, K = 8192: N = 8192 17.2 us against 18.4 with 8; N = 28672 60
+        // against 56).
+        return p.n <= 16384 ? launch_stream<16>(p, out, st) : launch_stream<8>(p, out, st);
+    }
+    const GemmWs w = carve_gemm(p, pl, ws);
+    TileArgs t{};
+    t.a = reinterpret_cast<const char*>(pl.pack_a ? w.a : p.a);
+    t.b = reinterpret_cast<const char*>(pl.pack_b ? w.b : p.b);
+    t.lda = pl.pack_a ? pl.ld : p.lda;
+    t.ldb = pl.pack_b ? pl.ld : p.ldb;
+    t.m = int(p.m);
+    t.n = int(p.n);
+    t.steps = t.b_steps = int(ceil_div(p.k, 128));
+    // A packed row is whole; beside one that is not, it only has to reach as far.
+    t.tail = (pl.pack_a && pl.pack_b) || p.k % 128 == 0 ? 128 : int(round_up(p.k % 128, 16));
+    if (pl.pack_a) {
+        const hipError_t e = pack_bytes(p.a, p.lda, p.m, p.k, w.a, pl.ld, st);
+        if (e != hipSuccess) return e;
+    }
+    if (pl.pack_b) {
+        const hipError_t e = pack_bytes(p.b, p.ldb, p.n, p.k, w.b, pl.ld, st);
+        if (e != hipSuccess) return e;
+    }
+    return launch_tiles<Mma::I8>(t, pl.tiles, out, w.part, st);
+}
+
+// ---- gradients -----------------------------------------------------------
+//
+// Both are a product of G with the 8-bit operand q, whose rows run across the
+// sum; q is turned so that they run along it, in 16 bits, with its scales
+// multiplied in.  bf16 gradients: q * scale rounded to bf16 (as dequantizing
+// the operand to bf16 does; the result's error is that of its own rounding
+// times sqrt 2).  f16: q * scale * 2^e rounded to f16.  f32: q is exact in
+// bf16; G * scale becomes three bf16 planes that hold all its 24 bits, and the
+// sum runs over the planes.
+
+struct GradPlan {
+    bool pack_g;
+    int planes;
+    int64_t depth;  // of packed rows, in elements
+    TilePlan tiles;
+};
+
+GradPlan plan_grad(const I8Grad& p) {
+    GradPlan pl{};
+    const int64_t size = p.type == TG_FLOAT32 ? 4 : 2;
+    pl.planes = p.type == TG_FLOAT32 ? 3 : 1;
+    pl.pack_g = p.type == TG_FLOAT32 || p.transposed || !in_place(p.g, p.ldg * size, p.depth * size);
+    pl.depth = round_up(p.depth, 64);
+    pl.tiles = plan_tiles(p.rows, p.cols, pl.depth / 64 * pl.planes);
+    return pl;
+}
+
+struct GradWs {
+    void *g, *q, *part;
+    float* range;
+    size_t bytes;
+};
+
+GradWs carve_grad(const I8Grad& p, const GradPlan& pl, void* ws) {
+    Carver c{static_cast<char*>(ws)};
+    GradWs w{};
+    if (p.rows == 0 || p.cols == 0 || p.depth == 0) return w;
+    if (pl.pack_g) w.g = c.take(size_t(p.rows) * size_t(pl.depth) * size_t(pl.planes) * 2);
+    w.q = c.take(size_t(p.cols) * size_t(pl.depth) * 2);
+    if (p.type == TG_F16) w.range = static_cast<float*>(c.take(8));
+    w.part = c.take(part_bytes(pl.tiles, p.rows, p.cols));
+    w.bytes = c.used;
+    return w;
+}
+
+template <typename S, typename D, int PLANES>
+hipError_t pack_turned(const void* src, int64_t ld, int64_t rows, int64_t cols, const float* scale,
+                       const float* factor, void* dst, int64_t depth, hipStream_t st) {
+    const int64_t tiles_r = depth / 64, tiles = tiles_r * ceil_div(cols, 64);
+    if (tiles >= (int64_t(1) << 24)) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((tg_i8_pack_turned<S, D, PLANES>), dim3(unsigned(tiles)), dim3(256), 0, st,
+                       static_cast<const S*>(src), ld, rows, cols, scale, factor, static_cast<D*>(dst), depth, tiles_r);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t grad_typed(const I8Grad& p, void* ws, hipStream_t st) {
+    constexpr bool F32 = std::is_same<T, float>::value;
+    using D = std::conditional_t<std::is_same<T, f16_t>::value, f16_t, bf16_t>;
+    TileStore<T> out{nullptr, nullptr, nullptr, nullptr, static_cast<T*>(p.out), p.cols};
+    if (p.depth == 0) return launch_join<float>(nullptr, 0, p.rows, p.cols, out, st);
+    const GradPlan pl = plan_grad(p);
+    const GradWs w = carve_grad(p, pl, ws);
+    hipError_t e = hipSuccess;
+    if (p.type == TG_F16) {
+        hipLaunchKernelGGL(tg_i8_scale_range, dim3(1), dim3(1024), 0, st, p.scale, p.depth, w.range);
+        e = hipGetLastError();
+        out.all = w.range + 1;
+    }
+    if (e == hipSuccess)
+        e = pack_turned<int8_t, D, 1>(p.q, p.ldq, p.depth, p.cols, F32 ? nullptr : p.scale,
+                                      p.type == TG_F16 ? w.range : nullptr, w.q, pl.depth, st);
+    if (e == hipSuccess && pl.pack_g) {
+        if (p.transposed) {
+            e = pack_turned<T, D, F32 ? 3 : 1>(p.g, p.ldg, p.depth, p.rows, F32 ? p.scale : nullptr, nullptr, w.g,
+                                               pl.depth, st);
+        } else if constexpr (F32) {
+            hipLaunchKernelGGL(tg_i8_pack_split, dim3(stride_grid(p.rows * pl.depth / 8)), dim3(256), 0, st,
+                               static_cast<const float*>(p.g), p.ldg, p.rows, p.depth, p.scale,
+                               static_cast<bf16_t*>(w.g), pl.depth);
+            e = hipGetLastError();
+        } else {
+            e = pack_bytes(p.g, p.ldg * 2, p.rows, p.depth * 2, w.g, pl.depth * 2, st);
         }
+    }
+    if (e != hipSuccess) return e;
+    TileArgs t{};
+    t.a = static_cast<const char*>(pl.pack_g ? w.g : p.g);
+    t.b = static_cast<const char*>(w.q);
+    t.lda = pl.pack_g ? pl.depth * pl.planes * 2 : p.ldg * 2;
+    t.ldb = pl.depth * 2;
+    t.m = int(p.rows);
+    t.n = int(p.cols);
+    t.b_steps = int(pl.depth / 64);
+    t.steps = t.b_steps * pl.planes;
+    t.tail = pl.pack_g || p.depth % 64 == 0 ? 128 : int(p.depth % 64 * 2);
+    return launch_tiles<std::is_same<D, f16_t>::value ? Mma::F16 : Mma::BF16>(t, pl.tiles, out, w.part, st);
 }
 
 }  // namespace
 
-size_t i8_gemm_ws(const I8Gemm&) { return 0; }
+size_t i8_gemm_ws(const I8Gemm& p) { return carve_gemm(p, plan_gemm(p), nullptr).bytes; }
 
-hipError_t i8_gemm(const I8Gemm& p, void*, hipStream_t st) {
+hipError_t i8_gemm(const I8Gemm& p, void* ws, hipStream_t st) {
     if (p.m == 0 || p.n == 0) return hipSuccess;
-    return by_type(p.type, [&](auto tag) {
-        using T = decltype(tag);
-        const int64_t tn = ceil_div(p.n, 64);
-        hipLaunchKernelGGL((tg_i8_gemm_tiles<T>), dim3(unsigned(ceil_div(p.m, 64) * tn)), dim3(256), 0, st, p.a,
-                           p.lda, p.a_scale, p.b, p.ldb, p.b_scale, static_cast<const T*>(p.bias),
-                           static_cast<T*>(p.c), p.m, p.n, p.k, tn);
-        return hipGetLastError();
-    });
+    return by_type(p.type, [&](auto tag) { return gemm_typed<decltype(tag)>(p, ws, st); });
 }
 
-size_t i8_grad_ws(const I8Grad&) { return 0; }
+size_t i8_grad_ws(const I8Grad& p) { return carve_grad(p, plan_grad(p), nullptr).bytes; }
 
-hipError_t i8_grad(const I8Grad& p, void*, hipStream_t st) {
+hipError_t i8_grad(const I8Grad& p, void* ws, hipStream_t st) {
     if (p.rows == 0 || p.cols == 0) return hipSuccess;
-    return by_type(p.type, [&](auto tag) {
-        using T = decltype(tag);
-        const int64_t tn = ceil_div(p.cols, 64);
-        const auto kernel = p.transposed ? &tg_i8_grad_tiles<T, true> : &tg_i8_grad_tiles<T, false>;
-        hipLaunchKernelGGL(kernel, dim3(unsigned(ceil_div(p.rows, 64) * tn)), dim3(256), 0, st,
-                           static_cast<const T*>(p.g), p.ldg, p.q, p.ldq, p.scale, static_cast<T*>(p.out),
-                           p.rows, p.cols, p.depth, tn);
-        return hipGetLastError();
-    });
+    return by_type(p.type, [&](auto tag) { return grad_typed<decltype(tag)>(p, ws, st); });
 }
 
 }  // namespace tg

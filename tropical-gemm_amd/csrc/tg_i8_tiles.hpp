@@ -1,0 +1,416 @@
+// tg_i8_tiles.hpp -- C = A B^T on matrix instructions, for operands whose
+// rows run along the sum: A is M rows and B is N rows of `bytes` bytes each,
+// of 8-bit integers, bf16 or f16.  One kernel for the 8-bit product and (after
+// tg_i8_pack.hpp) for the gradients.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "tg_i8_types.hpp"
+
+namespace tg {
+
+enum class Mma { I8, BF16, F16 };
+
+// Matrix instructions of FS x FS outputs: 64 bytes of the sum for FS 16, 32
+// bytes for FS 32.
+//
+// D += X Y^T: lane l holds bytes (l / FS) * 16 ... + 15 of row l % FS of both,
+// and of D the column l % FS: rows 4 * (l / 16) + e (FS 16, e < 4), or
+// 8 * (e / 4) + 4 * (l / 32) + e % 4 (FS 32, e < 16).
+template <Mma KIND, int FS>
+struct MmaAcc {
+    typedef float type __attribute__((ext_vector_type(FS * FS / 64)));
+};
+template <int FS>
+struct MmaAcc<Mma::I8, FS> {
+    typedef int32_t type __attribute__((ext_vector_type(FS * FS / 64)));
+};
+
+template <Mma KIND, int FS>
+__device__ __forceinline__ typename MmaAcc<KIND, FS>::type mma(u32x4 x, u32x4 y, typename MmaAcc<KIND, FS>::type d) {
+    if constexpr (KIND == Mma::I8) {
+        typedef int32_t V __attribute__((ext_vector_type(4)));
+        const V a = __builtin_bit_cast(V, x), b = __builtin_bit_cast(V, y);
+        if constexpr (FS == 16) return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, d, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, d, 0, 0, 0);
+    } else if constexpr (KIND == Mma::BF16) {
+        typedef __bf16 V __attribute__((ext_vector_type(8)));
+        const V a = __builtin_bit_cast(V, x), b = __builtin_bit_cast(V, y);
+        if constexpr (FS == 16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, d, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, d, 0, 0, 0);
+    } else {
+        typedef _Float16 V __attribute__((ext_vector_type(8)));
+        const V a = __builtin_bit_cast(V, x), b = __builtin_bit_cast(V, y);
+        if constexpr (FS == 16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, d, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, d, 0, 0, 0);
+    }
+}
+
+// Bytes of LDS.
+typedef __attribute__((address_space(3))) char lds_t;
+
+// One 16-byte load per lane straight into LDS: from base + off (off differs by
+// lane) to lds + lane * 16.  base and lds are the same in all lanes.  Written
+// as an instruction so that the compiler does not wait for it before every
+// later LDS read (tile_wait() is the wait); it has no output registers, and
+// m0 has no other use here.
+__device__ __forceinline__ void tile_load(const char* base, uint32_t off, uint32_t lds) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base));
+}
+
+// At most N of this wave's loads into LDS are outstanding and every LDS read
+// of it is done; then all waves of the workgroup meet.
+template <int N>
+__device__ __forceinline__ void tile_wait() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
+}
+
+struct TileArgs {
+    const char *a, *b;  // 16-byte aligned; row strides lda, ldb in bytes: multiples of 16 below 2^23
+    int64_t lda, ldb;
+    int m, n;           // rows of A and B
+    int steps;          // 128-byte steps of the whole sum
+    int tail;           // bytes of the last step that count: a multiple of 16, 16 ... 128
+    int b_steps;        // A's step s meets B's step s % b_steps
+    int tiles_m, tiles_n;
+    int slice;          // steps of one blockIdx.y (tg_i8_tiles_slice)
+};
+
+// Tile of a workgroup: WM x WN waves, each FM x FN fragments of FS x FS.
+//
+// LDS holds a ring of NS stages of BM + BN rows of 128 bytes.  One step is two
+// halves of 64 bytes.  While the matrix unit works on one half's fragments, the
+// other half's are read from LDS into registers; the step's barrier stands
+// between the halves, where the next step's loads have landed and this step's
+// LDS is free for the loads of the step NS later.
+//
+// The 16-byte chunk c of a row lies at place c ^ key(row).  LDS serves 16
+// lanes of a 16-byte read at a time, lanes {0-3, 12-15, 20-27} and {4-11,
+// 16-19, 28-31} of each 32, and key makes those 16 meet 16 different places of
+// the 256 bytes that two rows take (no bank conflict is counted).  B's rows
+// are taken so that a lane's FN fragments hold VPF FN neighbouring columns of C
+// (whole 16-byte stores); B is the first operand, so that a fragment's values
+// of a lane are neighbours in a row of C.
+template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NS>
+struct Tile {
+    static constexpr int BM = WM * FM * FS, BN = WN * FN * FS, NT = WM * WN * 64;
+    static constexpr int KS = FS / 16;       // instructions along half a step
+    static constexpr int VPF = FS * FS / 64;  // values of a fragment per lane
+    static constexpr int LOADS_A = BM * 8 / NT, LOADS_B = BN * 8 / NT, LOADS = LOADS_A + LOADS_B;
+    static constexpr int STAGE = (BM + BN) * 128, LDS = NS * STAGE;
+    static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0 && NT % 64 == 0, "whole loads");
+    static_assert(NS >= 2 && NS <= 6, "wait_for's cases");
+    using Acc = typename MmaAcc<KIND, FS>::type;
+    using Value = std::conditional_t<KIND == Mma::I8, int32_t, float>;
+
+    static __device__ __forceinline__ int key_a(int r) { return FS == 16 ? r & 7 : r / 2 & 7; }
+    static __device__ __forceinline__ int key_b(int r) {
+        return FS == 16 ? (r & 3) | (r / (VPF * FN) & 1) << 2 : r / 2 & 7;
+    }
+
+    // The workgroup's tile: consecutive workgroups go round the 8 XCDs, so
+    // each XCD takes a contiguous run of tiles, in bands of 8 tile rows, whose
+    // panels its L2 then holds.
+    static __device__ __forceinline__ void place(const TileArgs& p, int& tm, int& tn) {
+        const int total = p.tiles_m * p.tiles_n, per = total / 8, rest = total % 8;
+        const int x = int(blockIdx.x) % 8;
+        int id = x * per + (x < rest ? x : rest) + int(blockIdx.x) / 8;
+        const int band = id / (8 * p.tiles_n);
+        const int height = p.tiles_m - band * 8 < 8 ? p.tiles_m - band * 8 : 8;
+        id -= band * 8 * p.tiles_n;
+        tm = band * 8 + id % height;
+        tn = id / height;
+    }
+
+    // Sums steps [s0, s1), at least one, of tile (tm, tn) into acc.
+    static __device__ __forceinline__ void run(const TileArgs& p, int tm, int tn, int s0, int s1, lds_t* lds,
+                                               Acc (&acc)[FM][FN]) {
+        const int t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64);
+        const uint32_t lds0 = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>(lds))) + wave * 1024;
+        const char* a0 = p.a + int64_t(tm) * BM * p.lda;
+        const char* b0 = p.b + int64_t(tn) * BN * p.ldb;
+        const bool cut = s1 == p.steps && p.tail < 128;  // the last step is a partial one
+
+        // Thread t loads place t % 8 of rows t / 8, t / 8 + NT / 8, ...; rows
+        // past the matrix repeat its last one (their outputs are not stored),
+        // chunks past a partial last step repeat the last that counts (A's
+        // are cleared in registers before they are used).
+        uint32_t off_a[LOADS_A], off_b[LOADS_B];
+        auto chunk_a = [&](int i) { return (t % 8) ^ key_a(t / 8 + i * (NT / 8)); };
+        auto chunk_b = [&](int i) { return (t % 8) ^ key_b(t / 8 + i * (NT / 8)); };
+#pragma unroll
+        for (int i = 0; i < LOADS_A; ++i) {
+            const int r = t / 8 + i * (NT / 8), last = p.m - 1 - tm * BM;
+            off_a[i] = uint32_t(r < last ? r : last) * uint32_t(p.lda) + chunk_a(i) * 16;
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS_B; ++i) {
+            const int r = t / 8 + i * (NT / 8), last = p.n - 1 - tn * BN;
+            off_b[i] = uint32_t(r < last ? r : last) * uint32_t(p.ldb) + chunk_b(i) * 16;
+        }
+        // Loads of the step that comes next, `count` of them from load `first`
+        // on; `over` is at most a chunk's own offset in its row, so off - over
+        // stays inside the row.
+        int next = s0, next_b = s0 % p.b_steps;
+        uint32_t next_lds = lds0;
+        auto load = [&](int first, int count) {
+            const bool partial = cut && next == s1 - 1;
+            const char *pa = a0 + int64_t(next) * 128, *pb = b0 + int64_t(next_b) * 128;
+#pragma unroll
+            for (int i = first; i < first + count; ++i) {
+                const int past = (i < LOADS_A ? chunk_a(i) : chunk_b(i - LOADS_A)) * 16 + 16 - p.tail;
+                const uint32_t over = partial && past > 0 ? uint32_t(past) : 0;
+                if (i < LOADS_A) tile_load(pa, off_a[i] - over, next_lds + i * (NT * 16));
+                else tile_load(pb, off_b[i - LOADS_A] - over, next_lds + i * (NT * 16));
+            }
+        };
+        auto loaded = [&] {
+            ++next;
+            next_b = next_b + 1 == p.b_steps ? 0 : next_b + 1;
+            next_lds = next_lds == lds0 + (NS - 1) * STAGE ? lds0 : next_lds + STAGE;
+        };
+        // Waits until all but the newest `steps` steps' loads have landed.
+        auto wait_for = [&](int steps) {
+            if (NS > 5 && steps >= 4) tile_wait<(NS > 5 ? 4 : 0) * LOADS>();
+            else if (NS > 4 && steps >= 3) tile_wait<(NS > 4 ? 3 : 0) * LOADS>();
+            else if (NS > 3 && steps >= 2) tile_wait<(NS > 3 ? 2 : 0) * LOADS>();
+            else if (NS > 2 && steps >= 1) tile_wait<(NS > 2 ? 1 : 0) * LOADS>();
+            else tile_wait<0>();
+        };
+
+        const int wm = wave / WN, wn = wave % WN, li = lane % FS, lg = lane / FS;
+        const int group = FS == 16 ? li / 4 : li / 4 % 2, value = FS == 16 ? li % 4 : li / 8 * 4 + li % 4;
+        const int row_a = wm * FM * FS + li, row_b = wn * FN * FS + group * (VPF * FN) + value;
+        // Fragment j's row, row_b + VPF j, has row_b's key, as fragment i's of
+        // A, row_a + FS i, has row_a's.
+        const int at_a = row_a * 128 + ((lg ^ key_a(row_a)) << 4);
+        const int at_b = BM * 128 + row_b * 128 + ((lg ^ key_b(row_b)) << 4);
+        typedef const __attribute__((address_space(3))) u32x4* frag_t;
+        u32x4 xa[2][FM][KS], xb[2][FN][KS];
+        // Part i of FM of a half's fragments.
+        auto read_part = [&](int i, int half, int at) {
+            const lds_t* from = lds + at;
+#pragma unroll
+            for (int u = 0; u < KS; ++u)
+                xa[half][i][u] = *reinterpret_cast<frag_t>(from + (at_a ^ (half * 64 + u * 32)) + i * FS * 128);
+#pragma unroll
+            for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j)
+#pragma unroll
+                for (int u = 0; u < KS; ++u)
+                    xb[half][j][u] = *reinterpret_cast<frag_t>(from + (at_b ^ (half * 64 + u * 32)) + j * VPF * 128);
+        };
+        // Multiplies the fragments of half h, row by row.  Behind each row's
+        // products come its parts of a later step's loads (spread over all
+        // rows: 393 us against 419 for 8192^3 in 8 bits with all of them
+        // behind the first half of the rows) and of the next half's reads
+        // (done one row before the end, so that they are there in time).
+        auto products = [&](int h, auto reads, auto loads, int at) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+#pragma unroll
+                for (int u = 0; u < KS; ++u)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = mma<KIND, FS>(xb[h][j][u], xa[h][i][u], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (decltype(loads)::value) {
+                    load(i * LOADS / FM, (i + 1) * LOADS / FM - i * LOADS / FM);
+                }
+                if constexpr (decltype(reads)::value) {
+                    if (i == 0) read_part(0, h ^ 1, at);
+                    if (i + 1 < FM) read_part(i + 1, h ^ 1, at);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // Clears the chunks of A's fragments that lie past the sum's end.
+        auto clear = [&](int h) {
+#pragma unroll
+            for (int u = 0; u < KS; ++u)
+                if ((lg + 2 * u + 4 * h) * 16 >= p.tail) {
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) xa[h][i][u] = u32x4{0, 0, 0, 0};
+                }
+        };
+        const std::true_type yes;
+        const std::false_type no;
+
+        for (int s = s0; s < s1 && s < s0 + NS; ++s) {
+            load(0, LOADS);
+            loaded();
+        }
+        if (s1 - s0 >= NS) tile_wait<(NS - 1) * LOADS>();
+        else tile_wait<0>();
+#pragma unroll
+        for (int i = 0; i < FM; ++i) read_part(i, 0, 0);
+        int s = s0, at = 0, then = STAGE;  // places of this step's and the next one's stage
+        auto step_done = [&] {
+            at = then;
+            then = then == (NS - 1) * STAGE ? 0 : then + STAGE;
+        };
+        for (; s < s1 - NS; ++s) {
+            products(0, yes, no, at);
+            tile_wait<(NS - 2) * LOADS>();
+            products(1, yes, yes, then);
+            loaded();
+            step_done();
+        }
+        for (; s < s1 - 1; ++s) {  // nothing is left to load
+            products(0, yes, no, at);
+            wait_for(s1 - 2 - s);
+            products(1, yes, no, then);
+            step_done();
+        }
+        if (cut) clear(0);
+        products(0, yes, no, at);
+        if (cut) clear(1);
+        products(1, no, no, 0);
+    }
+
+    // Hands the lane's outputs to `out` in groups of eight neighbours in a row.
+    // Its scales are loaded together first: a load before each group's store
+    // would cost its latency FM times over (2.7 us a tile more at 256 x 256).
+    template <typename Out>
+    static __device__ __forceinline__ void outputs(const TileArgs& p, int tm, int tn, const Acc (&acc)[FM][FN],
+                                                   const Out& out) {
+        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, li = lane % FS, lg = lane / FS;
+        const int m0 = tm * BM + wave / WN * FM * FS + li, n0 = tn * BN + wave % WN * FN * FS + lg * VPF * FN;
+        constexpr int GROUPS = FN * VPF / 8;
+        static_assert(FN * VPF % 8 == 0, "groups of eight");
+        typename Out::Row rows[FM];
+        typename Out::Cols cols[GROUPS];
+        auto each = [&](auto inside) {
+            constexpr bool IN = decltype(inside)::value;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+                if (IN || m0 + i * FS < p.m) rows[i] = out.row(m0 + i * FS);
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g)
+                if (IN || n0 + g * 8 < p.n) cols[g] = out.cols(n0 + g * 8, IN ? 8 : p.n - n0 - g * 8);
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                if (!IN && m0 + i * FS >= p.m) continue;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    if (!IN && n0 + g * 8 >= p.n) continue;
+                    Value v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = acc[i][(g * 8 + e) / VPF][(g * 8 + e) % VPF];
+                    out.store(m0 + i * FS, n0 + g * 8, IN ? 8 : p.n - n0 - g * 8, v, rows[i], cols[g]);
+                }
+            }
+        };
+        if ((tm + 1) * BM <= p.m && (tn + 1) * BN <= p.n) each(std::true_type());
+        else each(std::false_type());
+    }
+};
+
+// C = sum * a_scale[m] * b_scale[n] + bias[n], rounded to T; a_scale, b_scale
+// and bias may be null, `all` is one more factor where it is not.
+template <typename T>
+struct TileStore {
+    const float *a_scale, *b_scale, *all;
+    const T* bias;
+    T* c;
+    int64_t n;
+
+    struct Row {
+        float scale;
+    };
+    struct Cols {
+        float scale[8], bias[8];
+    };
+    __device__ __forceinline__ Row row(int m) const { return {a_scale != nullptr ? a_scale[m] : 1.0f}; }
+    __device__ __forceinline__ Cols cols(int col, int left) const {
+        Cols c;
+        const float f = all != nullptr ? *all : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c.scale[i] = f, c.bias[i] = 0.0f;
+        if (b_scale != nullptr) load_upto8(b_scale + col, left, c.scale);
+        if (bias != nullptr) load_upto8(bias + col, left, c.bias);
+        return c;
+    }
+    template <typename V>
+    __device__ __forceinline__ void store(int m, int col, int left, const V (&x)[8], const Row& r,
+                                          const Cols& c8) const {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = float(x[i]) * r.scale * c8.scale[i];
+        if (bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += c8.bias[i];
+        }
+        store_upto8(c + int64_t(m) * n + col, left, v);
+    }
+};
+
+// Sums of a slice as they are, in rows of `ld` (a multiple of 8) 32-bit values.
+template <typename V>
+struct TilePartial {
+    V* c;
+    int64_t ld;
+    struct Row {};
+    struct Cols {};
+    __device__ __forceinline__ Row row(int) const { return {}; }
+    __device__ __forceinline__ Cols cols(int, int) const { return {}; }
+    __device__ __forceinline__ void store(int m, int col, int, const V (&x)[8], const Row&, const Cols&) const {
+        typedef V V4 __attribute__((ext_vector_type(4)));
+        V4* to = reinterpret_cast<V4*>(c + int64_t(m) * ld + col);
+        to[0] = V4{x[0], x[1], x[2], x[3]};
+        to[1] = V4{x[4], x[5], x[6], x[7]};
+    }
+};
+
+template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NS, int PER_CU, typename T>
+__global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_i8_tiles(TileArgs p, TileStore<T> out) {
+    using Cfg = Tile<KIND, FS, WM, WN, FM, FN, NS>;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typename Cfg::Acc acc[FM][FN] = {};
+    int tm, tn;
+    Cfg::place(p, tm, tn);
+    Cfg::run(p, tm, tn, 0, p.steps, (lds_t*)(smem), acc);
+    Cfg::outputs(p, tm, tn, acc, out);
+}
+
+// Slice blockIdx.y of the sum: its sums to part + blockIdx.y * M * ld.
+template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NS, int PER_CU>
+__global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_i8_tiles_slice(
+    TileArgs p, TilePartial<typename Tile<KIND, FS, WM, WN, FM, FN, NS>::Value> out) {
+    using Cfg = Tile<KIND, FS, WM, WN, FM, FN, NS>;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typename Cfg::Acc acc[FM][FN] = {};
+    int tm, tn;
+    Cfg::place(p, tm, tn);
+    const int s0 = int(blockIdx.y) * p.slice, s1 = s0 + p.slice < p.steps ? s0 + p.slice : p.steps;
+    Cfg::run(p, tm, tn, s0, s1, (lds_t*)(smem), acc);
+    out.c += int64_t(blockIdx.y) * p.m * out.ld;
+    Cfg::outputs(p, tm, tn, acc, out);
+}
+
+// C from the slices' sums, added in their order (none: an empty sum).
+template <typename V, typename T>
+__global__ __launch_bounds__(256) void tg_i8_tiles_join(const V* __restrict__ part, int64_t ld, int slices, int64_t m,
+                                                        int64_t n, TileStore<T> out) {
+    typedef V V4 __attribute__((ext_vector_type(4)));
+    const int64_t groups = ld / 8, total = m * groups;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+        const int64_t row = i / groups, col = (i - row * groups) * 8;
+        const V4* from = reinterpret_cast<const V4*>(part + row * ld + col);
+        V4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+        for (int s = 0; s < slices; ++s, from += m * ld / 4) {
+            a += from[0];
+            b += from[1];
+        }
+        const V v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        const int left = int(n - col < 8 ? n - col : 8);
+        out.store(int(row), int(col), left, v, out.row(int(row)), out.cols(int(col), left));
+    }
+}
+
+}  // namespace tg
