@@ -104,6 +104,16 @@ unsigned stride_grid(int64_t items) {
     return unsigned(blocks < 65536 ? blocks : 65536);
 }
 
+// Both jobs in one launch: what the second one's own launch would cost (2.5 us)
+// is more than most small operands take.
+template <typename A, typename B>
+hipError_t launch_pack(const A& a, const B& b, hipStream_t st) {
+    const int64_t na = a.blocks(), nb = b.blocks();
+    if (na + nb >= int64_t(1) << 24) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((tg_i8_pack<A, B>), dim3(unsigned(na + nb)), dim3(256), 0, st, a, b, int(na), int(nb));
+    return hipGetLastError();
+}
+
 template <typename V, typename T>
 hipError_t launch_join(const V* part, int slices, int64_t m, int64_t n, const TileStore<T>& out, hipStream_t st) {
     const int64_t ld = round_up(n, 8);
@@ -203,11 +213,8 @@ GemmWs carve_gemm(const I8Gemm& p, const GemmPlan& pl, void* ws) {
     return w;
 }
 
-hipError_t pack_bytes(const void* src, int64_t ld_src, int64_t rows, int64_t bytes, void* dst, int64_t ld,
-                      hipStream_t st) {
-    hipLaunchKernelGGL(tg_i8_pack_bytes, dim3(stride_grid(rows * ld / 16)), dim3(256), 0, st,
-                       static_cast<const int8_t*>(src), ld_src, rows, int(bytes), static_cast<int8_t*>(dst), ld);
-    return hipGetLastError();
+PackBytes bytes_job(const void* src, int64_t ld_src, int64_t rows, int64_t bytes, void* dst, int64_t ld) {
+    return {static_cast<const int8_t*>(src), ld_src, rows, int(bytes), static_cast<int8_t*>(dst), ld};
 }
 
 template <int W, typename T>
@@ -241,12 +248,10 @@ hipError_t gemm_typed(const I8Gemm& p, void* ws, hipStream_t st) {
     t.steps = t.b_steps = int(ceil_div(p.k, 128));
     // A packed row is whole; beside one that is not, it only has to reach as far.
     t.tail = (pl.pack_a && pl.pack_b) || p.k % 128 == 0 ? 128 : int(round_up(p.k % 128, 16));
-    if (pl.pack_a) {
-        const hipError_t e = pack_bytes(p.a, p.lda, p.m, p.k, w.a, pl.ld, st);
-        if (e != hipSuccess) return e;
-    }
-    if (pl.pack_b) {
-        const hipError_t e = pack_bytes(p.b, p.ldb, p.n, p.k, w.b, pl.ld, st);
+    if (pl.pack_a || pl.pack_b) {
+        const PackBytes a = bytes_job(p.a, p.lda, pl.pack_a ? p.m : 0, p.k, w.a, pl.ld);
+        const PackBytes b = bytes_job(p.b, p.ldb, pl.pack_b ? p.n : 0, p.k, w.b, pl.ld);
+        const hipError_t e = launch_pack(a, b, st);
         if (e != hipSuccess) return e;
     }
     return launch_tiles<Mma::I8>(t, pl.tiles, out, w.part, st);
@@ -297,16 +302,6 @@ GradWs carve_grad(const I8Grad& p, const GradPlan& pl, void* ws) {
     return w;
 }
 
-template <typename S, typename D, int PLANES>
-hipError_t pack_turned(const void* src, int64_t ld, int64_t rows, int64_t cols, const float* scale,
-                       const float* factor, void* dst, int64_t depth, hipStream_t st) {
-    const int64_t tiles_r = depth / 64, tiles = tiles_r * ceil_div(cols, 64);
-    if (tiles >= (int64_t(1) << 24)) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((tg_i8_pack_turned<S, D, PLANES>), dim3(unsigned(tiles)), dim3(256), 0, st,
-                       static_cast<const S*>(src), ld, rows, cols, scale, factor, static_cast<D*>(dst), depth, tiles_r);
-    return hipGetLastError();
-}
-
 template <typename T>
 hipError_t grad_typed(const I8Grad& p, void* ws, hipStream_t st) {
     constexpr bool F32 = std::is_same<T, float>::value;
@@ -321,21 +316,23 @@ hipError_t grad_typed(const I8Grad& p, void* ws, hipStream_t st) {
         e = hipGetLastError();
         out.all = w.range + 1;
     }
-    if (e == hipSuccess)
-        e = pack_turned<int8_t, D, 1>(p.q, p.ldq, p.depth, p.cols, F32 ? nullptr : p.scale,
-                                      p.type == TG_F16 ? w.range : nullptr, w.q, pl.depth, st);
-    if (e == hipSuccess && pl.pack_g) {
-        if (p.transposed) {
-            e = pack_turned<T, D, F32 ? 3 : 1>(p.g, p.ldg, p.depth, p.rows, F32 ? p.scale : nullptr, nullptr, w.g,
-                                               pl.depth, st);
-        } else if constexpr (F32) {
-            hipLaunchKernelGGL(tg_i8_pack_split, dim3(stride_grid(p.rows * pl.depth / 8)), dim3(256), 0, st,
-                               static_cast<const float*>(p.g), p.ldg, p.rows, p.depth, p.scale,
-                               static_cast<bf16_t*>(w.g), pl.depth);
-            e = hipGetLastError();
-        } else {
-            e = pack_bytes(p.g, p.ldg * 2, p.rows, p.depth * 2, w.g, pl.depth * 2, st);
-        }
+    if (e != hipSuccess) return e;
+    const PackTurned<int8_t, D, 1> q{p.q, p.ldq, p.depth, p.cols, F32 ? nullptr : p.scale,
+                                     p.type == TG_F16 ? w.range : nullptr, static_cast<D*>(w.q), pl.depth};
+    if (!pl.pack_g) {
+        e = launch_pack(q, PackNothing(), st);
+    } else if (p.transposed) {
+        e = launch_pack(q,
+                        PackTurned<T, D, F32 ? 3 : 1>{static_cast<const T*>(p.g), p.ldg, p.depth, p.rows,
+                                                      F32 ? p.scale : nullptr, nullptr, static_cast<D*>(w.g), pl.depth},
+                        st);
+    } else if constexpr (F32) {
+        e = launch_pack(q,
+                        PackSplit{static_cast<const float*>(p.g), p.ldg, p.rows, p.depth, p.scale,
+                                  static_cast<bf16_t*>(w.g), pl.depth},
+                        st);
+    } else {
+        e = launch_pack(q, bytes_job(p.g, p.ldg * 2, p.rows, p.depth * 2, w.g, pl.depth * 2), st);
     }
     if (e != hipSuccess) return e;
     TileArgs t{};

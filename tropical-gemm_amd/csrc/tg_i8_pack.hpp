@@ -10,39 +10,67 @@
 
 namespace tg {
 
+inline int64_t pack_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// A job is run by `count` workgroups of 256 threads, each with its number.
+
+struct PackNothing {
+    static constexpr int kLdsWords = 1;
+    int64_t blocks() const { return 0; }
+    __device__ __forceinline__ void run(int, int, uint32_t*) const {}
+};
+
 // Rows of `bytes` bytes at any address to rows of `ld` bytes (a multiple of
 // 128): 16 bytes a thread.
-__global__ __launch_bounds__(256) void tg_i8_pack_bytes(const int8_t* __restrict__ src, int64_t ld_src, int64_t rows,
-                                                        int bytes, int8_t* __restrict__ dst, int64_t ld) {
-    const int64_t chunks = ld / 16, total = rows * chunks;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-        const int64_t row = i / chunks, c = i - row * chunks;
-        *reinterpret_cast<u32x4*>(dst + row * ld + c * 16) = stream_tail(src + row * ld_src, int(c) * 16, bytes);
+struct PackBytes {
+    static constexpr int kLdsWords = 1;
+    const int8_t* src;
+    int64_t ld_src, rows;
+    int bytes;
+    int8_t* dst;
+    int64_t ld;
+    int64_t blocks() const {
+        const int64_t n = pack_ceil(rows * (ld / 16), 256);
+        return n < 65536 ? n : 65536;
     }
+    __device__ __forceinline__ void run(int block, int count, uint32_t*) const {
+        const int64_t chunks = ld / 16, total = rows * chunks;
+        for (int64_t i = int64_t(block) * 256 + threadIdx.x; i < total; i += int64_t(count) * 256) {
+            const int64_t row = i / chunks, c = i - row * chunks;
+            *reinterpret_cast<u32x4*>(dst + row * ld + c * 16) = stream_tail(src + row * ld_src, int(c) * 16, bytes);
+        }
+    }
+};
+
+// |s|, or 0 where it is not finite.
+__device__ __forceinline__ float finite_size(float s) {
+    s = fabsf(s);
+    return s < __builtin_huge_valf() ? s : 0.0f;
 }
 
-// The factor 2^e that puts the largest finite scale into [64, 128), and its
-// inverse, for products q * scale * 2^e in f16: at most 127 * 128, and with
-// all of f16's bits down to 2^-21 of the largest scale.
+// e such that top * 2^e lies in [64, 128) (0 for top 0; |e| at most 120), for
+// products q * scale * 2^e in f16 with top the largest scale: at most 127 *
+// 128, and with all of f16's bits down to 2^-21 of the largest scale.
+__device__ __forceinline__ int range_exponent(float top) {
+    if (!(top > 0.0f)) return 0;
+    int e = 0;
+    (void)frexpf(top, &e);  // top in [2^(e-1), 2^e)
+    e = 7 - e;
+    return e > 120 ? 120 : e < -120 ? -120 : e;
+}
+
+// 2^e for all the scales, and its inverse.
 __global__ __launch_bounds__(1024) void tg_i8_scale_range(const float* __restrict__ scale, int64_t n,
                                                           float* __restrict__ out) {
     __shared__ float part[16];
     float top = 0.0f;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) {
-        const float s = fabsf(scale[i]);
-        if (s < __builtin_huge_valf()) top = fmaxf(top, s);
-    }
+    for (int64_t i = threadIdx.x; i < n; i += 1024) top = fmaxf(top, finite_size(scale[i]));
     top = wave_max(top);
     if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = top;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 1; i < 16; ++i) top = fmaxf(top, part[i]);
-        int e = 0;
-        if (top > 0.0f) {
-            (void)frexpf(top, &e);  // top in [2^(e-1), 2^e)
-            e = 7 - e;
-            e = e > 120 ? 120 : e < -120 ? -120 : e;
-        }
+        const int e = range_exponent(top);
         out[0] = ldexpf(1.0f, e);
         out[1] = ldexpf(1.0f, -e);
     }
@@ -65,82 +93,108 @@ __device__ __forceinline__ void split_value(float v, D (&d)[PLANES]) {
 // factor may be null), rows of dst of PLANES planes of `depth` (a multiple of
 // 64, at least rows) elements, zeros from r = rows on.  A workgroup takes 64
 // rows by 64 columns through LDS: pairs of rows are written there as words of
-// two, 33 words a column, so that a wave's 8 x 8 words meet 64 banks.
+// two, 33 words a column, so that a wave's 8 x 8 words meet 64 banks.  Bound by
+// memory (8192 x 4096 from 8 to 16 bits: 100 MB in 24 us).
 template <typename S, typename D, int PLANES>
-__global__ __launch_bounds__(256) void tg_i8_pack_turned(const S* __restrict__ src, int64_t ld_src, int64_t rows,
-                                                         int64_t cols, const float* __restrict__ scale,
-                                                         const float* __restrict__ factor, D* __restrict__ dst,
-                                                         int64_t depth, int64_t tiles_r) {
+struct PackTurned {
     static_assert(sizeof(D) == 2, "pairs are words");
-    __shared__ uint32_t tile[PLANES][64][33];
-    const int t = threadIdx.x;
-    const int64_t r0 = int64_t(blockIdx.x) % tiles_r * 64, c0 = int64_t(blockIdx.x) / tiles_r * 64;
-    {
-        const int cg = t % 8, rp = t / 8;
-        const int64_t c = c0 + cg * 8;
-        const int left = cols - c < 8 ? int(cols - c) : 8;
-        float v[2][8] = {};
+    const S* src;
+    int64_t ld_src, rows, cols;
+    const float *scale, *factor;
+    D* dst;
+    int64_t depth;
+    static constexpr int kLdsWords = PLANES * 64 * 33;
+    int64_t blocks() const { return depth / 64 * pack_ceil(cols, 64); }
+    __device__ __forceinline__ void run(int block, int, uint32_t* lds) const {
+        uint32_t(*tile)[64][33] = reinterpret_cast<uint32_t(*)[64][33]>(lds);
+        const int t = threadIdx.x, tiles_r = int(depth / 64);
+        const int64_t r0 = int64_t(block % tiles_r) * 64, c0 = int64_t(block / tiles_r) * 64;
+        {
+            const int cg = t % 8, rp = t / 8;
+            const int64_t c = c0 + cg * 8;
+            const int left = cols - c < 8 ? int(cols - c) : 8;
+            float v[2][8] = {};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t r = r0 + rp * 2 + h;
-            if (r >= rows || left <= 0) continue;
-            if constexpr (sizeof(S) == 1) load_i8_upto8(src + r * ld_src + c, left, v[h]);
-            else load_upto8(src + r * ld_src + c, left, v[h]);
-            if (scale != nullptr) {
-                const float s = factor != nullptr ? scale[r] * factor[0] : scale[r];
+            for (int h = 0; h < 2; ++h) {
+                const int64_t r = r0 + rp * 2 + h;
+                if (r >= rows || left <= 0) continue;
+                if constexpr (sizeof(S) == 1) load_i8_upto8(src + r * ld_src + c, left, v[h]);
+                else load_upto8(src + r * ld_src + c, left, v[h]);
+                if (scale != nullptr) {
+                    const float s = factor != nullptr ? scale[r] * factor[0] : scale[r];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[h][i] *= s;
+                    for (int i = 0; i < 8; ++i) v[h][i] *= s;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                D lo[PLANES], hi[PLANES];
+                split_value<D, PLANES>(v[0][i], lo);
+                split_value<D, PLANES>(v[1][i], hi);
+#pragma unroll
+                for (int p = 0; p < PLANES; ++p)
+                    tile[p][cg * 8 + i][rp] = uint32_t(__builtin_bit_cast(uint16_t, lo[p])) |
+                                              uint32_t(__builtin_bit_cast(uint16_t, hi[p])) << 16;
             }
         }
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            D lo[PLANES], hi[PLANES];
-            split_value<D, PLANES>(v[0][i], lo);
-            split_value<D, PLANES>(v[1][i], hi);
+        for (int p = 0; p < PLANES; ++p)
 #pragma unroll
-            for (int p = 0; p < PLANES; ++p)
-                tile[p][cg * 8 + i][rp] = uint32_t(__builtin_bit_cast(uint16_t, lo[p])) |
-                                          uint32_t(__builtin_bit_cast(uint16_t, hi[p])) << 16;
-        }
+            for (int pass = 0; pass < 2; ++pass) {
+                const int c = pass * 32 + t / 8, w = t % 8 * 4;
+                if (c0 + c >= cols) continue;
+                const u32x4 v = {tile[p][c][w], tile[p][c][w + 1], tile[p][c][w + 2], tile[p][c][w + 3]};
+                *reinterpret_cast<u32x4*>(dst + ((c0 + c) * PLANES + p) * depth + r0 + w * 2) = v;
+            }
     }
-    __syncthreads();
-#pragma unroll
-    for (int p = 0; p < PLANES; ++p)
-#pragma unroll
-        for (int pass = 0; pass < 2; ++pass) {
-            const int c = pass * 32 + t / 8, w = t % 8 * 4;
-            if (c0 + c >= cols) continue;
-            const u32x4 v = {tile[p][c][w], tile[p][c][w + 1], tile[p][c][w + 2], tile[p][c][w + 3]};
-            *reinterpret_cast<u32x4*>(dst + ((c0 + c) * PLANES + p) * depth + r0 + w * 2) = v;
-        }
-}
+};
 
 // f32 rows as three bf16 planes each: dst[i][p][r] from src[i][r] * scale[r].
-__global__ __launch_bounds__(256) void tg_i8_pack_split(const float* __restrict__ src, int64_t ld_src, int64_t rows,
-                                                        int64_t cols, const float* __restrict__ scale,
-                                                        bf16_t* __restrict__ dst, int64_t depth) {
-    const int64_t groups = depth / 8, total = rows * groups;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
-        const int64_t row = i / groups, at = (i - row * groups) * 8;
-        const int left = cols - at < 8 ? int(cols - at) : 8;
-        float v[8] = {}, s[8] = {};
-        if (left > 0) {
-            load_upto8(src + row * ld_src + at, left, v);
-            load_upto8(scale + at, left, s);
-        }
-        bf16_t d[8][3];
+struct PackSplit {
+    static constexpr int kLdsWords = 1;
+    const float* src;
+    int64_t ld_src, rows, cols;
+    const float* scale;
+    bf16_t* dst;
+    int64_t depth;
+    int64_t blocks() const {
+        const int64_t n = pack_ceil(rows * (depth / 8), 256);
+        return n < 65536 ? n : 65536;
+    }
+    __device__ __forceinline__ void run(int block, int count, uint32_t*) const {
+        const int64_t groups = depth / 8, total = rows * groups;
+        for (int64_t i = int64_t(block) * 256 + threadIdx.x; i < total; i += int64_t(count) * 256) {
+            const int64_t row = i / groups, at = (i - row * groups) * 8;
+            const int left = cols - at < 8 ? int(cols - at) : 8;
+            float v[8] = {}, s[8] = {};
+            if (left > 0) {
+                load_upto8(src + row * ld_src + at, left, v);
+                load_upto8(scale + at, left, s);
+            }
+            bf16_t d[8][3];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) split_value<bf16_t, 3>(v[e] * s[e], d[e]);
+            for (int e = 0; e < 8; ++e) split_value<bf16_t, 3>(v[e] * s[e], d[e]);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
-            u32x4 w;
+            for (int p = 0; p < 3; ++p) {
+                u32x4 w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                w[e] = uint32_t(__builtin_bit_cast(uint16_t, d[2 * e][p])) |
-                       uint32_t(__builtin_bit_cast(uint16_t, d[2 * e + 1][p])) << 16;
-            *reinterpret_cast<u32x4*>(dst + (row * 3 + p) * depth + at) = w;
+                for (int e = 0; e < 4; ++e)
+                    w[e] = uint32_t(__builtin_bit_cast(uint16_t, d[2 * e][p])) |
+                           uint32_t(__builtin_bit_cast(uint16_t, d[2 * e + 1][p])) << 16;
+                *reinterpret_cast<u32x4*>(dst + (row * 3 + p) * depth + at) = w;
+            }
         }
     }
+};
+
+// Job a on the first `na` workgroups, job b on the `nb` behind them.
+template <typename A, typename B>
+__global__ __launch_bounds__(256) void tg_i8_pack(A a, B b, int na, int nb) {
+    constexpr int WA = A::kLdsWords, WB = B::kLdsWords;
+    __shared__ uint32_t lds[WA > WB ? WA : WB];
+    if (int(blockIdx.x) < na) a.run(int(blockIdx.x), na, lds);
+    else b.run(int(blockIdx.x) - na, nb, lds);
 }
 
 }  // namespace tg

@@ -28,11 +28,12 @@ from .ops import _ptr, _stream
 
 _FLOAT = {torch.float32: nat.FLOAT["f32"], torch.bfloat16: nat.FLOAT["bf16"],
           torch.float16: nat.FLOAT["f16"]}
+_F32 = (torch.float32,)
 
 
 def _rows(name: str, t: torch.Tensor, dtype=None) -> int:
     """Checks a matrix on the GPU whose rows are neighbours; its row stride."""
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError("tropical_gemm GPU entry points need device tensors "
                          f"({name} is on {t.device.type}); move the tensors to the GPU first")
     if t.dim() != 2:
@@ -42,9 +43,11 @@ def _rows(name: str, t: torch.Tensor, dtype=None) -> int:
             raise ValueError(f"Unsupported dtype {t.dtype} of {name}: expected bfloat16, float16 or float32")
     elif t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.is_contiguous():
+        return t.shape[1]
     rows, cols = t.shape
     ld, step = t.stride()
-    if rows <= 1 or cols == 0:
+    if rows <= 1:
         ld = cols
     if (cols > 1 and step != 1) or ld < cols:
         raise ValueError(f"The elements of a row of {name} must be neighbours and its rows apart, got strides "
@@ -57,18 +60,15 @@ def _vector(name: str, t: torch.Tensor, n: int, dtypes) -> None:
         raise ValueError(f"Dimension mismatch: {name} has shape {tuple(t.shape)}, expected ({n},)")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if n > 1 and t.stride(0) != 1:
+    if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous (call .contiguous() on PyTorch tensors)")
 
 
-def _same_device(*named) -> torch.device:
-    """The device of the first of (name, tensor) pairs, which all others that
-    are not None must share."""
-    first, dev = named[0][0], named[0][1].device
-    for name, t in named[1:]:
+def _same_device(dev: torch.device, first: str, **others) -> None:
+    """All tensors that are not None are on `dev`, where `first` is."""
+    for name, t in others.items():
         if t is not None and t.device != dev:
             raise ValueError(f"Tensors must be on the same device: {first} is on {dev}, {name} is on {t.device}")
-    return dev
 
 
 def _same_shape(name: str, t: torch.Tensor, shape) -> None:
@@ -99,8 +99,9 @@ def dequantize(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.
     """``q * scale[:, None]`` rounded to ``dtype``."""
     ld = _rows("q", q, torch.int8)
     rows, cols = q.shape
-    _vector("scale", scale, rows, (torch.float32,))
-    dev = _same_device(("q", q), ("scale", scale))
+    _vector("scale", scale, rows, _F32)
+    dev = q.device
+    _same_device(dev, "q", scale=scale)
     _float_type(dtype)
     y = torch.empty((rows, cols), dtype=dtype, device=dev)
     nat.check(nat.load().tg_i8_dequantize(dev.index or 0, _FLOAT[dtype], q.data_ptr(), ld, scale.data_ptr(),
@@ -121,7 +122,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     ldx = _rows("x", x)
     rows, cols = x.shape
     _vector("weight", weight, cols, (x.dtype, torch.float32))
-    dev = _same_device(("x", x), ("weight", weight), ("residual", residual))
+    dev = x.device
+    _same_device(dev, "x", weight=weight, residual=residual)
     ldr, h = 0, x
     if residual is not None:
         ldr = _rows("residual", residual, x.dtype)
@@ -148,7 +150,8 @@ def rms_norm_backward(grad_y: torch.Tensor, h: torch.Tensor, weight: torch.Tenso
     _same_shape("grad_y", grad_y, h.shape)
     ldg = _rows("grad_y", grad_y, h.dtype)
     _vector("weight", weight, cols, (h.dtype, torch.float32))
-    dev = _same_device(("h", h), ("grad_y", grad_y), ("weight", weight), ("grad_h", grad_h))
+    dev = h.device
+    _same_device(dev, "h", grad_y=grad_y, weight=weight, grad_h=grad_h)
     ldgh = 0
     if grad_h is not None:
         _same_shape("grad_h", grad_h, h.shape)
@@ -177,12 +180,13 @@ def matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: tor
     n, k2 = b.shape
     if k != k2:
         raise ValueError(f"Dimension mismatch: a is {m}x{k}, b is {n}x{k2}")
-    _vector("a_scale", a_scale, m, (torch.float32,))
-    _vector("b_scale", b_scale, n, (torch.float32,))
+    _vector("a_scale", a_scale, m, _F32)
+    _vector("b_scale", b_scale, n, _F32)
     kind = _float_type(dtype)
     if bias is not None:
         _vector("bias", bias, n, (dtype,))
-    dev = _same_device(("a", a), ("b", b), ("a_scale", a_scale), ("b_scale", b_scale), ("bias", bias))
+    dev = a.device
+    _same_device(dev, "a", b=b, a_scale=a_scale, b_scale=b_scale, bias=bias)
     c = torch.empty((m, n), dtype=dtype, device=dev)
     lib = nat.load()
     pa, pb = a.data_ptr(), b.data_ptr()
@@ -201,8 +205,9 @@ def _backward(which: str, grad_c: torch.Tensor, q: torch.Tensor, scale: torch.Te
     depth, k = q.shape
     if depth != (n if which == "a" else m):
         raise ValueError(f"Dimension mismatch: grad_c is {m}x{n}, {other} is {depth}x{k}")
-    _vector(f"{other}_scale", scale, depth, (torch.float32,))
-    dev = _same_device(("grad_c", grad_c), (other, q), (f"{other}_scale", scale))
+    _vector(f"{other}_scale", scale, depth, _F32)
+    dev = grad_c.device
+    _same_device(dev, "grad_c", **{other: q, f"{other}_scale": scale})
     out = torch.empty((m if which == "a" else n, k), dtype=grad_c.dtype, device=dev)
     lib = nat.load()
     size, run = ((lib.tg_i8_backward_a_workspace_size, lib.tg_i8_backward_a) if which == "a" else
