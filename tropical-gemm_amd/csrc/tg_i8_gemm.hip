@@ -27,19 +27,20 @@ hipError_t by_type(int type, F&& f) {
 // ---- choice of a tile ----------------------------------------------------
 
 // A tile's sizes, workgroups per CU, and its time in us: `start` + step for
-// each 128 bytes of the sum while every workgroup has a CU of its own,
-// otherwise rounds of `round` + full for each 128 bytes.  Measured on MI355X
-// over 135 products (M 32 ... 8192, N 512 ... 8192, K 512 ... 8192 bytes), 8-bit
-// and bf16 alike (the time goes by bytes): the tile with the least time so
-// reckoned is 0.5% slower than the best one in the mean, 13% at most.
+// each 128 bytes of the sum while every workgroup has a CU of its own (`crowd`
+// more as the last CUs fill and share the way to memory), otherwise rounds of
+// `round` + full for each 128 bytes.  Fitted to 275 products on MI355X (M 32
+// ... 8192, N 512 ... 8192, K 512 ... 8192 bytes; 8-bit and bf16 alike, the time
+// goes by bytes): the tile with the least time so reckoned is 0.25% slower
+// than the best one in the mean, 18% at most.
 struct TileTime {
     int bm, bn, threads, per_cu;
-    double start, step, round, full;
+    double start, step, crowd, round, full;
 };
 constexpr TileTime kTiles[] = {
-    {256, 256, 512, 1, 6.8, 1.05, 8.3, 1.46}, {128, 128, 512, 1, 3.4, 0.365, 2.5, 0.49},
-    {128, 128, 256, 2, 3.4, 0.40, 3.2, 0.894}, {64, 128, 512, 2, 2.8, 0.267, 2.0, 0.58},
-    {64, 64, 256, 3, 2.7, 0.19, 1.1, 0.55},    {32, 64, 256, 3, 2.6, 0.165, 1.0, 0.42},
+    {256, 256, 512, 1, 7.67, 0.987, 0.659, 9.24, 1.359}, {128, 128, 512, 1, 4.00, 0.336, 0.145, 2.31, 0.447},
+    {128, 128, 256, 2, 3.79, 0.417, 0.137, 3.10, 0.848}, {64, 128, 512, 2, 3.16, 0.235, 0.065, 1.53, 0.547},
+    {64, 64, 256, 2, 2.78, 0.197, 0.022, 1.01, 0.336},   {32, 64, 256, 3, 2.67, 0.176, 0.001, 0.74, 0.362},
 };
 constexpr int kTileForms = sizeof(kTiles) / sizeof(kTiles[0]);
 
@@ -49,16 +50,13 @@ struct TilePlan {
 };
 
 double tile_time(const TileTime& c, int64_t tiles, int64_t steps) {
-    if (tiles <= 256) {
-        // A CU's neighbours take bandwidth from a 256 x 256 tile's step.
-        const double crowd = c.bm == 256 && tiles > 128 ? 0.9 * (c.full - c.step) * double(tiles - 128) / 128 : 0;
-        return c.start + double(steps) * (c.step + crowd);
-    }
+    const double alone = c.step + (tiles > 128 ? c.crowd * double((tiles < 256 ? tiles : 256) - 128) / 128 : 0);
+    if (tiles <= 256) return c.start + double(steps) * alone;
     const int64_t slots = 256 * int64_t(c.per_cu), whole = tiles / slots;
-    double t = 3 + double(whole) * (c.round + double(steps) * c.full);
     const double last = double(tiles - whole * slots) / double(slots), depth = last * c.per_cu;
+    double t = 3 + double(whole) * (c.round + double(steps) * c.full);
     if (last > 0 && c.per_cu > 1)
-        t += c.round + double(steps) * (depth <= 1 ? c.step : c.step + (c.full - c.step) * (depth - 1) / (c.per_cu - 1));
+        t += c.round + double(steps) * (depth <= 1 ? alone : alone + (c.full - alone) * (depth - 1) / (c.per_cu - 1));
     else if (last > 0)
         t += c.round + double(steps) * c.full * (0.75 + 0.25 * last);
     return t;
@@ -122,18 +120,18 @@ hipError_t launch_join(const V* part, int slices, int64_t m, int64_t n, const Ti
     return hipGetLastError();
 }
 
-template <Mma KIND, int WM, int WN, int FM, int FN, int NS, int PER_CU, typename T>
+template <Mma KIND, int WM, int WN, int FM, int FN, int NB, int PER_CU, typename T>
 hipError_t launch_form(TileArgs p, const TilePlan& pl, const TileStore<T>& out, void* part, hipStream_t st) {
-    using Cfg = Tile<KIND, 16, WM, WN, FM, FN, NS>;
+    using Cfg = Tile<KIND, 16, WM, WN, FM, FN, NB>;
     const dim3 grid(unsigned(pl.tiles_m * pl.tiles_n), unsigned(pl.slices));
     if (pl.slices == 1) {
-        const auto kernel = &tg_i8_tiles<KIND, 16, WM, WN, FM, FN, NS, PER_CU, T>;
+        const auto kernel = &tg_i8_tiles<KIND, 16, WM, WN, FM, FN, NB, PER_CU, T>;
         static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
         if (attr != hipSuccess) return attr;
         hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, out);
         return hipGetLastError();
     }
-    const auto kernel = &tg_i8_tiles_slice<KIND, 16, WM, WN, FM, FN, NS, PER_CU>;
+    const auto kernel = &tg_i8_tiles_slice<KIND, 16, WM, WN, FM, FN, NB, PER_CU>;
     static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
     if (attr != hipSuccess) return attr;
     auto* sums = static_cast<typename Cfg::Value*>(part);
@@ -152,7 +150,7 @@ hipError_t launch_tiles(TileArgs p, const TilePlan& pl, const TileStore<T>& out,
         case 1: return launch_form<KIND, 2, 4, 4, 2, 4, 1>(p, pl, out, part, st);
         case 2: return launch_form<KIND, 2, 2, 4, 4, 2, 2>(p, pl, out, part, st);
         case 3: return launch_form<KIND, 2, 4, 2, 2, 3, 2>(p, pl, out, part, st);
-        case 4: return launch_form<KIND, 2, 2, 2, 2, 3, 3>(p, pl, out, part, st);
+        case 4: return launch_form<KIND, 2, 2, 2, 2, 3, 2>(p, pl, out, part, st);
         default: return launch_form<KIND, 2, 2, 1, 2, 4, 3>(p, pl, out, part, st);
     }
 }

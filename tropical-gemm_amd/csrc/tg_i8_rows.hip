@@ -202,13 +202,34 @@ __global__ __launch_bounds__(256) void tg_i8_restore(const int8_t* __restrict__ 
     }
 }
 
+// A group of eight elements as it is loaded.
+template <typename T>
+struct Eight {
+    T v[8];
+    __device__ __forceinline__ void load(const T* p, int64_t left) {
+        typedef uint32_t words __attribute__((ext_vector_type(sizeof(T) * 2), aligned(sizeof(T))));
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        if (left >= 8) {
+            typedef uint32_t raw __attribute__((ext_vector_type(sizeof(T) * 2)));
+            const t8 x = __builtin_bit_cast(t8, raw(*reinterpret_cast<const words*>(p)));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = x[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : T(0.0f);
+        }
+    }
+};
+
 // Backward of the norm.  u = gy * w, rstd and c = rstd^2 * mean(u * h) of each
 // row, gx = rstd * (u - h * c) + gh; the workgroup adds gy * h * rstd of its
 // rows (blockIdx.x, + gridDim.x, ...) in that order in registers, and writes
 // that sum of each column to part[blockIdx.x].  The columns of a thread are as
-// in tg_i8_rows; blockIdx.y takes the next NT * VPT * 8 of them when COLS
-// does not hold the row (then every workgroup of a row reduces all of it).
-template <typename T, typename W, int NT, int VPT>
+// in tg_i8_rows; its weights stay in registers, and the next row is loaded
+// before this one is reduced, so that loads are always on their way.  A row
+// longer than NT * VPT * 8 is shared by blockIdx.y; then every workgroup
+// reduces all of it.
+template <typename T, typename W, bool GH, int NT, int VPT>
 __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
     const T* __restrict__ gy, int64_t ldg, const T* __restrict__ h, int64_t ldh, const W* __restrict__ w,
     float eps, const T* __restrict__ gh, int64_t ldgh, T* __restrict__ gx, float* __restrict__ part,
@@ -217,96 +238,132 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
     __shared__ float red[2][2][W64];
     const int t = threadIdx.x, wave = t / 64;
     const int64_t base = int64_t(blockIdx.y) * (NT * VPT * 8);
-    float acc[VPT][8] = {};
-    int flip = 0;
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, flip ^= 1) {
-        float g[VPT][8], hv[VPT][8];
-        float ss = 0.0f, dot = 0.0f;
-        auto add = [&](int64_t at, float(&gv)[8], float(&hh)[8]) {
-            const int n = cols - at < 8 ? int(cols - at) : 8;
-            float wv[8];
-            load_upto8(gy + row * ldg + at, n, gv);
-            load_upto8(h + row * ldh + at, n, hh);
-            load_upto8(w + at, n, wv);
+    auto at = [&](int k) { return base + int64_t(k * NT + t) * 8; };
+    float acc[VPT][8] = {}, wv[VPT][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                ss += hh[i] * hh[i];
-                dot += gv[i] * wv[i] * hh[i];
-            }
-        };
+    for (int k = 0; k < VPT; ++k)
+        if (at(k) < cols) load_upto8(w + at(k), int(cols - at(k) < 8 ? cols - at(k) : 8), wv[k]);
+    struct Row {
+        Eight<T> g[VPT], h[VPT], gh[VPT];
+    } x[2];
+    auto load = [&](int64_t row, Row& r) {
+        if (row >= rows) return;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int64_t left = cols - at(k);
+            if (left <= 0) continue;
+            r.g[k].load(gy + row * ldg + at(k), left);
+            r.h[k].load(h + row * ldh + at(k), left);
+            if constexpr (GH) r.gh[k].load(gh + row * ldgh + at(k), left);
+        }
+    };
+    const float inv_n = 1.0f / float(cols);
+    auto finish = [&](int64_t row, const Row& r, int flip) {
+        float ss = 0.0f, dot = 0.0f;
         if (gridDim.y > 1) {  // the part of the row that other workgroups hold
-            float a[8], b[8];
-            for (int64_t at = int64_t(t) * 8; at < cols; at += NT * 8)
-                if (at < base || at >= base + NT * VPT * 8) add(at, a, b);
+            for (int64_t c = int64_t(t) * 8; c < cols; c += NT * 8) {
+                if (c >= base && c < base + NT * VPT * 8) continue;
+                const int n = cols - c < 8 ? int(cols - c) : 8;
+                float a[8], b[8], d[8];
+                load_upto8(gy + row * ldg + c, n, a);
+                load_upto8(h + row * ldh + c, n, b);
+                load_upto8(w + c, n, d);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    ss += b[i] * b[i];
+                    dot += a[i] * d[i] * b[i];
+                }
+            }
         }
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int64_t at = base + int64_t(k * NT + t) * 8;
-            if (at < cols) add(at, g[k], hv[k]);
+            if (at(k) >= cols) continue;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float hv = to_f32(r.h[k].v[i]);
+                ss += hv * hv;
+                dot += to_f32(r.g[k].v[i]) * wv[k][i] * hv;
+            }
         }
         ss = wave_sum(ss);
         dot = wave_sum(dot);
-        if (t % 64 == 0) {
-            red[flip][0][wave] = ss;
-            red[flip][1][wave] = dot;
-        }
-        __syncthreads();
-        ss = dot = 0.0f;
+        if constexpr (W64 > 1) {
+            if (t % 64 == 0) {
+                red[flip][0][wave] = ss;
+                red[flip][1][wave] = dot;
+            }
+            __syncthreads();
+            ss = dot = 0.0f;
 #pragma unroll
-        for (int i = 0; i < W64; ++i) {
-            ss += red[flip][0][i];
-            dot += red[flip][1][i];
+            for (int i = 0; i < W64; ++i) {
+                ss += red[flip][0][i];
+                dot += red[flip][1][i];
+            }
         }
-        const float inv_n = 1.0f / float(cols);
         const float rstd = 1.0f / sqrtf(ss * inv_n + eps);
         const float c = dot * inv_n * rstd * rstd;
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
-            const int64_t at = base + int64_t(k * NT + t) * 8;
-            if (at >= cols) continue;
-            const int n = cols - at < 8 ? int(cols - at) : 8;
-            float wv[8], o[8];
-            load_upto8(w + at, n, wv);
+            const int64_t left = cols - at(k);
+            if (left <= 0) continue;
+            float o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                acc[k][i] += g[k][i] * (hv[k][i] * rstd);
-                o[i] = rstd * (g[k][i] * wv[i] - hv[k][i] * c);
+                const float g = to_f32(r.g[k].v[i]), hv = to_f32(r.h[k].v[i]);
+                acc[k][i] += g * (hv * rstd);
+                o[i] = rstd * (g * wv[k][i] - hv * c);
+                if constexpr (GH) o[i] += to_f32(r.gh[k].v[i]);
             }
-            if (gh != nullptr) {
-                float a[8];
-                load_upto8(gh + row * ldgh + at, n, a);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] += a[i];
-            }
-            store_upto8(gx + row * cols + at, n, o);
+            store_upto8(gx + row * cols + at(k), left < 8 ? int(left) : 8, o);
         }
+    };
+    const int64_t stride = gridDim.x;
+    load(blockIdx.x, x[0]);
+    for (int64_t row = blockIdx.x; row < rows; row += 2 * stride) {
+        load(row + stride, x[1]);
+        finish(row, x[0], 0);
+        load(row + 2 * stride, x[0]);
+        if (row + stride < rows) finish(row + stride, x[1], 1);
     }
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-        const int64_t at = base + int64_t(k * NT + t) * 8;
-        if (at < cols) store_upto8(part + int64_t(blockIdx.x) * cols + at, cols - at < 8 ? int(cols - at) : 8, acc[k]);
+        const int64_t left = cols - at(k);
+        if (left > 0) store_upto8(part + int64_t(blockIdx.x) * cols + at(k), left < 8 ? int(left) : 8, acc[k]);
     }
 }
 
-// gw[j] = sum over the parts, in their order within each of the 16 slices and
-// then over the slices: the same bits in every run.
+// gw[j] = sum over the parts: 64 slices of them, each in order, four of its
+// loads on their way at a time, then the slices in order.  The same bits in
+// every run.
 template <typename W>
 __global__ __launch_bounds__(1024) void tg_i8_sum_parts(const float* __restrict__ part, int64_t parts,
                                                         W* __restrict__ gw, int64_t cols) {
-    __shared__ float s[16][64];
-    const int c = threadIdx.x % 64, y = threadIdx.x / 64;
-    const int64_t col = int64_t(blockIdx.x) * 64 + c;
+    __shared__ float s[64][17];
+    const int c = threadIdx.x % 16, y = threadIdx.x / 16;
+    const int64_t col = int64_t(blockIdx.x) * 16 + c;
     float a = 0.0f;
-    if (col < cols)
-        for (int64_t r = y; r < parts; r += 16) a += part[r * cols + col];
+    if (col < cols) {
+        for (int64_t r = y; r < parts; r += 256) {
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = r + 64 * i < parts ? part[(r + 64 * i) * cols + col] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a += v[i];
+        }
+    }
     s[y][c] = a;
     __syncthreads();
-    if (y == 0 && col < cols) {
-        for (int i = 1; i < 16; ++i) a += s[i][c];
+    if (threadIdx.x < 16 && col < cols) {
+        a = s[0][c];
+#pragma unroll
+        for (int i = 1; i < 64; ++i) a += s[i][c];
         gw[col] = static_cast<W>(a);
     }
 }
 
+// Workgroups along the rows, each with a part of the weight's gradient: two
+// for each CU (a part costs cols * 8 bytes of traffic, as much as a row's
+// gradient or two).
 int64_t backward_parts(int64_t rows) { return rows < 512 ? rows : 512; }
 
 template <typename T, typename W, int NT, int VPT>
@@ -314,14 +371,15 @@ hipError_t launch_norm_backward(const I8NormBackward& p, float* part, hipStream_
     const int64_t parts = backward_parts(p.rows);
     if (parts > 0) {
         const dim3 grid(unsigned(parts), unsigned(ceil_div(p.cols, NT * VPT * 8)));
-        hipLaunchKernelGGL((tg_i8_norm_backward<T, W, NT, VPT>), grid, dim3(NT), 0, st,
-                           static_cast<const T*>(p.grad_y), p.ldg, static_cast<const T*>(p.h), p.ldh,
-                           static_cast<const W*>(p.weight), p.eps, static_cast<const T*>(p.grad_h), p.ldgh,
-                           static_cast<T*>(p.grad_x), part, p.rows, p.cols);
+        const auto kernel = p.grad_h != nullptr ? &tg_i8_norm_backward<T, W, true, NT, VPT>
+                                                : &tg_i8_norm_backward<T, W, false, NT, VPT>;
+        hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, st, static_cast<const T*>(p.grad_y), p.ldg,
+                           static_cast<const T*>(p.h), p.ldh, static_cast<const W*>(p.weight), p.eps,
+                           static_cast<const T*>(p.grad_h), p.ldgh, static_cast<T*>(p.grad_x), part, p.rows, p.cols);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((tg_i8_sum_parts<W>), dim3(unsigned(ceil_div(p.cols, 64))), dim3(1024), 0, st, part,
+    hipLaunchKernelGGL((tg_i8_sum_parts<W>), dim3(unsigned(ceil_div(p.cols, 16))), dim3(1024), 0, st, part,
                        parts, static_cast<W*>(p.grad_weight), p.cols);
     return hipGetLastError();
 }
@@ -330,8 +388,10 @@ template <typename T, typename W>
 hipError_t norm_backward_typed(const I8NormBackward& p, float* part, hipStream_t st) {
     const int64_t groups = ceil_div(p.cols, 8);
     if (groups <= 64) return launch_norm_backward<T, W, 64, 1>(p, part, st);
+    if (groups <= 128) return launch_norm_backward<T, W, 128, 1>(p, part, st);
     if (groups <= 256) return launch_norm_backward<T, W, 256, 1>(p, part, st);
-    return launch_norm_backward<T, W, 512, 2>(p, part, st);
+    if (groups <= 512) return launch_norm_backward<T, W, 512, 1>(p, part, st);
+    return launch_norm_backward<T, W, 1024, 1>(p, part, st);
 }
 
 }  // namespace

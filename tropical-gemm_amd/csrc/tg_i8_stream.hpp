@@ -84,8 +84,29 @@ __global__ __launch_bounds__(W * 64) void tg_i8_stream(StreamArgs p, TileStore<T
     const int at_a = int(reinterpret_cast<uintptr_t>(pa) & 3), at_b = int(reinterpret_cast<uintptr_t>(pb) & 3);
     Acc acc = {};
     const int units = p.k / 128;
-    int u = wave;
-    for (; u < units; u += W) {
+    // What does not need the sum is loaded before it, so that its latency is
+    // not added to the end: the bytes behind the whole units, and scales.
+    const bool last = wave == units % W;
+    u32x4 ta[2], tb[2];
+    if (last) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            tb[i] = stream_tail(pb, units * 128 + i * 64 + lg * 16, p.k);
+            ta[i] = stream_tail(pa, units * 128 + i * 64 + lg * 16, p.k);
+        }
+    }
+    const bool stores = wave == 0 && li < p.m;
+    float sa = 0, sb[4] = {}, bias[4] = {};
+    if (stores) {
+        sa = out.a_scale[li];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int n = n0 + lg * 4 + e < p.n ? n0 + lg * 4 + e : p.n - 1;
+            sb[e] = out.b_scale[n];
+            if (out.bias != nullptr) bias[e] = to_f32(out.bias[n]);
+        }
+    }
+    for (int u = wave; u < units; u += W) {
         StreamRaw<WORDS> xa[2], xb[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -95,25 +116,21 @@ __global__ __launch_bounds__(W * 64) void tg_i8_stream(StreamArgs p, TileStore<T
 #pragma unroll
         for (int i = 0; i < 2; ++i) acc = mma<Mma::I8, 16>(xb[i].get(at_b), xa[i].get(at_a), acc);
     }
-    if (u == units) {  // the bytes behind the whole units
+    if (last) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int k = u * 128 + i * 64 + lg * 16;
-            acc = mma<Mma::I8, 16>(stream_tail(pb, k, p.k), stream_tail(pa, k, p.k), acc);
-        }
+        for (int i = 0; i < 2; ++i) acc = mma<Mma::I8, 16>(tb[i], ta[i], acc);
     }
     part[wave][lane] = acc;
     __syncthreads();
-    if (wave != 0 || li >= p.m) return;
+    if (!stores) return;
 #pragma unroll
     for (int w = 1; w < W; ++w) acc += part[w][lane];
-    const float sa = out.a_scale[li];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int n = n0 + lg * 4 + e;
         if (n >= p.n) continue;
-        float v = float(acc[e]) * sa * out.b_scale[n];
-        if (out.bias != nullptr) v += to_f32(out.bias[n]);
+        float v = float(acc[e]) * sa * sb[e];
+        if (out.bias != nullptr) v += bias[e];
         out.c[int64_t(li) * p.n + n] = static_cast<T>(v);
     }
 }

@@ -85,11 +85,15 @@ struct TileArgs {
 
 // Tile of a workgroup: WM x WN waves, each FM x FN fragments of FS x FS.
 //
-// LDS holds a ring of NS stages of BM + BN rows of 128 bytes.  One step is two
-// halves of 64 bytes.  While the matrix unit works on one half's fragments, the
-// other half's are read from LDS into registers; the step's barrier stands
-// between the halves, where the next step's loads have landed and this step's
-// LDS is free for the loads of the step NS later.
+// LDS holds a ring of NB + 1 stages of A's BM rows of 128 bytes and one of NB
+// stages of B's BN rows.  One step is two halves of 64 bytes.  While the matrix
+// unit works on one half's fragments, the other half's are read from LDS into
+// registers; the step's barrier stands between the halves, where the next
+// step's loads have landed and this step's LDS is free.  A's loads of the step
+// NB later go in the half before it (A's ring has a stage more), B's in the
+// half behind it: a CU takes one 1 KiB load in 16 clocks at most, and waves
+// that issue them faster stand still (8192^3 in 8 bits: 396 us; with A's and
+// B's behind the barrier 421, all behind its first four rows 440).
 //
 // The 16-byte chunk c of a row lies at place c ^ key(row).  LDS serves 16
 // lanes of a 16-byte read at a time, lanes {0-3, 12-15, 20-27} and {4-11,
@@ -98,15 +102,15 @@ struct TileArgs {
 // are taken so that a lane's FN fragments hold VPF FN neighbouring columns of C
 // (whole 16-byte stores); B is the first operand, so that a fragment's values
 // of a lane are neighbours in a row of C.
-template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NS>
+template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB>
 struct Tile {
     static constexpr int BM = WM * FM * FS, BN = WN * FN * FS, NT = WM * WN * 64;
     static constexpr int KS = FS / 16;       // instructions along half a step
     static constexpr int VPF = FS * FS / 64;  // values of a fragment per lane
     static constexpr int LOADS_A = BM * 8 / NT, LOADS_B = BN * 8 / NT, LOADS = LOADS_A + LOADS_B;
-    static constexpr int STAGE = (BM + BN) * 128, LDS = NS * STAGE;
+    static constexpr int NA = NB + 1, STAGE_A = BM * 128, STAGE_B = BN * 128, LDS = NA * STAGE_A + NB * STAGE_B;
     static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0 && NT % 64 == 0, "whole loads");
-    static_assert(NS >= 2 && NS <= 6, "wait_for's cases");
+    static_assert(NB >= 2 && NB <= 5, "wait_for's cases");
     using Acc = typename MmaAcc<KIND, FS>::type;
     using Value = std::conditional_t<KIND == Mma::I8, int32_t, float>;
 
@@ -155,33 +159,41 @@ struct Tile {
             const int r = t / 8 + i * (NT / 8), last = p.n - 1 - tn * BN;
             off_b[i] = uint32_t(r < last ? r : last) * uint32_t(p.ldb) + chunk_b(i) * 16;
         }
-        // Loads of the step that comes next, `count` of them from load `first`
-        // on; `over` is at most a chunk's own offset in its row, so off - over
-        // stays inside the row.
-        int next = s0, next_b = s0 % p.b_steps;
-        uint32_t next_lds = lds0;
-        auto load = [&](int first, int count) {
-            const bool partial = cut && next == s1 - 1;
-            const char *pa = a0 + int64_t(next) * 128, *pb = b0 + int64_t(next_b) * 128;
-#pragma unroll
-            for (int i = first; i < first + count; ++i) {
-                const int past = (i < LOADS_A ? chunk_a(i) : chunk_b(i - LOADS_A)) * 16 + 16 - p.tail;
-                const uint32_t over = partial && past > 0 ? uint32_t(past) : 0;
-                if (i < LOADS_A) tile_load(pa, off_a[i] - over, next_lds + i * (NT * 16));
-                else tile_load(pb, off_b[i - LOADS_A] - over, next_lds + i * (NT * 16));
-            }
+        // `count` loads from load `first` on of the step that comes next, A's
+        // before B's; `over` is at most a chunk's own offset in its row, so
+        // off - over stays inside the row.
+        int next_a = s0, next_b = s0, turn_b = s0 % p.b_steps;
+        uint32_t to_a = lds0, to_b = lds0 + NA * STAGE_A;
+        auto over = [&](int step, int chunk) {
+            const int past = chunk * 16 + 16 - p.tail;
+            return uint32_t(cut && step == s1 - 1 && past > 0 ? past : 0);
         };
-        auto loaded = [&] {
-            ++next;
-            next_b = next_b + 1 == p.b_steps ? 0 : next_b + 1;
-            next_lds = next_lds == lds0 + (NS - 1) * STAGE ? lds0 : next_lds + STAGE;
+        auto load_a = [&](int first, int count) {
+            const char* from = a0 + int64_t(next_a) * 128;
+#pragma unroll
+            for (int i = first; i < first + count; ++i)
+                tile_load(from, off_a[i] - over(next_a, chunk_a(i)), to_a + i * (NT * 16));
+        };
+        auto load_b = [&](int first, int count) {
+            const char* from = b0 + int64_t(turn_b) * 128;
+#pragma unroll
+            for (int i = first; i < first + count; ++i)
+                tile_load(from, off_b[i] - over(next_b, chunk_b(i)), to_b + i * (NT * 16));
+        };
+        auto loaded_a = [&] {
+            ++next_a;
+            to_a = to_a == lds0 + (NA - 1) * STAGE_A ? lds0 : to_a + STAGE_A;
+        };
+        auto loaded_b = [&] {
+            ++next_b;
+            turn_b = turn_b + 1 == p.b_steps ? 0 : turn_b + 1;
+            to_b = to_b == lds0 + NA * STAGE_A + (NB - 1) * STAGE_B ? lds0 + NA * STAGE_A : to_b + STAGE_B;
         };
         // Waits until all but the newest `steps` steps' loads have landed.
         auto wait_for = [&](int steps) {
-            if (NS > 5 && steps >= 4) tile_wait<(NS > 5 ? 4 : 0) * LOADS>();
-            else if (NS > 4 && steps >= 3) tile_wait<(NS > 4 ? 3 : 0) * LOADS>();
-            else if (NS > 3 && steps >= 2) tile_wait<(NS > 3 ? 2 : 0) * LOADS>();
-            else if (NS > 2 && steps >= 1) tile_wait<(NS > 2 ? 1 : 0) * LOADS>();
+            if (NB > 4 && steps >= 3) tile_wait<(NB > 4 ? 3 : 0) * LOADS>();
+            else if (NB > 3 && steps >= 2) tile_wait<(NB > 3 ? 2 : 0) * LOADS>();
+            else if (NB > 2 && steps >= 1) tile_wait<(NB > 2 ? 1 : 0) * LOADS>();
             else tile_wait<0>();
         };
 
@@ -191,27 +203,25 @@ struct Tile {
         // Fragment j's row, row_b + VPF j, has row_b's key, as fragment i's of
         // A, row_a + FS i, has row_a's.
         const int at_a = row_a * 128 + ((lg ^ key_a(row_a)) << 4);
-        const int at_b = BM * 128 + row_b * 128 + ((lg ^ key_b(row_b)) << 4);
+        const int at_b = NA * STAGE_A + row_b * 128 + ((lg ^ key_b(row_b)) << 4);
         typedef const __attribute__((address_space(3))) u32x4* frag_t;
         u32x4 xa[2][FM][KS], xb[2][FN][KS];
-        // Part i of FM of a half's fragments.
-        auto read_part = [&](int i, int half, int at) {
-            const lds_t* from = lds + at;
+        // Part i of FM of a half's fragments, from the stages at (pa, pb).
+        auto read_part = [&](int i, int half, int pa, int pb) {
+            const lds_t *from_a = lds + pa, *from_b = lds + pb;
 #pragma unroll
             for (int u = 0; u < KS; ++u)
-                xa[half][i][u] = *reinterpret_cast<frag_t>(from + (at_a ^ (half * 64 + u * 32)) + i * FS * 128);
+                xa[half][i][u] = *reinterpret_cast<frag_t>(from_a + (at_a ^ (half * 64 + u * 32)) + i * FS * 128);
 #pragma unroll
             for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j)
 #pragma unroll
                 for (int u = 0; u < KS; ++u)
-                    xb[half][j][u] = *reinterpret_cast<frag_t>(from + (at_b ^ (half * 64 + u * 32)) + j * VPF * 128);
+                    xb[half][j][u] = *reinterpret_cast<frag_t>(from_b + (at_b ^ (half * 64 + u * 32)) + j * VPF * 128);
         };
         // Multiplies the fragments of half h, row by row.  Behind each row's
-        // products come its parts of a later step's loads (spread over all
-        // rows: 393 us against 419 for 8192^3 in 8 bits with all of them
-        // behind the first half of the rows) and of the next half's reads
-        // (done one row before the end, so that they are there in time).
-        auto products = [&](int h, auto reads, auto loads, int at) {
+        // products come its parts of a later step's loads and of the next
+        // half's reads (done one row before the end, to be there in time).
+        auto products = [&](int h, auto reads, auto loads_a, auto loads_b, int pa, int pb) {
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
 #pragma unroll
@@ -219,12 +229,13 @@ struct Tile {
 #pragma unroll
                     for (int j = 0; j < FN; ++j) acc[i][j] = mma<KIND, FS>(xb[h][j][u], xa[h][i][u], acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (decltype(loads)::value) {
-                    load(i * LOADS / FM, (i + 1) * LOADS / FM - i * LOADS / FM);
-                }
+                if constexpr (decltype(loads_a)::value)
+                    load_a(i * LOADS_A / FM, (i + 1) * LOADS_A / FM - i * LOADS_A / FM);
+                if constexpr (decltype(loads_b)::value)
+                    load_b(i * LOADS_B / FM, (i + 1) * LOADS_B / FM - i * LOADS_B / FM);
                 if constexpr (decltype(reads)::value) {
-                    if (i == 0) read_part(0, h ^ 1, at);
-                    if (i + 1 < FM) read_part(i + 1, h ^ 1, at);
+                    if (i == 0) read_part(0, h ^ 1, pa, pb);
+                    if (i + 1 < FM) read_part(i + 1, h ^ 1, pa, pb);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -241,58 +252,84 @@ struct Tile {
         const std::true_type yes;
         const std::false_type no;
 
-        for (int s = s0; s < s1 && s < s0 + NS; ++s) {
-            load(0, LOADS);
-            loaded();
+        for (int s = s0; s < s1 && s < s0 + NB; ++s) {
+            load_a(0, LOADS_A);
+            load_b(0, LOADS_B);
+            loaded_a();
+            loaded_b();
         }
-        if (s1 - s0 >= NS) tile_wait<(NS - 1) * LOADS>();
+        if (s1 - s0 >= NB) tile_wait<(NB - 1) * LOADS>();
         else tile_wait<0>();
 #pragma unroll
-        for (int i = 0; i < FM; ++i) read_part(i, 0, 0);
-        int s = s0, at = 0, then = STAGE;  // places of this step's and the next one's stage
+        for (int i = 0; i < FM; ++i) read_part(i, 0, 0, 0);
+        // Places of this step's and the next one's stages.
+        int s = s0, pa = 0, pb = 0, then_a = STAGE_A, then_b = STAGE_B;
         auto step_done = [&] {
-            at = then;
-            then = then == (NS - 1) * STAGE ? 0 : then + STAGE;
+            pa = then_a;
+            pb = then_b;
+            then_a = then_a == (NA - 1) * STAGE_A ? 0 : then_a + STAGE_A;
+            then_b = then_b == (NB - 1) * STAGE_B ? 0 : then_b + STAGE_B;
         };
-        for (; s < s1 - NS; ++s) {
-            products(0, yes, no, at);
-            tile_wait<(NS - 2) * LOADS>();
-            products(1, yes, yes, then);
-            loaded();
+        for (; s < s1 - NB; ++s) {
+            products(0, yes, yes, no, pa, pb);
+            loaded_a();
+            tile_wait<(NB - 2) * LOADS + LOADS_A>();
+            products(1, yes, no, yes, then_a, then_b);
+            loaded_b();
             step_done();
         }
         for (; s < s1 - 1; ++s) {  // nothing is left to load
-            products(0, yes, no, at);
+            products(0, yes, no, no, pa, pb);
             wait_for(s1 - 2 - s);
-            products(1, yes, no, then);
+            products(1, yes, no, no, then_a, then_b);
             step_done();
         }
         if (cut) clear(0);
-        products(0, yes, no, at);
+        products(0, yes, no, no, pa, pb);
         if (cut) clear(1);
-        products(1, no, no, 0);
+        products(1, no, no, no, 0, 0);
+    }
+
+    // What `Out` needs beside the sums, for the lane's rows and groups of eight
+    // columns.
+    template <typename Out>
+    struct Beside {
+        typename Out::Row rows[FM];
+        typename Out::Cols cols[FN * VPF / 8];
+    };
+    static constexpr int GROUPS = FN * VPF / 8;
+    static_assert(FN * VPF % 8 == 0, "groups of eight");
+    // Loaded before the sum where registers allow it, so that its latency is
+    // not added to the end.
+    static constexpr bool EARLY_BESIDE = FM * FN <= 8;
+
+    static __device__ __forceinline__ int first_row(int tm) {
+        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+        return tm * BM + wave / WN * FM * FS + lane % FS;
+    }
+    static __device__ __forceinline__ int first_col(int tn) {
+        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+        return tn * BN + wave % WN * FN * FS + lane / FS * VPF * FN;
+    }
+
+    template <typename Out>
+    static __device__ __forceinline__ void beside(const TileArgs& p, int tm, int tn, const Out& out, Beside<Out>& x) {
+        const int m0 = first_row(tm), n0 = first_col(tn);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+            if (m0 + i * FS < p.m) x.rows[i] = out.row(m0 + i * FS);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+            if (n0 + g * 8 < p.n) x.cols[g] = out.cols(n0 + g * 8, p.n - n0 - g * 8);
     }
 
     // Hands the lane's outputs to `out` in groups of eight neighbours in a row.
-    // Its scales are loaded together first: a load before each group's store
-    // would cost its latency FM times over (2.7 us a tile more at 256 x 256).
     template <typename Out>
     static __device__ __forceinline__ void outputs(const TileArgs& p, int tm, int tn, const Acc (&acc)[FM][FN],
-                                                   const Out& out) {
-        const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, li = lane % FS, lg = lane / FS;
-        const int m0 = tm * BM + wave / WN * FM * FS + li, n0 = tn * BN + wave % WN * FN * FS + lg * VPF * FN;
-        constexpr int GROUPS = FN * VPF / 8;
-        static_assert(FN * VPF % 8 == 0, "groups of eight");
-        typename Out::Row rows[FM];
-        typename Out::Cols cols[GROUPS];
+                                                   const Out& out, const Beside<Out>& x) {
+        const int m0 = first_row(tm), n0 = first_col(tn);
         auto each = [&](auto inside) {
             constexpr bool IN = decltype(inside)::value;
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-                if (IN || m0 + i * FS < p.m) rows[i] = out.row(m0 + i * FS);
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g)
-                if (IN || n0 + g * 8 < p.n) cols[g] = out.cols(n0 + g * 8, IN ? 8 : p.n - n0 - g * 8);
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
                 if (!IN && m0 + i * FS >= p.m) continue;
@@ -302,12 +339,25 @@ struct Tile {
                     Value v[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] = acc[i][(g * 8 + e) / VPF][(g * 8 + e) % VPF];
-                    out.store(m0 + i * FS, n0 + g * 8, IN ? 8 : p.n - n0 - g * 8, v, rows[i], cols[g]);
+                    out.store(m0 + i * FS, n0 + g * 8, IN ? 8 : p.n - n0 - g * 8, v, x.rows[i], x.cols[g]);
                 }
             }
         };
         if ((tm + 1) * BM <= p.m && (tn + 1) * BN <= p.n) each(std::true_type());
         else each(std::false_type());
+    }
+
+    // The workgroup's tile over steps [s0, s1), from the sum to `out`.
+    template <typename Out>
+    static __device__ __forceinline__ void whole(const TileArgs& p, int s0, int s1, char* smem, const Out& out) {
+        Acc acc[FM][FN] = {};
+        Beside<Out> x;
+        int tm, tn;
+        place(p, tm, tn);
+        if (EARLY_BESIDE) beside(p, tm, tn, out, x);
+        run(p, tm, tn, s0, s1, (lds_t*)(smem), acc);
+        if (!EARLY_BESIDE) beside(p, tm, tn, out, x);
+        outputs(p, tm, tn, acc, out, x);
     }
 };
 
@@ -367,30 +417,20 @@ struct TilePartial {
     }
 };
 
-template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NS, int PER_CU, typename T>
+template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB, int PER_CU, typename T>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_i8_tiles(TileArgs p, TileStore<T> out) {
-    using Cfg = Tile<KIND, FS, WM, WN, FM, FN, NS>;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    typename Cfg::Acc acc[FM][FN] = {};
-    int tm, tn;
-    Cfg::place(p, tm, tn);
-    Cfg::run(p, tm, tn, 0, p.steps, (lds_t*)(smem), acc);
-    Cfg::outputs(p, tm, tn, acc, out);
+    Tile<KIND, FS, WM, WN, FM, FN, NB>::whole(p, 0, p.steps, smem, out);
 }
 
 // Slice blockIdx.y of the sum: its sums to part + blockIdx.y * M * ld.
-template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NS, int PER_CU>
+template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB, int PER_CU>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_i8_tiles_slice(
-    TileArgs p, TilePartial<typename Tile<KIND, FS, WM, WN, FM, FN, NS>::Value> out) {
-    using Cfg = Tile<KIND, FS, WM, WN, FM, FN, NS>;
+    TileArgs p, TilePartial<typename Tile<KIND, FS, WM, WN, FM, FN, NB>::Value> out) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    typename Cfg::Acc acc[FM][FN] = {};
-    int tm, tn;
-    Cfg::place(p, tm, tn);
     const int s0 = int(blockIdx.y) * p.slice, s1 = s0 + p.slice < p.steps ? s0 + p.slice : p.steps;
-    Cfg::run(p, tm, tn, s0, s1, (lds_t*)(smem), acc);
     out.c += int64_t(blockIdx.y) * p.m * out.ld;
-    Cfg::outputs(p, tm, tn, acc, out);
+    Tile<KIND, FS, WM, WN, FM, FN, NB>::whole(p, s0, s1, smem, out);
 }
 
 // C from the slices' sums, added in their order (none: an empty sum).
