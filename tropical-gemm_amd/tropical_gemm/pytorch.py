@@ -23,7 +23,7 @@ from __future__ import annotations
 
 import torch
 
-from . import cuda_available, ops
+from . import cuda_available, int8, ops
 
 GPU_AVAILABLE = cuda_available()
 _DLPACK_AVAILABLE = True
@@ -218,6 +218,97 @@ def tropical_maxmul_matmul_batched(a: torch.Tensor, b: torch.Tensor) -> torch.Te
     return TropicalMaxMulMatmulBatched.apply(a, b)
 
 
+# ---------------------------------------------------------------------------
+# Linear layers in 8 bits (no counterpart in the reference)
+# ---------------------------------------------------------------------------
+
+def _prep_int8(name: str, x: torch.Tensor, weight: torch.Tensor):
+    if not x.is_cuda or not weight.is_cuda:
+        raise RuntimeError(f"{name} requires GPU tensors.")
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
+        raise RuntimeError(f"{name} expects activations (tokens, k) and weights (n, k), got "
+                           f"{tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.dtype != weight.dtype:
+        raise RuntimeError(f"{name} expects one dtype, got {x.dtype} and {weight.dtype}")
+    return x.detach().contiguous(), weight.detach().contiguous()
+
+
+def _int8_product_backward(ctx, grad, q, scale, qw, scale_w, want_x: bool, want_w: bool):
+    grad = grad.contiguous()
+    return (int8.backward_a(grad, qw, scale_w) if want_x else None,
+            int8.backward_b(grad, q, scale) if want_w else None)
+
+
+class Int8LinearGPU(torch.autograd.Function):
+    """``y = x @ weight.T`` with both operands rounded to 8-bit rows, one scale
+    for each token and each output channel.
+
+    The backward pass reads the 8-bit rows, which are all that is kept of the
+    operands (half of bfloat16's bytes): the gradients are those of the product
+    of the rounded operands, passed through the rounding unchanged."""
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+        x, weight = _prep_int8("Int8LinearGPU", x, weight)
+        q, scale = int8.quantize(x)
+        qw, scale_w = int8.quantize(weight)
+        ctx.save_for_backward(q, scale, qw, scale_w)
+        return int8.matmul(q, scale, qw, scale_w, dtype=x.dtype)
+
+    @staticmethod
+    def backward(ctx, grad_y: torch.Tensor):
+        return _int8_product_backward(ctx, grad_y, *ctx.saved_tensors, *ctx.needs_input_grad)
+
+
+class RmsNormInt8LinearGPU(torch.autograd.Function):
+    """``(y, h)`` of one step of a residual stream: ``h = x + residual``,
+    ``y = rms_norm(h, norm_weight, eps) @ weight.T``, the norm's output rounded
+    to 8-bit rows as it is made and the weights to 8-bit rows beside it.
+
+    Kept for the backward pass: h, the 8-bit rows and the scales."""
+
+    @staticmethod
+    def forward(ctx, x, residual, norm_weight, weight, eps: float = 1e-6):
+        name = "RmsNormInt8LinearGPU"
+        x, weight = _prep_int8(name, x, weight)
+        norm_weight = norm_weight.detach().contiguous()
+        residual = None if residual is None else residual.detach().contiguous()
+        q, scale, h = int8.rms_norm(x, norm_weight, residual, eps)
+        if residual is None:
+            h = x.clone()  # an output of its own, which the caller may write
+        qw, scale_w = int8.quantize(weight)
+        ctx.save_for_backward(h, norm_weight, q, scale, qw, scale_w)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return int8.matmul(q, scale, qw, scale_w, dtype=x.dtype), h
+
+    @staticmethod
+    def backward(ctx, grad_y, grad_h):
+        h, norm_weight, q, scale, qw, scale_w = ctx.saved_tensors
+        want_x, want_r, want_nw, want_w, _ = ctx.needs_input_grad
+        want_norm = want_x or want_r or want_nw
+        if grad_y is None:
+            return grad_h, grad_h if want_r else None, None, None, None
+        grad_n, grad_w = _int8_product_backward(ctx, grad_y, q, scale, qw, scale_w, want_norm, want_w)
+        if not want_norm:
+            return None, None, None, grad_w, None
+        grad_h = None if grad_h is None else grad_h.contiguous()
+        grad_x, grad_nw = int8.rms_norm_backward(grad_n, h, norm_weight, ctx.eps, grad_h)
+        return grad_x, grad_x if want_r else None, grad_nw, grad_w, None
+
+
+def int8_linear_gpu(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """``x @ weight.T`` in 8 bits, with gradients (``Int8LinearGPU``)."""
+    return Int8LinearGPU.apply(x, weight)
+
+
+def rms_norm_int8_linear_gpu(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: torch.Tensor,
+                             weight: torch.Tensor, eps: float = 1e-6):
+    """``(rms_norm(x + residual) @ weight.T, x + residual)`` in 8 bits, with
+    gradients (``RmsNormInt8LinearGPU``)."""
+    return RmsNormInt8LinearGPU.apply(x, residual, norm_weight, weight, eps)
+
+
 __all__ = [
     "TropicalMaxPlusMatmulGPU",
     "TropicalMinPlusMatmulGPU",
@@ -231,6 +322,10 @@ __all__ = [
     "tropical_maxplus_matmul_batched",
     "tropical_minplus_matmul_batched",
     "tropical_maxmul_matmul_batched",
+    "Int8LinearGPU",
+    "RmsNormInt8LinearGPU",
+    "int8_linear_gpu",
+    "rms_norm_int8_linear_gpu",
     "GPU_AVAILABLE",
     "_DLPACK_AVAILABLE",
 ]
