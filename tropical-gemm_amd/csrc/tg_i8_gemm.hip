@@ -5,6 +5,7 @@
 
 #include "../../include/tropical_gemm_hip.h"
 #include "tg_i8.hpp"
+#include "tg_i8_any.hpp"
 #include "tg_i8_pack.hpp"
 #include "tg_i8_stream.hpp"
 #include "tg_i8_tiles.hpp"
@@ -65,7 +66,7 @@ double tile_time(const TileTime& c, int64_t tiles, int64_t steps) {
 // Tile and slices of the sum: slices where tiles are few, as long as the time
 // they save outweighs their partial sums' way through memory and the launch
 // that joins them (2.5 us and 4 TB/s).
-TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps) {
+TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps, double* time = nullptr) {
     if (m <= 0 || n <= 0 || steps <= 0) return {0, 1, 0, 0, 1};
     TilePlan best = {0, 1, ceil_div(m, 256), ceil_div(n, 256), steps};
     double least = 1e30;
@@ -85,6 +86,7 @@ TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps) {
             }
         }
     }
+    if (time != nullptr) *time = least;
     return best;
 }
 
@@ -178,10 +180,30 @@ struct Carver {
 constexpr int64_t kStreamRows = 16;
 
 struct GemmPlan {
-    bool stream, pack_a, pack_b;
+    bool stream, any, pack_a, pack_b;
     int64_t ld;  // of packed rows
     TilePlan tiles;
 };
+
+// A launch that lays out rows: what it takes beside the bytes' way through
+// memory, in us.
+constexpr double kPackTime = 2.5;
+// How much longer than two launches one may take, in us: it saves the caller's
+// thread a launch and a workspace, 5 us.
+constexpr double kOneLaunch = 2.0;
+
+// Time of tg_i8_any in us, as tile_time gives it for the others.  Measured on
+// 96 products of odd sizes (M 32 ... 8192, N 65 ... 4097, K 129 ... 8191): the
+// way taken with it is at most 3 us slower than the other one but for more
+// than 1000 tiles of one or two steps (19 us, or 26 as it is chosen).  Longer
+// sums than 4096 are always laid out first (M = 64, N = 4097, K = 8191: 25 us
+// against 35).
+double any_time(const I8Gemm& p) {
+    const int64_t tiles = ceil_div(p.m, 64) * ceil_div(p.n, 64);
+    if (tiles >= int64_t(1) << 24 || p.k > 4096) return 1e30;
+    const double per_cu = double(tiles) / 256, step = 0.48 * per_cu;
+    return 4.0 + per_cu + double(ceil_div(p.k, 128)) * (step > 0.37 ? step : 0.37);
+}
 
 GemmPlan plan_gemm(const I8Gemm& p) {
     GemmPlan pl{};
@@ -190,7 +212,12 @@ GemmPlan plan_gemm(const I8Gemm& p) {
     pl.pack_a = !in_place(p.a, p.lda, p.k);
     pl.pack_b = !in_place(p.b, p.ldb, p.k);
     pl.ld = round_up(p.k, 128);
-    pl.tiles = plan_tiles(p.m, p.n, ceil_div(p.k, 128));
+    double time = 0;
+    pl.tiles = plan_tiles(p.m, p.n, ceil_div(p.k, 128), &time);
+    if (pl.pack_a || pl.pack_b) {
+        const double bytes = 2 * double(pl.ld) * (double(p.m) * pl.pack_a + double(p.n) * pl.pack_b);
+        pl.any = any_time(p) < time + kPackTime + bytes / 4e6 + kOneLaunch;
+    }
     return pl;
 }
 
@@ -203,7 +230,7 @@ struct GemmWs {
 GemmWs carve_gemm(const I8Gemm& p, const GemmPlan& pl, void* ws) {
     Carver c{static_cast<char*>(ws)};
     GemmWs w{};
-    if (p.m == 0 || p.n == 0 || p.k == 0 || pl.stream) return w;
+    if (p.m == 0 || p.n == 0 || p.k == 0 || pl.stream || pl.any) return w;
     if (pl.pack_a) w.a = static_cast<int8_t*>(c.take(size_t(p.m) * size_t(pl.ld)));
     if (pl.pack_b) w.b = static_cast<int8_t*>(c.take(size_t(p.n) * size_t(pl.ld)));
     w.part = c.take(part_bytes(pl.tiles, p.m, p.n));
@@ -234,6 +261,11 @@ hipError_t gemm_typed(const I8Gemm& p, void* ws, hipStream_t st) {
         // 13, K = 8192: N = 8192 17.2 us against 18.4 with 8; N = 28672 60
         // against 56).
         return p.n <= 16384 ? launch_stream<16>(p, out, st) : launch_stream<8>(p, out, st);
+    }
+    if (pl.any) {
+        const AnyArgs args{p.a, p.lda, p.b, p.ldb, int(p.m), int(p.n), int(p.k), int(ceil_div(p.m, 64)), int(ceil_div(p.n, 64))};
+        hipLaunchKernelGGL((tg_i8_any<T>), dim3(unsigned(args.tiles_m * args.tiles_n)), dim3(256), 0, st, args, out);
+        return hipGetLastError();
     }
     const GemmWs w = carve_gemm(p, pl, ws);
     TileArgs t{};

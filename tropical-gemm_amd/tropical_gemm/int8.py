@@ -88,7 +88,7 @@ def quantize(x: torch.Tensor):
     ld = _rows("x", x)
     rows, cols = x.shape
     dev = x.device
-    q = torch.empty((rows, cols), dtype=torch.int8, device=dev)
+    q = torch.empty(rows, cols, dtype=torch.int8, device=dev)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
     nat.check(nat.load().tg_i8_quantize(dev.index or 0, _FLOAT[x.dtype], x.data_ptr(), ld, q.data_ptr(),
                                         scale.data_ptr(), rows, cols, _stream(dev)))
@@ -103,7 +103,7 @@ def dequantize(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.
     dev = q.device
     _same_device(dev, "q", scale=scale)
     _float_type(dtype)
-    y = torch.empty((rows, cols), dtype=dtype, device=dev)
+    y = torch.empty(rows, cols, dtype=dtype, device=dev)
     nat.check(nat.load().tg_i8_dequantize(dev.index or 0, _FLOAT[dtype], q.data_ptr(), ld, scale.data_ptr(),
                                           y.data_ptr(), rows, cols, _stream(dev)))
     return y
@@ -128,8 +128,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     if residual is not None:
         ldr = _rows("residual", residual, x.dtype)
         _same_shape("residual", residual, x.shape)
-        h = torch.empty((rows, cols), dtype=x.dtype, device=dev)
-    q = torch.empty((rows, cols), dtype=torch.int8, device=dev)
+        h = torch.empty(rows, cols, dtype=x.dtype, device=dev)
+    q = torch.empty(rows, cols, dtype=torch.int8, device=dev)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
     nat.check(nat.load().tg_i8_rms_norm(
         dev.index or 0, _FLOAT[x.dtype], _FLOAT[weight.dtype], x.data_ptr(), ldx, _ptr(residual), ldr,
@@ -156,7 +156,7 @@ def rms_norm_backward(grad_y: torch.Tensor, h: torch.Tensor, weight: torch.Tenso
     if grad_h is not None:
         _same_shape("grad_h", grad_h, h.shape)
         ldgh = _rows("grad_h", grad_h, h.dtype)
-    grad_x = torch.empty((rows, cols), dtype=h.dtype, device=dev)
+    grad_x = torch.empty(rows, cols, dtype=h.dtype, device=dev)
     grad_weight = torch.empty(cols, dtype=weight.dtype, device=dev)
     lib = nat.load()
     nbytes = lib.tg_i8_rms_norm_backward_workspace_size(rows, cols)
@@ -187,7 +187,7 @@ def matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: tor
         _vector("bias", bias, n, (dtype,))
     dev = a.device
     _same_device(dev, "a", b=b, a_scale=a_scale, b_scale=b_scale, bias=bias)
-    c = torch.empty((m, n), dtype=dtype, device=dev)
+    c = torch.empty(m, n, dtype=dtype, device=dev)
     lib = nat.load()
     pa, pb = a.data_ptr(), b.data_ptr()
     nbytes = lib.tg_i8_gemm_workspace_size(pa, lda, pb, ldb, m, n, k) if k < 1 << 17 else 0
@@ -208,7 +208,7 @@ def _backward(which: str, grad_c: torch.Tensor, q: torch.Tensor, scale: torch.Te
     _vector(f"{other}_scale", scale, depth, _F32)
     dev = grad_c.device
     _same_device(dev, "grad_c", **{other: q, f"{other}_scale": scale})
-    out = torch.empty((m if which == "a" else n, k), dtype=grad_c.dtype, device=dev)
+    out = torch.empty(m if which == "a" else n, k, dtype=grad_c.dtype, device=dev)
     lib = nat.load()
     size, run = ((lib.tg_i8_backward_a_workspace_size, lib.tg_i8_backward_a) if which == "a" else
                  (lib.tg_i8_backward_b_workspace_size, lib.tg_i8_backward_b))
