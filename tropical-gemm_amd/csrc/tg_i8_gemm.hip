@@ -34,20 +34,24 @@ hipError_t by_type(int type, F&& f) {
 // ... 8192, N 512 ... 8192, K 512 ... 8192 bytes; 8-bit and bf16 alike, the time
 // goes by bytes): the tile with the least time so reckoned is 0.25% slower
 // than the best one in the mean, 18% at most.
+//
+// `planes`: a step takes that many planes of A (f32 gradients; fitted to 80
+// products, outputs of four bytes among the time).
 struct TileTime {
-    int bm, bn, threads, per_cu;
+    int bm, bn, threads, per_cu, planes;
     double start, step, crowd, round, full;
 };
 constexpr TileTime kTiles[] = {
-    {256, 256, 512, 1, 7.67, 0.987, 0.659, 9.24, 1.359}, {128, 128, 512, 1, 4.00, 0.336, 0.145, 2.31, 0.447},
-    {128, 128, 256, 2, 3.79, 0.417, 0.137, 3.10, 0.848}, {64, 128, 512, 2, 3.16, 0.235, 0.065, 1.53, 0.547},
-    {64, 64, 256, 2, 2.78, 0.197, 0.022, 1.01, 0.336},   {32, 64, 256, 3, 2.67, 0.176, 0.001, 0.74, 0.362},
+    {256, 256, 512, 1, 1, 7.67, 0.987, 0.659, 9.24, 1.359}, {128, 128, 512, 1, 1, 4.00, 0.336, 0.145, 2.31, 0.447},
+    {128, 128, 256, 2, 1, 3.79, 0.417, 0.137, 3.10, 0.848}, {64, 128, 512, 2, 1, 3.16, 0.235, 0.065, 1.53, 0.547},
+    {64, 64, 256, 2, 1, 2.78, 0.197, 0.022, 1.01, 0.336},   {32, 64, 256, 3, 1, 2.67, 0.176, 0.001, 0.74, 0.362},
+    {64, 128, 512, 1, 3, 3.40, 0.396, 0.220, 3.00, 0.620},  {32, 64, 256, 2, 3, 2.90, 0.220, 0.010, 1.75, 0.458},
 };
 constexpr int kTileForms = sizeof(kTiles) / sizeof(kTiles[0]);
 
 struct TilePlan {
     int form, slices;
-    int64_t tiles_m, tiles_n, slice;
+    int64_t tiles_m, tiles_n, slice, steps;
 };
 
 double tile_time(const TileTime& c, int64_t tiles, int64_t steps) {
@@ -66,23 +70,27 @@ double tile_time(const TileTime& c, int64_t tiles, int64_t steps) {
 // Tile and slices of the sum: slices where tiles are few, as long as the time
 // they save outweighs their partial sums' way through memory and the launch
 // that joins them (2.5 us and 4 TB/s).
-TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps, double* time = nullptr) {
-    if (m <= 0 || n <= 0 || steps <= 0) return {0, 1, 0, 0, 1};
-    TilePlan best = {0, 1, ceil_div(m, 256), ceil_div(n, 256), steps};
+//
+// A sum of `planes` planes is `steps` steps of a form that takes all planes in
+// a step, or planes * steps of the largest form, one plane after another.
+TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps, int planes, double* time = nullptr) {
+    if (m <= 0 || n <= 0 || steps <= 0) return {0, 1, 0, 0, 1, 0};
+    TilePlan best = {0, 1, ceil_div(m, 256), ceil_div(n, 256), steps * planes, steps * planes};
     double least = 1e30;
     for (int f = 0; f < kTileForms; ++f) {
         const TileTime& c = kTiles[f];
-        const int64_t tm = ceil_div(m, c.bm), tn = ceil_div(n, c.bn);
+        if (c.planes != planes && f != 0) continue;
+        const int64_t tm = ceil_div(m, c.bm), tn = ceil_div(n, c.bn), all = c.planes == planes ? steps : steps * planes;
         // A launch's thread count stays below 2^32.
         if (tm * tn >= (int64_t(1) << 32) / c.threads) continue;
         for (int s = 1; s <= 32; s *= 2) {
-            const int64_t slice = ceil_div(steps, s);
+            const int64_t slice = ceil_div(all, s);
             if (s > 1 && (tm * tn * s > 512 || slice < 4)) break;
             double t = tile_time(c, tm * tn * s, slice);
             if (s > 1) t += 2.5 + double(s + 1) * double(m) * double(n) * 4 / 4e6;
             if (t < least) {
                 least = t;
-                best = {f, int(ceil_div(steps, slice)), tm, tn, slice};
+                best = {f, int(ceil_div(all, slice)), tm, tn, slice, all};
             }
         }
     }
@@ -122,18 +130,18 @@ hipError_t launch_join(const V* part, int slices, int64_t m, int64_t n, const Ti
     return hipGetLastError();
 }
 
-template <Mma KIND, int WM, int WN, int FM, int FN, int NB, int PER_CU, typename T>
+template <Mma KIND, int WM, int WN, int FM, int FN, int NB, int PER_CU, int P = 1, typename T>
 hipError_t launch_form(TileArgs p, const TilePlan& pl, const TileStore<T>& out, void* part, hipStream_t st) {
-    using Cfg = Tile<KIND, 16, WM, WN, FM, FN, NB>;
+    using Cfg = Tile<KIND, 16, WM, WN, FM, FN, NB, P>;
     const dim3 grid(unsigned(pl.tiles_m * pl.tiles_n), unsigned(pl.slices));
     if (pl.slices == 1) {
-        const auto kernel = &tg_i8_tiles<KIND, 16, WM, WN, FM, FN, NB, PER_CU, T>;
+        const auto kernel = &tg_i8_tiles<KIND, 16, WM, WN, FM, FN, NB, P, PER_CU, T>;
         static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
         if (attr != hipSuccess) return attr;
         hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, out);
         return hipGetLastError();
     }
-    const auto kernel = &tg_i8_tiles_slice<KIND, 16, WM, WN, FM, FN, NB, PER_CU>;
+    const auto kernel = &tg_i8_tiles_slice<KIND, 16, WM, WN, FM, FN, NB, P, PER_CU>;
     static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
     if (attr != hipSuccess) return attr;
     auto* sums = static_cast<typename Cfg::Value*>(part);
@@ -147,6 +155,11 @@ hipError_t launch_tiles(TileArgs p, const TilePlan& pl, const TileStore<T>& out,
     p.tiles_m = int(pl.tiles_m);
     p.tiles_n = int(pl.tiles_n);
     p.slice = int(pl.slice);
+    p.steps = int(pl.steps);
+    if constexpr (KIND == Mma::BF16 && std::is_same<T, float>::value) {
+        if (pl.form == 6) return launch_form<KIND, 2, 4, 2, 2, 2, 1, 3>(p, pl, out, part, st);
+        if (pl.form == 7) return launch_form<KIND, 2, 2, 1, 2, 3, 2, 3>(p, pl, out, part, st);
+    }
     switch (pl.form) {
         case 0: return launch_form<KIND, 2, 4, 8, 4, 2, 1>(p, pl, out, part, st);
         case 1: return launch_form<KIND, 2, 4, 4, 2, 4, 1>(p, pl, out, part, st);
@@ -213,7 +226,7 @@ GemmPlan plan_gemm(const I8Gemm& p) {
     pl.pack_b = !in_place(p.b, p.ldb, p.k);
     pl.ld = round_up(p.k, 128);
     double time = 0;
-    pl.tiles = plan_tiles(p.m, p.n, ceil_div(p.k, 128), &time);
+    pl.tiles = plan_tiles(p.m, p.n, ceil_div(p.k, 128), 1, &time);
     if (pl.pack_a || pl.pack_b) {
         const double bytes = 2 * double(pl.ld) * (double(p.m) * pl.pack_a + double(p.n) * pl.pack_b);
         pl.any = any_time(p) < time + kPackTime + bytes / 4e6 + kOneLaunch;
@@ -275,7 +288,7 @@ hipError_t gemm_typed(const I8Gemm& p, void* ws, hipStream_t st) {
     t.ldb = pl.pack_b ? pl.ld : p.ldb;
     t.m = int(p.m);
     t.n = int(p.n);
-    t.steps = t.b_steps = int(ceil_div(p.k, 128));
+    t.b_steps = int(ceil_div(p.k, 128));
     // A packed row is whole; beside one that is not, it only has to reach as far.
     t.tail = (pl.pack_a && pl.pack_b) || p.k % 128 == 0 ? 128 : int(round_up(p.k % 128, 16));
     if (pl.pack_a || pl.pack_b) {
@@ -294,8 +307,8 @@ hipError_t gemm_typed(const I8Gemm& p, void* ws, hipStream_t st) {
 // multiplied in.  bf16 gradients: q * scale rounded to bf16 (as dequantizing
 // the operand to bf16 does; the result's error is that of its own rounding
 // times sqrt 2).  f16: q * scale * 2^e rounded to f16.  f32: q is exact in
-// bf16; G * scale becomes three bf16 planes that hold all its 24 bits, and the
-// sum runs over the planes.
+// bf16; G * scale becomes three bf16 planes that hold all its 24 bits, each
+// multiplied with q.
 
 struct GradPlan {
     bool pack_g;
@@ -310,7 +323,7 @@ GradPlan plan_grad(const I8Grad& p) {
     pl.planes = p.type == TG_FLOAT32 ? 3 : 1;
     pl.pack_g = p.type == TG_FLOAT32 || p.transposed || !in_place(p.g, p.ldg * size, p.depth * size);
     pl.depth = round_up(p.depth, 64);
-    pl.tiles = plan_tiles(p.rows, p.cols, pl.depth / 64 * pl.planes);
+    pl.tiles = plan_tiles(p.rows, p.cols, pl.depth / 64, pl.planes);
     return pl;
 }
 
@@ -373,7 +386,7 @@ hipError_t grad_typed(const I8Grad& p, void* ws, hipStream_t st) {
     t.m = int(p.rows);
     t.n = int(p.cols);
     t.b_steps = int(pl.depth / 64);
-    t.steps = t.b_steps * pl.planes;
+    t.plane = pl.depth * 2;
     t.tail = pl.pack_g || p.depth % 64 == 0 ? 128 : int(p.depth % 64 * 2);
     return launch_tiles<std::is_same<D, f16_t>::value ? Mma::F16 : Mma::BF16>(t, pl.tiles, out, w.part, st);
 }

@@ -79,6 +79,7 @@ struct TileArgs {
     int steps;          // 128-byte steps of the whole sum
     int tail;           // bytes of the last step that count: a multiple of 16, 16 ... 128
     int b_steps;        // A's step s meets B's step s % b_steps
+    int64_t plane;      // bytes between the planes of a row of A
     int tiles_m, tiles_n;
     int slice;          // steps of one blockIdx.y (tg_i8_tiles_slice)
 };
@@ -102,14 +103,16 @@ struct TileArgs {
 // are taken so that a lane's FN fragments hold VPF FN neighbouring columns of C
 // (whole 16-byte stores); B is the first operand, so that a fragment's values
 // of a lane are neighbours in a row of C.
-template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB>
+//
+// P planes: a row of A is the sum of P rows, each multiplied with B's.
+template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB, int P = 1>
 struct Tile {
     static constexpr int BM = WM * FM * FS, BN = WN * FN * FS, NT = WM * WN * 64;
     static constexpr int KS = FS / 16;       // instructions along half a step
     static constexpr int VPF = FS * FS / 64;  // values of a fragment per lane
-    static constexpr int LOADS_A = BM * 8 / NT, LOADS_B = BN * 8 / NT, LOADS = LOADS_A + LOADS_B;
-    static constexpr int NA = NB + 1, STAGE_A = BM * 128, STAGE_B = BN * 128, LDS = NA * STAGE_A + NB * STAGE_B;
-    static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0 && NT % 64 == 0, "whole loads");
+    static constexpr int LOADS_A = P * BM * 8 / NT, LOADS_B = BN * 8 / NT, LOADS = LOADS_A + LOADS_B;
+    static constexpr int NA = NB + 1, STAGE_A = P * BM * 128, STAGE_B = BN * 128, LDS = NA * STAGE_A + NB * STAGE_B;
+    static_assert(BM * 8 * P % NT == 0 && BN * 8 % NT == 0 && NT % 64 == 0, "whole loads");
     static_assert(NB >= 2 && NB <= 5, "wait_for's cases");
     using Acc = typename MmaAcc<KIND, FS>::type;
     using Value = std::conditional_t<KIND == Mma::I8, int32_t, float>;
@@ -151,8 +154,8 @@ struct Tile {
         auto chunk_b = [&](int i) { return (t % 8) ^ key_b(t / 8 + i * (NT / 8)); };
 #pragma unroll
         for (int i = 0; i < LOADS_A; ++i) {
-            const int r = t / 8 + i * (NT / 8), last = p.m - 1 - tm * BM;
-            off_a[i] = uint32_t(r < last ? r : last) * uint32_t(p.lda) + chunk_a(i) * 16;
+            const int r = (t / 8 + i * (NT / 8)) % BM, k = (t / 8 + i * (NT / 8)) / BM, last = p.m - 1 - tm * BM;
+            off_a[i] = uint32_t(r < last ? r : last) * uint32_t(p.lda) + uint32_t(k) * uint32_t(p.plane) + chunk_a(i) * 16;
         }
 #pragma unroll
         for (int i = 0; i < LOADS_B; ++i) {
@@ -205,15 +208,17 @@ struct Tile {
         const int at_a = row_a * 128 + ((lg ^ key_a(row_a)) << 4);
         const int at_b = NA * STAGE_A + row_b * 128 + ((lg ^ key_b(row_b)) << 4);
         typedef const __attribute__((address_space(3))) u32x4* frag_t;
-        u32x4 xa[2][FM][KS], xb[2][FN][KS];
-        // Part i of FM of a half's fragments, from the stages at (pa, pb).
+        // Row f of A's fragments: plane f % P of fragment f / P.
+        constexpr int ROWS = FM * P;
+        u32x4 xa[2][ROWS][KS], xb[2][FN][KS];
+        // Part i of ROWS of a half's fragments, from the stages at (pa, pb).
         auto read_part = [&](int i, int half, int pa, int pb) {
             const lds_t *from_a = lds + pa, *from_b = lds + pb;
 #pragma unroll
             for (int u = 0; u < KS; ++u)
-                xa[half][i][u] = *reinterpret_cast<frag_t>(from_a + (at_a ^ (half * 64 + u * 32)) + i * FS * 128);
+                xa[half][i][u] = *reinterpret_cast<frag_t>(from_a + (at_a ^ (half * 64 + u * 32)) + (i % P * BM + i / P * FS) * 128);
 #pragma unroll
-            for (int j = i * FN / FM; j < (i + 1) * FN / FM; ++j)
+            for (int j = i * FN / ROWS; j < (i + 1) * FN / ROWS; ++j)
 #pragma unroll
                 for (int u = 0; u < KS; ++u)
                     xb[half][j][u] = *reinterpret_cast<frag_t>(from_b + (at_b ^ (half * 64 + u * 32)) + j * VPF * 128);
@@ -223,19 +228,19 @@ struct Tile {
         // half's reads (done one row before the end, to be there in time).
         auto products = [&](int h, auto reads, auto loads_a, auto loads_b, int pa, int pb) {
 #pragma unroll
-            for (int i = 0; i < FM; ++i) {
+            for (int i = 0; i < ROWS; ++i) {
 #pragma unroll
                 for (int u = 0; u < KS; ++u)
 #pragma unroll
-                    for (int j = 0; j < FN; ++j) acc[i][j] = mma<KIND, FS>(xb[h][j][u], xa[h][i][u], acc[i][j]);
+                    for (int j = 0; j < FN; ++j) acc[i / P][j] = mma<KIND, FS>(xb[h][j][u], xa[h][i][u], acc[i / P][j]);
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (decltype(loads_a)::value)
-                    load_a(i * LOADS_A / FM, (i + 1) * LOADS_A / FM - i * LOADS_A / FM);
+                    load_a(i * LOADS_A / ROWS, (i + 1) * LOADS_A / ROWS - i * LOADS_A / ROWS);
                 if constexpr (decltype(loads_b)::value)
-                    load_b(i * LOADS_B / FM, (i + 1) * LOADS_B / FM - i * LOADS_B / FM);
+                    load_b(i * LOADS_B / ROWS, (i + 1) * LOADS_B / ROWS - i * LOADS_B / ROWS);
                 if constexpr (decltype(reads)::value) {
                     if (i == 0) read_part(0, h ^ 1, pa, pb);
-                    if (i + 1 < FM) read_part(i + 1, h ^ 1, pa, pb);
+                    if (i + 1 < ROWS) read_part(i + 1, h ^ 1, pa, pb);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -246,7 +251,7 @@ struct Tile {
             for (int u = 0; u < KS; ++u)
                 if ((lg + 2 * u + 4 * h) * 16 >= p.tail) {
 #pragma unroll
-                    for (int i = 0; i < FM; ++i) xa[h][i][u] = u32x4{0, 0, 0, 0};
+                    for (int i = 0; i < ROWS; ++i) xa[h][i][u] = u32x4{0, 0, 0, 0};
                 }
         };
         const std::true_type yes;
@@ -261,7 +266,7 @@ struct Tile {
         if (s1 - s0 >= NB) tile_wait<(NB - 1) * LOADS>();
         else tile_wait<0>();
 #pragma unroll
-        for (int i = 0; i < FM; ++i) read_part(i, 0, 0, 0);
+        for (int i = 0; i < ROWS; ++i) read_part(i, 0, 0, 0);
         // Places of this step's and the next one's stages.
         int s = s0, pa = 0, pb = 0, then_a = STAGE_A, then_b = STAGE_B;
         auto step_done = [&] {
@@ -417,20 +422,20 @@ struct TilePartial {
     }
 };
 
-template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB, int PER_CU, typename T>
+template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB, int P, int PER_CU, typename T>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_i8_tiles(TileArgs p, TileStore<T> out) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    Tile<KIND, FS, WM, WN, FM, FN, NB>::whole(p, 0, p.steps, smem, out);
+    Tile<KIND, FS, WM, WN, FM, FN, NB, P>::whole(p, 0, p.steps, smem, out);
 }
 
 // Slice blockIdx.y of the sum: its sums to part + blockIdx.y * M * ld.
-template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB, int PER_CU>
+template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB, int P, int PER_CU>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_i8_tiles_slice(
-    TileArgs p, TilePartial<typename Tile<KIND, FS, WM, WN, FM, FN, NB>::Value> out) {
+    TileArgs p, TilePartial<typename Tile<KIND, FS, WM, WN, FM, FN, NB, P>::Value> out) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int s0 = int(blockIdx.y) * p.slice, s1 = s0 + p.slice < p.steps ? s0 + p.slice : p.steps;
     out.c += int64_t(blockIdx.y) * p.m * out.ld;
-    Tile<KIND, FS, WM, WN, FM, FN, NB>::whole(p, s0, s1, smem, out);
+    Tile<KIND, FS, WM, WN, FM, FN, NB, P>::whole(p, s0, s1, smem, out);
 }
 
 // C from the slices' sums, added in their order (none: an empty sum).
