@@ -477,3 +477,26 @@ def test_numbers_of_a_known_case():
     q, scale = int8.quantize(x)
     assert q.cpu().tolist() == [[127, 0, 2, 2, 0, -2, -127, 126]] and scale.item() == 1.0
     assert np.array_equal(int8.dequantize(q, scale, torch.float32).cpu().numpy(), q.cpu().numpy().astype(np.float32))
+
+
+@pytest.mark.parametrize("m", [4, 5, 16])
+def test_matmul_wide(m):
+    """More columns than the kernel for few rows takes, aligned rows and not."""
+    n, k = 12300, 144
+    for ldb, off in ((k, 0), (k + 1, 1)):
+        _say("matmul wide", m, n, k, ldb, off)
+        a, sa = _int8(1, m, k, full=True)
+        b, sb = _int8(2, n, k, ldb, off, full=True)
+        _check_matmul(int8.matmul(a, sa, b, sb), a, sa, b, sb, None, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+def test_gradients_of_long_sums(dtype):
+    """Few outputs and a long sum, which is cut into slices."""
+    m, n, k = 5000, 40, 72
+    g = _values(1, m, n, dtype)
+    a, sa = _int8(2, m, k)
+    f64 = lambda t: t.cpu().double()  # noqa: E731
+    _check_grad(int8.backward_b(g, a, sa), f64(g).t(), f64(a) * f64(sa)[:, None], dtype)
+    again = int8.backward_b(g, a, sa)
+    assert torch.equal(again, int8.backward_b(g, a, sa))

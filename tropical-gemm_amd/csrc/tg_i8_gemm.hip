@@ -69,7 +69,8 @@ double tile_time(const TileTime& c, int64_t tiles, int64_t steps) {
 
 // Tile and slices of the sum: slices where tiles are few, as long as the time
 // they save outweighs their partial sums' way through memory and the launch
-// that joins them (2.5 us and 4 TB/s).
+// that joins them (4.5 us and 4 TB/s; N = 256, K = 8192, M = 16: 9.8 us in
+// slices, 13.9 without).
 //
 // A sum of `planes` planes is `steps` steps of a form that takes all planes in
 // a step, or planes * steps of the largest form, one plane after another.
@@ -87,7 +88,7 @@ TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps, int planes, double* tim
             const int64_t slice = ceil_div(all, s);
             if (s > 1 && (tm * tn * s > 512 || slice < 4)) break;
             double t = tile_time(c, tm * tn * s, slice);
-            if (s > 1) t += 2.5 + double(s + 1) * double(m) * double(n) * 4 / 4e6;
+            if (s > 1) t += 4.5 + double(s + 1) * double(m) * double(n) * 4 / 4e6;
             if (t < least) {
                 least = t;
                 best = {f, int(ceil_div(all, slice)), tm, tn, slice, all};
@@ -188,9 +189,15 @@ struct Carver {
 
 // ---- the 8-bit product ---------------------------------------------------
 
-// Up to 16 rows of A take the kernel that streams B: M = 16 against a tile of
-// 32 x 64, N = K = 8192: 17 us against 18, and rows of any alignment.
-constexpr int64_t kStreamRows = 16;
+// Up to 16 rows of A take the kernel that streams B, rows of any alignment: M =
+// 16, N = K = 4096: 6.9 us against 8.4 with tiles; M = 1, N = K = 8192: 14.4
+// against 16.7.  Its reads of A count where there are more than a few rows,
+// and a wide matrix fills the GPU with tiles: M = 16, N = 28672, K = 8192: 60 us
+// against 44 with tiles (M = 4: 42 and 45; N = 8192: 17.8 and 17.3).
+bool streams(const I8Gemm& p) {
+    if (p.m > 16) return false;
+    return p.m <= 4 || p.n <= 12288 || !in_place(p.a, p.lda, p.k) || !in_place(p.b, p.ldb, p.k);
+}
 
 struct GemmPlan {
     bool stream, any, pack_a, pack_b;
@@ -220,7 +227,7 @@ double any_time(const I8Gemm& p) {
 
 GemmPlan plan_gemm(const I8Gemm& p) {
     GemmPlan pl{};
-    pl.stream = p.m <= kStreamRows;
+    pl.stream = streams(p);
     if (pl.stream) return pl;
     pl.pack_a = !in_place(p.a, p.lda, p.k);
     pl.pack_b = !in_place(p.b, p.ldb, p.k);

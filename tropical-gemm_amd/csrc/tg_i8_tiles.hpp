@@ -114,6 +114,7 @@ struct Tile {
     static constexpr int NA = NB + 1, STAGE_A = P * BM * 128, STAGE_B = BN * 128, LDS = NA * STAGE_A + NB * STAGE_B;
     static_assert(BM * 8 * P % NT == 0 && BN * 8 % NT == 0 && NT % 64 == 0, "whole loads");
     static_assert(NB >= 2 && NB <= 5, "wait_for's cases");
+    static_assert(FN >= 2, "work between two products");
     using Acc = typename MmaAcc<KIND, FS>::type;
     using Value = std::conditional_t<KIND == Mma::I8, int32_t, float>;
 
@@ -223,25 +224,31 @@ struct Tile {
                 for (int u = 0; u < KS; ++u)
                     xb[half][j][u] = *reinterpret_cast<frag_t>(from_b + (at_b ^ (half * 64 + u * 32)) + j * VPF * 128);
         };
-        // Multiplies the fragments of half h, row by row.  Behind each row's
-        // products come its parts of a later step's loads and of the next
+        // Multiplies the fragments of half h, row by row.  Between each row's
+        // products go its parts of a later step's loads and of the next
         // half's reads (done one row before the end, to be there in time).
         auto products = [&](int h, auto reads, auto loads_a, auto loads_b, int pa, int pb) {
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
+                auto product = [&](int j) {
 #pragma unroll
-                for (int u = 0; u < KS; ++u)
-#pragma unroll
-                    for (int j = 0; j < FN; ++j) acc[i / P][j] = mma<KIND, FS>(xb[h][j][u], xa[h][i][u], acc[i / P][j]);
+                    for (int u = 0; u < KS; ++u)
+                        acc[i / P][j] = mma<KIND, FS>(xb[h][j][u], xa[h][i][u], acc[i / P][j]);
+                };
+                product(0);
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (decltype(loads_a)::value)
                     load_a(i * LOADS_A / ROWS, (i + 1) * LOADS_A / ROWS - i * LOADS_A / ROWS);
                 if constexpr (decltype(loads_b)::value)
                     load_b(i * LOADS_B / ROWS, (i + 1) * LOADS_B / ROWS - i * LOADS_B / ROWS);
+                product(1);
+                __builtin_amdgcn_sched_barrier(0);
                 if constexpr (decltype(reads)::value) {
                     if (i == 0) read_part(0, h ^ 1, pa, pb);
                     if (i + 1 < ROWS) read_part(i + 1, h ^ 1, pa, pb);
                 }
+#pragma unroll
+                for (int j = 2; j < FN; ++j) product(j);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
