@@ -377,8 +377,23 @@ int tg_i8_gemm(int device, tg_float type, const int8_t* a, int64_t lda, const fl
                int64_t m, int64_t n, int64_t k, void* workspace, size_t workspace_bytes,
                void* stream);
 
+/* Name of the way tg_i8_gemm takes for these operands, e.g. "stream waves 16"
+ * (up to 16 rows: b is streamed into registers), "any" (one launch for
+ * unaligned rows), "tiles 256x256", "tiles 64x64 per_cu 2 slices 4 pack a"
+ * (the sum in four slices that are joined afterwards, a laid out first);
+ * "invalid" for arguments the call would reject.  Host logic only, as
+ * tg_gemm_plan: pointers are checked for alignment.  tg_i8_backward_plan is
+ * the same for grad_a (want_a not 0) or grad_b. */
+const char* tg_i8_gemm_plan(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, int64_t m,
+                            int64_t n, int64_t k);
+const char* tg_i8_backward_plan(tg_float type, int want_a, const void* grad_c, int64_t ldg,
+                                int64_t m, int64_t n, int64_t k);
+
 /* grad_a[i, k] = sum_j grad_c[i, j] * b_scale[j] * b[j, k]: the gradient of
- * a[i, k] * a_scale[i].  grad_c is m x n and grad_a m x k, of type. */
+ * a[i, k] * a_scale[i].  grad_c is m x n and grad_a m x k, of type.  The sum
+ * (over n; over m for grad_b) has at most 2^20 terms.  For bf16 and f16 the
+ * dequantized b * b_scale is rounded to that type, for f32 nothing is rounded
+ * but the f32 sums. */
 size_t tg_i8_backward_a_workspace_size(tg_float type, const void* grad_c, int64_t ldg, int64_t m,
                                        int64_t n, int64_t k);
 int tg_i8_backward_a(int device, tg_float type, const void* grad_c, int64_t ldg, const int8_t* b,

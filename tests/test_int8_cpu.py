@@ -127,3 +127,58 @@ def test_python_layer_refuses_host_tensors():
                  lambda: int8.backward_a(x[:, :2], q, s), lambda: int8.backward_b(x, q, s)):
         with pytest.raises(ValueError, match="need device tensors"):
             call()
+
+
+def _gemm_plan(m, n, k, lda=None, ldb=None, a=P, b=P):
+    return nat.load().tg_i8_gemm_plan(a, lda or k, b, ldb or k, m, n, k).decode()
+
+
+def _grad_plan(kind, want_a, m, n, k, ldg=None, g=P):
+    return nat.load().tg_i8_backward_plan(nat.FLOAT[kind], want_a, g, ldg or n, m, n, k).decode()
+
+
+@pytest.mark.parametrize("args,plan", [
+    ((1, 8192, 8192), "stream waves 16"),
+    ((13, 5003, 4099), "stream waves 16"),
+    ((4, 28672, 8192), "stream waves 8"),
+    ((16, 28672, 8192), "tiles 32x64 per_cu 3"),
+    ((16, 28672, 8191), "stream waves 8"),
+    ((8192, 8192, 8192), "tiles 256x256"),
+    ((512, 4096, 4096), "tiles 64x128 per_cu 2"),
+    ((2048, 2048, 2048), "tiles 128x128"),
+    ((2048, 4096, 2048), "tiles 128x128 per_cu 2"),
+    ((1024, 1024, 1024), "tiles 64x64 per_cu 2"),
+    ((32, 4096, 512), "tiles 32x64 per_cu 3"),
+    ((64, 256, 16384), "tiles 32x64 per_cu 3 slices 32"),
+    ((300, 500, 701), "any"),
+    ((8191, 8191, 8191), "tiles 256x256 pack a pack b"),
+    ((0, 8, 16), "none"),
+    ((8, 8, 0), "bias"),
+    ((8, 8, -1), "invalid"),
+    ((8, 8, 1 << 17), "invalid"),
+])
+def test_gemm_plans(args, plan):
+    assert _gemm_plan(*args) == plan
+
+
+def test_gemm_plans_of_strides():
+    assert _gemm_plan(8192, 8192, 8192, lda=8200) == "tiles 256x256 pack a"
+    assert _gemm_plan(8192, 8192, 8192, b=P + 8) == "tiles 256x256 pack b"
+    assert _gemm_plan(8192, 8192, 8192, ldb=1 << 23) == "tiles 256x256 pack b"
+    assert _gemm_plan(8, 8, 16, lda=15) == "invalid"
+
+
+@pytest.mark.parametrize("kind,want_a,args,plan", [
+    ("bf16", 1, (8192, 4096, 4096), "tiles 256x256"),
+    ("bf16", 0, (8192, 4096, 4096), "tiles 256x256 pack grad_c"),
+    ("f16", 1, (8192, 4095, 4096), "tiles 256x256 pack grad_c"),
+    ("f32", 1, (8192, 4096, 4096), "tiles 256x256 pack grad_c"),
+    ("f32", 1, (301, 1031, 2049), "tiles 32x64 per_cu 2 planes 3 pack grad_c"),
+    ("f32", 0, (1024, 2048, 2048), "tiles 64x128 planes 3 pack grad_c"),
+    ("bf16", 0, (8192, 64, 64), "tiles 32x64 per_cu 3 slices 32 pack grad_c"),
+    ("bf16", 1, (8, 0, 16), "zero"),
+    ("bf16", 1, (0, 8, 16), "none"),
+    ("bf16", 0, ((1 << 20) + 1, 8, 16), "invalid"),
+])
+def test_gradient_plans(kind, want_a, args, plan):
+    assert _grad_plan(kind, want_a, *args) == plan

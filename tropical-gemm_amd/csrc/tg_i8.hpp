@@ -56,6 +56,7 @@ struct I8Gemm {
 };
 size_t i8_gemm_ws(const I8Gemm& p);
 hipError_t i8_gemm(const I8Gemm& p, void* ws, hipStream_t st);
+std::string i8_gemm_plan(const I8Gemm& p);
 
 // out (rows x cols) = sum over r < depth of G(i, r) * scale[r] * q[r, j], with
 // G(i, r) = g[i * ldg + r], or g[r * ldg + i] when `transposed`.
@@ -72,5 +73,6 @@ struct I8Grad {
 };
 size_t i8_grad_ws(const I8Grad& p);
 hipError_t i8_grad(const I8Grad& p, void* ws, hipStream_t st);
+std::string i8_grad_plan(const I8Grad& p);
 
 }  // namespace tg

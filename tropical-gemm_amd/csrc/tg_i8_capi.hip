@@ -133,6 +133,18 @@ tg::I8Grad grad_b(tg_float type, const void* grad_c, int64_t ldg, const int8_t* 
     return {type, grad_c, ldg, true, a, lda, a_scale, out, n, k, m};
 }
 
+// A plan's name, the thread's until its next one.
+template <typename F>
+const char* named(F&& f) noexcept {
+    try {
+        static thread_local std::string name;
+        name = f();
+        return name.c_str();
+    } catch (...) {
+        return "invalid";
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -236,6 +248,19 @@ int tg_i8_gemm(int device, tg_float type, const int8_t* a, int64_t lda, const fl
         TG_CHECK(check_ws(tg::i8_gemm_ws(p), workspace, workspace_bytes));
         return launched(device, "tg_i8_gemm", [&] { return tg::i8_gemm(p, workspace, as_stream(stream)); });
     });
+}
+
+const char* tg_i8_gemm_plan(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, int64_t m, int64_t n,
+                            int64_t k) {
+    const tg::I8Gemm p{TG_BF16, a, lda, nullptr, b, ldb, nullptr, nullptr, nullptr, m, n, k};
+    return named([&] { return check_gemm(p) == TG_OK ? tg::i8_gemm_plan(p) : std::string("invalid"); });
+}
+
+const char* tg_i8_backward_plan(tg_float type, int want_a, const void* grad_c, int64_t ldg, int64_t m, int64_t n,
+                                int64_t k) {
+    const tg::I8Grad p = want_a != 0 ? grad_a(type, grad_c, ldg, nullptr, k, nullptr, nullptr, m, n, k)
+                                     : grad_b(type, grad_c, ldg, nullptr, k, nullptr, nullptr, m, n, k);
+    return named([&] { return check_grad(p, "q") == TG_OK ? tg::i8_grad_plan(p) : std::string("invalid"); });
 }
 
 size_t tg_i8_backward_a_workspace_size(tg_float type, const void* grad_c, int64_t ldg, int64_t m, int64_t n,

@@ -262,6 +262,11 @@ PackBytes bytes_job(const void* src, int64_t ld_src, int64_t rows, int64_t bytes
     return {static_cast<const int8_t*>(src), ld_src, rows, int(bytes), static_cast<int8_t*>(dst), ld};
 }
 
+// Waves of a workgroup of tg_i8_stream: 16 while the GPU holds all workgroups
+// at once (M = 13, K = 8192: N = 8192 17.2 us against 18.4 with 8; N = 28672 60
+// against 56).
+int stream_waves(int64_t n) { return n <= 16384 ? 16 : 8; }
+
 template <int W, typename T>
 hipError_t launch_stream(const I8Gemm& p, const TileStore<T>& out, hipStream_t st) {
     auto words = [](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 4 == 0 && ld % 4 == 0; };
@@ -276,12 +281,7 @@ hipError_t gemm_typed(const I8Gemm& p, void* ws, hipStream_t st) {
     const TileStore<T> out{p.a_scale, p.b_scale, nullptr, static_cast<const T*>(p.bias), static_cast<T*>(p.c), p.n};
     if (p.k == 0) return launch_join<int32_t>(nullptr, 0, p.m, p.n, out, st);
     const GemmPlan pl = plan_gemm(p);
-    if (pl.stream) {
-        // 16 waves a workgroup while the GPU holds all of them at once (M =
-        // 13, K = 8192: N = 8192 17.2 us against 18.4 with 8; N = 28672 60
-        // against 56).
-        return p.n <= 16384 ? launch_stream<16>(p, out, st) : launch_stream<8>(p, out, st);
-    }
+    if (pl.stream) return stream_waves(p.n) == 16 ? launch_stream<16>(p, out, st) : launch_stream<8>(p, out, st);
     if (pl.any) {
         const AnyArgs args{p.a, p.lda, p.b, p.ldb, int(p.m), int(p.n), int(p.k), int(ceil_div(p.m, 64)), int(ceil_div(p.n, 64))};
         hipLaunchKernelGGL((tg_i8_any<T>), dim3(unsigned(args.tiles_m * args.tiles_n)), dim3(256), 0, st, args, out);
@@ -398,7 +398,33 @@ hipError_t grad_typed(const I8Grad& p, void* ws, hipStream_t st) {
     return launch_tiles<std::is_same<D, f16_t>::value ? Mma::F16 : Mma::BF16>(t, pl.tiles, out, w.part, st);
 }
 
+// The tiles' part of a plan's name.
+std::string tiles_name(const TilePlan& pl) {
+    const TileTime& c = kTiles[pl.form];
+    std::string name = "tiles " + std::to_string(c.bm) + "x" + std::to_string(c.bn);
+    if (c.per_cu > 1) name += " per_cu " + std::to_string(c.per_cu);
+    if (c.planes > 1) name += " planes " + std::to_string(c.planes);
+    if (pl.slices > 1) name += " slices " + std::to_string(pl.slices);
+    return name;
+}
+
 }  // namespace
+
+std::string i8_gemm_plan(const I8Gemm& p) {
+    if (p.m == 0 || p.n == 0) return "none";
+    if (p.k == 0) return "bias";
+    const GemmPlan pl = plan_gemm(p);
+    if (pl.stream) return "stream waves " + std::to_string(stream_waves(p.n));
+    if (pl.any) return "any";
+    return tiles_name(pl.tiles) + (pl.pack_a ? " pack a" : "") + (pl.pack_b ? " pack b" : "");
+}
+
+std::string i8_grad_plan(const I8Grad& p) {
+    if (p.rows == 0 || p.cols == 0) return "none";
+    if (p.depth == 0) return "zero";
+    const GradPlan pl = plan_grad(p);
+    return tiles_name(pl.tiles) + (pl.pack_g ? " pack grad_c" : "");
+}
 
 size_t i8_gemm_ws(const I8Gemm& p) { return carve_gemm(p, plan_gemm(p), nullptr).bytes; }
 

@@ -92,60 +92,65 @@ __device__ __forceinline__ void split_value(float v, D (&d)[PLANES]) {
 // Transposes: dst[c][r] = src[r][c] * scale[r] * factor in type D (scale and
 // factor may be null), rows of dst of PLANES planes of `depth` (a multiple of
 // 64, at least rows) elements, zeros from r = rows on.  A workgroup takes 64
-// rows by 64 columns through LDS: pairs of rows are written there as words of
-// two, 33 words a column, so that a wave's 8 x 8 words meet 64 banks.  Bound by
-// memory (8192 x 4096 from 8 to 16 bits: 100 MB in 24 us).
+// rows by 128 bytes of them (at least 64 columns), whole lines both ways,
+// through LDS: pairs of rows are written there as words of two, 33 words a
+// column, so that the words of 8 x 8 lanes meet 64 banks.  Bound by memory.
 template <typename S, typename D, int PLANES>
 struct PackTurned {
     static_assert(sizeof(D) == 2, "pairs are words");
+    static constexpr int COLS = sizeof(S) == 1 ? 128 : 64, GROUPS = COLS / 8, PASSES = GROUPS * 32 / 256;
     const S* src;
     int64_t ld_src, rows, cols;
     const float *scale, *factor;
     D* dst;
     int64_t depth;
-    static constexpr int kLdsWords = PLANES * 64 * 33;
-    int64_t blocks() const { return depth / 64 * pack_ceil(cols, 64); }
-    __device__ __forceinline__ void run(int block, int, uint32_t* lds) const {
-        uint32_t(*tile)[64][33] = reinterpret_cast<uint32_t(*)[64][33]>(lds);
+    static constexpr int kLdsWords = PLANES * COLS * 33;
+    int64_t blocks() const { return depth / 64 * pack_ceil(cols, COLS); }
+    __device__ __forceinline__ void run(int block, int count, uint32_t* lds) const {
+        uint32_t(*tile)[COLS][33] = reinterpret_cast<uint32_t(*)[COLS][33]>(lds);
         const int t = threadIdx.x, tiles_r = int(depth / 64);
-        const int64_t r0 = int64_t(block % tiles_r) * 64, c0 = int64_t(block / tiles_r) * 64;
-        {
-            const int cg = t % 8, rp = t / 8;
-            const int64_t c = c0 + cg * 8;
-            const int left = cols - c < 8 ? int(cols - c) : 8;
-            float v[2][8] = {};
+        block = xcd_run(block, count);
+        const int64_t r0 = int64_t(block % tiles_r) * 64, c0 = int64_t(block / tiles_r) * COLS;
+        float v[PASSES][2][8] = {};
+        const int cg = t % GROUPS;
+        const int64_t c = c0 + cg * 8;
+        const int left = cols - c < 8 ? int(cols - c) : 8;
+#pragma unroll
+        for (int pass = 0; pass < PASSES; ++pass)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int64_t r = r0 + rp * 2 + h;
+                const int64_t r = r0 + (pass * (256 / GROUPS) + t / GROUPS) * 2 + h;
                 if (r >= rows || left <= 0) continue;
-                if constexpr (sizeof(S) == 1) load_i8_upto8(src + r * ld_src + c, left, v[h]);
-                else load_upto8(src + r * ld_src + c, left, v[h]);
+                if constexpr (sizeof(S) == 1) load_i8_upto8(src + r * ld_src + c, left, v[pass][h]);
+                else load_upto8(src + r * ld_src + c, left, v[pass][h]);
                 if (scale != nullptr) {
                     const float s = factor != nullptr ? scale[r] * factor[0] : scale[r];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[h][i] *= s;
+                    for (int i = 0; i < 8; ++i) v[pass][h][i] *= s;
                 }
             }
 #pragma unroll
+        for (int pass = 0; pass < PASSES; ++pass)
+#pragma unroll
             for (int i = 0; i < 8; ++i) {
                 D lo[PLANES], hi[PLANES];
-                split_value<D, PLANES>(v[0][i], lo);
-                split_value<D, PLANES>(v[1][i], hi);
+                split_value<D, PLANES>(v[pass][0][i], lo);
+                split_value<D, PLANES>(v[pass][1][i], hi);
 #pragma unroll
                 for (int p = 0; p < PLANES; ++p)
-                    tile[p][cg * 8 + i][rp] = uint32_t(__builtin_bit_cast(uint16_t, lo[p])) |
-                                              uint32_t(__builtin_bit_cast(uint16_t, hi[p])) << 16;
+                    tile[p][cg * 8 + i][pass * (256 / GROUPS) + t / GROUPS] =
+                        uint32_t(__builtin_bit_cast(uint16_t, lo[p])) |
+                        uint32_t(__builtin_bit_cast(uint16_t, hi[p])) << 16;
             }
-        }
         __syncthreads();
 #pragma unroll
         for (int p = 0; p < PLANES; ++p)
 #pragma unroll
-            for (int pass = 0; pass < 2; ++pass) {
-                const int c = pass * 32 + t / 8, w = t % 8 * 4;
-                if (c0 + c >= cols) continue;
-                const u32x4 v = {tile[p][c][w], tile[p][c][w + 1], tile[p][c][w + 2], tile[p][c][w + 3]};
-                *reinterpret_cast<u32x4*>(dst + ((c0 + c) * PLANES + p) * depth + r0 + w * 2) = v;
+            for (int pass = 0; pass < COLS / 32; ++pass) {
+                const int k = pass * 32 + t / 8, w = t % 8 * 4;
+                if (c0 + k >= cols) continue;
+                const u32x4 x = {tile[p][k][w], tile[p][k][w + 1], tile[p][k][w + 2], tile[p][k][w + 3]};
+                *reinterpret_cast<u32x4*>(dst + ((c0 + k) * PLANES + p) * depth + r0 + w * 2) = x;
             }
     }
 };

@@ -123,13 +123,10 @@ struct Tile {
         return FS == 16 ? (r & 3) | (r / (VPF * FN) & 1) << 2 : r / 2 & 7;
     }
 
-    // The workgroup's tile: consecutive workgroups go round the 8 XCDs, so
-    // each XCD takes a contiguous run of tiles, in bands of 8 tile rows, whose
-    // panels its L2 then holds.
+    // The workgroup's tile: each XCD takes a run of tiles in bands of 8 tile
+    // rows, whose panels its L2 then holds.
     static __device__ __forceinline__ void place(const TileArgs& p, int& tm, int& tn) {
-        const int total = p.tiles_m * p.tiles_n, per = total / 8, rest = total % 8;
-        const int x = int(blockIdx.x) % 8;
-        int id = x * per + (x < rest ? x : rest) + int(blockIdx.x) / 8;
+        int id = xcd_run(int(blockIdx.x), p.tiles_m * p.tiles_n);
         const int band = id / (8 * p.tiles_n);
         const int height = p.tiles_m - band * 8 < 8 ? p.tiles_m - band * 8 : 8;
         id -= band * 8 * p.tiles_n;

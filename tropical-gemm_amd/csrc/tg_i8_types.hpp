@@ -126,4 +126,11 @@ __device__ __forceinline__ float wave_max(float x) {
     return x;
 }
 
+// Workgroup `id` of `count`, renumbered so that each of the 8 XCDs, round which
+// consecutive workgroups go, takes a run of neighbours.
+__device__ __forceinline__ int xcd_run(int id, int count) {
+    const int per = count / 8, rest = count % 8, x = id % 8;
+    return x * per + (x < rest ? x : rest) + id / 8;
+}
+
 }  // namespace tg

@@ -92,6 +92,8 @@ SIGNATURES = {
     "tg_i8_gemm_workspace_size": ([_vp, _i64, _vp, _i64, _i64, _i64, _i64], _sz),
     "tg_i8_gemm": ([_i32, _i32, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _sz,
                     _vp], _i32),
+    "tg_i8_gemm_plan": ([_vp, _i64, _vp, _i64, _i64, _i64, _i64], ctypes.c_char_p),
+    "tg_i8_backward_plan": ([_i32, _i32, _vp, _i64, _i64, _i64, _i64], ctypes.c_char_p),
     "tg_i8_backward_a_workspace_size": ([_i32, _vp, _i64, _i64, _i64, _i64], _sz),
     "tg_i8_backward_a": ([_i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz,
                           _vp], _i32),
