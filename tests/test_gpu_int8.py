@@ -77,7 +77,7 @@ def _check_rows(q, scale, want):
     assert (q64[~live] == 0).all()
 
 
-COLS = [1, 7, 8, 64, 511, 512, 513, 2048, 2051, 4096, 8192, 8200, 40001]
+COLS = [1, 7, 8, 9, 64, 511, 512, 513, 1024, 1025, 2048, 2051, 2501, 3081, 4096, 5003, 6145, 8185, 8192, 8200, 40001]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)

@@ -26,7 +26,7 @@ struct AnyArgs {
 // Bound by the loads' latency.
 template <typename T>
 __global__ __launch_bounds__(256) void tg_i8_any(AnyArgs p, TileStore<T> out) {
-    using Cfg = Tile<Mma::I8, 16, 2, 2, 2, 2, 2>;
+    using Cfg = Tile<Mma::I8, 2, 2, 2, 2, 2>;
     constexpr int STAGE = Cfg::STAGE_A + Cfg::STAGE_B;
     __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
     lds_t* lds = (lds_t*)(smem);
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void tg_i8_any(AnyArgs p, TileStore<T> out) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = mma<Mma::I8, 16>(xb[j], xa[i], acc[i][j]);
+                for (int j = 0; j < 2; ++j) acc[i][j] = mma<Mma::I8>(xb[j], xa[i], acc[i][j]);
         }
     };
 

@@ -95,6 +95,10 @@ constexpr int64_t kMostK = (int64_t(1) << 17) - 1;
 // The operands laid out along the sum have row strides below 2^23 bytes.
 constexpr int64_t kMostDepth = int64_t(1) << 20;
 
+// The norm's backward pass counts a row's elements in f32 and has 64 threads
+// for each column of its widest launch.
+constexpr int64_t kMostBackwardCols = int64_t(1) << 24;
+
 int check_gemm(const tg::I8Gemm& p) {
     TG_CHECK(check_type(p.type));
     TG_CHECK(check_dims({p.m, p.n, p.k}));
@@ -213,6 +217,7 @@ int tg_i8_rms_norm_backward(int device, tg_float type, tg_float weight_type, con
         TG_CHECK(check_ld("h", ldh, cols));
         if (grad_h != nullptr) TG_CHECK(check_ld("grad_h", ldgh, cols));
         TG_CHECK(check_eps(eps));
+        if (cols > kMostBackwardCols) return bad_size("cols is " + std::to_string(cols) + ": at most 2^24 are supported");
         const bool any = rows > 0 && cols > 0;
         TG_CHECK(check_ptr("grad_y", grad_y, any));
         TG_CHECK(check_ptr("h", h, any));

@@ -133,16 +133,16 @@ hipError_t launch_join(const V* part, int slices, int64_t m, int64_t n, const Ti
 
 template <Mma KIND, int WM, int WN, int FM, int FN, int NB, int PER_CU, int P = 1, typename T>
 hipError_t launch_form(TileArgs p, const TilePlan& pl, const TileStore<T>& out, void* part, hipStream_t st) {
-    using Cfg = Tile<KIND, 16, WM, WN, FM, FN, NB, P>;
+    using Cfg = Tile<KIND, WM, WN, FM, FN, NB, P>;
     const dim3 grid(unsigned(pl.tiles_m * pl.tiles_n), unsigned(pl.slices));
     if (pl.slices == 1) {
-        const auto kernel = &tg_i8_tiles<KIND, 16, WM, WN, FM, FN, NB, P, PER_CU, T>;
+        const auto kernel = &tg_i8_tiles<KIND, WM, WN, FM, FN, NB, P, PER_CU, T>;
         static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
         if (attr != hipSuccess) return attr;
         hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, out);
         return hipGetLastError();
     }
-    const auto kernel = &tg_i8_tiles_slice<KIND, 16, WM, WN, FM, FN, NB, P, PER_CU>;
+    const auto kernel = &tg_i8_tiles_slice<KIND, WM, WN, FM, FN, NB, P, PER_CU>;
     static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
     if (attr != hipSuccess) return attr;
     auto* sums = static_cast<typename Cfg::Value*>(part);
@@ -193,9 +193,10 @@ struct Carver {
 // 16, N = K = 4096: 6.9 us against 8.4 with tiles; M = 1, N = K = 8192: 14.4
 // against 16.7.  Its reads of A count where there are more than a few rows,
 // and a wide matrix fills the GPU with tiles: M = 16, N = 28672, K = 8192: 60 us
-// against 44 with tiles (M = 4: 42 and 45; N = 8192: 17.8 and 17.3).
+// against 44 with tiles (M = 4: 42 and 45; N = 8192: 17.8 and 17.3).  (A launch's
+// thread count stays below 2^32.)
 bool streams(const I8Gemm& p) {
-    if (p.m > 16) return false;
+    if (p.m > 16 || p.n >= int64_t(1) << 27) return false;
     return p.m <= 4 || p.n <= 12288 || !in_place(p.a, p.lda, p.k) || !in_place(p.b, p.ldb, p.k);
 }
 

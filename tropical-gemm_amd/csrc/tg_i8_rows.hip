@@ -47,12 +47,40 @@ __device__ __forceinline__ void row_reduce(float& sum, float& top) {
     }
 }
 
+// A group of eight elements as it is loaded.
+template <typename T>
+struct Eight {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    t8 v;
+    // The eight from p on, at any address.
+    __device__ __forceinline__ void load(const T* p) {
+        typedef uint32_t words __attribute__((ext_vector_type(sizeof(T) * 2)));
+        typedef uint32_t words_any __attribute__((ext_vector_type(sizeof(T) * 2), aligned(sizeof(T))));
+        v = __builtin_bit_cast(t8, words(*reinterpret_cast<const words_any*>(p)));
+    }
+    // The first `left` of them, zeros behind.
+    __device__ __forceinline__ void load(const T* p, int64_t left) {
+        if (left >= 8) {
+            load(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : T(0.0f);
+        }
+    }
+};
+
 // h = round(x + residual); rstd = (mean h^2 + eps)^-1/2; v = h * w;
 // top = max(max |v|, tiny); q = rint(v * 127 / top); scale = top * rstd / 127.
 // rstd cancels in q, so q depends on no order of summation, and both
 // reductions of the row are made in one pass.  NORM false: v = x, rstd = 1.
 // A NaN or infinity makes the row's scale NaN or infinite with zeros in q, so
 // its values are NaN, as dividing by the row's maximum gives them.
+//
+// VPT > 0, for rows of at least eight elements: all loads of a thread are
+// issued before the first is used.  A group that would end past the row is
+// moved back to end with it, so that no load depends on a branch; the elements
+// it shares with the group before it are written twice, with the same values,
+// and counted once.
 // VPT 0: rows of any length, read again (through L2) after the reduction.
 template <typename T, typename W, bool NORM, bool RES, int NT, int VPT>
 __global__ __launch_bounds__(kBlock<NT>) void tg_i8_rows(const T* __restrict__ x, int64_t ldx,
@@ -68,78 +96,109 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_i8_rows(const T* __restrict__ x
     const T* rr = RES ? res + row * ldr : nullptr;
     float sum = 0.0f, top = 0.0f;
 
-    // One group: the (rounded) stream and its weighted values.
-    auto take = [&](int64_t at, float(&v)[8], bool first) {
-        const int n = cols - at < 8 ? int(cols - at) : 8;
-        load_upto8(xr + at, n, v);
-        if constexpr (RES) {
-            float r[8];
-            load_upto8(rr + at, n, r);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_f32(static_cast<T>(v[i] + r[i]));
-            if (first) store_upto8(h + row * cols + at, n, v);
-        }
-        if constexpr (NORM) {
-            float g[8];
-            load_upto8(w + at, n, g);
-            if (first) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum += v[i] * v[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= g[i];
-        }
-        if (first) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[i]));
-        }
-    };
-    auto give = [&](int64_t at, const float(&v)[8], float inv) {
+    auto give = [&](int64_t at, int n, const float(&v)[8], float inv) {
         int o[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int r = __float2int_rn(v[i] * inv);
             o[i] = r > 127 ? 127 : (r < -127 ? -127 : r);
         }
-        store_i8_upto8(q + row * cols + at, cols - at < 8 ? int(cols - at) : 8, o);
+        store_i8_upto8(q + row * cols + at, n, o);
+    };
+    // Reduces the row, stores its scale and gives 127 / top.
+    auto reduce = [&] {
+        row_reduce<NT>(sum, top);
+        top = max_nan(top, kI8TinyTop);
+        if (live && t == 0) {
+            if constexpr (NORM) {
+                const float rstd = 1.0f / sqrtf(sum / float(cols > 0 ? cols : 1) + eps);
+                scale[row] = top * rstd / 127.0f;
+            } else {
+                scale[row] = top / 127.0f;
+            }
+        }
+        return 127.0f / top;
     };
 
-    constexpr int G = VPT > 0 ? VPT : 1;
-    float v[G][8];
-    if (live) {
-        if constexpr (VPT > 0) {
+    if constexpr (VPT > 0) {
+        float v[VPT][8];
+        auto start = [&](int g) { return int64_t(g * NT + t) * 8; };
+        auto from = [&](int g) { return start(g) <= cols - 8 ? start(g) : cols - 8; };
+        if (live) {
+            Eight<T> a[VPT], b[VPT];
+            Eight<W> f[VPT];
 #pragma unroll
             for (int g = 0; g < VPT; ++g) {
-                const int64_t at = int64_t(g * NT + t) * 8;
-                if (at < cols) take(at, v[g], true);
+                a[g].load(xr + from(g));
+                if constexpr (RES) b[g].load(rr + from(g));
             }
-        } else {
-            for (int64_t at = int64_t(t) * 8; at < cols; at += NT * 8) take(at, v[0], true);
-        }
-    }
-    row_reduce<NT>(sum, top);
-    if (!live) return;
-    top = max_nan(top, kI8TinyTop);
-    const float inv = 127.0f / top;
-    if (t == 0) {
-        if constexpr (NORM) {
-            const float rstd = 1.0f / sqrtf(sum / float(cols > 0 ? cols : 1) + eps);
-            scale[row] = top * rstd / 127.0f;
-        } else {
-            scale[row] = top / 127.0f;
-        }
-    }
-    if constexpr (VPT > 0) {
+            if constexpr (NORM) {
 #pragma unroll
-        for (int g = 0; g < VPT; ++g) {
-            const int64_t at = int64_t(g * NT + t) * 8;
-            if (at < cols) give(at, v[g], inv);
+                for (int g = 0; g < VPT; ++g) f[g].load(w + from(g));
+            }
+#pragma unroll
+            for (int g = 0; g < VPT; ++g) {
+                const int again = int(start(g) - from(g));  // of the group before it; 8 and more: all
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[g][i] = to_f32(a[g].v[i]);
+                if constexpr (RES) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[g][i] = to_f32(static_cast<T>(v[g][i] + to_f32(b[g].v[i])));
+                    if (again < 8) store8(h + row * cols + from(g), v[g]);
+                }
+                if constexpr (NORM) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        sum += i >= again ? v[g][i] * v[g][i] : 0.0f;
+                        v[g][i] *= to_f32(f[g].v[i]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[g][i]));
+            }
+        }
+        const float inv = reduce();
+        if (live) {
+#pragma unroll
+            for (int g = 0; g < VPT; ++g)
+                if (start(g) < cols) give(from(g), 8, v[g], inv);
         }
     } else {
-        for (int64_t at = int64_t(t) * 8; at < cols; at += NT * 8) {
-            take(at, v[0], false);
-            give(at, v[0], inv);
-        }
+        // One group: the (rounded) stream and its weighted values.
+        auto take = [&](int64_t at, int n, float(&v)[8], bool first) {
+            load_upto8(xr + at, n, v);
+            if constexpr (RES) {
+                float r[8];
+                load_upto8(rr + at, n, r);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = to_f32(static_cast<T>(v[i] + r[i]));
+                if (first) store_upto8(h + row * cols + at, n, v);
+            }
+            if constexpr (NORM) {
+                float g[8];
+                load_upto8(w + at, n, g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (first) sum += v[i] * v[i];
+                    v[i] *= g[i];
+                }
+            }
+            if (first) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[i]));
+            }
+        };
+        auto each = [&](auto&& f) {
+            if (!live) return;
+            for (int64_t at = int64_t(t) * 8; at < cols; at += NT * 8) f(at, cols - at < 8 ? int(cols - at) : 8);
+        };
+        float v[8];
+        each([&](int64_t at, int n) { take(at, n, v, true); });
+        const float inv = reduce();
+        each([&](int64_t at, int n) {
+            take(at, n, v, false);
+            give(at, n, v, inv);
+        });
     }
 }
 
@@ -160,12 +219,23 @@ hipError_t launch_rows(const I8Norm& p, hipStream_t st) {
     return hipSuccess;
 }
 
+// Few threads a row, so that a workgroup's barrier stops few loads, and two
+// groups each (three where two would leave more than a quarter of the threads
+// without one, or with one they share): bf16 norm with residual of 16384 rows
+// of 1024: 19.7 us, 21.1 with one group a thread on twice the threads; of 2501:
+// 56.6 us as 128 x 3, 70.3 as 256 x 2; 8192 rows of 8192: 81.9 us as 512 x 2
+// (5.7 TB/s), 85.1 as 256 x 4, 85.0 as 1024 x 1.
 template <typename T, typename W, bool NORM, bool RES>
 hipError_t rows_form(const I8Norm& p, hipStream_t st) {
     const int64_t groups = ceil_div(p.cols, 8);
+    if (p.cols < 8) return launch_rows<T, W, NORM, RES, 64, 0>(p, st);
     if (groups <= 64) return launch_rows<T, W, NORM, RES, 64, 1>(p, st);
-    if (groups <= 256) return launch_rows<T, W, NORM, RES, 256, 1>(p, st);
-    if (groups <= 1024) return launch_rows<T, W, NORM, RES, 256, 4>(p, st);
+    if (groups <= 128) return launch_rows<T, W, NORM, RES, 64, 2>(p, st);
+    if (groups <= 256) return launch_rows<T, W, NORM, RES, 128, 2>(p, st);
+    if (groups <= 384) return launch_rows<T, W, NORM, RES, 128, 3>(p, st);
+    if (groups <= 512) return launch_rows<T, W, NORM, RES, 256, 2>(p, st);
+    if (groups <= 768) return launch_rows<T, W, NORM, RES, 256, 3>(p, st);
+    if (groups <= 1024) return launch_rows<T, W, NORM, RES, 512, 2>(p, st);
     return launch_rows<T, W, NORM, RES, 1024, 0>(p, st);
 }
 
@@ -201,25 +271,6 @@ __global__ __launch_bounds__(256) void tg_i8_restore(const int8_t* __restrict__ 
         store_upto8(y + row * cols + at, n, v);
     }
 }
-
-// A group of eight elements as it is loaded.
-template <typename T>
-struct Eight {
-    T v[8];
-    __device__ __forceinline__ void load(const T* p, int64_t left) {
-        typedef uint32_t words __attribute__((ext_vector_type(sizeof(T) * 2), aligned(sizeof(T))));
-        typedef T t8 __attribute__((ext_vector_type(8)));
-        if (left >= 8) {
-            typedef uint32_t raw __attribute__((ext_vector_type(sizeof(T) * 2)));
-            const t8 x = __builtin_bit_cast(t8, raw(*reinterpret_cast<const words*>(p)));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = x[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : T(0.0f);
-        }
-    }
-};
 
 // Backward of the norm.  u = gy * w, rstd and c = rstd^2 * mean(u * h) of each
 // row, gx = rstd * (u - h * c) + gh; the workgroup adds gy * h * rstd of its

@@ -74,7 +74,7 @@ struct StreamRaw<false> {
 // start at multiples of four bytes.
 template <int W, bool WORDS, typename T>
 __global__ __launch_bounds__(W * 64) void tg_i8_stream(StreamArgs p, TileStore<T> out) {
-    typedef MmaAcc<Mma::I8, 16>::type Acc;
+    typedef MmaAcc<Mma::I8>::type Acc;
     __shared__ Acc part[W][64];
     const int t = threadIdx.x, lane = t % 64, wave = t / 64, li = lane % 16, lg = lane / 16;
     const int n0 = int(blockIdx.x) * 16;
@@ -114,11 +114,11 @@ __global__ __launch_bounds__(W * 64) void tg_i8_stream(StreamArgs p, TileStore<T
             xa[i].load(pa + u * 128 + i * 64 + lg * 16);
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) acc = mma<Mma::I8, 16>(xb[i].get(at_b), xa[i].get(at_a), acc);
+        for (int i = 0; i < 2; ++i) acc = mma<Mma::I8>(xb[i].get(at_b), xa[i].get(at_a), acc);
     }
     if (last) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) acc = mma<Mma::I8, 16>(tb[i], ta[i], acc);
+        for (int i = 0; i < 2; ++i) acc = mma<Mma::I8>(tb[i], ta[i], acc);
     }
     part[wave][lane] = acc;
     __syncthreads();

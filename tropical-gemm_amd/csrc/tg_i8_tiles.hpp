@@ -15,38 +15,31 @@ namespace tg {
 
 enum class Mma { I8, BF16, F16 };
 
-// Matrix instructions of FS x FS outputs: 64 bytes of the sum for FS 16, 32
-// bytes for FS 32.
+// Matrix instructions of 16 x 16 outputs, 64 bytes of the sum.
 //
-// D += X Y^T: lane l holds bytes (l / FS) * 16 ... + 15 of row l % FS of both,
-// and of D the column l % FS: rows 4 * (l / 16) + e (FS 16, e < 4), or
-// 8 * (e / 4) + 4 * (l / 32) + e % 4 (FS 32, e < 16).
-template <Mma KIND, int FS>
+// D += X Y^T: lane l holds bytes (l / 16) * 16 ... + 15 of row l % 16 of both,
+// and of D rows 4 * (l / 16) ... + 3 of column l % 16.  (32 x 32 outputs read
+// less from LDS and were not faster: the multiplier is the bound either way.)
+template <Mma KIND>
 struct MmaAcc {
-    typedef float type __attribute__((ext_vector_type(FS * FS / 64)));
+    typedef float type __attribute__((ext_vector_type(4)));
 };
-template <int FS>
-struct MmaAcc<Mma::I8, FS> {
-    typedef int32_t type __attribute__((ext_vector_type(FS * FS / 64)));
+template <>
+struct MmaAcc<Mma::I8> {
+    typedef int32_t type __attribute__((ext_vector_type(4)));
 };
 
-template <Mma KIND, int FS>
-__device__ __forceinline__ typename MmaAcc<KIND, FS>::type mma(u32x4 x, u32x4 y, typename MmaAcc<KIND, FS>::type d) {
+template <Mma KIND>
+__device__ __forceinline__ typename MmaAcc<KIND>::type mma(u32x4 x, u32x4 y, typename MmaAcc<KIND>::type d) {
     if constexpr (KIND == Mma::I8) {
         typedef int32_t V __attribute__((ext_vector_type(4)));
-        const V a = __builtin_bit_cast(V, x), b = __builtin_bit_cast(V, y);
-        if constexpr (FS == 16) return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, d, 0, 0, 0);
-        else return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, d, 0, 0, 0);
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(V, x), __builtin_bit_cast(V, y), d, 0, 0, 0);
     } else if constexpr (KIND == Mma::BF16) {
         typedef __bf16 V __attribute__((ext_vector_type(8)));
-        const V a = __builtin_bit_cast(V, x), b = __builtin_bit_cast(V, y);
-        if constexpr (FS == 16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, d, 0, 0, 0);
-        else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, d, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V, x), __builtin_bit_cast(V, y), d, 0, 0, 0);
     } else {
         typedef _Float16 V __attribute__((ext_vector_type(8)));
-        const V a = __builtin_bit_cast(V, x), b = __builtin_bit_cast(V, y);
-        if constexpr (FS == 16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, d, 0, 0, 0);
-        else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, d, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V, x), __builtin_bit_cast(V, y), d, 0, 0, 0);
     }
 }
 
@@ -84,7 +77,7 @@ struct TileArgs {
     int slice;          // steps of one blockIdx.y (tg_i8_tiles_slice)
 };
 
-// Tile of a workgroup: WM x WN waves, each FM x FN fragments of FS x FS.
+// Tile of a workgroup: WM x WN waves, each FM x FN fragments of 16 x 16.
 //
 // LDS holds a ring of NB + 1 stages of A's BM rows of 128 bytes and one of NB
 // stages of B's BN rows.  One step is two halves of 64 bytes.  While the matrix
@@ -105,23 +98,20 @@ struct TileArgs {
 // of a lane are neighbours in a row of C.
 //
 // P planes: a row of A is the sum of P rows, each multiplied with B's.
-template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB, int P = 1>
+template <Mma KIND, int WM, int WN, int FM, int FN, int NB, int P = 1>
 struct Tile {
+    static constexpr int FS = 16, VPF = 4;  // a fragment's rows, and its values in a lane
     static constexpr int BM = WM * FM * FS, BN = WN * FN * FS, NT = WM * WN * 64;
-    static constexpr int KS = FS / 16;       // instructions along half a step
-    static constexpr int VPF = FS * FS / 64;  // values of a fragment per lane
     static constexpr int LOADS_A = P * BM * 8 / NT, LOADS_B = BN * 8 / NT, LOADS = LOADS_A + LOADS_B;
     static constexpr int NA = NB + 1, STAGE_A = P * BM * 128, STAGE_B = BN * 128, LDS = NA * STAGE_A + NB * STAGE_B;
     static_assert(BM * 8 * P % NT == 0 && BN * 8 % NT == 0 && NT % 64 == 0, "whole loads");
-    static_assert(NB >= 2 && NB <= 5, "wait_for's cases");
+    static_assert(NB >= 2 && NB <= 4, "wait_for's cases");
     static_assert(FN >= 2, "work between two products");
-    using Acc = typename MmaAcc<KIND, FS>::type;
+    using Acc = typename MmaAcc<KIND>::type;
     using Value = std::conditional_t<KIND == Mma::I8, int32_t, float>;
 
-    static __device__ __forceinline__ int key_a(int r) { return FS == 16 ? r & 7 : r / 2 & 7; }
-    static __device__ __forceinline__ int key_b(int r) {
-        return FS == 16 ? (r & 3) | (r / (VPF * FN) & 1) << 2 : r / 2 & 7;
-    }
+    static __device__ __forceinline__ int key_a(int r) { return r & 7; }
+    static __device__ __forceinline__ int key_b(int r) { return (r & 3) | (r / (VPF * FN) & 1) << 2; }
 
     // The workgroup's tile: each XCD takes a run of tiles in bands of 8 tile
     // rows, whose panels its L2 then holds.
@@ -192,15 +182,13 @@ struct Tile {
         };
         // Waits until all but the newest `steps` steps' loads have landed.
         auto wait_for = [&](int steps) {
-            if (NB > 4 && steps >= 3) tile_wait<(NB > 4 ? 3 : 0) * LOADS>();
-            else if (NB > 3 && steps >= 2) tile_wait<(NB > 3 ? 2 : 0) * LOADS>();
+            if (NB > 3 && steps >= 2) tile_wait<(NB > 3 ? 2 : 0) * LOADS>();
             else if (NB > 2 && steps >= 1) tile_wait<(NB > 2 ? 1 : 0) * LOADS>();
             else tile_wait<0>();
         };
 
         const int wm = wave / WN, wn = wave % WN, li = lane % FS, lg = lane / FS;
-        const int group = FS == 16 ? li / 4 : li / 4 % 2, value = FS == 16 ? li % 4 : li / 8 * 4 + li % 4;
-        const int row_a = wm * FM * FS + li, row_b = wn * FN * FS + group * (VPF * FN) + value;
+        const int row_a = wm * FM * FS + li, row_b = wn * FN * FS + li / 4 * (VPF * FN) + li % 4;
         // Fragment j's row, row_b + VPF j, has row_b's key, as fragment i's of
         // A, row_a + FS i, has row_a's.
         const int at_a = row_a * 128 + ((lg ^ key_a(row_a)) << 4);
@@ -208,18 +196,14 @@ struct Tile {
         typedef const __attribute__((address_space(3))) u32x4* frag_t;
         // Row f of A's fragments: plane f % P of fragment f / P.
         constexpr int ROWS = FM * P;
-        u32x4 xa[2][ROWS][KS], xb[2][FN][KS];
+        u32x4 xa[2][ROWS], xb[2][FN];
         // Part i of ROWS of a half's fragments, from the stages at (pa, pb).
         auto read_part = [&](int i, int half, int pa, int pb) {
             const lds_t *from_a = lds + pa, *from_b = lds + pb;
-#pragma unroll
-            for (int u = 0; u < KS; ++u)
-                xa[half][i][u] = *reinterpret_cast<frag_t>(from_a + (at_a ^ (half * 64 + u * 32)) + (i % P * BM + i / P * FS) * 128);
+            xa[half][i] = *reinterpret_cast<frag_t>(from_a + (at_a ^ (half * 64)) + (i % P * BM + i / P * FS) * 128);
 #pragma unroll
             for (int j = i * FN / ROWS; j < (i + 1) * FN / ROWS; ++j)
-#pragma unroll
-                for (int u = 0; u < KS; ++u)
-                    xb[half][j][u] = *reinterpret_cast<frag_t>(from_b + (at_b ^ (half * 64 + u * 32)) + j * VPF * 128);
+                xb[half][j] = *reinterpret_cast<frag_t>(from_b + (at_b ^ (half * 64)) + j * VPF * 128);
         };
         // Multiplies the fragments of half h, row by row.  Between each row's
         // products go its parts of a later step's loads and of the next
@@ -227,11 +211,7 @@ struct Tile {
         auto products = [&](int h, auto reads, auto loads_a, auto loads_b, int pa, int pb) {
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
-                auto product = [&](int j) {
-#pragma unroll
-                    for (int u = 0; u < KS; ++u)
-                        acc[i / P][j] = mma<KIND, FS>(xb[h][j][u], xa[h][i][u], acc[i / P][j]);
-                };
+                auto product = [&](int j) { acc[i / P][j] = mma<KIND>(xb[h][j], xa[h][i], acc[i / P][j]); };
                 product(0);
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (decltype(loads_a)::value)
@@ -251,12 +231,9 @@ struct Tile {
         };
         // Clears the chunks of A's fragments that lie past the sum's end.
         auto clear = [&](int h) {
+            if ((lg + 4 * h) * 16 < p.tail) return;
 #pragma unroll
-            for (int u = 0; u < KS; ++u)
-                if ((lg + 2 * u + 4 * h) * 16 >= p.tail) {
-#pragma unroll
-                    for (int i = 0; i < ROWS; ++i) xa[h][i][u] = u32x4{0, 0, 0, 0};
-                }
+            for (int i = 0; i < ROWS; ++i) xa[h][i] = u32x4{0, 0, 0, 0};
         };
         const std::true_type yes;
         const std::false_type no;
@@ -352,7 +329,7 @@ struct Tile {
                 }
             }
         };
-        if ((tm + 1) * BM <= p.m && (tn + 1) * BN <= p.n) each(std::true_type());
+        if (int64_t(tm + 1) * BM <= p.m && int64_t(tn + 1) * BN <= p.n) each(std::true_type());
         else each(std::false_type());
     }
 
@@ -426,20 +403,20 @@ struct TilePartial {
     }
 };
 
-template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB, int P, int PER_CU, typename T>
+template <Mma KIND, int WM, int WN, int FM, int FN, int NB, int P, int PER_CU, typename T>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_i8_tiles(TileArgs p, TileStore<T> out) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    Tile<KIND, FS, WM, WN, FM, FN, NB, P>::whole(p, 0, p.steps, smem, out);
+    Tile<KIND, WM, WN, FM, FN, NB, P>::whole(p, 0, p.steps, smem, out);
 }
 
 // Slice blockIdx.y of the sum: its sums to part + blockIdx.y * M * ld.
-template <Mma KIND, int FS, int WM, int WN, int FM, int FN, int NB, int P, int PER_CU>
+template <Mma KIND, int WM, int WN, int FM, int FN, int NB, int P, int PER_CU>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_i8_tiles_slice(
-    TileArgs p, TilePartial<typename Tile<KIND, FS, WM, WN, FM, FN, NB, P>::Value> out) {
+    TileArgs p, TilePartial<typename Tile<KIND, WM, WN, FM, FN, NB, P>::Value> out) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int s0 = int(blockIdx.y) * p.slice, s1 = s0 + p.slice < p.steps ? s0 + p.slice : p.steps;
     out.c += int64_t(blockIdx.y) * p.m * out.ld;
-    Tile<KIND, FS, WM, WN, FM, FN, NB, P>::whole(p, s0, s1, smem, out);
+    Tile<KIND, WM, WN, FM, FN, NB, P>::whole(p, s0, s1, smem, out);
 }
 
 // C from the slices' sums, added in their order (none: an empty sum).
