@@ -23,7 +23,9 @@ struct AnyArgs {
 // Tile's LDS rows and fragments.  Rows come through registers (a load straight
 // into LDS needs aligned addresses), two steps ahead of their use, and LDS
 // holds two steps.  Bytes past the sum's end are zeros of both operands.
-// Bound by the loads' latency.
+// Bound by the loads' latency.  GPU time of M x N x K here and in two launches:
+// 1001 x 1001 x 515: 7.0 and 7.7 us; 64 x 1031 x 2049: 11.1 and 9.2; 33 x 5003 x
+// 4095: 15.7 and 21.7; 2049 x 1031 x 1031, which takes the two, 16.3 and 14.1.
 template <typename T>
 __global__ __launch_bounds__(256) void tg_i8_any(AnyArgs p, TileStore<T> out) {
     using Cfg = Tile<Mma::I8, 2, 2, 2, 2, 2>;

@@ -4,7 +4,7 @@
 //
 // All of them are bound by HBM: every input element is read once, every
 // output written once, a row's values stay in registers between its reduction
-// and its output.
+// and its output.  (A copy of 1 GiB reaches 4.95 TB/s on the same GPU.)
 #include "../../include/tropical_gemm_hip.h"
 #include "tg_i8.hpp"
 #include "tg_i8_types.hpp"
@@ -82,6 +82,9 @@ struct Eight {
 // it shares with the group before it are written twice, with the same values,
 // and counted once.
 // VPT 0: rows of any length, read again (through L2) after the reduction.
+// bf16, 8192 x 8192: norm with residual 87 us (470 MB, 5.4 TB/s), without norm
+// 38.7 us (201 MB, 5.2 TB/s); one row of 4096: 2.8 us, the loads' latency and
+// the launch's.
 template <typename T, typename W, bool NORM, bool RES, int NT, int VPT>
 __global__ __launch_bounds__(kBlock<NT>) void tg_i8_rows(const T* __restrict__ x, int64_t ldx,
                                                          const T* __restrict__ res, int64_t ldr,
@@ -254,7 +257,8 @@ hipError_t by_type(int type, F&& f) {
     }
 }
 
-// y = round(q * scale), eight elements a thread.
+// y = round(q * scale), eight elements a thread.  bf16, 8192 x 8192: 31.8 us
+// behind the kernel that wrote q (201 MB, 6.3 TB/s, q still in the last cache).
 template <typename T>
 __global__ __launch_bounds__(256) void tg_i8_restore(const int8_t* __restrict__ q, int64_t ldq,
                                                      const float* __restrict__ scale, T* __restrict__ y,
@@ -279,7 +283,8 @@ __global__ __launch_bounds__(256) void tg_i8_restore(const int8_t* __restrict__ 
 // in tg_i8_rows; its weights stay in registers, and the next row is loaded
 // before this one is reduced, so that loads are always on their way.  A row
 // longer than NT * VPT * 8 is shared by blockIdx.y; then every workgroup
-// reduces all of it.
+// reduces all of it.  bf16, 8192 x 4096 with gh: 49.9 us (277 MB with the
+// parts, 5.5 TB/s); f32, 777 x 2501: 11.1 us, two rows one after the other.
 template <typename T, typename W, bool GH, int NT, int VPT>
 __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
     const T* __restrict__ gy, int64_t ldg, const T* __restrict__ h, int64_t ldh, const W* __restrict__ w,
@@ -385,7 +390,7 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
 
 // gw[j] = sum over the parts: 64 slices of them, each in order, four of its
 // loads on their way at a time, then the slices in order.  The same bits in
-// every run.
+// every run.  512 parts of 4096: 4.8 us, a launch and a few loads' latency.
 template <typename W>
 __global__ __launch_bounds__(1024) void tg_i8_sum_parts(const float* __restrict__ part, int64_t parts,
                                                         W* __restrict__ gw, int64_t cols) {
