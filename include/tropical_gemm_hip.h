@@ -377,8 +377,9 @@ int tg_i8_gemm(int device, tg_float type, const int8_t* a, int64_t lda, const fl
                int64_t m, int64_t n, int64_t k, void* workspace, size_t workspace_bytes,
                void* stream);
 
-/* Name of the way tg_i8_gemm takes for these operands, e.g. "stream waves 16"
- * (up to 16 rows: b is streamed into registers), "any" (one launch for
+/* Name of the way tg_i8_gemm takes for these operands, e.g. "stream rows 16
+ * words" (up to 16 rows: b is streamed into registers; rows are 32-bit
+ * aligned), "any" (one launch for
  * unaligned rows), "tiles 256x256", "tiles 64x64 per_cu 2 slices 4 pack a"
  * (the sum in four slices that are joined afterwards, a laid out first);
  * "invalid" for arguments the call would reject.  Host logic only, as

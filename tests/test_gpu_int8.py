@@ -225,7 +225,7 @@ SIZES = [(1, 1, 1), (1, 64, 128), (1, 1000, 4096), (1, 333, 1001), (2, 17, 15), 
          (33, 65, 127), (48, 1024, 2048), (63, 63, 63), (64, 512, 1000), (65, 300, 144), (100, 1, 500),
          (128, 128, 128), (129, 127, 255), (200, 1000, 1600), (255, 257, 256), (256, 512, 1024), (257, 256, 130),
          (300, 600, 16), (511, 1030, 384), (513, 300, 4000), (1000, 1000, 1000), (1024, 768, 2304),
-         (2049, 130, 272)]
+         (2049, 130, 272), (20, 300, 1040), (32, 48, 100), (40, 77, 515), (50, 200, 300), (64, 129, 2000), (90, 200, 17)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES, ids=lambda v: str(v))
@@ -479,9 +479,9 @@ def test_numbers_of_a_known_case():
     assert np.array_equal(int8.dequantize(q, scale, torch.float32).cpu().numpy(), q.cpu().numpy().astype(np.float32))
 
 
-@pytest.mark.parametrize("m", [4, 5, 16])
+@pytest.mark.parametrize("m", [4, 5, 16, 17, 32, 33, 64])
 def test_matmul_wide(m):
-    """More columns than the kernel for few rows takes, aligned rows and not."""
+    """More columns than some of the ways for few rows take, aligned rows and not."""
     n, k = 12300, 144
     for ldb, off in ((k, 0), (k + 1, 1)):
         _say("matmul wide", m, n, k, ldb, off)

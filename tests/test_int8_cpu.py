@@ -138,17 +138,21 @@ def _grad_plan(kind, want_a, m, n, k, ldg=None, g=P):
 
 
 @pytest.mark.parametrize("args,plan", [
-    ((1, 8192, 8192), "stream waves 16"),
-    ((13, 5003, 4099), "stream waves 16"),
-    ((4, 28672, 8192), "stream waves 8"),
-    ((16, 28672, 8192), "tiles 32x64 per_cu 3"),
-    ((16, 28672, 8191), "stream waves 8"),
+    ((1, 8192, 8192), "stream rows 16 words"),
+    ((13, 5003, 4099), "stream rows 16"),
+    ((16, 28672, 8192), "stream rows 16 words"),
+    ((17, 28672, 8192), "tiles 32x64 per_cu 3"),
+    ((17, 28672, 8191), "stream rows 32"),
+    ((32, 4096, 4100), "stream rows 32 words"),
+    ((33, 4096, 4095), "stream rows 48"),
+    ((64, 4096, 4095), "stream rows 64"),
+    ((64, 16384, 4095), "any"),
     ((8192, 8192, 8192), "tiles 256x256"),
     ((512, 4096, 4096), "tiles 64x128 per_cu 2"),
     ((2048, 2048, 2048), "tiles 128x128"),
     ((2048, 4096, 2048), "tiles 128x128 per_cu 2"),
     ((1024, 1024, 1024), "tiles 64x64 per_cu 2"),
-    ((32, 4096, 512), "tiles 32x64 per_cu 3"),
+    ((64, 4096, 512), "tiles 32x64 per_cu 3"),
     ((64, 256, 16384), "tiles 32x64 per_cu 3 slices 32"),
     ((300, 500, 701), "any"),
     ((8191, 8191, 8191), "tiles 256x256 pack a pack b"),

@@ -11,6 +11,7 @@
 
 namespace tg {
 
+// At least 16 bytes of the sum (k).
 struct AnyArgs {
     const int8_t* a;
     int64_t lda;
@@ -22,10 +23,12 @@ struct AnyArgs {
 // 64 x 64 outputs a workgroup of 2 x 2 waves, 128 bytes of the sum a step, on
 // Tile's LDS rows and fragments.  Rows come through registers (a load straight
 // into LDS needs aligned addresses), two steps ahead of their use, and LDS
-// holds two steps.  Bytes past the sum's end are zeros of both operands.
-// Bound by the loads' latency.  GPU time of M x N x K here and in two launches:
-// 1001 x 1001 x 515: 7.0 and 7.7 us; 64 x 1031 x 2049: 11.1 and 9.2; 33 x 5003 x
-// 4095: 15.7 and 21.7; 2049 x 1031 x 1031, which takes the two, 16.3 and 14.1.
+// holds two steps.  A row's chunk that would end past it is its last 16 bytes,
+// shifted on their way into LDS, zeros from the sum's end on.
+// Bound by the loads' latency (as aligned words and the next lane's first, one
+// more load a row: a third slower).  GPU time of M x N x K here and in two
+// launches, us: 1001 x 1001 x 515: 6.4 and 7.8; 257 x 1031 x 1031: 7.6 and 8.0;
+// 128 x 4096 x 4095: 16.1 and 19.7; 2049 x 1031 x 1031: 16.2 and 14.4.
 template <typename T>
 __global__ __launch_bounds__(256) void tg_i8_any(AnyArgs p, TileStore<T> out) {
     using Cfg = Tile<Mma::I8, 2, 2, 2, 2, 2>;
@@ -62,18 +65,19 @@ __global__ __launch_bounds__(256) void tg_i8_any(AnyArgs p, TileStore<T> out) {
     }
     u32x4 raw[2][4];
     auto load = [&](int s, u32x4(&v)[4]) {
+        if (s * 128 >= p.k) return;
         const int k = s * 128 + chunk * 16;
-        if (s * 128 + 128 <= p.k) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const u32x4_any*>(row[i] + k);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = stream_tail(row[i], k, p.k);
-        }
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const u32x4_any*>(row[i] + (k < p.k - 16 ? k : p.k - 16));
     };
-    auto put = [&](int stage, const u32x4(&v)[4]) {
+    auto put = [&](int s, u32x4(&v)[4]) {
+        if (s * 128 + 128 > p.k) {
+            const int k = s * 128 + chunk * 16;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<put_t>(lds + stage * STAGE + to[i]) = v[i];
+            for (int i = 0; i < 4; ++i) v[i] = shift_out(v[i], k < p.k - 16 ? 0 : k - (p.k - 16));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<put_t>(lds + s % 2 * STAGE + to[i]) = v[i];
     };
     const int lane = t % 64, wave = t / 64, li = lane % 16, lg = lane / 16;
     const int row_a = wave / 2 * 32 + li, row_b = wave % 2 * 32 + li / 4 * 8 + li % 4;
@@ -105,11 +109,11 @@ __global__ __launch_bounds__(256) void tg_i8_any(AnyArgs p, TileStore<T> out) {
     __syncthreads();
     for (int s = 0; s < steps; s += 2) {
         products(0);
-        put(1, raw[1]);
+        put(s + 1, raw[1]);
         load(s + 3, raw[1]);
         __syncthreads();
         if (s + 1 < steps) products(1);
-        put(0, raw[0]);
+        put(s + 2, raw[0]);
         load(s + 4, raw[0]);
         __syncthreads();
     }

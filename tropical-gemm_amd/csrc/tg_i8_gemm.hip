@@ -189,19 +189,29 @@ struct Carver {
 
 // ---- the 8-bit product ---------------------------------------------------
 
-// Up to 16 rows of A take the kernel that streams B, rows of any alignment: M =
-// 16, N = K = 4096: 6.9 us against 8.4 with tiles; M = 1, N = K = 8192: 14.4
-// against 16.7.  Its reads of A count where there are more than a few rows,
-// and a wide matrix fills the GPU with tiles: M = 16, N = 28672, K = 8192: 60 us
-// against 44 with tiles (M = 4: 42 and 45; N = 8192: 17.8 and 17.3).  (A launch's
-// thread count stays below 2^32.)
-bool streams(const I8Gemm& p) {
-    if (p.m > 16 || p.n >= int64_t(1) << 27) return false;
-    return p.m <= 4 || p.n <= 12288 || !in_place(p.a, p.lda, p.k) || !in_place(p.b, p.ldb, p.k);
+// Rows of A that tg_i8_stream takes (in sixteens; 0: others take the product):
+// B is read once and needs no layout, but every 16 rows of B read all of A, so
+// more rows than 16 only where B is narrow or would have to be laid out first.
+// us, cold weights, tg_i8_stream and the best other way, M x N x K:
+//     16 x 4096 x 4096    6.6   10.7     16 x 28672 x 8192  47.2   44.7
+//     32 x 4096 x 4096    7.2   10.9     32 x  8192 x 8192  19.8   19.5
+//                                        32 x 16384 x 4096  19.9   16.3
+// and unaligned
+//     32 x 1024 x 8191    9.7   35.7     32 x 16384 x 4095  27.7   26.9
+//     64 x 1024 x 8191   15.2   35.2     64 x  8192 x 8191  39.4   45.6
+//     64 x 4096 x 4095   12.8   24.6     64 x 16384 x 4095  40.9   26.8
+int stream_rows(const I8Gemm& p) {
+    // A launch's thread count stays below 2^32.
+    if (p.m > 64 || p.n >= int64_t(1) << 26) return 0;
+    if (p.m <= 16) return 16;
+    const bool ready = in_place(p.a, p.lda, p.k) && in_place(p.b, p.ldb, p.k);
+    if (p.m <= 32) return p.n <= 8192 || !ready ? 32 : 0;
+    return p.n <= 8192 && !ready ? int(round_up(p.m, 16)) : 0;
 }
 
 struct GemmPlan {
-    bool stream, any, pack_a, pack_b;
+    int stream;  // rows of A of tg_i8_stream
+    bool any, pack_a, pack_b;
     int64_t ld;  // of packed rows
     TilePlan tiles;
 };
@@ -221,15 +231,15 @@ constexpr double kOneLaunch = 2.0;
 // against 35).
 double any_time(const I8Gemm& p) {
     const int64_t tiles = ceil_div(p.m, 64) * ceil_div(p.n, 64);
-    if (tiles >= int64_t(1) << 24 || p.k > 4096) return 1e30;
+    if (tiles >= int64_t(1) << 24 || p.k < 16 || p.k > 4096) return 1e30;
     const double per_cu = double(tiles) / 256, step = 0.48 * per_cu;
     return 4.0 + per_cu + double(ceil_div(p.k, 128)) * (step > 0.37 ? step : 0.37);
 }
 
 GemmPlan plan_gemm(const I8Gemm& p) {
     GemmPlan pl{};
-    pl.stream = streams(p);
-    if (pl.stream) return pl;
+    pl.stream = stream_rows(p);
+    if (pl.stream != 0) return pl;
     pl.pack_a = !in_place(p.a, p.lda, p.k);
     pl.pack_b = !in_place(p.b, p.ldb, p.k);
     pl.ld = round_up(p.k, 128);
@@ -251,7 +261,7 @@ struct GemmWs {
 GemmWs carve_gemm(const I8Gemm& p, const GemmPlan& pl, void* ws) {
     Carver c{static_cast<char*>(ws)};
     GemmWs w{};
-    if (p.m == 0 || p.n == 0 || p.k == 0 || pl.stream || pl.any) return w;
+    if (p.m == 0 || p.n == 0 || p.k == 0 || pl.stream != 0 || pl.any) return w;
     if (pl.pack_a) w.a = static_cast<int8_t*>(c.take(size_t(p.m) * size_t(pl.ld)));
     if (pl.pack_b) w.b = static_cast<int8_t*>(c.take(size_t(p.n) * size_t(pl.ld)));
     w.part = c.take(part_bytes(pl.tiles, p.m, p.n));
@@ -263,18 +273,32 @@ PackBytes bytes_job(const void* src, int64_t ld_src, int64_t rows, int64_t bytes
     return {static_cast<const int8_t*>(src), ld_src, rows, int(bytes), static_cast<int8_t*>(dst), ld};
 }
 
-// Waves of a workgroup of tg_i8_stream: 16 while the GPU holds all workgroups
-// at once (M = 13, K = 8192: N = 8192 17.2 us against 18.4 with 8; N = 28672 60
-// against 56).
-int stream_waves(int64_t n) { return n <= 16384 ? 16 : 8; }
-
-template <int W, typename T>
-hipError_t launch_stream(const I8Gemm& p, const TileStore<T>& out, hipStream_t st) {
+// 32-bit aligned rows.
+bool in_words(const I8Gemm& p) {
     auto words = [](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 4 == 0 && ld % 4 == 0; };
+    return words(p.a, p.lda) && words(p.b, p.ldb);
+}
+
+template <int R, int W, bool WORDS, typename T>
+hipError_t launch_stream(const I8Gemm& p, const TileStore<T>& out, hipStream_t st) {
     const StreamArgs args{p.a, p.lda, p.b, p.ldb, int(p.m), int(p.n), int(p.k)};
-    const auto kernel = words(p.a, p.lda) && words(p.b, p.ldb) ? &tg_i8_stream<W, true, T> : &tg_i8_stream<W, false, T>;
-    hipLaunchKernelGGL(kernel, dim3(unsigned(ceil_div(p.n, 16))), dim3(W * 64), 0, st, args, out);
+    hipLaunchKernelGGL((tg_i8_stream<R, W, WORDS, T>), dim3(unsigned(ceil_div(p.n, 16))), dim3(W * 64), 0, st, args, out);
     return hipGetLastError();
+}
+
+// Eight waves of a workgroup; 16 for a few aligned rows (M = 1, cold weights, N
+// x K: 8192 x 8192 14.6 us and 15.1 with 8, 4096 x 4096 6.1 and 6.5; unaligned
+// 8192 x 8191 14.5 and 14.0).  Beyond 32 rows the way for any address serves
+// all.
+template <typename T>
+hipError_t stream_typed(const I8Gemm& p, int rows, const TileStore<T>& out, hipStream_t st) {
+    const bool words = in_words(p);
+    switch (rows) {
+        case 16: return words ? launch_stream<1, 16, true>(p, out, st) : launch_stream<1, 8, false>(p, out, st);
+        case 32: return words ? launch_stream<2, 8, true>(p, out, st) : launch_stream<2, 8, false>(p, out, st);
+        case 48: return launch_stream<3, 8, false>(p, out, st);
+        default: return launch_stream<4, 8, false>(p, out, st);
+    }
 }
 
 template <typename T>
@@ -282,7 +306,7 @@ hipError_t gemm_typed(const I8Gemm& p, void* ws, hipStream_t st) {
     const TileStore<T> out{p.a_scale, p.b_scale, nullptr, static_cast<const T*>(p.bias), static_cast<T*>(p.c), p.n};
     if (p.k == 0) return launch_join<int32_t>(nullptr, 0, p.m, p.n, out, st);
     const GemmPlan pl = plan_gemm(p);
-    if (pl.stream) return stream_waves(p.n) == 16 ? launch_stream<16>(p, out, st) : launch_stream<8>(p, out, st);
+    if (pl.stream != 0) return stream_typed(p, pl.stream, out, st);
     if (pl.any) {
         const AnyArgs args{p.a, p.lda, p.b, p.ldb, int(p.m), int(p.n), int(p.k), int(ceil_div(p.m, 64)), int(ceil_div(p.n, 64))};
         hipLaunchKernelGGL((tg_i8_any<T>), dim3(unsigned(args.tiles_m * args.tiles_n)), dim3(256), 0, st, args, out);
@@ -415,7 +439,7 @@ std::string i8_gemm_plan(const I8Gemm& p) {
     if (p.m == 0 || p.n == 0) return "none";
     if (p.k == 0) return "bias";
     const GemmPlan pl = plan_gemm(p);
-    if (pl.stream) return "stream waves " + std::to_string(stream_waves(p.n));
+    if (pl.stream != 0) return "stream rows " + std::to_string(pl.stream) + (in_words(p) && pl.stream <= 32 ? " words" : "");
     if (pl.any) return "any";
     return tiles_name(pl.tiles) + (pl.pack_a ? " pack a" : "") + (pl.pack_b ? " pack b" : "");
 }

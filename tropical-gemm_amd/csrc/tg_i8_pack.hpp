@@ -37,7 +37,9 @@ struct PackBytes {
         const int64_t chunks = ld / 16, total = rows * chunks;
         for (int64_t i = int64_t(block) * 256 + threadIdx.x; i < total; i += int64_t(count) * 256) {
             const int64_t row = i / chunks, c = i - row * chunks;
-            *reinterpret_cast<u32x4*>(dst + row * ld + c * 16) = stream_tail(src + row * ld_src, int(c) * 16, bytes);
+            StreamTail x;
+            x.load(src + row * ld_src, int(c) * 16, bytes);
+            *reinterpret_cast<u32x4*>(dst + row * ld + c * 16) = x.get();
         }
     }
 };
