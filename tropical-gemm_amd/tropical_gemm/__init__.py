@@ -12,6 +12,9 @@ and the ``mod gpu`` functions of ``crates/tropical-gemm-python/src/lib.rs:1657-2
 * ``cuda_available()`` (lib.rs:2341-2344), true when a HIP device and the
   native library are present.
 
+``tropical_gemm.int8`` holds the operators of an 8-bit linear layer (no
+counterpart in the reference).
+
 The reference's numpy GPU functions hand row-major numpy data to its
 column-major API without the operand swap (lib.rs:1904-1907), which is wrong
 for non-symmetric inputs; these functions compute the row-major product.
