@@ -31,17 +31,26 @@ _FLOAT = {torch.float32: nat.FLOAT["f32"], torch.bfloat16: nat.FLOAT["bf16"],
 _F32 = (torch.float32,)
 
 
-def _rows(name: str, t: torch.Tensor, dtype=None) -> int:
-    """Checks a matrix on the GPU whose rows are neighbours; its row stride."""
-    if not t.is_cuda:
+def _elsewhere(name: str, t: torch.Tensor, dev: int | None):
+    if dev is None:
         raise ValueError("tropical_gemm GPU entry points need device tensors "
                          f"({name} is on {t.device.type}); move the tensors to the GPU first")
+    raise ValueError(f"Tensors must be on the same device, cuda:{dev}: {name} is on {t.device}")
+
+
+# The checks take the device as an index: comparing torch.device objects costs
+# a small call as much as an allocation.
+def _rows(name: str, t: torch.Tensor, dtype=None, dev: int | None = None) -> int:
+    """Checks a matrix on a GPU (on `dev`) whose rows are neighbours; its row stride."""
+    on = t.get_device()
+    if on < 0 or dev is not None and on != dev:
+        _elsewhere(name, t, dev)
     if t.dim() != 2:
         raise ValueError(f"Expected a 2D tensor for {name}, got {t.dim()} dims")
     if dtype is None:
         if t.dtype not in _FLOAT:
             raise ValueError(f"Unsupported dtype {t.dtype} of {name}: expected bfloat16, float16 or float32")
-    elif t.dtype != dtype:
+    elif t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if t.is_contiguous():
         return t.shape[1]
@@ -55,20 +64,15 @@ def _rows(name: str, t: torch.Tensor, dtype=None) -> int:
     return ld
 
 
-def _vector(name: str, t: torch.Tensor, n: int, dtypes) -> None:
-    if t.dim() != 1 or t.shape[0] != n:
+def _vector(name: str, t: torch.Tensor, n: int, dtypes, dev: int) -> None:
+    if t.shape != (n,):
         raise ValueError(f"Dimension mismatch: {name} has shape {tuple(t.shape)}, expected ({n},)")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.get_device() != dev:
+        _elsewhere(name, t, dev)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous (call .contiguous() on PyTorch tensors)")
-
-
-def _same_device(dev: torch.device, first: str, **others) -> None:
-    """All tensors that are not None are on `dev`, where `first` is."""
-    for name, t in others.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"Tensors must be on the same device: {first} is on {dev}, {name} is on {t.device}")
 
 
 def _same_shape(name: str, t: torch.Tensor, shape) -> None:
@@ -95,7 +99,7 @@ def quantize(x: torch.Tensor):
     dev = x.device
     q = _matrix(rows, cols, torch.int8, dev)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
-    nat.check(nat.load().tg_i8_quantize(dev.index or 0, _FLOAT[x.dtype], x.data_ptr(), ld, q.data_ptr(),
+    nat.check(nat.load().tg_i8_quantize(dev.index, _FLOAT[x.dtype], x.data_ptr(), ld, q.data_ptr(),
                                         scale.data_ptr(), rows, cols, _stream(dev)))
     return q, scale
 
@@ -104,12 +108,11 @@ def dequantize(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.
     """``q * scale[:, None]`` rounded to ``dtype``."""
     ld = _rows("q", q, torch.int8)
     rows, cols = q.shape
-    _vector("scale", scale, rows, _F32)
     dev = q.device
-    _same_device(dev, "q", scale=scale)
+    _vector("scale", scale, rows, _F32, dev.index)
     _float_type(dtype)
     y = _matrix(rows, cols, dtype, dev)
-    nat.check(nat.load().tg_i8_dequantize(dev.index or 0, _FLOAT[dtype], q.data_ptr(), ld, scale.data_ptr(),
+    nat.check(nat.load().tg_i8_dequantize(dev.index, _FLOAT[dtype], q.data_ptr(), ld, scale.data_ptr(),
                                           y.data_ptr(), rows, cols, _stream(dev)))
     return y
 
@@ -126,18 +129,17 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     scales.  ``weight`` is of x's type or float32."""
     ldx = _rows("x", x)
     rows, cols = x.shape
-    _vector("weight", weight, cols, (x.dtype, torch.float32))
     dev = x.device
-    _same_device(dev, "x", weight=weight, residual=residual)
+    _vector("weight", weight, cols, (x.dtype, torch.float32), dev.index)
     ldr, h = 0, x
     if residual is not None:
-        ldr = _rows("residual", residual, x.dtype)
+        ldr = _rows("residual", residual, x.dtype, dev.index)
         _same_shape("residual", residual, x.shape)
         h = _matrix(rows, cols, x.dtype, dev)
     q = _matrix(rows, cols, torch.int8, dev)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
     nat.check(nat.load().tg_i8_rms_norm(
-        dev.index or 0, _FLOAT[x.dtype], _FLOAT[weight.dtype], x.data_ptr(), ldx, _ptr(residual), ldr,
+        dev.index, _FLOAT[x.dtype], _FLOAT[weight.dtype], x.data_ptr(), ldx, _ptr(residual), ldr,
         weight.data_ptr(), eps, q.data_ptr(), scale.data_ptr(), None if residual is None else h.data_ptr(), rows,
         cols, _stream(dev)))
     return q, scale, h
@@ -150,24 +152,23 @@ def rms_norm_backward(grad_y: torch.Tensor, h: torch.Tensor, weight: torch.Tenso
     ``grad_h``, the gradient of the stream h from elsewhere, added to grad_x.
     grad_x is the gradient of x and of the residual.  Equal calls give equal
     bits."""
+    dev = h.device
     ldh = _rows("h", h)
     rows, cols = h.shape
     _same_shape("grad_y", grad_y, h.shape)
-    ldg = _rows("grad_y", grad_y, h.dtype)
-    _vector("weight", weight, cols, (h.dtype, torch.float32))
-    dev = h.device
-    _same_device(dev, "h", grad_y=grad_y, weight=weight, grad_h=grad_h)
+    ldg = _rows("grad_y", grad_y, h.dtype, dev.index)
+    _vector("weight", weight, cols, (h.dtype, torch.float32), dev.index)
     ldgh = 0
     if grad_h is not None:
         _same_shape("grad_h", grad_h, h.shape)
-        ldgh = _rows("grad_h", grad_h, h.dtype)
+        ldgh = _rows("grad_h", grad_h, h.dtype, dev.index)
     grad_x = _matrix(rows, cols, h.dtype, dev)
     grad_weight = torch.empty(cols, dtype=weight.dtype, device=dev)
     lib = nat.load()
     nbytes = lib.tg_i8_rms_norm_backward_workspace_size(rows, cols)
     ws = _workspace(nbytes, dev)
     nat.check(lib.tg_i8_rms_norm_backward(
-        dev.index or 0, _FLOAT[h.dtype], _FLOAT[weight.dtype], grad_y.data_ptr(), ldg, h.data_ptr(), ldh,
+        dev.index, _FLOAT[h.dtype], _FLOAT[weight.dtype], grad_y.data_ptr(), ldg, h.data_ptr(), ldh,
         weight.data_ptr(), eps, _ptr(grad_h), ldgh, grad_x.data_ptr(), grad_weight.data_ptr(), rows, cols,
         _ptr(ws), nbytes, _stream(dev)))
     return grad_x, grad_weight
@@ -179,40 +180,38 @@ def matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: tor
     int8 activations, ``b`` (n, k) an int8 weight matrix with one row for each
     output, f32 scales, ``bias`` of ``dtype``.  The integer sum is exact
     (k < 2**17)."""
+    dev = a.device
     lda = _rows("a", a, torch.int8)
-    ldb = _rows("b", b, torch.int8)
+    ldb = _rows("b", b, torch.int8, dev.index)
     m, k = a.shape
     n, k2 = b.shape
     if k != k2:
         raise ValueError(f"Dimension mismatch: a is {m}x{k}, b is {n}x{k2}")
-    _vector("a_scale", a_scale, m, _F32)
-    _vector("b_scale", b_scale, n, _F32)
+    _vector("a_scale", a_scale, m, _F32, dev.index)
+    _vector("b_scale", b_scale, n, _F32, dev.index)
     kind = _float_type(dtype)
     if bias is not None:
-        _vector("bias", bias, n, (dtype,))
-    dev = a.device
-    _same_device(dev, "a", b=b, a_scale=a_scale, b_scale=b_scale, bias=bias)
+        _vector("bias", bias, n, (dtype,), dev.index)
     c = _matrix(m, n, dtype, dev)
     lib = nat.load()
     pa, pb = a.data_ptr(), b.data_ptr()
     nbytes = lib.tg_i8_gemm_workspace_size(pa, lda, pb, ldb, m, n, k) if k < 1 << 17 else 0
     ws = _workspace(nbytes, dev)
-    nat.check(lib.tg_i8_gemm(dev.index or 0, kind, pa, lda, a_scale.data_ptr(), pb, ldb, b_scale.data_ptr(),
+    nat.check(lib.tg_i8_gemm(dev.index, kind, pa, lda, a_scale.data_ptr(), pb, ldb, b_scale.data_ptr(),
                              _ptr(bias), c.data_ptr(), m, n, k, _ptr(ws), nbytes, _stream(dev)))
     return c
 
 
 def _backward(which: str, grad_c: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    dev = grad_c.device
     ldg = _rows("grad_c", grad_c)
     other = "b" if which == "a" else "a"
-    ldq = _rows(other, q, torch.int8)
+    ldq = _rows(other, q, torch.int8, dev.index)
     m, n = grad_c.shape
     depth, k = q.shape
     if depth != (n if which == "a" else m):
         raise ValueError(f"Dimension mismatch: grad_c is {m}x{n}, {other} is {depth}x{k}")
-    _vector(f"{other}_scale", scale, depth, _F32)
-    dev = grad_c.device
-    _same_device(dev, "grad_c", **{other: q, f"{other}_scale": scale})
+    _vector(f"{other}_scale", scale, depth, _F32, dev.index)
     out = _matrix(m if which == "a" else n, k, grad_c.dtype, dev)
     lib = nat.load()
     size, run = ((lib.tg_i8_backward_a_workspace_size, lib.tg_i8_backward_a) if which == "a" else
@@ -220,7 +219,7 @@ def _backward(which: str, grad_c: torch.Tensor, q: torch.Tensor, scale: torch.Te
     kind = _FLOAT[grad_c.dtype]
     nbytes = size(kind, grad_c.data_ptr(), ldg, m, n, k)
     ws = _workspace(nbytes, dev)
-    nat.check(run(dev.index or 0, kind, grad_c.data_ptr(), ldg, q.data_ptr(), ldq, scale.data_ptr(),
+    nat.check(run(dev.index, kind, grad_c.data_ptr(), ldg, q.data_ptr(), ldq, scale.data_ptr(),
                   out.data_ptr(), m, n, k, _ptr(ws), nbytes, _stream(dev)))
     return out
 
