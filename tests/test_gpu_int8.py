@@ -282,7 +282,8 @@ def test_scales_that_are_not_finite_stay_in_their_rows():
 
 GRADS = [(1, 1, 1), (1, 70, 130), (2, 3, 5), (16, 64, 128), (17, 33, 65), (64, 64, 64), (100, 130, 70), (127, 129, 255),
          (128, 256, 128), (130, 1000, 520), (301, 515, 260), (512, 512, 512), (700, 96, 1040), (1031, 257, 129),
-         (1536, 1024, 768)]
+         (1536, 1024, 768), (40, 2050, 72), (2050, 40, 72), (300, 2100, 1030), (2100, 300, 1030), (1000, 1100, 1200),
+         (9, 20, 8), (66, 8, 9), (65, 190, 63), (129, 7, 40), (7, 100, 40)]
 
 
 def _check_grad(got, g, x, dtype):

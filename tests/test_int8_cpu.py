@@ -180,6 +180,10 @@ def test_gemm_plans_of_strides():
     ("f32", 1, (301, 1031, 2049), "tiles 32x64 per_cu 2 planes 3 pack grad_c"),
     ("f32", 0, (1024, 2048, 2048), "tiles 64x128 planes 3 pack grad_c"),
     ("bf16", 0, (8192, 64, 64), "tiles 32x64 per_cu 3 slices 32 pack grad_c"),
+    ("bf16", 1, (64, 256, 256), "turn"),
+    ("f16", 0, (513, 1024, 1024), "turn"),
+    ("f32", 0, (64, 301, 1031), "turn"),
+    ("bf16", 0, (64, 256, 7), "tiles 32x64 per_cu 3 pack grad_c"),
     ("bf16", 1, (8, 0, 16), "zero"),
     ("bf16", 1, (0, 8, 16), "none"),
     ("bf16", 0, ((1 << 20) + 1, 8, 16), "invalid"),

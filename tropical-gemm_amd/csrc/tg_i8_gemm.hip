@@ -9,6 +9,7 @@
 #include "tg_i8_pack.hpp"
 #include "tg_i8_stream.hpp"
 #include "tg_i8_tiles.hpp"
+#include "tg_i8_turn.hpp"
 
 namespace tg {
 namespace {
@@ -219,9 +220,10 @@ struct GemmPlan {
 // A launch that lays out rows: what it takes beside the bytes' way through
 // memory, in us.
 constexpr double kPackTime = 2.5;
-// How much longer than two launches one may take, in us: it saves the caller's
-// thread a launch and a workspace, 5 us.
-constexpr double kOneLaunch = 2.0;
+// One launch of `one` us instead of two of `two`: it may take 2 us more where the
+// GPU waits for the caller's thread, which spends 13 us on two launches and a
+// workspace, 9 on one.
+bool one_launch(double one, double two) { return one < two + (one < 12 ? 2 : 0); }
 
 // Time of tg_i8_any in us, as tile_time gives it for the others.  Measured on
 // 96 products of odd sizes (M 32 ... 8192, N 65 ... 4097, K 129 ... 8191): the
@@ -247,7 +249,7 @@ GemmPlan plan_gemm(const I8Gemm& p) {
     pl.tiles = plan_tiles(p.m, p.n, ceil_div(p.k, 128), 1, &time);
     if (pl.pack_a || pl.pack_b) {
         const double bytes = 2 * double(pl.ld) * (double(p.m) * pl.pack_a + double(p.n) * pl.pack_b);
-        pl.any = any_time(p) < time + kPackTime + bytes / 4e6 + kOneLaunch;
+        pl.any = one_launch(any_time(p), time + kPackTime + bytes / 4e6);
     }
     return pl;
 }
@@ -343,11 +345,29 @@ hipError_t gemm_typed(const I8Gemm& p, void* ws, hipStream_t st) {
 // multiplied with q.
 
 struct GradPlan {
+    bool turn;  // one launch of tg_i8_turn
     bool pack_g;
     int planes;
     int64_t depth;  // of packed rows, in elements
     TilePlan tiles;
 };
+
+// Time of tg_i8_turn in us, as tile_time gives it for the others: a step takes
+// the vector unit as long for each of a CU's tiles, and a little longer where
+// they share it.  Fitted to 576 gradients (rows and columns 65 ... 4096, sums 64
+// ... 2049; 13% off in the root mean square).  Chosen with it, 64% of those in
+// 16 bits take one launch and 3.3 us less in the mean, half of those in f32 1.3
+// us less; the worst choices lose 3 us (f32: 7 of 23, 1024 terms for a few columns).
+double turn_time(const I8Grad& p) {
+    const int64_t tiles = ceil_div(p.rows, 64) * ceil_div(p.cols, 64);
+    if (tiles >= int64_t(1) << 23 || !turn_fits(p.transposed, p.rows, p.cols, p.depth)) return 1e30;
+    // A CU holds `slots` tiles at a time; a last round takes at least one tile's time.
+    const int64_t slots = p.type == TG_FLOAT32 ? 2 : 4, rest = tiles % (256 * slots);
+    const double last = rest > 256 ? double(rest) / 256 : rest > 0 ? 1 : 0;
+    const double per_cu = double(tiles / (256 * slots) * slots) + last, steps = double(ceil_div(p.depth, 64));
+    if (p.type == TG_FLOAT32) return 3.0 + 0.38 * per_cu + steps * (1.04 * per_cu + (tiles > 256 ? 0.35 : 0));
+    return 3.45 + 0.11 * per_cu + steps * (0.49 * per_cu + (tiles > 256 ? 0.18 : 0));
+}
 
 GradPlan plan_grad(const I8Grad& p) {
     GradPlan pl{};
@@ -355,7 +375,11 @@ GradPlan plan_grad(const I8Grad& p) {
     pl.planes = p.type == TG_FLOAT32 ? 3 : 1;
     pl.pack_g = p.type == TG_FLOAT32 || p.transposed || !in_place(p.g, p.ldg * size, p.depth * size);
     pl.depth = round_up(p.depth, 64);
-    pl.tiles = plan_tiles(p.rows, p.cols, pl.depth / 64, pl.planes);
+    double time = 0;
+    pl.tiles = plan_tiles(p.rows, p.cols, pl.depth / 64, pl.planes, &time);
+    const double bytes = double(pl.depth) * (3 * double(p.cols) + (pl.pack_g ? double(size + 2 * pl.planes) * double(p.rows) : 0));
+    const int launches = p.type == TG_F16 ? 2 : 1;  // before the tiles'
+    pl.turn = one_launch(turn_time(p), time + kPackTime * launches + bytes / 4e6);
     return pl;
 }
 
@@ -368,13 +392,25 @@ struct GradWs {
 GradWs carve_grad(const I8Grad& p, const GradPlan& pl, void* ws) {
     Carver c{static_cast<char*>(ws)};
     GradWs w{};
-    if (p.rows == 0 || p.cols == 0 || p.depth == 0) return w;
+    if (p.rows == 0 || p.cols == 0 || p.depth == 0 || pl.turn) return w;
     if (pl.pack_g) w.g = c.take(size_t(p.rows) * size_t(pl.depth) * size_t(pl.planes) * 2);
     w.q = c.take(size_t(p.cols) * size_t(pl.depth) * 2);
     if (p.type == TG_F16) w.range = static_cast<float*>(c.take(8));
     w.part = c.take(part_bytes(pl.tiles, p.rows, p.cols));
     w.bytes = c.used;
     return w;
+}
+
+template <typename T, bool TRANS>
+hipError_t launch_turn(const I8Grad& p, const TileStore<T>& out, hipStream_t st) {
+    using Cfg = Turn<T, TRANS>;
+    const auto kernel = &tg_i8_turn<T, TRANS>;
+    static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+    if (attr != hipSuccess) return attr;
+    const TurnArgs args{p.g, p.ldg, p.q, p.ldq, p.scale, int(p.rows), int(p.cols), int(p.depth),
+                        int(ceil_div(p.rows, 64)), int(ceil_div(p.cols, 64))};
+    hipLaunchKernelGGL(kernel, dim3(unsigned(args.tiles_m * args.tiles_n)), dim3(Cfg::NT), Cfg::LDS, st, args, out);
+    return hipGetLastError();
 }
 
 template <typename T>
@@ -384,6 +420,7 @@ hipError_t grad_typed(const I8Grad& p, void* ws, hipStream_t st) {
     TileStore<T> out{nullptr, nullptr, nullptr, nullptr, static_cast<T*>(p.out), p.cols};
     if (p.depth == 0) return launch_join<float>(nullptr, 0, p.rows, p.cols, out, st);
     const GradPlan pl = plan_grad(p);
+    if (pl.turn) return p.transposed ? launch_turn<T, true>(p, out, st) : launch_turn<T, false>(p, out, st);
     const GradWs w = carve_grad(p, pl, ws);
     hipError_t e = hipSuccess;
     if (p.type == TG_F16) {
@@ -448,6 +485,7 @@ std::string i8_grad_plan(const I8Grad& p) {
     if (p.rows == 0 || p.cols == 0) return "none";
     if (p.depth == 0) return "zero";
     const GradPlan pl = plan_grad(p);
+    if (pl.turn) return "turn";
     return tiles_name(pl.tiles) + (pl.pack_g ? " pack grad_c" : "");
 }
 
