@@ -384,7 +384,8 @@ int tg_i8_gemm(int device, tg_float type, const int8_t* a, int64_t lda, const fl
  * (the sum in four slices that are joined afterwards, a laid out first);
  * "invalid" for arguments the call would reject.  Host logic only, as
  * tg_gemm_plan: pointers are checked for alignment.  tg_i8_backward_plan is
- * the same for grad_a (want_a not 0) or grad_b. */
+ * the same for grad_a (want_a not 0) or grad_b; "turn" is one launch for small
+ * ones. */
 const char* tg_i8_gemm_plan(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, int64_t m,
                             int64_t n, int64_t k);
 const char* tg_i8_backward_plan(tg_float type, int want_a, const void* grad_c, int64_t ldg,

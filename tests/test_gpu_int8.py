@@ -310,6 +310,44 @@ def test_gradients(dtype, m, n, k):
         _check_grad(int8.backward_b(g, a, sa), f64(g).t(), f64(a) * f64(sa)[:, None], dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("m,n,k", [(70, 90, 100), (300, 2100, 1030), (2100, 300, 1030), (40, 2050, 72), (2050, 40, 72)],
+                         ids=lambda v: str(v))
+def test_gradients_that_are_not_finite(dtype, m, n, k):
+    """NaN and infinity in grad_c and in a scale reach the outputs that they are
+    a term of, and no others."""
+    nan, inf = float("nan"), float("inf")
+    for pad in (0, 1):
+        _say("backward not finite", IDS[dtype], m, n, k, pad)
+        g = _values(1, m, n, dtype, n + pad)
+        a, sa = _int8(2, m, k, k + pad)
+        b, sb = _int8(3, n, k, k + pad)
+        clean = int8.backward_a(g, b, sb), int8.backward_b(g, a, sa)
+        g[1, n - 1], g[3, 4], g[m - 1, n - 2] = nan, inf, -inf
+        b[4], b[n - 2], a[3], a[m - 1] = 3, 5, -2, 7  # no zeros where infinities meet them
+        got_a, got_b = int8.backward_a(g, b, sb), int8.backward_b(g, a, sa)
+        assert torch.isnan(got_a[1]).all() and torch.isnan(got_b[n - 1]).all()
+        assert (got_a[3] == inf).all() and (got_a[m - 1] == -inf).all()
+        assert (got_b[4] == -inf).all() and (got_b[n - 2] == -inf).all()
+        for got, was, hit in ((got_a, clean[0], (1, 3, m - 1)), (got_b, clean[1], (n - 1, 4, n - 2))):
+            rest = torch.ones(got.shape[0], dtype=torch.bool, device=DEV)
+            rest[list(hit)] = False
+            assert torch.isfinite(got[rest]).all()
+        sb[n - 1], sa[0] = nan, nan
+        assert torch.isnan(int8.backward_a(g, b, sb)).all() and torch.isnan(int8.backward_b(g, a, sa)).all()
+
+
+def test_gradients_of_the_largest_numbers():
+    """Close to the end of f32's range nothing overflows on the way."""
+    top = float(torch.finfo(torch.float32).max)
+    for m, n in ((64, 64), (2100, 300)):
+        g = torch.zeros(m, n, device=DEV)
+        g[:, 5] = top
+        b = torch.ones(n, 72, dtype=torch.int8, device=DEV)
+        out = int8.backward_a(g, b, torch.ones(n, device=DEV))
+        assert torch.equal(out, torch.full_like(out, top))
+
+
 def test_gradients_against_differences():
     """sum(G * (A B^T)) is linear in either operand, so its difference along any
     direction is the gradient's product with it."""
@@ -330,7 +368,11 @@ def test_gradients_against_differences():
 def test_gradients_of_wide_range():
     """Gradients and scales far from one: nothing is lost below or above the
     16-bit types' ranges on the way."""
-    m, n, k = 130, 200, 96
+    for m, n, k in ((130, 200, 96), (2050, 40, 72)):
+        _check_wide_range(m, n, k)
+
+
+def _check_wide_range(m, n, k):
     for dtype, gs, ss in ((torch.bfloat16, 1e-20, 1e-6), (torch.bfloat16, 1e15, 1e3), (torch.float16, 1e-3, 1e-5),
                           (torch.float16, 1e3, 1e-5), (torch.float16, 1e-4, 3e2), (torch.float32, 1e-15, 1e-10)):
         _say("wide", IDS[dtype], gs, ss)

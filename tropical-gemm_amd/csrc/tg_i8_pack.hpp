@@ -78,16 +78,22 @@ __global__ __launch_bounds__(1024) void tg_i8_scale_range(const float* __restric
     }
 }
 
-// v as 1 or 3 numbers of type D that add up to it: one rounding, or all of an
-// f32's 24 bits in three bf16 numbers.
+// v as 1 or 3 numbers of type D that add up to it: one rounding, or an f32's 24
+// bits cut into three bf16 numbers of eight (cut, not rounded: the largest
+// numbers stay finite, and it is less work).
 template <typename D, int PLANES>
 __device__ __forceinline__ void split_value(float v, D (&d)[PLANES]) {
-    d[0] = static_cast<D>(v);
-    if constexpr (PLANES == 3) {
-        // An infinity or NaN stays in the first.
-        const float r = fabsf(v) < __builtin_huge_valf() ? v - static_cast<float>(d[0]) : 0.0f;
-        d[1] = static_cast<D>(r);
-        d[2] = static_cast<D>(r - static_cast<float>(d[1]));
+    if constexpr (PLANES == 1) {
+        d[0] = static_cast<D>(v);
+    } else {
+        float r = v;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const uint32_t bits = __builtin_bit_cast(uint32_t, r);
+            d[i] = __builtin_bit_cast(D, uint16_t(bits >> 16));
+            r -= __builtin_bit_cast(float, bits & 0xffff0000u);
+            if (i == 0) r = fabsf(v) < __builtin_huge_valf() ? r : v != v ? v : 0.0f;  // an infinity stays in the first
+        }
     }
 }
 
