@@ -240,6 +240,23 @@ def test_matmul(m, n, k):
         _check_matmul(int8.matmul(a, sa, b, sb, bias, dtype), a, sa, b, sb, bias, dtype)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("m,n,k", [(8192, 4097, 128), (2048, 2049, 384), (4096, 2049, 128), (512, 4095, 640), (1024, 1023, 256)],
+                         ids=lambda v: str(v))
+def test_matmul_odd_columns(dtype, m, n, k):
+    """Rows of the output that start at any half of a word, in every tile size:
+    the same values as with one column more."""
+    _say("matmul odd columns", IDS[dtype], m, n, k)
+    a, sa = _int8(1, m, k, full=True)
+    b, sb = _int8(2, n + 1, k, full=True)
+    bias = torch.randn(n + 1, generator=_gen(3)).to(dtype).to(DEV)
+    even = int8.matmul(a, sa, b, sb, bias, dtype)
+    assert torch.equal(int8.matmul(a, sa, b[:n], sb[:n], bias[:n], dtype), even[:, :n])
+    rows = torch.tensor([0, 1, m // 2 + 1, m - 1])
+    want = (a[rows].cpu().double() @ b.cpu().double().t()) * sa[rows].cpu().double()[:, None] * sb.cpu().double() + bias.cpu().double()
+    assert torch.allclose(even[rows].cpu().double(), want, rtol=1e-5 if dtype == torch.float32 else 1e-2, atol=1e-4)
+
+
 @pytest.mark.parametrize("m,n", [(1, 40), (20, 40), (130, 70)])
 def test_matmul_largest_sums(m, n):
     """-128 * -128 over the longest k: 2^14 (2^17 - 1), just inside i32."""

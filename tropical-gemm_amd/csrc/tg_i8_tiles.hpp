@@ -335,8 +335,56 @@ struct Tile {
                 }
             }
         };
-        if (int64_t(tm + 1) * BM <= p.m && int64_t(tn + 1) * BN <= p.n) each(std::true_type());
+        const bool in = int64_t(tm + 1) * BM <= p.m && int64_t(tn + 1) * BN <= p.n;
+        if constexpr (Out::HALVES) {
+            if (in && out.odd_rows()) return halves(m0, n0, acc, out, x);
+        }
+        if (in) each(std::true_type());
         else each(std::false_type());
+    }
+
+    // The same for 16-bit outputs inside the matrix, where rows start at any
+    // half of a word: a store of 16 bytes at an odd half takes several times as
+    // long as one at a word, so a lane stores the whole words of its columns, the
+    // last with the next lane's first column (8-bit product of 8192 x 4097 x
+    // 1024: 64 us with the stores at halves, 54 so; with 4094 columns 48).
+    template <typename Out>
+    static __device__ __forceinline__ void halves(int m0, int n0, const Acc (&acc)[FM][FN], const Out& out,
+                                                  const Beside<Out>& x) {
+        constexpr int W = GROUPS * 4;
+        const int lg = threadIdx.x % 64 / FS;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            uint32_t w[W + 1];
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                Value v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = acc[i][(g * 8 + e) / VPF][(g * 8 + e) % VPF];
+                const u32x4 q = out.pack(v, x.rows[i], x.cols[g]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[g * 4 + e] = q[e];
+            }
+            w[W] = __shfl_down(w[0], FS);
+            char* to = out.at(m0 + i * FS, n0);
+            const int odd = int(reinterpret_cast<uintptr_t>(to) & 2);
+            if (odd != 0 && lg == 0) *reinterpret_cast<uint16_t*>(to) = uint16_t(w[0]);
+            uint32_t s[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) s[e] = __builtin_amdgcn_alignbyte(w[e + 1], w[e], odd);
+            to += odd;
+#pragma unroll
+            for (int g = 0; g + 1 < GROUPS; ++g)
+                *reinterpret_cast<u32x4_word*>(to + g * 16) = u32x4{s[g * 4], s[g * 4 + 1], s[g * 4 + 2], s[g * 4 + 3]};
+            to += (GROUPS - 1) * 16;
+            if (odd != 0 && lg == 3) {  // the next lane's columns are another wave's
+                *reinterpret_cast<u32x2_word*>(to) = u32x2{s[W - 4], s[W - 3]};
+                *reinterpret_cast<uint32_t*>(to + 8) = s[W - 2];
+                *reinterpret_cast<uint16_t*>(to + 12) = uint16_t(s[W - 1]);
+            } else {
+                *reinterpret_cast<u32x4_word*>(to) = u32x4{s[W - 4], s[W - 3], s[W - 2], s[W - 1]};
+            }
+        }
     }
 
     // The workgroup's tile over steps [s0, s1), from the sum to `out`.
@@ -368,6 +416,23 @@ struct TileStore {
     struct Cols {
         float scale[8], bias[8];
     };
+    static constexpr bool HALVES = sizeof(T) == 2;
+    // Not all rows start at a word.
+    __device__ __forceinline__ bool odd_rows() const { return n % 2 != 0 || reinterpret_cast<uintptr_t>(c) % 4 != 0; }
+    __device__ __forceinline__ char* at(int m, int col) const {
+        return reinterpret_cast<char*>(c + int64_t(m) * n + col);
+    }
+    // Eight 16-bit outputs.
+    template <typename V>
+    __device__ __forceinline__ u32x4 pack(const V (&x)[8], const Row& r, const Cols& c8) const {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        float v[8];
+        scaled(x, r, c8, v);
+        t8 t;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t[i] = static_cast<T>(v[i]);
+        return __builtin_bit_cast(u32x4, t);
+    }
     __device__ __forceinline__ Row row(int m) const { return {a_scale != nullptr ? a_scale[m] : 1.0f}; }
     __device__ __forceinline__ Cols cols(int col, int left) const {
         Cols c;
@@ -379,15 +444,19 @@ struct TileStore {
         return c;
     }
     template <typename V>
-    __device__ __forceinline__ void store(int m, int col, int left, const V (&x)[8], const Row& r,
-                                          const Cols& c8) const {
-        float v[8];
+    __device__ __forceinline__ void scaled(const V (&x)[8], const Row& r, const Cols& c8, float (&v)[8]) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = float(x[i]) * r.scale * c8.scale[i];
         if (bias != nullptr) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] += c8.bias[i];
         }
+    }
+    template <typename V>
+    __device__ __forceinline__ void store(int m, int col, int left, const V (&x)[8], const Row& r,
+                                          const Cols& c8) const {
+        float v[8];
+        scaled(x, r, c8, v);
         store_upto8(c + int64_t(m) * n + col, left, v);
     }
 };
@@ -395,6 +464,7 @@ struct TileStore {
 // Sums of a slice as they are, in rows of `ld` (a multiple of 8) 32-bit values.
 template <typename V>
 struct TilePartial {
+    static constexpr bool HALVES = false;
     V* c;
     int64_t ld;
     struct Row {};

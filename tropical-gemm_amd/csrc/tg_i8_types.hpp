@@ -16,6 +16,7 @@ using f16_t = _Float16;
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef uint32_t u32x4_word __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_word __attribute__((ext_vector_type(2), aligned(4)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
