@@ -358,7 +358,7 @@ int tg_i8_rms_norm(int device, tg_float type, tg_float weight_type, const void* 
  *   grad_weight = sum_i grad_y * xh            (of weight_type).
  * grad_h, the gradient that reaches h from elsewhere, may be NULL.  grad_x is
  * the gradient of x and of residual.  Sums are made in a fixed order: equal
- * calls give equal bits. */
+ * calls give equal bits.  cols is at most 2^24. */
 size_t tg_i8_rms_norm_backward_workspace_size(int64_t rows, int64_t cols);
 int tg_i8_rms_norm_backward(int device, tg_float type, tg_float weight_type, const void* grad_y,
                             int64_t ldg, const void* h, int64_t ldh, const void* weight, float eps,

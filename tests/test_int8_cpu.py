@@ -60,6 +60,7 @@ def test_dimensions(name, value, needle):
     ("tg_i8_rms_norm_backward", dict(ldg=7), "row stride of grad_y"),
     ("tg_i8_rms_norm_backward", dict(ldh=-8), "row stride of h"),
     ("tg_i8_rms_norm_backward", dict(ldgh=0), "row stride of grad_h"),
+    ("tg_i8_rms_norm_backward", dict(cols=(1 << 24) + 1, ldg=1 << 25, ldh=1 << 25, ldgh=1 << 25), "at most 2^24"),
     ("tg_i8_gemm", dict(lda=15), "row stride of a"),
     ("tg_i8_gemm", dict(ldb=15), "row stride of b"),
     ("tg_i8_gemm", dict(k=1 << 17, lda=1 << 17, ldb=1 << 17), "exact up to k = 131071"),

@@ -1,6 +1,6 @@
 // tg_i8_capi.hip -- C entry points of the 8-bit layer: argument checks (before
 // any HIP call), device selection and dispatch.
-#include <new>
+#include <exception>
 #include <string>
 
 #include "../../include/tropical_gemm_hip.h"
@@ -16,9 +16,14 @@ template <typename F>
 int guarded(F&& f) noexcept {
     try {
         return f();
+    } catch (const std::exception& e) {
+        try {
+            return host_fail(TG_ERR_DRIVER, e.what());
+        } catch (...) {
+        }
     } catch (...) {
-        return TG_ERR_DRIVER;
     }
+    return TG_ERR_DRIVER;
 }
 
 int bad_argument(const std::string& msg) { return host_fail(TG_ERR_INVALID_ARGUMENT, msg); }
