@@ -169,7 +169,8 @@ def _norm_grads(gy, h, w, eps, gh):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 4096), (3, 7), (70, 512), (700, 129), (33, 2048), (20, 8192),
-                                       (9, 8193), (5, 20011), (2500, 264), (1100, 2052)])
+                                       (9, 8193), (5, 20011), (2500, 264), (1100, 2052), (40, 9), (600, 4095), (300, 8190),
+                                       (700, 5001)])
 def test_rms_norm_backward(dtype, rows, cols):
     for wtype, residual in ((dtype, True), (torch.float32, False)):
         _say("rms_norm_backward", IDS[dtype], IDS[wtype], rows, cols, residual)

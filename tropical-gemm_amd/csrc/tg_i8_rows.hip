@@ -282,10 +282,13 @@ __global__ __launch_bounds__(256) void tg_i8_restore(const int8_t* __restrict__ 
 // that sum of each column to part[blockIdx.x].  The columns of a thread are as
 // in tg_i8_rows; its weights stay in registers, and the next row is loaded
 // before this one is reduced, so that loads are always on their way.  A row
-// longer than NT * VPT * 8 is shared by blockIdx.y; then every workgroup
-// reduces all of it.  bf16, 8192 x 4096 with gh: 49.9 us (277 MB with the
-// parts, 5.5 TB/s); f32, 777 x 2501: 11.1 us, two rows one after the other.
-template <typename T, typename W, bool GH, int NT, int VPT>
+// longer than NT * 8 is shared by blockIdx.y; then every workgroup reduces all
+// of it.  A row's last group is moved back to end with the row, as in
+// tg_i8_rows, so that no load waits for a branch (bf16, 8192 rows of 4095: 62 us
+// for the whole pass with branches, 45 so); TINY, rows below eight elements, is
+// one group with a bound.  bf16, 8192 x 4096 with gh: 48.7 us (277 MB with the
+// parts, 5.7 TB/s); f32, 777 x 2501: 11 us, two rows one after the other.
+template <typename T, typename W, bool GH, int NT, bool TINY>
 __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
     const T* __restrict__ gy, int64_t ldg, const T* __restrict__ h, int64_t ldh, const W* __restrict__ w,
     float eps, const T* __restrict__ gh, int64_t ldgh, T* __restrict__ gx, float* __restrict__ part,
@@ -293,37 +296,38 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
     constexpr int W64 = NT / 64;
     __shared__ float red[2][2][W64];
     const int t = threadIdx.x, wave = t / 64;
-    const int64_t base = int64_t(blockIdx.y) * (NT * VPT * 8);
-    auto at = [&](int k) { return base + int64_t(k * NT + t) * 8; };
-    float acc[VPT][8] = {}, wv[VPT][8];
-#pragma unroll
-    for (int k = 0; k < VPT; ++k)
-        if (at(k) < cols) load_upto8(w + at(k), int(cols - at(k) < 8 ? cols - at(k) : 8), wv[k]);
+    const int64_t base = int64_t(blockIdx.y) * (NT * 8), start = base + int64_t(t) * 8;
+    const int64_t at = TINY ? 0 : start <= cols - 8 ? start : cols - 8;
+    const bool live = start < cols;
+    const int again = live ? int(start - at) : 8;  // elements of the group before this one
+    const int n = TINY ? int(cols) : 8;
+    auto load8_of = [&](const auto* from, auto& x) {
+        if constexpr (TINY) x.load(from, n);
+        else x.load(from);
+    };
+    Eight<W> wv;
+    load8_of(w + at, wv);
+    float acc[8] = {};
     struct Row {
-        Eight<T> g[VPT], h[VPT], gh[VPT];
+        Eight<T> g, h, gh;
     } x[2];
     auto load = [&](int64_t row, Row& r) {
         if (row >= rows) return;
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            const int64_t left = cols - at(k);
-            if (left <= 0) continue;
-            r.g[k].load(gy + row * ldg + at(k), left);
-            r.h[k].load(h + row * ldh + at(k), left);
-            if constexpr (GH) r.gh[k].load(gh + row * ldgh + at(k), left);
-        }
+        load8_of(gy + row * ldg + at, r.g);
+        load8_of(h + row * ldh + at, r.h);
+        if constexpr (GH) load8_of(gh + row * ldgh + at, r.gh);
     };
     const float inv_n = 1.0f / float(cols);
     auto finish = [&](int64_t row, const Row& r, int flip) {
         float ss = 0.0f, dot = 0.0f;
         if (gridDim.y > 1) {  // the part of the row that other workgroups hold
             for (int64_t c = int64_t(t) * 8; c < cols; c += NT * 8) {
-                if (c >= base && c < base + NT * VPT * 8) continue;
-                const int n = cols - c < 8 ? int(cols - c) : 8;
+                if (c >= base && c < base + NT * 8) continue;
+                const int left = cols - c < 8 ? int(cols - c) : 8;
                 float a[8], b[8], d[8];
-                load_upto8(gy + row * ldg + c, n, a);
-                load_upto8(h + row * ldh + c, n, b);
-                load_upto8(w + c, n, d);
+                load_upto8(gy + row * ldg + c, left, a);
+                load_upto8(h + row * ldh + c, left, b);
+                load_upto8(w + c, left, d);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     ss += b[i] * b[i];
@@ -332,14 +336,10 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
             }
         }
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            if (at(k) >= cols) continue;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float hv = to_f32(r.h[k].v[i]);
-                ss += hv * hv;
-                dot += to_f32(r.g[k].v[i]) * wv[k][i] * hv;
-            }
+        for (int i = 0; i < 8; ++i) {
+            const float hv = i >= again ? to_f32(r.h.v[i]) : 0.0f;
+            ss += hv * hv;
+            dot += i >= again ? to_f32(r.g.v[i]) * to_f32(wv.v[i]) * hv : 0.0f;
         }
         ss = wave_sum(ss);
         dot = wave_sum(dot);
@@ -358,20 +358,15 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
         }
         const float rstd = 1.0f / sqrtf(ss * inv_n + eps);
         const float c = dot * inv_n * rstd * rstd;
+        float o[8];
 #pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            const int64_t left = cols - at(k);
-            if (left <= 0) continue;
-            float o[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float g = to_f32(r.g[k].v[i]), hv = to_f32(r.h[k].v[i]);
-                acc[k][i] += g * (hv * rstd);
-                o[i] = rstd * (g * wv[k][i] - hv * c);
-                if constexpr (GH) o[i] += to_f32(r.gh[k].v[i]);
-            }
-            store_upto8(gx + row * cols + at(k), left < 8 ? int(left) : 8, o);
+        for (int i = 0; i < 8; ++i) {
+            const float g = to_f32(r.g.v[i]), hv = to_f32(r.h.v[i]);
+            acc[i] += g * (hv * rstd);
+            o[i] = rstd * (g * to_f32(wv.v[i]) - hv * c);
+            if constexpr (GH) o[i] += to_f32(r.gh.v[i]);
         }
+        if (live) store_upto8(gx + row * cols + at, n, o);
     };
     const int64_t stride = gridDim.x;
     load(blockIdx.x, x[0]);
@@ -381,11 +376,7 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
         load(row + 2 * stride, x[0]);
         if (row + stride < rows) finish(row + stride, x[1], 1);
     }
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-        const int64_t left = cols - at(k);
-        if (left > 0) store_upto8(part + int64_t(blockIdx.x) * cols + at(k), left < 8 ? int(left) : 8, acc[k]);
-    }
+    if (live) store_upto8(part + int64_t(blockIdx.x) * cols + at, n, acc);
 }
 
 // gw[j] = sum over the parts: 64 slices of them, each in order, four of its
@@ -417,18 +408,21 @@ __global__ __launch_bounds__(1024) void tg_i8_sum_parts(const float* __restrict_
     }
 }
 
-// Workgroups along the rows, each with a part of the weight's gradient: two
-// for each CU (a part costs cols * 8 bytes of traffic, as much as a row's
-// gradient or two).
-int64_t backward_parts(int64_t rows) { return rows < 512 ? rows : 512; }
+// Workgroups along the rows, each with a part of the weight's gradient: as many
+// as the GPU holds at once, two for each CU, or one of 1024 threads (a part
+// costs cols * 8 bytes of traffic, as much as a row's gradient or two).
+int64_t backward_parts(int64_t rows, int64_t cols) {
+    const int64_t most = cols > 4096 ? 256 : 512;
+    return rows < most ? rows : most;
+}
 
-template <typename T, typename W, int NT, int VPT>
+template <typename T, typename W, int NT, bool TINY = false>
 hipError_t launch_norm_backward(const I8NormBackward& p, float* part, hipStream_t st) {
-    const int64_t parts = backward_parts(p.rows);
+    const int64_t parts = backward_parts(p.rows, p.cols);
     if (parts > 0) {
-        const dim3 grid(unsigned(parts), unsigned(ceil_div(p.cols, NT * VPT * 8)));
-        const auto kernel = p.grad_h != nullptr ? &tg_i8_norm_backward<T, W, true, NT, VPT>
-                                                : &tg_i8_norm_backward<T, W, false, NT, VPT>;
+        const dim3 grid(unsigned(parts), unsigned(ceil_div(p.cols, NT * 8)));
+        const auto kernel = p.grad_h != nullptr ? &tg_i8_norm_backward<T, W, true, NT, TINY>
+                                                : &tg_i8_norm_backward<T, W, false, NT, TINY>;
         hipLaunchKernelGGL(kernel, grid, dim3(NT), 0, st, static_cast<const T*>(p.grad_y), p.ldg,
                            static_cast<const T*>(p.h), p.ldh, static_cast<const W*>(p.weight), p.eps,
                            static_cast<const T*>(p.grad_h), p.ldgh, static_cast<T*>(p.grad_x), part, p.rows, p.cols);
@@ -443,11 +437,12 @@ hipError_t launch_norm_backward(const I8NormBackward& p, float* part, hipStream_
 template <typename T, typename W>
 hipError_t norm_backward_typed(const I8NormBackward& p, float* part, hipStream_t st) {
     const int64_t groups = ceil_div(p.cols, 8);
-    if (groups <= 64) return launch_norm_backward<T, W, 64, 1>(p, part, st);
-    if (groups <= 128) return launch_norm_backward<T, W, 128, 1>(p, part, st);
-    if (groups <= 256) return launch_norm_backward<T, W, 256, 1>(p, part, st);
-    if (groups <= 512) return launch_norm_backward<T, W, 512, 1>(p, part, st);
-    return launch_norm_backward<T, W, 1024, 1>(p, part, st);
+    if (p.cols < 8) return launch_norm_backward<T, W, 64, true>(p, part, st);
+    if (groups <= 64) return launch_norm_backward<T, W, 64>(p, part, st);
+    if (groups <= 128) return launch_norm_backward<T, W, 128>(p, part, st);
+    if (groups <= 256) return launch_norm_backward<T, W, 256>(p, part, st);
+    if (groups <= 512) return launch_norm_backward<T, W, 512>(p, part, st);
+    return launch_norm_backward<T, W, 1024>(p, part, st);
 }
 
 }  // namespace
@@ -481,7 +476,7 @@ hipError_t i8_dequantize(int type, const int8_t* q, int64_t ldq, const float* sc
 }
 
 size_t i8_rms_norm_backward_ws(int64_t rows, int64_t cols) {
-    return size_t(backward_parts(rows)) * size_t(cols) * sizeof(float);
+    return size_t(backward_parts(rows, cols)) * size_t(cols) * sizeof(float);
 }
 
 hipError_t i8_rms_norm_backward(const I8NormBackward& p, void* ws, hipStream_t st) {
