@@ -69,6 +69,19 @@ struct Eight {
     }
 };
 
+// v * 127 / top with one rounding: 127 / top as a sum of two numbers.  Where it
+// is a whole number and a half exactly, as for half of the row's maximum, the
+// result is too, and goes to the even neighbour; 127 / top rounded once misses
+// one such tie in twenty.
+struct Steps {
+    float hi, lo;
+    __device__ __forceinline__ explicit Steps(float top) {
+        hi = 127.0f / top;
+        lo = fmaf(-hi, top, 127.0f) / top;
+    }
+    __device__ __forceinline__ float of(float v) const { return fmaf(v, hi, v * lo); }
+};
+
 // h = round(x + residual); rstd = (mean h^2 + eps)^-1/2; v = h * w;
 // top = max(max |v|, tiny); q = rint(v * 127 / top); scale = top * rstd / 127.
 // rstd cancels in q, so q depends on no order of summation, and both
@@ -99,11 +112,11 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_i8_rows(const T* __restrict__ x
     const T* rr = RES ? res + row * ldr : nullptr;
     float sum = 0.0f, top = 0.0f;
 
-    auto give = [&](int64_t at, int n, const float(&v)[8], float inv) {
+    auto give = [&](int64_t at, int n, const float(&v)[8], const Steps& s) {
         int o[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int r = __float2int_rn(v[i] * inv);
+            const int r = __float2int_rn(s.of(v[i]));
             o[i] = r > 127 ? 127 : (r < -127 ? -127 : r);
         }
         store_i8_upto8(q + row * cols + at, n, o);
@@ -120,7 +133,7 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_i8_rows(const T* __restrict__ x
                 scale[row] = top / 127.0f;
             }
         }
-        return 127.0f / top;
+        return Steps(top);
     };
 
     if constexpr (VPT > 0) {
@@ -160,11 +173,11 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_i8_rows(const T* __restrict__ x
                 for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[g][i]));
             }
         }
-        const float inv = reduce();
+        const Steps steps = reduce();
         if (live) {
 #pragma unroll
             for (int g = 0; g < VPT; ++g)
-                if (start(g) < cols) give(from(g), 8, v[g], inv);
+                if (start(g) < cols) give(from(g), 8, v[g], steps);
         }
     } else {
         // One group: the (rounded) stream and its weighted values.
@@ -197,10 +210,10 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_i8_rows(const T* __restrict__ x
         };
         float v[8];
         each([&](int64_t at, int n) { take(at, n, v, true); });
-        const float inv = reduce();
+        const Steps steps = reduce();
         each([&](int64_t at, int n) {
             take(at, n, v, false);
-            give(at, n, v, inv);
+            give(at, n, v, steps);
         });
     }
 }
