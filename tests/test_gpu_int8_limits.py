@@ -56,3 +56,26 @@ def test_ties_go_to_the_even_integer(dtype):
     wide[:, :x.shape[1]] = x
     for q in (int8.quantize(x)[0], int8.rms_norm(x, ones)[0], int8.quantize(wide)[0][:, :x.shape[1]]):
         assert torch.equal(q.cpu().long(), want)
+
+
+@pytest.mark.parametrize("cols", [8193, 8194, 8195, 8196, 8197, 8198, 8199, 16385, 16391])
+def test_norm_backward_has_one_writer_for_each_column(cols):
+    """Rows shared by workgroups of 8192 columns, the last one's fewer than eight:
+    the columns before it belong to the workgroup before, bit for bit, and equal
+    calls give equal bits."""
+    rows, base = 3000, (cols - 1) // 8192 * 8192
+    _say("norm backward", rows, cols)
+    g, h = (torch.randn(rows, cols, generator=_gen(s)) * torch.exp(2 * torch.randn(rows, cols, generator=_gen(s + 2)))
+            for s in (1, 2))
+    w = torch.randn(cols, generator=_gen(5))
+    last = slice(cols - 8, base)  # columns whose group the last workgroup loads too
+    for t in (g, h, w):
+        t[..., last] = t[..., base - 8192:base - 8191]  # as the first column of their workgroup
+    g, h, w = g.to(DEV), h.to(DEV), w.to(DEV)
+    gx, gw = int8.rms_norm_backward(g, h, w)
+    first = slice(base - 8192, base - 8191)
+    assert torch.equal(gx[:, last], gx[:, first].expand_as(gx[:, last]))
+    assert torch.equal(gw[last], gw[first].expand_as(gw[last]))
+    for _ in range(3):
+        again = int8.rms_norm_backward(g, h, w)
+        assert torch.equal(gx, again[0]) and torch.equal(gw, again[1])

@@ -5,6 +5,8 @@
 // All of them are bound by HBM: every input element is read once, every
 // output written once, a row's values stay in registers between its reduction
 // and its output.  (A copy of 1 GiB reaches 4.95 TB/s on the same GPU.)
+#include <type_traits>
+
 #include "../../include/tropical_gemm_hip.h"
 #include "tg_i8.hpp"
 #include "tg_i8_types.hpp"
@@ -296,7 +298,8 @@ __global__ __launch_bounds__(256) void tg_i8_restore(const int8_t* __restrict__ 
 // in tg_i8_rows; its weights stay in registers, and the next row is loaded
 // before this one is reduced, so that loads are always on their way.  A row
 // longer than NT * 8 is shared by blockIdx.y; then every workgroup reduces all
-// of it.  A row's last group is moved back to end with the row, as in
+// of it, its own columns last, so that two of them may differ in the sums' last
+// bit: each column is stored by its own workgroup alone.  A row's last group is moved back to end with the row, as in
 // tg_i8_rows, so that no load waits for a branch (bf16, 8192 rows of 4095: 62 us
 // for the whole pass with branches, 45 so); TINY, rows below eight elements, is
 // one group with a bound.  bf16, 8192 x 4096 with gh: 48.7 us (277 MB with the
@@ -314,6 +317,16 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
     const bool live = start < cols;
     const int again = live ? int(start - at) : 8;  // elements of the group before this one
     const int n = TINY ? int(cols) : 8;
+    // Stores the thread's group, without the columns before the workgroup's first.
+    auto store = [&](auto* to, const float(&v)[8]) {
+        if (at >= base) {
+            store_upto8(to, n, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i >= again) to[i] = static_cast<std::remove_reference_t<decltype(*to)>>(v[i]);
+        }
+    };
     auto load8_of = [&](const auto* from, auto& x) {
         if constexpr (TINY) x.load(from, n);
         else x.load(from);
@@ -379,7 +392,7 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
             o[i] = rstd * (g * to_f32(wv.v[i]) - hv * c);
             if constexpr (GH) o[i] += to_f32(r.gh.v[i]);
         }
-        if (live) store_upto8(gx + row * cols + at, n, o);
+        if (live) store(gx + row * cols + at, o);
     };
     const int64_t stride = gridDim.x;
     load(blockIdx.x, x[0]);
@@ -389,7 +402,7 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
         load(row + 2 * stride, x[0]);
         if (row + stride < rows) finish(row + stride, x[1], 1);
     }
-    if (live) store_upto8(part + int64_t(blockIdx.x) * cols + at, n, acc);
+    if (live) store(part + int64_t(blockIdx.x) * cols + at, acc);
 }
 
 // gw[j] = sum over the parts: 64 slices of them, each in order, four of its
