@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from tropical_gemm import int8
+from tropical_gemm import pytorch as tgt
 
 pytestmark = pytest.mark.gpu
 
@@ -79,3 +80,12 @@ def test_norm_backward_has_one_writer_for_each_column(cols):
     for _ in range(3):
         again = int8.rms_norm_backward(g, h, w)
         assert torch.equal(gx, again[0]) and torch.equal(gw, again[1])
+
+
+def test_second_derivatives_are_refused():
+    x, w = (torch.randn(8, 16, generator=_gen(s)).to(DEV).requires_grad_() for s in (1, 2))
+    nw = torch.ones(16, device=DEV)
+    for y in (tgt.int8_linear_gpu(x, w), tgt.rms_norm_int8_linear_gpu(x, None, nw, w)[0]):
+        grad, = torch.autograd.grad(y.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="no second derivatives"):
+            (y.sum() + grad.square().sum()).backward()

@@ -233,10 +233,34 @@ def _prep_int8(name: str, x: torch.Tensor, weight: torch.Tensor):
     return x.detach().contiguous(), weight.detach().contiguous()
 
 
-def _int8_product_backward(ctx, grad, q, scale, qw, scale_w, want_x: bool, want_w: bool):
+def _int8_product_backward(grad, q, scale, qw, scale_w, want_x: bool, want_w: bool):
     grad = grad.contiguous()
     return (int8.backward_a(grad, qw, scale_w) if want_x else None,
             int8.backward_b(grad, q, scale) if want_w else None)
+
+
+class _FirstDerivative(torch.autograd.Function):
+    """A gradient as it is, whose own gradient is an error."""
+
+    @staticmethod
+    def forward(ctx, name: str, grad: torch.Tensor) -> torch.Tensor:
+        ctx.name = name
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"{ctx.name} has no second derivatives: its gradients cannot be differentiated again.")
+
+
+def _first_derivatives(name: str, *grads):
+    """The gradients of a backward pass whose kernels record nothing.  Where the
+    caller asked for a graph of that pass (``create_graph=True``), they are part
+    of one that refuses, or a loss that holds them would silently lack their
+    derivatives.  (``once_differentiable`` marks them only where the incoming
+    gradient needs one itself, which a loss's ones do not.)"""
+    if not torch.is_grad_enabled():
+        return grads
+    return tuple(g if g is None else _FirstDerivative.apply(name, g.detach().requires_grad_()) for g in grads)
 
 
 class Int8LinearGPU(torch.autograd.Function):
@@ -245,7 +269,8 @@ class Int8LinearGPU(torch.autograd.Function):
 
     The backward pass reads the 8-bit rows, which are all that is kept of the
     operands (half of bfloat16's bytes): the gradients are those of the product
-    of the rounded operands, passed through the rounding unchanged."""
+    of the rounded operands, passed through the rounding unchanged.  They have
+    no gradients of their own: differentiating them is an error."""
 
     @staticmethod
     def forward(ctx, x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
@@ -257,7 +282,9 @@ class Int8LinearGPU(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_y: torch.Tensor):
-        return _int8_product_backward(ctx, grad_y, *ctx.saved_tensors, *ctx.needs_input_grad)
+        with torch.no_grad():
+            grads = _int8_product_backward(grad_y, *ctx.saved_tensors, *ctx.needs_input_grad)
+        return _first_derivatives("Int8LinearGPU", *grads)
 
 
 class RmsNormInt8LinearGPU(torch.autograd.Function):
@@ -265,7 +292,8 @@ class RmsNormInt8LinearGPU(torch.autograd.Function):
     ``y = rms_norm(h, norm_weight, eps) @ weight.T``, the norm's output rounded
     to 8-bit rows as it is made and the weights to 8-bit rows beside it.
 
-    Kept for the backward pass: h, the 8-bit rows and the scales."""
+    Kept for the backward pass: h, the 8-bit rows and the scales.  The gradients
+    have no gradients of their own: differentiating them is an error."""
 
     @staticmethod
     def forward(ctx, x, residual, norm_weight, weight, eps: float = 1e-6):
@@ -289,11 +317,13 @@ class RmsNormInt8LinearGPU(torch.autograd.Function):
         want_norm = want_x or want_r or want_nw
         if grad_y is None:
             return grad_h, grad_h if want_r else None, None, None, None
-        grad_n, grad_w = _int8_product_backward(ctx, grad_y, q, scale, qw, scale_w, want_norm, want_w)
-        if not want_norm:
-            return None, None, None, grad_w, None
-        grad_h = None if grad_h is None else grad_h.contiguous()
-        grad_x, grad_nw = int8.rms_norm_backward(grad_n, h, norm_weight, ctx.eps, grad_h)
+        with torch.no_grad():
+            grad_n, grad_w = _int8_product_backward(grad_y, q, scale, qw, scale_w, want_norm, want_w)
+            grad_x = grad_nw = None
+            if want_norm:
+                grad_h = None if grad_h is None else grad_h.contiguous()
+                grad_x, grad_nw = int8.rms_norm_backward(grad_n, h, norm_weight, ctx.eps, grad_h)
+        grad_x, grad_nw, grad_w = _first_derivatives("RmsNormInt8LinearGPU", grad_x, grad_nw, grad_w)
         return grad_x, grad_x if want_r else None, grad_nw, grad_w, None
 
 
