@@ -89,3 +89,29 @@ def test_second_derivatives_are_refused():
         grad, = torch.autograd.grad(y.sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match="no second derivatives"):
             (y.sum() + grad.square().sum()).backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("m,n,k", [(2100, 296, 1030), (296, 2100, 1030), (1000, 72, 4096), (520, 4008, 1024), (70, 90, 100),
+                                   (300, 2100, 1030)], ids=lambda v: str(v))
+def test_infinite_scales_make_infinite_gradients(dtype, m, n, k):
+    """Where no term is zero, an infinite scale's term decides the sign, also in a
+    sum whose length is no whole number of steps."""
+    g = torch.rand(m, n, generator=_gen(1)) + 0.5
+    a, b = (torch.randint(1, 128, (r, k), generator=_gen(r)).to(torch.int8) for r in (m, n))
+    for at in (0, -1, -3, -9):
+        _say("infinite scale", IDS[dtype], m, n, k, at)
+        sa, sb = torch.full((m,), 0.01), torch.full((n,), 0.01)
+        sa[at] = sb[at] = float("inf")
+        g2, a2, b2 = g.clone(), a.clone(), b.clone()
+        g2[::2, at] *= -1
+        g2[at] *= -1
+        b2[at, ::3] *= -1
+        a2[at, ::3] *= -1
+        g2, a2, b2 = g2.to(dtype).to(DEV), a2.to(DEV), b2.to(DEV)
+        got = int8.backward_a(g2, b2, sb.to(DEV))
+        want = torch.sign(g2[:, at].float())[:, None] * torch.sign(b2[at].float()) * float("inf")
+        assert torch.equal(got.float(), want)
+        got = int8.backward_b(g2, a2, sa.to(DEV))
+        want = torch.sign(g2[at].float())[:, None] * torch.sign(a2[at].float()) * float("inf")
+        assert torch.equal(got.float(), want)

@@ -141,7 +141,7 @@ struct Tile {
 
         // Thread t loads place t % 8 of rows t / 8, t / 8 + NT / 8, ...; rows
         // past the matrix repeat its last one (their outputs are not stored),
-        // chunks past a partial last step repeat the last that counts (A's
+        // chunks past a partial last step repeat the last that counts (they
         // are cleared in registers before they are used).
         uint32_t off_a[LOADS_A], off_b[LOADS_B];
         auto chunk_a = [&](int i) { return (t % 8) ^ key_a(t / 8 + i * (NT / 8)); };
@@ -235,11 +235,16 @@ struct Tile {
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        // Clears the chunks of A's fragments that lie past the sum's end.
+        // Clears the fragments' chunks that lie past the sum's end: B's too but
+        // for integers, as an infinity there would make NaN of A's zeros.
         auto clear = [&](int h) {
             if ((lg + 4 * h) * 16 < p.tail) return;
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) xa[h][i] = u32x4{0, 0, 0, 0};
+            if constexpr (KIND != Mma::I8) {
+#pragma unroll
+                for (int j = 0; j < FN; ++j) xb[h][j] = u32x4{0, 0, 0, 0};
+            }
         };
         const std::true_type yes;
         const std::false_type no;
