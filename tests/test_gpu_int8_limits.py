@@ -115,3 +115,61 @@ def test_infinite_scales_make_infinite_gradients(dtype, m, n, k):
         got = int8.backward_b(g2, a2, sa.to(DEV))
         want = torch.sign(g2[at].float())[:, None] * torch.sign(a2[at].float()) * float("inf")
         assert torch.equal(got.float(), want)
+
+
+def _huge_rows(seed, rows, cols, dtype):
+    """Rows of ordinary values, of values whose squares pass f32, and of one such
+    value among ordinary ones, in turn."""
+    x = torch.randn(rows, cols, generator=_gen(seed))
+    x[1::4] *= 1e19
+    x[2::4] *= 5e36
+    x[3::4, cols // 2] = 3e20
+    return x.to(dtype)
+
+
+HUGE = [(6, 1), (9, 7), (9, 8), (33, 300), (10, 513), (21, 1025), (21, 2051), (10, 3081), (10, 4096), (10, 6145), (10, 8192),
+        (5, 8200), (5, 20011)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=IDS.get)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,cols", HUGE, ids=lambda v: str(v))
+def test_norm_of_huge_rows(dtype, residual, rows, cols):
+    """q within half a step (and f32's rounding of it), scales within 1e-5: f32 sums
+    of squares, as for ordinary rows."""
+    _say("norm of huge rows", IDS[dtype], rows, cols, residual)
+    x = _huge_rows(cols, rows, cols, dtype)
+    r = _huge_rows(cols + 1, rows, cols, dtype) if residual else None
+    w = (1 + 0.3 * torch.randn(cols, generator=_gen(3))).to(dtype)
+    q, scale, h = int8.rms_norm(x.to(DEV), w.to(DEV), None if r is None else r.to(DEV), 1e-5)
+    h64 = h.cpu().double()
+    assert torch.isfinite(h64).all()
+    want = h64 * ((h64 * h64).mean(1, keepdim=True) + 1e-5).rsqrt() * w.double()
+    step = want.abs().amax(1, keepdim=True) / 127
+    assert ((scale.cpu().double()[:, None] - step).abs() <= 1e-5 * step).all()
+    assert ((q.cpu().double() * step - want).abs() <= step * (0.5 + 127 * 4 * 2.0 ** -24 + 1e-9)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=IDS.get)
+@pytest.mark.parametrize("rows,cols", HUGE + [(1600, 264), (1025, 520), (1100, 4099), (600, 8195)], ids=lambda v: str(v))
+def test_norm_backward_of_huge_rows(dtype, rows, cols):
+    """Within 2e-5 of the magnitudes added, as for ordinary rows, then one rounding;
+    numbers below f32's normal ones within their last bit.  More rows than
+    workgroups, too."""
+    _say("norm backward of huge rows", IDS[dtype], rows, cols)
+    g = (torch.randn(rows, cols, generator=_gen(1)) * torch.exp(torch.randn(rows, 1, generator=_gen(2)))).to(dtype)
+    h = _huge_rows(cols, rows, cols, dtype)
+    w = (1 + 0.3 * torch.randn(cols, generator=_gen(3))).to(dtype)
+    gx, gw = int8.rms_norm_backward(g.to(DEV), h.to(DEV), w.to(DEV), 1e-5)
+    g64, h64, w64 = g.double(), h.double(), w.double()
+    rstd = ((h64 * h64).mean(1, keepdim=True) + 1e-5).rsqrt()
+    xh, u = h64 * rstd, g64 * w64
+    want = rstd * (u - xh * (u * xh).mean(1, keepdim=True))
+    size = rstd * (u.abs() + xh.abs() * (u * xh).abs().mean(1, keepdim=True))
+    unit = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    least = 2.0 ** -133 if dtype == torch.bfloat16 else 2.0 ** -148
+    assert ((gx.cpu().double() - want).abs() <= unit * want.abs() + 2e-5 * size + least).all()
+    want, size = (g64 * xh).sum(0), (g64 * xh).abs().sum(0)
+    again = int8.rms_norm_backward(g.to(DEV), h.to(DEV), w.to(DEV), 1e-5)
+    assert torch.equal(gx, again[0]) and torch.equal(gw, again[1])
+    assert ((gw.cpu().double() - want).abs() <= unit * want.abs() + 2e-5 * size).all()

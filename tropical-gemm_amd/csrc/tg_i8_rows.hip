@@ -25,6 +25,13 @@ constexpr int kRowsPerBlock = NT < 256 ? 256 / NT : 1;
 template <int NT>
 constexpr int kBlock = NT < 256 ? 256 : NT;
 
+// Squares of numbers above 2^64 pass f32.  A row whose sum of squares is not
+// finite is summed again with its values times kShrink: the largest, below
+// 2^128, become 2^48, of which 2^31 squares stay in f32, and the row's maximum,
+// at least 2^48 in a sum of 2^31 squares that passes 2^128, becomes 2^-32.
+constexpr float kHuge = __builtin_huge_valf();
+constexpr float kShrink = 0x1p-80f;
+
 // Reduces (sum, top) over the NT threads of each row; every thread gets both.
 template <int NT>
 __device__ __forceinline__ void row_reduce(float& sum, float& top) {
@@ -123,13 +130,36 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_i8_rows(const T* __restrict__ x
         }
         store_i8_upto8(q + row * cols + at, n, o);
     };
+    // The sum of squares of the row times kShrink; every wave makes it all.
+    auto shrunk_sum = [&] {
+        float s = 0.0f;
+        for (int64_t at = int64_t(threadIdx.x % 64) * 8; at < cols; at += 512) {
+            const int n = cols - at < 8 ? int(cols - at) : 8;
+            float v[8], r[8] = {};
+            load_upto8(xr + at, n, v);
+            if constexpr (RES) load_upto8(rr + at, n, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float hs = (RES ? to_f32(static_cast<T>(v[i] + r[i])) : v[i]) * kShrink;
+                s += hs * hs;
+            }
+        }
+        return wave_sum(s);
+    };
     // Reduces the row, stores its scale and gives 127 / top.
     auto reduce = [&] {
         row_reduce<NT>(sum, top);
         top = max_nan(top, kI8TinyTop);
+        float shrink = 1.0f;
+        if constexpr (NORM) {
+            if (live && !(sum < kHuge)) {
+                sum = shrunk_sum();
+                shrink = kShrink;
+            }
+        }
         if (live && t == 0) {
             if constexpr (NORM) {
-                const float rstd = 1.0f / sqrtf(sum / float(cols > 0 ? cols : 1) + eps);
+                const float rstd = shrink / sqrtf(sum / float(cols > 0 ? cols : 1) + eps * shrink * shrink);
                 scale[row] = top * rstd / 127.0f;
             } else {
                 scale[row] = top / 127.0f;
@@ -299,10 +329,10 @@ __global__ __launch_bounds__(256) void tg_i8_restore(const int8_t* __restrict__ 
 // before this one is reduced, so that loads are always on their way.  A row
 // longer than NT * 8 is shared by blockIdx.y; then every workgroup reduces all
 // of it, its own columns last, so that two of them may differ in the sums' last
-// bit: each column is stored by its own workgroup alone.  A row's last group is moved back to end with the row, as in
-// tg_i8_rows, so that no load waits for a branch (bf16, 8192 rows of 4095: 62 us
-// for the whole pass with branches, 45 so); TINY, rows below eight elements, is
-// one group with a bound.  bf16, 8192 x 4096 with gh: 48.7 us (277 MB with the
+// bit: each column is stored by its own workgroup alone.  A row's last group is
+// moved back to end with the row, as in tg_i8_rows, so that no load waits for a
+// branch (bf16, 8192 rows of 4095: 62 us for the whole pass with branches, 45
+// so); TINY, rows below eight elements, is one group with a bound.  bf16, 8192 x 4096 with gh: 48.7 us (277 MB with the
 // parts, 5.7 TB/s); f32, 777 x 2501: 11 us, two rows one after the other.
 template <typename T, typename W, bool GH, int NT, bool TINY>
 __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
@@ -344,8 +374,11 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
         if constexpr (GH) load8_of(gh + row * ldgh + at, r.gh);
     };
     const float inv_n = 1.0f / float(cols);
-    auto finish = [&](int64_t row, const Row& r, int flip) {
-        float ss = 0.0f, dot = 0.0f;
+    float ss = 0.0f, dot = 0.0f;
+    // The row's sums of h * h and u * h, of h times `shrink`, by way of
+    // red[slot]: never the same slot twice in turn, so that one barrier is enough.
+    auto sums = [&](int64_t row, const Row& r, float shrink, int slot) {
+        ss = dot = 0.0f;
         if (gridDim.y > 1) {  // the part of the row that other workgroups hold
             for (int64_t c = int64_t(t) * 8; c < cols; c += NT * 8) {
                 if (c >= base && c < base + NT * 8) continue;
@@ -356,14 +389,15 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
                 load_upto8(w + c, left, d);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    ss += b[i] * b[i];
-                    dot += a[i] * d[i] * b[i];
+                    const float hv = b[i] * shrink;
+                    ss += hv * hv;
+                    dot += a[i] * d[i] * hv;
                 }
             }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float hv = i >= again ? to_f32(r.h.v[i]) : 0.0f;
+            const float hv = i >= again ? to_f32(r.h.v[i]) * shrink : 0.0f;
             ss += hv * hv;
             dot += i >= again ? to_f32(r.g.v[i]) * to_f32(wv.v[i]) * hv : 0.0f;
         }
@@ -371,28 +405,37 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
         dot = wave_sum(dot);
         if constexpr (W64 > 1) {
             if (t % 64 == 0) {
-                red[flip][0][wave] = ss;
-                red[flip][1][wave] = dot;
+                red[slot][0][wave] = ss;
+                red[slot][1][wave] = dot;
             }
             __syncthreads();
             ss = dot = 0.0f;
 #pragma unroll
             for (int i = 0; i < W64; ++i) {
-                ss += red[flip][0][i];
-                dot += red[flip][1][i];
+                ss += red[slot][0][i];
+                dot += red[slot][1][i];
             }
         }
-        const float rstd = 1.0f / sqrtf(ss * inv_n + eps);
+    };
+    // Its part of the gradients.
+    auto give = [&](int64_t row, const Row& r, float shrink) {
+        const float rstd = 1.0f / sqrtf(ss * inv_n + eps * shrink * shrink);  // of h times `shrink`
         const float c = dot * inv_n * rstd * rstd;
         float o[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float g = to_f32(r.g.v[i]), hv = to_f32(r.h.v[i]);
+            const float g = to_f32(r.g.v[i]), hv = to_f32(r.h.v[i]) * shrink;
             acc[i] += g * (hv * rstd);
-            o[i] = rstd * (g * to_f32(wv.v[i]) - hv * c);
+            o[i] = rstd * shrink * (g * to_f32(wv.v[i]) - hv * c);
             if constexpr (GH) o[i] += to_f32(r.gh.v[i]);
         }
         if (live) store(gx + row * cols + at, o);
+    };
+    bool huge = false;
+    auto finish = [&](int64_t row, const Row& r, int flip) {
+        sums(row, r, 1.0f, flip);
+        huge |= !(ss < kHuge);
+        give(row, r, 1.0f);
     };
     const int64_t stride = gridDim.x;
     load(blockIdx.x, x[0]);
@@ -401,6 +444,20 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
         finish(row, x[0], 0);
         load(row + 2 * stride, x[0]);
         if (row + stride < rows) finish(row + stride, x[1], 1);
+    }
+    // Rows whose squares passed f32 had rstd 0, and nothing of them (or a NaN, of
+    // rows that are not finite) is in acc.  A second pass: as a branch of the
+    // first it makes the loads on their way wait (55 us there, 69).
+    if (huge) {  // the same in the whole workgroup
+        __syncthreads();
+        int slot = 0;  // another one each time, as above
+        for (int64_t row = blockIdx.x; row < rows; row += stride, slot ^= 1) {
+            load(row, x[0]);
+            sums(row, x[0], 1.0f, slot);
+            if (ss < kHuge) continue;
+            sums(row, x[0], kShrink, slot ^= 1);
+            give(row, x[0], kShrink);
+        }
     }
     if (live) store(part + int64_t(blockIdx.x) * cols + at, acc);
 }
