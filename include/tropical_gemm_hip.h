@@ -394,8 +394,10 @@ const char* tg_i8_backward_plan(tg_float type, int want_a, const void* grad_c, i
 /* grad_a[i, k] = sum_j grad_c[i, j] * b_scale[j] * b[j, k]: the gradient of
  * a[i, k] * a_scale[i].  grad_c is m x n and grad_a m x k, of type.  The sum
  * (over n; over m for grad_b) has at most 2^20 terms.  For bf16 and f16 the
- * dequantized b * b_scale is rounded to that type, for f32 nothing is rounded
- * but the f32 sums. */
+ * dequantized b * b_scale is rounded to that type's bits; where b_scale's finite
+ * values (above 2^-70) lie further apart than 2^20, which f16 does not hold,
+ * grad_c * b_scale is rounded to 16 bits instead, in about twice the time.  For
+ * f32, grad_c * b_scale is rounded to f32 and has to stay in its range. */
 size_t tg_i8_backward_a_workspace_size(tg_float type, const void* grad_c, int64_t ldg, int64_t m,
                                        int64_t n, int64_t k);
 int tg_i8_backward_a(int device, tg_float type, const void* grad_c, int64_t ldg, const int8_t* b,

@@ -173,3 +173,55 @@ def test_norm_backward_of_huge_rows(dtype, rows, cols):
     again = int8.rms_norm_backward(g.to(DEV), h.to(DEV), w.to(DEV), 1e-5)
     assert torch.equal(gx, again[0]) and torch.equal(gw, again[1])
     assert ((gw.cpu().double() - want).abs() <= unit * want.abs() + 2e-5 * size).all()
+
+
+F16_RANGES = [(64, 96, 80), (70, 90, 100), (300, 200, 264), (2100, 296, 1030), (296, 2100, 1030), (520, 4008, 1024),
+              (5000, 40, 72)]
+
+
+def _check_f16(got, g, x):
+    """Each term's factor rounded once (2^-11 of it) and f32 sums, then one rounding;
+    the 2-norm within 1.2 * 2^-11, as for the ordinary gradients."""
+    want, size = g @ x, g.abs() @ x.abs()
+    fine = want.abs() < 6e4
+    off = (got.cpu().double() - want)[fine]
+    u = 2.0 ** -11
+    assert fine.any() and torch.isfinite(got.cpu()[fine]).all()
+    assert (off.abs() <= ((1.01 * u + g.shape[1] * 2.0 ** -24) * size + u * want.abs())[fine] + 2.0 ** -24).all()
+    assert off.norm() <= 1.2 * u * want[fine].norm() + 2.0 ** -24 * off.numel() ** 0.5
+
+
+@pytest.mark.parametrize("m,n,k", F16_RANGES, ids=lambda v: str(v))
+@pytest.mark.parametrize("spread", [-100, -40, -19, 15, 19, 21, 30, 36, 60, 100])
+def test_f16_gradients_beside_a_scale_far_from_the_others(m, n, k, spread):
+    """One scale 2^spread times the others; a large one meets a gradient of zero, or
+    integers of zero (a padded position that holds anything)."""
+    g = torch.randn(m, n, generator=_gen(1)).half()
+    a, b = (torch.randint(-127, 128, (r, k), generator=_gen(r)).to(torch.int8) for r in (m, n))
+    sa, sb = (torch.rand(r, generator=_gen(r + 1)) * 0.02 + 1e-3 for r in (m, n))
+    sa[3] *= 2.0 ** spread
+    sb[3] *= 2.0 ** spread
+    for zero in ("gradient", "integers"):
+        _say("f16 range", m, n, k, spread, zero)
+        ga, gb, a2, b2 = g.clone(), g.clone(), a.clone(), b.clone()
+        if zero == "gradient":
+            ga[:, 3], gb[3] = 0, 0
+        else:
+            a2[3], b2[3] = 0, 0
+        f64 = lambda q, s: q.double() * s.double()[:, None]  # noqa: E731
+        _check_f16(int8.backward_a(ga.to(DEV), b2.to(DEV), sb.to(DEV)), ga.double(), f64(b2, sb))
+        _check_f16(int8.backward_b(gb.to(DEV), a2.to(DEV), sa.to(DEV)), gb.double().t(), f64(a2, sa))
+
+
+@pytest.mark.parametrize("m,n,k", F16_RANGES, ids=lambda v: str(v))
+def test_f16_gradients_of_terms_of_one_size_from_scales_of_many(m, n, k):
+    """Scales over 2^24 with gradients that make up for them: every term counts."""
+    _say("f16 balanced", m, n, k)
+    a, b = (torch.randint(-127, 128, (r, k), generator=_gen(r)).to(torch.int8) for r in (m, n))
+    ea, eb = (torch.randint(-12, 13, (r,), generator=_gen(r + 1)).double() for r in (m, n))
+    sa, sb = (0.01 * 2.0 ** -ea).float(), (0.01 * 2.0 ** -eb).float()
+    g = torch.randn(m, n, generator=_gen(1)).double()
+    ga, gb = (g * 2.0 ** eb).half(), (g * 2.0 ** ea[:, None]).half()
+    f64 = lambda q, s: q.double() * s.double()[:, None]  # noqa: E731
+    _check_f16(int8.backward_a(ga.to(DEV), b.to(DEV), sb.to(DEV)), ga.double(), f64(b, sb))
+    _check_f16(int8.backward_b(gb.to(DEV), a.to(DEV), sa.to(DEV)), gb.double().t(), f64(a, sa))

@@ -340,9 +340,10 @@ hipError_t gemm_typed(const I8Gemm& p, void* ws, hipStream_t st) {
 // sum; q is turned so that they run along it, in 16 bits, with its scales
 // multiplied in.  bf16 gradients: q * scale rounded to bf16 (as dequantizing
 // the operand to bf16 does; the result's error is that of its own rounding
-// times sqrt 2).  f16: q * scale * 2^e rounded to f16.  f32: q is exact in
-// bf16; G * scale becomes three bf16 planes that hold all its 24 bits, each
-// multiplied with q.
+// times sqrt 2).  f16: q * scale * 2^e rounded to f16, or G * scale as two bf16
+// planes where the scales' range is too wide for that (known on the GPU alone:
+// ScaleRange).  f32: q is exact in bf16; G * scale, rounded to f32, becomes three
+// bf16 planes that hold all its 24 bits, each multiplied with q.
 
 struct GradPlan {
     bool turn;  // one launch of tg_i8_turn
@@ -385,7 +386,7 @@ GradPlan plan_grad(const I8Grad& p) {
 
 struct GradWs {
     void *g, *q, *part;
-    float* range;
+    ScaleRange* range;
     size_t bytes;
 };
 
@@ -393,9 +394,10 @@ GradWs carve_grad(const I8Grad& p, const GradPlan& pl, void* ws) {
     Carver c{static_cast<char*>(ws)};
     GradWs w{};
     if (p.rows == 0 || p.cols == 0 || p.depth == 0 || pl.turn) return w;
-    if (pl.pack_g) w.g = c.take(size_t(p.rows) * size_t(pl.depth) * size_t(pl.planes) * 2);
+    const int planes = p.type == TG_F16 ? 2 : pl.planes;  // f16: in case the range is wide
+    if (pl.pack_g || planes > 1) w.g = c.take(size_t(p.rows) * size_t(pl.depth) * size_t(planes) * 2);
     w.q = c.take(size_t(p.cols) * size_t(pl.depth) * 2);
-    if (p.type == TG_F16) w.range = static_cast<float*>(c.take(8));
+    if (p.type == TG_F16) w.range = static_cast<ScaleRange*>(c.take(sizeof(ScaleRange)));
     w.part = c.take(part_bytes(pl.tiles, p.rows, p.cols));
     w.bytes = c.used;
     return w;
@@ -413,41 +415,68 @@ hipError_t launch_turn(const I8Grad& p, const TileStore<T>& out, hipStream_t st)
     return hipGetLastError();
 }
 
+// Lays out q in `D` and, where it has to be, G in PLANES planes of D.
+template <typename T, typename D, int PLANES>
+hipError_t pack_grad(const I8Grad& p, const GradPlan& pl, const GradWs& w, hipStream_t st) {
+    const T* g = static_cast<const T*>(p.g);
+    const float* scale_g = PLANES > 1 ? p.scale : nullptr;  // the scales go with one operand
+    const PackTurned<int8_t, D, 1> q{p.q, p.ldq, p.depth, p.cols, PLANES > 1 ? nullptr : p.scale, nullptr, static_cast<D*>(w.q), pl.depth};
+    if (!pl.pack_g) return launch_pack(q, PackNothing(), st);
+    if (p.transposed)
+        return launch_pack(q, PackTurned<T, D, PLANES>{g, p.ldg, p.depth, p.rows, scale_g, nullptr, static_cast<D*>(w.g), pl.depth}, st);
+    if constexpr (PLANES > 1)
+        return launch_pack(q, PackSplit<T, PLANES>{g, p.ldg, p.rows, p.depth, p.scale, static_cast<D*>(w.g), pl.depth}, st);
+    else
+        return launch_pack(q, bytes_job(p.g, p.ldg * 2, p.rows, p.depth * 2, w.g, pl.depth * 2), st);
+}
+
+// f16: one way or the other by the scales' range.
+hipError_t pack_grad_f16(const I8Grad& p, const GradPlan& pl, const GradWs& w, hipStream_t st) {
+    const f16_t* g = static_cast<const f16_t*>(p.g);
+    bf16_t* wide_g = static_cast<bf16_t*>(w.g);
+    using Narrow = PackTurned<int8_t, f16_t, 1>;
+    using Wide = PackTurned<int8_t, bf16_t, 1>;
+    const PackEither<Narrow, Wide> q{
+        Narrow{p.q, p.ldq, p.depth, p.cols, p.scale, &w.range->factor, static_cast<f16_t*>(w.q), pl.depth},
+        Wide{p.q, p.ldq, p.depth, p.cols, nullptr, nullptr, static_cast<bf16_t*>(w.q), pl.depth}, w.range};
+    if (pl.pack_g && p.transposed) {
+        using NarrowG = PackTurned<f16_t, f16_t, 1>;
+        using WideG = PackTurned<f16_t, bf16_t, 2>;
+        return launch_pack(q,
+                           PackEither<NarrowG, WideG>{
+                               NarrowG{g, p.ldg, p.depth, p.rows, nullptr, nullptr, static_cast<f16_t*>(w.g), pl.depth},
+                               WideG{g, p.ldg, p.depth, p.rows, p.scale, nullptr, wide_g, pl.depth}, w.range},
+                           st);
+    }
+    const PackSplit<f16_t, 2> wide{g, p.ldg, p.rows, p.depth, p.scale, wide_g, pl.depth};
+    if (!pl.pack_g) return launch_pack(q, PackEither<PackNothing, PackSplit<f16_t, 2>>{{}, wide, w.range}, st);
+    const PackBytes narrow = bytes_job(p.g, p.ldg * 2, p.rows, p.depth * 2, w.g, pl.depth * 2);
+    return launch_pack(q, PackEither<PackBytes, PackSplit<f16_t, 2>>{narrow, wide, w.range}, st);
+}
+
 template <typename T>
 hipError_t grad_typed(const I8Grad& p, void* ws, hipStream_t st) {
-    constexpr bool F32 = std::is_same<T, float>::value;
-    using D = std::conditional_t<std::is_same<T, f16_t>::value, f16_t, bf16_t>;
+    constexpr bool F32 = std::is_same<T, float>::value, F16 = std::is_same<T, f16_t>::value;
     TileStore<T> out{nullptr, nullptr, nullptr, nullptr, static_cast<T*>(p.out), p.cols};
     if (p.depth == 0) return launch_join<float>(nullptr, 0, p.rows, p.cols, out, st);
     const GradPlan pl = plan_grad(p);
     if (pl.turn) return p.transposed ? launch_turn<T, true>(p, out, st) : launch_turn<T, false>(p, out, st);
     const GradWs w = carve_grad(p, pl, ws);
     hipError_t e = hipSuccess;
-    if (p.type == TG_F16) {
+    TileArgs t{};
+    if constexpr (F16) {
         hipLaunchKernelGGL(tg_i8_scale_range, dim3(1), dim3(1024), 0, st, p.scale, p.depth, w.range);
         e = hipGetLastError();
-        out.all = w.range + 1;
-    }
-    if (e != hipSuccess) return e;
-    const PackTurned<int8_t, D, 1> q{p.q, p.ldq, p.depth, p.cols, F32 ? nullptr : p.scale,
-                                     p.type == TG_F16 ? w.range : nullptr, static_cast<D*>(w.q), pl.depth};
-    if (!pl.pack_g) {
-        e = launch_pack(q, PackNothing(), st);
-    } else if (p.transposed) {
-        e = launch_pack(q,
-                        PackTurned<T, D, F32 ? 3 : 1>{static_cast<const T*>(p.g), p.ldg, p.depth, p.rows,
-                                                      F32 ? p.scale : nullptr, nullptr, static_cast<D*>(w.g), pl.depth},
-                        st);
-    } else if constexpr (F32) {
-        e = launch_pack(q,
-                        PackSplit{static_cast<const float*>(p.g), p.ldg, p.rows, p.depth, p.scale,
-                                  static_cast<bf16_t*>(w.g), pl.depth},
-                        st);
+        if (e != hipSuccess) return e;
+        out.all = &w.range->back;
+        t.wide = &w.range->wide;
+        t.wide_a = static_cast<const char*>(w.g);
+        t.wide_lda = pl.depth * 2 * 2;
+        e = pack_grad_f16(p, pl, w, st);
     } else {
-        e = launch_pack(q, bytes_job(p.g, p.ldg * 2, p.rows, p.depth * 2, w.g, pl.depth * 2), st);
+        e = pack_grad<T, bf16_t, F32 ? 3 : 1>(p, pl, w, st);
     }
     if (e != hipSuccess) return e;
-    TileArgs t{};
     t.a = static_cast<const char*>(pl.pack_g ? w.g : p.g);
     t.b = static_cast<const char*>(w.q);
     t.lda = pl.pack_g ? pl.depth * pl.planes * 2 : p.ldg * 2;
@@ -457,7 +486,7 @@ hipError_t grad_typed(const I8Grad& p, void* ws, hipStream_t st) {
     t.b_steps = int(pl.depth / 64);
     t.plane = pl.depth * 2;
     t.tail = pl.pack_g || p.depth % 64 == 0 ? 128 : int(p.depth % 64 * 2);
-    return launch_tiles<std::is_same<D, f16_t>::value ? Mma::F16 : Mma::BF16>(t, pl.tiles, out, w.part, st);
+    return launch_tiles<F16 ? Mma::F16 : Mma::BF16>(t, pl.tiles, out, w.part, st);
 }
 
 // The tiles' part of a plan's name.

@@ -51,8 +51,8 @@ __device__ __forceinline__ float finite_size(float s) {
 }
 
 // e such that top * 2^e lies in [64, 128) (0 for top 0; |e| at most 120), for
-// products q * scale * 2^e in f16 with top the largest scale: at most 127 *
-// 128, and with all of f16's bits down to 2^-21 of the largest scale.
+// products q * scale * 2^e in f16 with top the largest scale: at most 128 *
+// 128, and with all of f16's bits down to 2^-20 of the largest scale.
 __device__ __forceinline__ int range_exponent(float top) {
     if (!(top > 0.0f)) return 0;
     int e = 0;
@@ -61,26 +61,56 @@ __device__ __forceinline__ int range_exponent(float top) {
     return e > 120 ? 120 : e < -120 ? -120 : e;
 }
 
-// 2^e for all the scales, and its inverse.
+// What f16 gradients take of their scales: q * scale * 2^e in f16 where no scale
+// that matters lies further than 2^20 below the largest.  Otherwise, `wide`, q
+// stays an integer (exact in bf16) and the gradient times its scales becomes two
+// bf16 planes, 16 bits of any size, for twice the products (8192 x 4096 x 4096:
+// 403 us instead of 223, 407 instead of 249).  Only the GPU knows which: every
+// kernel behind this one looks.
+//
+// Scales below 2^-70 do not matter: |g| < 2^16, |q| <= 2^7, and 2^20 such terms
+// stay below 2^-27, an eighth of f16's least number.
+struct ScaleRange {
+    float factor, back;  // 2^e and its inverse (1 for `wide`)
+    int wide;
+};
+constexpr float kLeastScale = 0x1p-70f;
+__device__ __forceinline__ void add_scale(float s, float& top, float& low) {
+    s = finite_size(s);
+    top = fmaxf(top, s);
+    if (s >= kLeastScale) low = fminf(low, s);
+}
+__device__ __forceinline__ ScaleRange scale_range(float top, float low) {
+    const int e = range_exponent(top);
+    const bool wide = low < top * 0x1p-20f;
+    return {ldexpf(1.0f, e), wide ? 1.0f : ldexpf(1.0f, -e), wide};
+}
+
+// The range of all the scales.
 __global__ __launch_bounds__(1024) void tg_i8_scale_range(const float* __restrict__ scale, int64_t n,
-                                                          float* __restrict__ out) {
-    __shared__ float part[16];
-    float top = 0.0f;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) top = fmaxf(top, finite_size(scale[i]));
+                                                          ScaleRange* __restrict__ out) {
+    __shared__ float part[2][16];
+    float top = 0.0f, low = __builtin_huge_valf();
+    for (int64_t i = threadIdx.x; i < n; i += 1024) add_scale(scale[i], top, low);
     top = wave_max(top);
-    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = top;
+    low = -wave_max(-low);
+    if (threadIdx.x % 64 == 0) {
+        part[0][threadIdx.x / 64] = top;
+        part[1][threadIdx.x / 64] = low;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, part[i]);
-        const int e = range_exponent(top);
-        out[0] = ldexpf(1.0f, e);
-        out[1] = ldexpf(1.0f, -e);
+        for (int i = 1; i < 16; ++i) {
+            top = fmaxf(top, part[0][i]);
+            low = fminf(low, part[1][i]);
+        }
+        *out = scale_range(top, low);
     }
 }
 
-// v as 1 or 3 numbers of type D that add up to it: one rounding, or an f32's 24
-// bits cut into three bf16 numbers of eight (cut, not rounded: the largest
-// numbers stay finite, and it is less work).
+// v as 1 to 3 numbers of type D that add up to it: one rounding, an f32's first
+// 16 bits as two bf16 numbers, or its 24 bits as three (cut, not rounded, but for
+// the second of two: the largest numbers stay finite, and it is less work).
 template <typename D, int PLANES>
 __device__ __forceinline__ void split_value(float v, D (&d)[PLANES]) {
     if constexpr (PLANES == 1) {
@@ -88,9 +118,9 @@ __device__ __forceinline__ void split_value(float v, D (&d)[PLANES]) {
     } else {
         float r = v;
 #pragma unroll
-        for (int i = 0; i < 3; ++i) {
+        for (int i = 0; i < PLANES; ++i) {
             const uint32_t bits = __builtin_bit_cast(uint32_t, r);
-            d[i] = __builtin_bit_cast(D, uint16_t(bits >> 16));
+            d[i] = PLANES == 2 && i == 1 ? static_cast<D>(r) : __builtin_bit_cast(D, uint16_t(bits >> 16));
             r -= __builtin_bit_cast(float, bits & 0xffff0000u);
             if (i == 0) r = fabsf(v) < __builtin_huge_valf() ? r : v != v ? v : 0.0f;  // an infinity stays in the first
         }
@@ -165,10 +195,11 @@ struct PackTurned {
     }
 };
 
-// f32 rows as three bf16 planes each: dst[i][p][r] from src[i][r] * scale[r].
+// Rows as PLANES bf16 planes each: dst[i][p][r] from src[i][r] * scale[r].
+template <typename S, int PLANES>
 struct PackSplit {
     static constexpr int kLdsWords = 1;
-    const float* src;
+    const S* src;
     int64_t ld_src, rows, cols;
     const float* scale;
     bf16_t* dst;
@@ -187,19 +218,37 @@ struct PackSplit {
                 load_upto8(src + row * ld_src + at, left, v);
                 load_upto8(scale + at, left, s);
             }
-            bf16_t d[8][3];
+            bf16_t d[8][PLANES];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) split_value<bf16_t, 3>(v[e] * s[e], d[e]);
+            for (int e = 0; e < 8; ++e) split_value<bf16_t, PLANES>(v[e] * s[e], d[e]);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) {
+            for (int p = 0; p < PLANES; ++p) {
                 u32x4 w;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     w[e] = uint32_t(__builtin_bit_cast(uint16_t, d[2 * e][p])) |
                            uint32_t(__builtin_bit_cast(uint16_t, d[2 * e + 1][p])) << 16;
-                *reinterpret_cast<u32x4*>(dst + (row * 3 + p) * depth + at) = w;
+                *reinterpret_cast<u32x4*>(dst + (row * PLANES + p) * depth + at) = w;
             }
         }
+    }
+};
+
+// Job n, or w where the scales' range is wide: both of as many workgroups, or
+// each fit for any number of them.  Where n is nothing, few workgroups look.
+template <typename N, typename W>
+struct PackEither {
+    static constexpr int kLdsWords = N::kLdsWords > W::kLdsWords ? N::kLdsWords : W::kLdsWords;
+    N n;
+    W w;
+    const ScaleRange* range;
+    int64_t blocks() const {
+        const int64_t a = n.blocks(), b = w.blocks();
+        return a > 0 ? a : b < 2048 ? b : 2048;
+    }
+    __device__ __forceinline__ void run(int block, int count, uint32_t* lds) const {
+        if (range->wide != 0) w.run(block, count, lds);
+        else n.run(block, count, lds);
     }
 };
 

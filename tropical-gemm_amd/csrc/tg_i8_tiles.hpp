@@ -75,6 +75,9 @@ struct TileArgs {
     int64_t plane;      // bytes between the planes of a row of A
     int tiles_m, tiles_n;
     int slice;          // steps of one blockIdx.y (tg_i8_tiles_slice)
+    const int* wide;    // f16: where it is not 0, A is two bf16 planes in a row of wide_a, B is bf16
+    const char* wide_a;
+    int64_t wide_lda;
 };
 
 // Tile of a workgroup: WM x WN waves, each FM x FN fragments of 16 x 16.
@@ -392,9 +395,10 @@ struct Tile {
         }
     }
 
-    // The workgroup's tile over steps [s0, s1), from the sum to `out`.
+    // The workgroup's tile over slice `y` of the sum, from there to `out`.
     template <typename Out>
-    static __device__ __forceinline__ void whole(const TileArgs& p, int s0, int s1, char* smem, const Out& out) {
+    static __device__ __forceinline__ void whole(const TileArgs& p, int y, char* smem, const Out& out) {
+        const int s0 = y * p.slice, s1 = s0 + p.slice < p.steps ? s0 + p.slice : p.steps;
         Acc acc[FM][FN] = {};
         Beside<Out> x;
         int tm, tn;
@@ -484,10 +488,28 @@ struct TilePartial {
     }
 };
 
+// Slice `y` of the sum on KIND's instructions, or on bf16's where f16 operands
+// have been laid out as such.
+template <Mma KIND, int WM, int WN, int FM, int FN, int NB, int P, typename Out>
+__device__ __forceinline__ void tiles_slice(TileArgs p, int y, char* smem, const Out& out) {
+    if constexpr (KIND == Mma::F16) {
+        if (*p.wide != 0) {
+            p.a = p.wide_a;
+            p.lda = p.wide_lda;
+            p.steps *= 2;
+            p.slice *= 2;
+            p.tail = 128;
+            Tile<Mma::BF16, WM, WN, FM, FN, NB, P>::whole(p, y, smem, out);
+            return;
+        }
+    }
+    Tile<KIND, WM, WN, FM, FN, NB, P>::whole(p, y, smem, out);
+}
+
 template <Mma KIND, int WM, int WN, int FM, int FN, int NB, int P, int PER_CU, typename T>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_i8_tiles(TileArgs p, TileStore<T> out) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    Tile<KIND, WM, WN, FM, FN, NB, P>::whole(p, 0, p.steps, smem, out);
+    tiles_slice<KIND, WM, WN, FM, FN, NB, P>(p, 0, smem, out);
 }
 
 // Slice blockIdx.y of the sum: its sums to part + blockIdx.y * M * ld.
@@ -495,9 +517,8 @@ template <Mma KIND, int WM, int WN, int FM, int FN, int NB, int P, int PER_CU>
 __global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_i8_tiles_slice(
     TileArgs p, TilePartial<typename Tile<KIND, WM, WN, FM, FN, NB, P>::Value> out) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const int s0 = int(blockIdx.y) * p.slice, s1 = s0 + p.slice < p.steps ? s0 + p.slice : p.steps;
     out.c += int64_t(blockIdx.y) * p.m * out.ld;
-    Tile<KIND, WM, WN, FM, FN, NB, P>::whole(p, s0, s1, smem, out);
+    tiles_slice<KIND, WM, WN, FM, FN, NB, P>(p, int(blockIdx.y), smem, out);
 }
 
 // C from the slices' sums, added in their order (none: an empty sum).

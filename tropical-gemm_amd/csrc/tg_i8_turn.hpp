@@ -50,12 +50,17 @@ __device__ __forceinline__ u32x2 turn_read(const lds_t* at) {
 // Values past the matrices' edges are not stored and may be anything; a line's
 // 16 bytes that would end past it are its last ones, shifted into place.  Terms
 // past the sum's end are zeros of both operands.
-template <typename T, bool TRANS>
+//
+// WIDE: f16 of a wide range of scales (ScaleRange), G as two bf16 planes: up to
+// 2.6 times as long (1024 x 1024 x 1024: 29 us and 20 for 11.6 and 12.0).
+template <typename T, bool TRANS, bool WIDE = false>
 struct Turn {
     static constexpr bool F32 = std::is_same<T, float>::value, F16 = std::is_same<T, f16_t>::value;
-    using D = std::conditional_t<F16, f16_t, bf16_t>;
-    static constexpr int P = F32 ? 3 : 1, SIZE = sizeof(T);
-    static constexpr Mma KIND = F16 ? Mma::F16 : Mma::BF16;
+    using D = std::conditional_t<F16 && !WIDE, f16_t, bf16_t>;
+    // Planes of G; more than one: G takes the scales, q stays an integer.
+    static constexpr int P = F32 ? 3 : WIDE ? 2 : 1, SIZE = sizeof(T);
+    static constexpr bool SPLIT = P > 1;
+    static constexpr Mma KIND = std::is_same<D, f16_t>::value ? Mma::F16 : Mma::BF16;
     using Shape = Tile<KIND, 4, 2, 1, 2, 2>;  // places and stores of the outputs
     using Acc = typename Shape::Acc;
     static constexpr int NT = 512, ROW = 160, PLANE = TRANS ? 64 * ROW : 64 * 128, STAGE = P * PLANE + 64 * ROW;
@@ -67,12 +72,11 @@ struct Turn {
     struct Raw {
         u32x2 q;
         u32x4 g[LOADS];
-        float s;                                   // of q's term
-        float sg[F32 ? (TRANS ? LOADS : PER) : 1];  // of G's terms
+        float s;                                     // of q's term
+        float sg[SPLIT ? (TRANS ? LOADS : PER) : 1];  // of G's terms
     };
 
     typedef __attribute__((address_space(3))) u32x4* put16_t;
-    typedef __attribute__((address_space(3))) u32x2* put8_t;
 
     // 16 bytes of a line of `count` elements from element `at` on, or its last.
     template <typename E>
@@ -136,13 +140,13 @@ struct Turn {
             }
         }
         x.s = p.scale[r0 + t / 8 < last ? r0 + t / 8 : last];
-        if constexpr (F32 && TRANS) {
+        if constexpr (SPLIT && TRANS) {
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int r = r0 + t / CHUNKS + i * LINES;
                 x.sg[i] = p.scale[r < last ? r : last];
             }
-        } else if constexpr (F32) {
+        } else if constexpr (SPLIT) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) x.sg[i] = p.scale[r0 + at + i < last ? r0 + at + i : last];
         }
@@ -159,11 +163,14 @@ struct Turn {
     static __device__ __forceinline__ void put_step(const TurnArgs& p, int m0, int n0, int r0, lds_t* stage,
                                                     float factor, const Raw& x) {
         typedef D d8 __attribute__((ext_vector_type(8)));
-        typedef D d4 __attribute__((ext_vector_type(4)));
+        typedef D d_per __attribute__((ext_vector_type(PER)));
+        typedef T t_per __attribute__((ext_vector_type(PER)));
+        typedef std::conditional_t<PER == 8, u32x4, u32x2> words;
+        typedef __attribute__((address_space(3))) words* put_t;
         const int t = threadIdx.x;
         {
             u32x2 w = x.q;
-            float s = F32 ? 1.0f : x.s * factor;
+            float s = SPLIT ? 1.0f : x.s * factor;
             if constexpr (!INSIDE) {
                 const int past = n0 + t % 8 * 8 + 8 - p.n;
                 const uint64_t all = __builtin_bit_cast(uint64_t, w);
@@ -189,21 +196,21 @@ struct Turn {
             }
             const int chunk = at / 8;
             lds_t* to = stage + (TRANS ? line * ROW + chunk * 16 : line * 128 + ((chunk ^ (line & 7)) << 4));
-            if constexpr (F32) {
-                const f32x4 f = __builtin_bit_cast(f32x4, w);
-                d4 d[3];
+            if constexpr (SPLIT) {
+                const t_per f = __builtin_bit_cast(t_per, w);
+                d_per d[P];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < PER; ++e) {
                     // A term past the end is zero whatever its scale.
                     const bool live = INSIDE || (TRANS ? r0 + line < p.depth : r0 + at + e < p.depth);
-                    D part[3];
-                    split_value<D, 3>(live ? f[e] * x.sg[TRANS ? i : e] : 0.0f, part);
+                    D part[P];
+                    split_value<D, P>(live ? to_f32(f[e]) * x.sg[TRANS ? i : e] : 0.0f, part);
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) d[k][e] = part[k];
+                    for (int k = 0; k < P; ++k) d[k][e] = part[k];
                 }
 #pragma unroll
-                for (int k = 0; k < 3; ++k)
-                    *reinterpret_cast<put8_t>(to + k * PLANE + at % 8 * 2) = __builtin_bit_cast(u32x2, d[k]);
+                for (int k = 0; k < P; ++k)
+                    *reinterpret_cast<put_t>(to + k * PLANE + at % 8 * 2) = __builtin_bit_cast(words, d[k]);
             } else {
                 *reinterpret_cast<put16_t>(to) = w;
             }
@@ -243,6 +250,44 @@ struct Turn {
     }
 };
 
+// The range of a sum's scales, as tg_i8_scale_range finds it, in every workgroup.
+__device__ __forceinline__ ScaleRange turn_range(const TurnArgs& p) {
+    __shared__ float part[2][8];
+    float top = 0.0f, low = __builtin_huge_valf();
+    for (int i = threadIdx.x; i < p.depth; i += 512) add_scale(p.scale[i], top, low);
+    top = wave_max(top);
+    low = -wave_max(-low);
+    if (threadIdx.x % 64 == 0) {
+        part[0][threadIdx.x / 64] = top;
+        part[1][threadIdx.x / 64] = low;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        top = fmaxf(top, part[0][i]);
+        low = fminf(low, part[1][i]);
+    }
+    return scale_range(top, low);
+}
+
+// The sum of a wide range, without haste: one step's operands at a time in the
+// LDS that the other way's two take.
+template <bool TRANS>
+__device__ __forceinline__ void turn_wide(const TurnArgs& p, int m0, int n0, lds_t* lds,
+                                          typename Turn<f16_t, TRANS, true>::Acc (&acc)[1][2]) {
+    using Cfg = Turn<f16_t, TRANS, true>;
+    static_assert(Cfg::STAGE <= Turn<f16_t, TRANS>::LDS, "one stage");
+    const typename Cfg::Lines l = Cfg::lines(p, m0, n0);
+    for (int r0 = 0; r0 < p.depth; r0 += 64) {
+        typename Cfg::Raw x;
+        Cfg::load(p, m0, n0, r0, l, x);
+        Cfg::put(p, m0, n0, r0, lds, 1.0f, x);
+        __syncthreads();
+        Cfg::products(lds, acc);
+        __syncthreads();
+    }
+}
+
 template <typename T, bool TRANS>
 __global__ __launch_bounds__(512) void tg_i8_turn(TurnArgs p, TileStore<T> out) {
     using Cfg = Turn<T, TRANS>;
@@ -261,39 +306,30 @@ __global__ __launch_bounds__(512) void tg_i8_turn(TurnArgs p, TileStore<T> out) 
     typename Cfg::Raw x[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) Cfg::load(p, m0, n0, i * 64, l, x[i]);
-    float factor = 1.0f, back = 1.0f;
-    if constexpr (Cfg::F16) {
-        // The range of the scales, as tg_i8_scale_range finds it, in every workgroup.
-        __shared__ float part[8];
-        float top = 0.0f;
-        for (int i = threadIdx.x; i < p.depth; i += 512) top = fmaxf(top, finite_size(p.scale[i]));
-        top = wave_max(top);
-        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = top;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, part[i]);
-        const int e = range_exponent(top);
-        factor = ldexpf(1.0f, e);
-        back = ldexpf(1.0f, -e);
-    }
+    ScaleRange range{1.0f, 1.0f, 0};
+    if constexpr (Cfg::F16) range = turn_range(p);
     typename Cfg::Acc acc[1][2] = {};
-    Cfg::put(p, m0, n0, 0, lds, factor, x[0]);
-    Cfg::load(p, m0, n0, AHEAD * 64, l, x[0]);
-    __syncthreads();
-    for (int s0 = 0; s0 < steps; s0 += AHEAD) {
+    if (range.wide != 0) {
+        if constexpr (Cfg::F16) turn_wide<TRANS>(p, m0, n0, lds, acc);
+    } else {
+        Cfg::put(p, m0, n0, 0, lds, range.factor, x[0]);
+        Cfg::load(p, m0, n0, AHEAD * 64, l, x[0]);
+        __syncthreads();
+        for (int s0 = 0; s0 < steps; s0 += AHEAD) {
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int s = s0 + i;
-            if (s >= steps) break;
-            Cfg::products(lds + i % 2 * Cfg::STAGE, acc);
-            Cfg::put(p, m0, n0, (s + 1) * 64, lds + (i + 1) % 2 * Cfg::STAGE, factor, x[(i + 1) % AHEAD]);
-            Cfg::load(p, m0, n0, (s + 1 + AHEAD) * 64, l, x[(i + 1) % AHEAD]);
-            __syncthreads();
+            for (int i = 0; i < AHEAD; ++i) {
+                const int s = s0 + i;
+                if (s >= steps) break;
+                Cfg::products(lds + i % 2 * Cfg::STAGE, acc);
+                Cfg::put(p, m0, n0, (s + 1) * 64, lds + (i + 1) % 2 * Cfg::STAGE, range.factor, x[(i + 1) % AHEAD]);
+                Cfg::load(p, m0, n0, (s + 1 + AHEAD) * 64, l, x[(i + 1) % AHEAD]);
+                __syncthreads();
+            }
         }
     }
     if constexpr (Cfg::F16) {
-        acc[0][0] *= back;
-        acc[0][1] *= back;
+        acc[0][0] *= range.back;
+        acc[0][1] *= range.back;
     }
     typename Cfg::Shape::template Beside<TileStore<T>> beside;
     Cfg::Shape::beside(tile, tm, tn, out, beside);
