@@ -225,3 +225,17 @@ def test_f16_gradients_of_terms_of_one_size_from_scales_of_many(m, n, k):
     f64 = lambda q, s: q.double() * s.double()[:, None]  # noqa: E731
     _check_f16(int8.backward_a(ga.to(DEV), b.to(DEV), sb.to(DEV)), ga.double(), f64(b, sb))
     _check_f16(int8.backward_b(gb.to(DEV), a.to(DEV), sa.to(DEV)), gb.double().t(), f64(a, sa))
+
+
+@pytest.mark.parametrize("n", [(1 << 26) - 16, (1 << 26) - 15, (1 << 26) - 1])
+def test_one_row_times_the_most_columns(n):
+    """Both sides of the limit of one launch for few rows."""
+    _say("matmul", 1, n, 16)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    b = torch.randint(-127, 128, (n, 16), generator=g, device=DEV, dtype=torch.int8)
+    a = torch.randint(-127, 128, (1, 16), generator=g, device=DEV, dtype=torch.int8)
+    sb = torch.rand(n, generator=g, device=DEV)
+    c = int8.matmul(a, torch.full((1,), 0.5, device=DEV), b, sb, dtype=torch.float32)
+    want = (b.float() * a.float()).sum(1) * 0.5 * sb  # whole numbers below 2^24
+    assert torch.equal(c[0], want)

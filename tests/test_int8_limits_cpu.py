@@ -4,6 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from tropical_gemm import _native as nat  # noqa: E402
 from tropical_gemm import int8  # noqa: E402
 from tropical_gemm import pytorch as tgt  # noqa: E402
 
@@ -83,3 +84,15 @@ def test_gradient_of_the_stream_alone(on_host):
     grads = torch.autograd.grad((h ** 3).sum(), (x, r), create_graph=True)
     second, = torch.autograd.grad(grads[0].sum(), x)
     assert torch.allclose(grads[1], 3 * (x + r) ** 2) and torch.allclose(second, 6 * (x + r))
+
+
+@pytest.mark.parametrize("m,k", [(1, 16), (16, 16), (16, 17), (32, 17), (64, 17)])
+def test_products_of_few_rows_launch_fewer_than_2_to_the_32_threads(m, k):
+    """Sixteen columns take up to 1024 threads: 2^26 - 16 columns are the most."""
+    lib = nat.load()
+    most = (1 << 26) - 16
+    plan = lambda n: lib.tg_i8_gemm_plan(4096, k, 4096, k, m, n, k).decode()  # noqa: E731
+    if m <= 16:
+        assert plan(most).startswith("stream")
+    for n in (most + 1, most + 15, 1 << 26):
+        assert not plan(n).startswith("stream") and plan(n) != "invalid"

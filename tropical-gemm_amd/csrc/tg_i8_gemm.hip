@@ -202,8 +202,8 @@ struct Carver {
 //     64 x 1024 x 8191   15.2   35.2     64 x  8192 x 8191  39.4   45.6
 //     64 x 4096 x 4095   12.8   24.6     64 x 16384 x 4095  40.9   26.8
 int stream_rows(const I8Gemm& p) {
-    // A launch's thread count stays below 2^32.
-    if (p.m > 64 || p.n >= int64_t(1) << 26) return 0;
+    // A launch's thread count stays below 2^32: 1024 threads for 16 columns.
+    if (p.m > 64 || p.n > (int64_t(1) << 26) - 16) return 0;
     if (p.m <= 16) return 16;
     const bool ready = in_place(p.a, p.lda, p.k) && in_place(p.b, p.ldb, p.k);
     if (p.m <= 32) return p.n <= 8192 || !ready ? 32 : 0;
