@@ -239,3 +239,60 @@ def test_one_row_times_the_most_columns(n):
     c = int8.matmul(a, torch.full((1,), 0.5, device=DEV), b, sb, dtype=torch.float32)
     want = (b.float() * a.float()).sum(1) * 0.5 * sb  # whole numbers below 2^24
     assert torch.equal(c[0], want)
+
+
+def _rel(a, b):
+    return ((a.detach().cpu().double() - b).norm() / b.norm()).item()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=IDS.get)
+@pytest.mark.parametrize("m,n,k", [(70, 130, 257), (300, 256, 512), (1100, 520, 1030)], ids=lambda v: str(v))
+def test_linear_gradients_in_16_bits(dtype, m, n, k):
+    """y: one rounding of every value, u.  Gradients: one of every value and one of
+    every factor, 1.2 u in the 2-norm as for the operators alone."""
+    u = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    x, w, g = (torch.randn(*s, generator=_gen(i)).to(dtype).to(DEV) for i, s in enumerate(((m, k), (n, k), (m, n))))
+    x.requires_grad_()
+    w.requires_grad_()
+    y = tgt.int8_linear_gpu(x, w)
+    y.backward(g)
+    f64 = lambda q, s: q.cpu().double() * s.cpu().double()[:, None]  # noqa: E731
+    xr, wr = f64(*int8.quantize(x.detach())), f64(*int8.quantize(w.detach()))
+    g64 = g.cpu().double()
+    assert y.dtype == x.grad.dtype == w.grad.dtype == dtype
+    assert _rel(y, xr @ wr.t()) < 1.01 * u
+    assert _rel(x.grad, g64 @ wr) < 1.2 * u
+    assert _rel(w.grad, g64.t() @ xr) < 1.2 * u
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=IDS.get)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("m,n,k", [(130, 96, 300), (700, 512, 1024)], ids=lambda v: str(v))
+def test_norm_linear_gradients_in_16_bits(dtype, residual, m, n, k):
+    """As above, with the product's gradient rounded (1.2 u) before the norm's
+    backward pass, which is linear in it and stretches it by at most the largest
+    weight, 1.5, and its result rounded (u): less than 3 u.  The stream is what
+    is stored of it."""
+    u = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    shapes = ((m, k), (m, k), (k,), (n, k), (m, n), (m, k))
+    x, r, nw, w, gy, gh = (torch.randn(*s, generator=_gen(i)) for i, s in enumerate(shapes))
+    x, r, nw, w, gy, gh = (t.to(dtype) for t in (x, r, 1 + 0.1 * nw, w, gy, gh))
+    ours = [t.to(DEV).requires_grad_() for t in (x, r, nw, w)]
+    if not residual:
+        ours[1] = None
+    y, h = tgt.rms_norm_int8_linear_gpu(*ours, 1e-5)
+    torch.autograd.backward([y, h], [gy.to(DEV), gh.to(DEV)])
+
+    ref = [t.double().requires_grad_() for t in (x, r, nw, w)]
+    h64 = ref[0] + ref[1] if residual else ref[0] * 1.0
+    h64 = h64 + (h.detach().cpu().double() - h64).detach()
+    norm = h64 * (h64.square().mean(1, keepdim=True) + 1e-5).rsqrt() * ref[2]
+    f64 = lambda q, s: q.cpu().double() * s.cpu().double()[:, None]  # noqa: E731
+    rows = f64(*int8.rms_norm(h.detach(), nw.to(DEV), None, 1e-5)[:2])
+    wr = f64(*int8.quantize(w.to(DEV)))
+    y64 = (norm + (rows - norm).detach()) @ (ref[3] + (wr - ref[3]).detach()).t()
+    torch.autograd.backward([y64, h64], [gy.double(), gh.double()])
+    assert _rel(y, y64.detach()) < 1.01 * u
+    for a, b in zip(ours, ref):
+        if a is not None:
+            assert a.grad.dtype == dtype and _rel(a.grad, b.grad) < 3 * u

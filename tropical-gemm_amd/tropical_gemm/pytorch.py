@@ -303,7 +303,7 @@ class RmsNormInt8LinearGPU(torch.autograd.Function):
         residual = None if residual is None else residual.detach().contiguous()
         q, scale, h = int8.rms_norm(x, norm_weight, residual, eps)
         if residual is None:
-            h = x.clone()  # an output of its own, which the caller may write
+            h = x.clone()  # an output that shares no memory with an input
         qw, scale_w = int8.quantize(weight)
         ctx.save_for_backward(h, norm_weight, q, scale, qw, scale_w)
         ctx.eps = eps
