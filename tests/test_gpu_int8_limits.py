@@ -296,3 +296,52 @@ def test_norm_linear_gradients_in_16_bits(dtype, residual, m, n, k):
     for a, b in zip(ours, ref):
         if a is not None:
             assert a.grad.dtype == dtype and _rel(a.grad, b.grad) < 3 * u
+
+
+@pytest.mark.parametrize("m,n,k", [(64, 8191, 64), (8192, 64, 64), (1000, 1003, 5), (2048, 2048, 512), (2048, 2049, 2050),
+                                   (4096, 4100, 520), (4096, 1024, 4096)], ids=lambda v: str(v))
+@pytest.mark.parametrize("spread", [10, 40])
+def test_f16_gradients_in_every_tile_size(m, n, k, spread):
+    """As above, in slices, in larger tiles, in place and laid out; a gradient past
+    its scale's row is zero.  The 64-bit products are torch's on the GPU."""
+    _say("f16 tiles", m, n, k, spread)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    grad = torch.randn(m, n, generator=g, device=DEV).half()
+    a, b = (torch.randint(-127, 128, (r, k), generator=g, device=DEV).to(torch.int8) for r in (m, n))
+    sa, sb = (torch.rand(r, generator=g, device=DEV) * 0.02 + 1e-3 for r in (m, n))
+    sa[3] *= 2.0 ** spread
+    sb[3] *= 2.0 ** spread
+    grad[3], grad[:, 3] = 0, 0
+    f64 = lambda q, s: q.double() * s.double()[:, None]  # noqa: E731
+    u = 2.0 ** -11
+    for got, x, y in ((int8.backward_a(grad, b, sb), grad.double(), f64(b, sb)),
+                      (int8.backward_b(grad, a, sa), grad.double().t().contiguous(), f64(a, sa))):
+        want, size = torch.mm(x, y), torch.mm(x.abs(), y.abs())
+        off = got.double() - want
+        assert (off.abs() <= (1.01 * u + x.shape[1] * 2.0 ** -24) * size + u * want.abs() + 2.0 ** -24).all()
+        assert off.norm() <= 1.2 * u * want.norm() + 2.0 ** -24 * off.numel() ** 0.5
+
+
+@pytest.mark.parametrize("m,n,k", [(100, 96, 80), (520, 4008, 1024)], ids=lambda v: str(v))
+def test_f16_gradients_in_a_graph_follow_their_scales(m, n, k):
+    """Replays with scales of one size and far from each other, in turn."""
+    _say("f16 graph", m, n, k)
+    grad = torch.randn(m, n, generator=_gen(1)).half().to(DEV)
+    a, b = (torch.randint(-127, 128, (r, k), generator=_gen(r)).to(torch.int8).to(DEV) for r in (m, n))
+    sa, sb = (torch.rand(r, generator=_gen(r + 1)).to(DEV) * 0.02 + 1e-3 for r in (m, n))
+    grad[3], grad[:, 3] = 0, 0
+    step = lambda: (int8.backward_a(grad, b, sb), int8.backward_b(grad, a, sa))  # noqa: E731
+    first = step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(5):
+        sa[3] = sb[3] = 1e9 if i % 2 else 0.01
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        for u, v, w in zip(got, step(), first):
+            assert torch.equal(u, v)
+            assert (u.float() - w.float()).norm() <= 2.0 ** -9 * w.float().norm()
