@@ -378,10 +378,10 @@ int tg_i8_gemm(int device, tg_float type, const int8_t* a, int64_t lda, const fl
                void* stream);
 
 /* Name of the way tg_i8_gemm takes for these operands, e.g. "stream rows 16
- * words" (up to 16 rows: b is streamed into registers; rows are 32-bit
- * aligned), "any" (one launch for
- * unaligned rows), "tiles 256x256", "tiles 64x64 per_cu 2 slices 4 pack a"
- * (the sum in four slices that are joined afterwards, a laid out first);
+ * words" (a few rows of a, here up to 16, at most 64: b is streamed into
+ * registers; rows are 32-bit aligned), "any" (one launch for unaligned rows),
+ * "tiles 256x256", "tiles 64x64 per_cu 2 slices 4 pack a" (the sum in four
+ * slices that are joined afterwards, a laid out first);
  * "invalid" for arguments the call would reject.  Host logic only, as
  * tg_gemm_plan: pointers are checked for alignment.  tg_i8_backward_plan is
  * the same for grad_a (want_a not 0) or grad_b; "turn" is one launch for small

@@ -133,8 +133,8 @@ __device__ __forceinline__ void split_value(float v, D (&d)[PLANES]) {
 // rows by 128 bytes of them (at least 64 columns), whole lines both ways,
 // through LDS: pairs of rows are written there as words of two, 33 words a
 // column, so that the words of 8 x 8 lanes meet 64 banks.  Bound by memory:
-// 8192 x 4096 bf16 and as many 8-bit integers in one launch 43.4 us (235 MB,
-// 5.4 TB/s); 4096 x 4096 8-bit integers 14.3 us (50 MB, 3.5 TB/s).
+// 8192 x 4096 bf16 and as many 8-bit integers in one launch 42.9 us (235 MB,
+// 5.5 TB/s); 4096 x 4096 8-bit integers 13.5 us (50 MB, 3.7 TB/s).
 template <typename S, typename D, int PLANES>
 struct PackTurned {
     static_assert(sizeof(D) == 2, "pairs are words");

@@ -104,9 +104,9 @@ struct Steps {
 // it shares with the group before it are written twice, with the same values,
 // and counted once.
 // VPT 0: rows of any length, read again (through L2) after the reduction.
-// bf16, 8192 x 8192: norm with residual 87 us (470 MB, 5.4 TB/s), without norm
-// 38.7 us (201 MB, 5.2 TB/s); one row of 4096: 2.8 us, the loads' latency and
-// the launch's.
+// bf16, 8192 x 8192: norm with residual 89 us (470 MB, 5.3 TB/s), without norm
+// 40 us (201 MB, 5.0 TB/s); one row of 4096: 2.7 us, the loads' latency and
+// the launch's (medians of 60 runs).
 template <typename T, typename W, bool NORM, bool RES, int NT, int VPT>
 __global__ __launch_bounds__(kBlock<NT>) void tg_i8_rows(const T* __restrict__ x, int64_t ldx,
                                                          const T* __restrict__ res, int64_t ldr,
@@ -271,8 +271,8 @@ hipError_t launch_rows(const I8Norm& p, hipStream_t st) {
 // groups each (three where two would leave more than a quarter of the threads
 // without one, or with one they share): bf16 norm with residual of 16384 rows
 // of 1024: 19.7 us, 21.1 with one group a thread on twice the threads; of 2501:
-// 56.6 us as 128 x 3, 70.3 as 256 x 2; 8192 rows of 8192: 81.9 us as 512 x 2
-// (5.7 TB/s), 85.1 as 256 x 4, 85.0 as 1024 x 1.
+// 56.6 us as 128 x 3, 70.3 as 256 x 2; 8192 rows of 8192: 81.9 us as 512 x 2,
+// 85.1 as 256 x 4, 85.0 as 1024 x 1 (each the least of 30 runs).
 template <typename T, typename W, bool NORM, bool RES>
 hipError_t rows_form(const I8Norm& p, hipStream_t st) {
     const int64_t groups = ceil_div(p.cols, 8);
@@ -302,8 +302,8 @@ hipError_t by_type(int type, F&& f) {
     }
 }
 
-// y = round(q * scale), eight elements a thread.  bf16, 8192 x 8192: 31.8 us
-// behind the kernel that wrote q (201 MB, 6.3 TB/s, q still in the last cache).
+// y = round(q * scale), eight elements a thread.  bf16, 8192 x 8192: 32.8 us
+// behind the kernel that wrote q (201 MB, 6.1 TB/s, q still in the last cache).
 template <typename T>
 __global__ __launch_bounds__(256) void tg_i8_restore(const int8_t* __restrict__ q, int64_t ldq,
                                                      const float* __restrict__ scale, T* __restrict__ y,
@@ -332,8 +332,8 @@ __global__ __launch_bounds__(256) void tg_i8_restore(const int8_t* __restrict__ 
 // bit: each column is stored by its own workgroup alone.  A row's last group is
 // moved back to end with the row, as in tg_i8_rows, so that no load waits for a
 // branch (bf16, 8192 rows of 4095: 62 us for the whole pass with branches, 45
-// so); TINY, rows below eight elements, is one group with a bound.  bf16, 8192 x 4096 with gh: 48.7 us (277 MB with the
-// parts, 5.7 TB/s); f32, 777 x 2501: 11 us, two rows one after the other.
+// so); TINY, rows below eight elements, is one group with a bound.  bf16, 8192 x 4096 with gh: 51 us (277 MB with the
+// parts, 5.4 TB/s); f32, 777 x 2501: 11 us, two rows one after the other.
 template <typename T, typename W, bool GH, int NT, bool TINY>
 __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
     const T* __restrict__ gy, int64_t ldg, const T* __restrict__ h, int64_t ldh, const W* __restrict__ w,
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(NT) void tg_i8_norm_backward(
 
 // gw[j] = sum over the parts: 64 slices of them, each in order, four of its
 // loads on their way at a time, then the slices in order.  The same bits in
-// every run.  512 parts of 4096: 4.8 us, a launch and a few loads' latency.
+// every run.  512 parts of 4096: 5.1 us, a launch and a few loads' latency.
 template <typename W>
 __global__ __launch_bounds__(1024) void tg_i8_sum_parts(const float* __restrict__ part, int64_t parts,
                                                         W* __restrict__ gw, int64_t cols) {

@@ -1,4 +1,4 @@
-// tg_i8_stream.hpp -- the 8-bit product of a few rows of A (up to 16) with a
+// tg_i8_stream.hpp -- the 8-bit product of a few rows of A (up to 64) with a
 // weight matrix: every row of B is read once, straight into registers.
 #pragma once
 

@@ -91,12 +91,14 @@ struct TileArgs {
 // half behind it: a CU takes one 1 KiB load in 16 clocks at most, and waves
 // that issue them faster stand still (8192^3 in 8 bits: 396 us; with A's and
 // B's behind the barrier 421, all behind its first four rows 440; one build of
-// each in turn, kept ones measure 396 to 420 from GPU to GPU, 2.6 to 2.8 P
-// operations/s).  There the matrix unit is busy 68% of the cycles (79% in
-// bf16: 8192 x 4096 x 4096 in 190 us, 1.45 PFLOP/s) and the clock falls to
-// 1.8 GHz under the load.  Products of few tiles are bound by their loads:
-// M = 512, N = K = 4096 in 12.5 us, 24 KiB of loads in
-// 0.24 us on each CU.
+// each in turn, kept ones measure 396 to 426 from GPU to GPU, 2.6 to 2.8 P
+// operations/s).  There the matrix unit is busy 67% of the cycles (79% in bf16:
+// 8192 x 4096 x 4096 in 190 us once the clock has settled, 196 to 207 in the
+// median of a run, 1.3 to 1.45 PFLOP/s) and the clock falls to 1.8 GHz under the
+// load.  In products of few tiles a step takes longer than the issue of its
+// loads: M = 512, N = K = 4096 in 12.4 to 12.9 us, 0.24 us a step on each CU for
+// 24 KiB, which is 0.16 us at the rate above and 2.4 GHz (the rest, latency and
+// the barrier, was not measured apart).
 //
 // The 16-byte chunk c of a row lies at place c ^ key(row).  LDS serves 16
 // lanes of a 16-byte read at a time, lanes {0-3, 12-15, 20-27} and {4-11,

@@ -14,7 +14,6 @@ using f16_t = _Float16;
 // and written unaligned by one instruction on gfx950, so rows need no
 // alignment of their own.
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
-typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef uint32_t u32x4_word __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_word __attribute__((ext_vector_type(2), aligned(4)));
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
