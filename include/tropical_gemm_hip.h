@@ -346,7 +346,8 @@ int tg_i8_dequantize(int device, tg_float type, const int8_t* q, int64_t ldq, co
 /* h = x + residual, rounded to type (residual and h NULL: h stands for x);
  * y = h * (mean_j h^2 + eps)^-1/2 * weight, given as q and scale (q * scale is
  * y to 8 bits of the row's maximum, as in tg_i8_quantize).  weight is of type
- * or f32.  Squares may pass f32, h * weight may not. */
+ * or f32.  Squares may pass f32 (those below its range count as zero beside
+ * eps), h * weight may not. */
 int tg_i8_rms_norm(int device, tg_float type, tg_float weight_type, const void* x, int64_t ldx,
                    const void* residual, int64_t ldr, const void* weight, float eps, int8_t* q,
                    float* scale, void* h, int64_t rows, int64_t cols, void* stream);
