@@ -414,6 +414,127 @@ int tg_i8_backward_b(int device, tg_float type, const void* grad_c, int64_t ldg,
                      int64_t lda, const float* a_scale, void* grad_b, int64_t m, int64_t n,
                      int64_t k, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- layer in 8-bit floating point ---------------------------------------
+ *
+ * A linear layer whose operands are e4m3 numbers (OCP: 4 exponent and 3 mantissa
+ * bits, largest 448, no infinities) with one power of two, an e8m0 byte s that
+ * stands for 2^(s - 127) (255: NaN), for each block: 1 x 128 elements of
+ * activations, 128 x 128 of weights; the last block of a row or column may be
+ * smaller.  A power of two costs a floating-point number no bits.  The block's
+ * scale of row block r and column block c is at scale[r * scale_row + c *
+ * scale_col]: any order in memory (scale_row at most 2^22); the products are
+ * fastest where those of a column of blocks are neighbours, as tg_f8_quantize
+ * writes them.  No counterpart in the reference.  Conventions as for the 8-bit
+ * layer above. */
+
+/* top = the block's largest magnitude, e = the least integer with top <= 448 *
+ * 2^e, at least -100: scale = 2^e, q = x * 2^-e rounded to e4m3 (nearest, ties
+ * to even).  A block that holds a NaN or an infinity becomes NaNs with scale 1.
+ * block_rows is 1 or 128; scale is dense, [column block][row block].  cols is at
+ * most 2^30. */
+int tg_f8_quantize(int device, tg_float type, const void* x, int64_t ldx, int64_t block_rows,
+                   uint8_t* q, uint8_t* scale, int64_t rows, int64_t cols, void* stream);
+
+/* y = q times its scale, rounded to type (exact in bf16 and f32 for scales from
+ * 2^-100 on). */
+int tg_f8_dequantize(int device, tg_float type, const uint8_t* q, int64_t ldq, const uint8_t* scale,
+                     int64_t scale_row, int64_t scale_col, int64_t block_rows, void* y,
+                     int64_t rows, int64_t cols, void* stream);
+
+/* c[i, j] = sum_k (a[i, k] * its scale) * (b[j, k] * its scale) + bias[j]: a is m
+ * x k with a scale for 1 x 128, b is n x k (a weight matrix as it is stored) with
+ * a scale for 128 x 128, bias of type or NULL, c is m x n of type.  k is at most
+ * 2^20; k == 0 gives the bias (or zero).  Sums are f32.  For f32 outputs every
+ * product is exact (scales of 2^-100 to 2^111); for bf16 and f16 the matrix
+ * instructions add groups of a few products first, dropping what lies 2^-13 below
+ * the largest of them: 1.5e-5 of the result in the mean, less than these types'
+ * own rounding. */
+size_t tg_f8_gemm_workspace_size(tg_float type, const uint8_t* a, int64_t lda, const uint8_t* b,
+                                 int64_t ldb, int64_t m, int64_t n, int64_t k);
+int tg_f8_gemm(int device, tg_float type, const uint8_t* a, int64_t lda, const uint8_t* a_scale,
+               int64_t a_scale_row, int64_t a_scale_col, const uint8_t* b, int64_t ldb,
+               const uint8_t* b_scale, int64_t b_scale_row, int64_t b_scale_col, const void* bias,
+               void* c, int64_t m, int64_t n, int64_t k, void* workspace, size_t workspace_bytes,
+               void* stream);
+
+/* Name of the way tg_f8_gemm takes for these operands ("stream rows 16 words",
+ * "tiles 256x256", "tiles 64x64 slices 4 pack a"; "wide ..." in bf16 for f32 outputs), as tg_i8_gemm_plan; and of
+ * the gradients' (want_a not 0: grad_a). */
+const char* tg_f8_gemm_plan(tg_float type, const uint8_t* a, int64_t lda, const uint8_t* b,
+                            int64_t ldb, int64_t m, int64_t n, int64_t k);
+const char* tg_f8_backward_plan(tg_float type, int want_a, const void* grad_c, int64_t ldg,
+                                int64_t m, int64_t n, int64_t k);
+
+/* grad_a[i, k] = sum_j grad_c[i, j] * b[j, k] * its scale.  grad_c is m x n and
+ * grad_a m x k, of type.  Every product is exact for scales of 2^-100 to 2^111
+ * (the 8-bit operand in bf16, f16 and f32 gradients as two and three bf16 numbers
+ * that add up to them; numbers of a f32 gradient below 2^-110 may lose bits),
+ * sums are f32, of at most 2^20 terms. */
+size_t tg_f8_backward_a_workspace_size(tg_float type, const void* grad_c, int64_t ldg, int64_t m,
+                                       int64_t n, int64_t k);
+int tg_f8_backward_a(int device, tg_float type, const void* grad_c, int64_t ldg, const uint8_t* b,
+                     int64_t ldb, const uint8_t* b_scale, int64_t b_scale_row, int64_t b_scale_col,
+                     void* grad_a, int64_t m, int64_t n, int64_t k, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* grad_b[j, k] = sum_i grad_c[i, j] * a[i, k] * its scale, from the 8-bit
+ * activations that the forward pass kept.  grad_b is n x k of type. */
+size_t tg_f8_backward_b_workspace_size(tg_float type, const void* grad_c, int64_t ldg, int64_t m,
+                                       int64_t n, int64_t k);
+int tg_f8_backward_b(int device, tg_float type, const void* grad_c, int64_t ldg, const uint8_t* a,
+                     int64_t lda, const uint8_t* a_scale, int64_t a_scale_row, int64_t a_scale_col,
+                     void* grad_b, int64_t m, int64_t n, int64_t k, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* ---- layer norm and dropout ----------------------------------------------
+ *
+ * Dropout keeps no mask: which elements it keeps follows from the seed, the
+ * offset and an element's row and column alone, and every call that needs it
+ * makes it again.  Philox4x32-10 with the seed as its key (low word first) and
+ * the counter (column / 8, row, offset's low word, its high word) gives four
+ * words for eight columns: column j takes the low (j even) or high half of word j
+ * % 8 / 2, and is dropped where those 16 bits are below t = rint(p * 65536), p
+ * between 0 and 1.  Kept elements are multiplied by 65536 / (65536 - t), which
+ * keeps their mean; dropped ones are zero, whatever they held.  Calls of one seed
+ * have to differ in the offset, or they drop the same elements.  seed_at, where
+ * it is not NULL, points to the seed on the GPU, read when the kernel runs: a
+ * captured call then follows what is written there.  The same conventions as
+ * above.  No counterpart in the reference. */
+
+/* y = dropout(x) + residual (NULL: none), rounded to type.  The gradient of x is
+ * the same call on the gradient of y, without residual. */
+int tg_dropout(int device, tg_float type, const void* x, int64_t ldx, const void* residual,
+               int64_t ldr, double p, uint64_t seed, const uint64_t* seed_at, uint64_t offset,
+               void* y, int64_t rows, int64_t cols, void* stream);
+
+/* h = dropout(x) + residual, rounded to type (p 0 and residual NULL: h stands
+ * for x and may be NULL); mean and rstd = (variance + eps)^-1/2 of each row of h
+ * in f32; y = (h - mean) * rstd * weight + bias.  weight and bias (NULL: none)
+ * are of weight_type, which is type or f32.  The variance is of deviations from
+ * the mean; deviations and sums may pass f32.  cols is at most 2^24. */
+int tg_layer_norm(int device, tg_float type, tg_float weight_type, const void* x, int64_t ldx,
+                  const void* residual, int64_t ldr, const void* weight, const void* bias,
+                  float eps, double p, uint64_t seed, const uint64_t* seed_at, uint64_t offset,
+                  void* y, void* h, float* mean, float* rstd, int64_t rows, int64_t cols,
+                  void* stream);
+
+/* Gradients, from h, mean and rstd as tg_layer_norm gave them:
+ *   xh = (h - mean) * rstd, u = grad_y * weight,
+ *   grad_residual = rstd * (u - mean_j(u) - xh * mean_j(u * xh)) + grad_h,
+ *   grad_x = dropout(grad_residual)   (p 0: not written, may be NULL),
+ *   grad_weight = sum_i grad_y * xh, grad_bias = sum_i grad_y   (of weight_type).
+ * grad_h, the gradient that reaches h from elsewhere, may be NULL.  grad_x is
+ * made of grad_residual before its rounding.  Sums are made in a fixed order:
+ * equal calls give equal bits. */
+size_t tg_layer_norm_backward_workspace_size(int64_t rows, int64_t cols);
+int tg_layer_norm_backward(int device, tg_float type, tg_float weight_type, const void* grad_y,
+                           int64_t ldg, const void* h, int64_t ldh, const float* mean,
+                           const float* rstd, const void* weight, const void* grad_h, int64_t ldgh,
+                           double p, uint64_t seed, const uint64_t* seed_at, uint64_t offset,
+                           void* grad_x, void* grad_residual, void* grad_weight, void* grad_bias,
+                           int64_t rows, int64_t cols, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,378 @@
+// tg_f8_gemm.hip -- launches of the products in 8-bit floating point: rows times
+// rows with a power of two for each block, and the two gradients, which read one
+// 8-bit operand.
+#include "../../include/tropical_gemm_hip.h"
+#include "tg_f8.hpp"
+#include "tg_f8_pack.hpp"
+#include "tg_f8_stream.hpp"
+#include "tg_f8_tiles.hpp"
+#include "tg_i8.hpp"
+
+namespace tg {
+namespace {
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+template <typename F>
+hipError_t by_type(int type, F&& f) {
+    switch (type) {
+        case TG_BF16: return f(bf16_t());
+        case TG_F16: return f(f16_t());
+        default: return f(float());
+    }
+}
+
+// ---- choice of a tile ----------------------------------------------------
+
+// A tile's sizes, workgroups per CU, and its time in us: `start` + `step` for each
+// block of the sum while every workgroup has a CU of its own, otherwise rounds of
+// `round` + `full` for each block.
+struct TileTime {
+    int bm, bn, per_cu;
+    double start, step, round, full;
+};
+constexpr TileTime kTiles[] = {
+    {256, 256, 1, 7.0, 1.1, 7.0, 1.2}, {128, 128, 2, 4.0, 0.42, 3.0, 0.80}, {64, 64, 3, 2.8, 0.20, 1.0, 0.48},
+};
+constexpr int kTileForms = sizeof(kTiles) / sizeof(kTiles[0]);
+
+struct TilePlan {
+    int form, slices;
+    int64_t tiles_m, tiles_n, slice, steps;
+};
+
+double tile_time(const TileTime& c, int64_t tiles, int64_t steps) {
+    if (tiles <= 256) return c.start + double(steps) * c.step;
+    const int64_t slots = 256 * int64_t(c.per_cu);
+    return 3 + double(ceil_div(tiles, slots)) * (c.round + double(steps) * c.full);
+}
+
+TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps) {
+    TilePlan best = {0, 1, ceil_div(m, 256), ceil_div(n, 256), steps, steps};
+    double least = 1e30;
+    for (int f = 0; f < kTileForms; ++f) {
+        const TileTime& c = kTiles[f];
+        const int64_t tm = ceil_div(m, c.bm), tn = ceil_div(n, c.bn);
+        if (tm * tn >= int64_t(1) << 24) continue;  // a launch's thread count stays below 2^32
+        for (int s = 1; s <= 32; s *= 2) {
+            const int64_t slice = ceil_div(steps, s);
+            if (s > 1 && (tm * tn * s > 512 || slice < 4)) break;
+            double t = tile_time(c, tm * tn * s, slice);
+            // Partial sums' way through memory and the launch that joins them.
+            if (s > 1) t += 4.5 + double(s + 1) * double(m) * double(n) * 4 / 4e6;
+            if (t < least) {
+                least = t;
+                best = {f, int(ceil_div(steps, slice)), tm, tn, slice, steps};
+            }
+        }
+    }
+    return best;
+}
+
+std::string tiles_name(const TilePlan& pl) {
+    const TileTime& c = kTiles[pl.form];
+    std::string name = "tiles " + std::to_string(c.bm) + "x" + std::to_string(c.bn);
+    if (pl.slices > 1) name += " slices " + std::to_string(pl.slices);
+    return name;
+}
+
+size_t part_bytes(const TilePlan& pl, int64_t m, int64_t n) {
+    return pl.slices > 1 ? size_t(pl.slices) * size_t(m) * size_t(round_up(n, 8)) * 4 : 0;
+}
+
+template <typename K>
+hipError_t allow_lds(K* kernel, int bytes) {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+unsigned stride_grid(int64_t items) {
+    const int64_t blocks = ceil_div(items, 256);
+    return unsigned(blocks < 65536 ? blocks : 65536);
+}
+
+template <typename A, typename B>
+hipError_t launch_pack(const A& a, const B& b, hipStream_t st) {
+    const int64_t na = a.blocks(), nb = b.blocks();
+    if (na + nb >= int64_t(1) << 24) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((tg_i8_pack<A, B>), dim3(unsigned(na + nb)), dim3(256), 0, st, a, b, int(na), int(nb));
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_join(const float* part, int slices, int64_t m, int64_t n, const TileStore<T>& out, hipStream_t st) {
+    const int64_t ld = round_up(n, 8);
+    hipLaunchKernelGGL((tg_i8_tiles_join<float, T>), dim3(stride_grid(m * ld / 8)), dim3(256), 0, st, part, ld, slices, m,
+                       n, out);
+    return hipGetLastError();
+}
+
+template <int WM, int WN, int FM, int FN, int NB, int PER_CU, typename T>
+hipError_t launch_form(F8TileArgs p, const TilePlan& pl, const TileStore<T>& out, void* part, hipStream_t st) {
+    using Cfg = F8Tile<WM, WN, FM, FN, NB>;
+    const dim3 grid(unsigned(pl.tiles_m * pl.tiles_n), unsigned(pl.slices));
+    if (pl.slices == 1) {
+        const auto kernel = &tg_f8_tiles<WM, WN, FM, FN, NB, PER_CU, T>;
+        static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+        if (attr != hipSuccess) return attr;
+        hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, out);
+        return hipGetLastError();
+    }
+    const auto kernel = &tg_f8_tiles_slice<WM, WN, FM, FN, NB, PER_CU>;
+    static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+    if (attr != hipSuccess) return attr;
+    float* sums = static_cast<float*>(part);
+    hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, TilePartial<float>{sums, round_up(p.n, 8)});
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : launch_join(sums, pl.slices, p.m, p.n, out, st);
+}
+
+template <typename T>
+hipError_t launch_tiles(F8TileArgs p, const TilePlan& pl, const TileStore<T>& out, void* part, hipStream_t st) {
+    p.tiles_m = int(pl.tiles_m);
+    p.tiles_n = int(pl.tiles_n);
+    p.slice = int(pl.slice);
+    p.steps = int(pl.steps);
+    switch (pl.form) {
+        case 0: return launch_form<2, 2, 4, 4, 2, 1>(p, pl, out, part, st);
+        case 1: return launch_form<2, 2, 2, 2, 2, 2>(p, pl, out, part, st);
+        default: return launch_form<2, 2, 1, 1, 3, 3>(p, pl, out, part, st);
+    }
+}
+
+// True when the tiles can read rows of `bytes` bytes in place.
+bool in_place(const void* p, int64_t ld_bytes, int64_t bytes) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0 && ld_bytes < (int64_t(1) << 23) && bytes % 16 == 0;
+}
+
+// Carves 256-byte aligned parts out of a workspace.
+struct Carver {
+    char* at;
+    size_t used = 0;
+    void* take(size_t bytes) {
+        void* p = at == nullptr ? nullptr : at + used;
+        used += (bytes + 255) / 256 * 256;
+        return p;
+    }
+};
+
+// ---- the product ---------------------------------------------------------
+
+// Rows of A that tg_f8_stream takes (in sixteens; 0: the tiles take the
+// product): B is read once and needs no layout, but every 16 rows of B read all
+// of A.
+int stream_rows(const F8Gemm& p) {
+    // A launch's thread count stays below 2^32: 1024 threads for 16 columns.
+    if (p.m > 64 || p.n > (int64_t(1) << 26) - 16) return 0;
+    if (p.m <= 16) return 16;
+    const bool ready = in_place(p.a, p.lda, p.k) && in_place(p.b, p.ldb, p.k);
+    if (p.m <= 32) return p.n <= 8192 || !ready ? 32 : 0;
+    return p.n <= 8192 && !ready ? int(round_up(p.m, 16)) : 0;
+}
+
+struct GemmPlan {
+    int stream;  // rows of A of tg_f8_stream
+    bool wide;   // f32: both operands laid out in bf16
+    bool pack_a, pack_b;
+    int64_t ld;  // of packed rows, in bytes
+    TilePlan tiles;
+};
+
+GemmPlan plan_gemm(const F8Gemm& p) {
+    GemmPlan pl{};
+    pl.stream = stream_rows(p);
+    if (pl.stream != 0) return pl;
+    pl.wide = p.type == TG_FLOAT32;
+    if (pl.wide) {
+        pl.pack_a = pl.pack_b = true;
+        pl.ld = round_up(p.k, 64) * 2;
+        return pl;
+    }
+    pl.pack_a = !in_place(p.a, p.lda, p.k);
+    pl.pack_b = !in_place(p.b, p.ldb, p.k);
+    pl.ld = round_up(p.k, 128);
+    pl.tiles = plan_tiles(p.m, p.n, ceil_div(p.k, 128));
+    return pl;
+}
+
+struct GemmWs {
+    uint8_t *a, *b;
+    void* part;
+    size_t bytes;
+};
+
+GemmWs carve_gemm(const F8Gemm& p, const GemmPlan& pl, void* ws) {
+    Carver c{static_cast<char*>(ws)};
+    GemmWs w{};
+    if (p.m == 0 || p.n == 0 || p.k == 0 || pl.stream != 0) return w;
+    if (pl.pack_a) w.a = static_cast<uint8_t*>(c.take(size_t(p.m) * size_t(pl.ld)));
+    if (pl.pack_b) w.b = static_cast<uint8_t*>(c.take(size_t(p.n) * size_t(pl.ld)));
+    w.part = c.take(pl.wide ? plane_gemm_ws(p.m, p.n, pl.ld / 128, 1) : part_bytes(pl.tiles, p.m, p.n));
+    w.bytes = c.used;
+    return w;
+}
+
+PackBytes bytes_job(const void* src, int64_t ld_src, int64_t rows, int64_t bytes, void* dst, int64_t ld) {
+    return {static_cast<const int8_t*>(src), ld_src, rows, int(bytes), static_cast<int8_t*>(dst), ld};
+}
+
+// 32-bit aligned rows.
+bool in_words(const F8Gemm& p) {
+    auto words = [](const void* q, int64_t ld) { return reinterpret_cast<uintptr_t>(q) % 4 == 0 && ld % 4 == 0; };
+    return words(p.a, p.lda) && words(p.b, p.ldb);
+}
+
+template <int R, int W, bool WORDS, typename T>
+hipError_t launch_stream(const F8Gemm& p, const TileStore<T>& out, hipStream_t st) {
+    const F8StreamArgs args{p.a, p.b, p.lda, p.ldb, p.a_scale.p, p.b_scale.p, p.a_scale.row, p.a_scale.col,
+                            p.b_scale.row, p.b_scale.col, int(p.m), int(p.n), int(p.k)};
+    hipLaunchKernelGGL((tg_f8_stream<R, W, WORDS, T>), dim3(unsigned(ceil_div(p.n, 16))), dim3(W * 64), 0, st, args, out);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t stream_typed(const F8Gemm& p, int rows, const TileStore<T>& out, hipStream_t st) {
+    const bool words = in_words(p);
+    switch (rows) {
+        case 16: return words ? launch_stream<1, 16, true>(p, out, st) : launch_stream<1, 8, false>(p, out, st);
+        case 32: return words ? launch_stream<2, 8, true>(p, out, st) : launch_stream<2, 8, false>(p, out, st);
+        case 48: return launch_stream<3, 8, false>(p, out, st);
+        default: return launch_stream<4, 8, false>(p, out, st);
+    }
+}
+
+template <typename T>
+hipError_t gemm_typed(const F8Gemm& p, void* ws, hipStream_t st) {
+    const TileStore<T> out{nullptr, nullptr, nullptr, static_cast<const T*>(p.bias), static_cast<T*>(p.c), p.n};
+    if (p.k == 0) return launch_join(nullptr, 0, p.m, p.n, out, st);
+    const GemmPlan pl = plan_gemm(p);
+    if (pl.stream != 0) return stream_typed(p, pl.stream, out, st);
+    const GemmWs w = carve_gemm(p, pl, ws);
+    if (pl.wide) {
+        const hipError_t e = launch_pack(
+            PackF8Rows{p.a, p.lda, p.m, p.k, p.a_scale, 0, reinterpret_cast<bf16_t*>(w.a), pl.ld / 2},
+            PackF8Rows{p.b, p.ldb, p.n, p.k, p.b_scale, 7, reinterpret_cast<bf16_t*>(w.b), pl.ld / 2}, st);
+        if (e != hipSuccess) return e;
+        return plane_gemm(PlaneGemm{p.type, 1, w.a, w.b, pl.ld, pl.ld, pl.ld / 128, 128, p.bias, p.c, p.m, p.n}, w.part, st);
+    }
+    F8TileArgs t{};
+    t.a = pl.pack_a ? w.a : p.a;
+    t.b = pl.pack_b ? w.b : p.b;
+    t.lda = pl.pack_a ? pl.ld : p.lda;
+    t.ldb = pl.pack_b ? pl.ld : p.ldb;
+    t.sa = p.a_scale.p, t.sa_row = p.a_scale.row, t.sa_col = p.a_scale.col;
+    t.sb = p.b_scale.p, t.sb_row = p.b_scale.row, t.sb_col = p.b_scale.col;
+    t.m = int(p.m);
+    t.n = int(p.n);
+    // A packed row is whole; beside one that is not, it only has to reach as far.
+    t.tail = (pl.pack_a && pl.pack_b) || p.k % 128 == 0 ? 128 : int(round_up(p.k % 128, 16));
+    if (pl.pack_a || pl.pack_b) {
+        const PackBytes a = bytes_job(p.a, p.lda, pl.pack_a ? p.m : 0, p.k, w.a, pl.ld);
+        const PackBytes b = bytes_job(p.b, p.ldb, pl.pack_b ? p.n : 0, p.k, w.b, pl.ld);
+        const hipError_t e = launch_pack(a, b, st);
+        if (e != hipSuccess) return e;
+    }
+    return launch_tiles(t, pl.tiles, out, w.part, st);
+}
+
+// ---- gradients -----------------------------------------------------------
+//
+// Both are a product of G with the 8-bit operand q, whose rows run across the
+// sum; q is turned so that they run along it, in bf16 with its scales multiplied
+// in, which is exact.  G in bf16 is taken as it is, in f16 as two bf16 planes that
+// add up to it (8 + 3 bits), in f32 as three (8 + 8 + 8): every product is exact,
+// and the sums are f32.
+
+struct GradPlan {
+    bool pack_g;
+    int planes, tail;
+    int64_t depth, steps;  // of packed rows, in elements and in 128 bytes
+};
+
+GradPlan plan_grad(const F8Grad& p) {
+    GradPlan pl{};
+    pl.planes = p.type == TG_FLOAT32 ? 3 : p.type == TG_F16 ? 2 : 1;
+    pl.pack_g = pl.planes > 1 || p.transposed || !in_place(p.g, p.ldg * 2, p.depth * 2);
+    pl.depth = round_up(p.depth, 64);
+    pl.steps = pl.depth / 64;
+    pl.tail = pl.pack_g || p.depth % 64 == 0 ? 128 : int(p.depth % 64 * 2);
+    return pl;
+}
+
+struct GradWs {
+    void *g, *q, *part;
+    size_t bytes;
+};
+
+GradWs carve_grad(const F8Grad& p, const GradPlan& pl, void* ws) {
+    Carver c{static_cast<char*>(ws)};
+    GradWs w{};
+    if (p.rows == 0 || p.cols == 0 || p.depth == 0) return w;
+    if (pl.pack_g) w.g = c.take(size_t(p.rows) * size_t(pl.depth) * size_t(pl.planes) * 2);
+    w.q = c.take(size_t(p.cols) * size_t(pl.depth) * 2);
+    w.part = c.take(plane_gemm_ws(p.rows, p.cols, pl.steps, pl.planes));
+    w.bytes = c.used;
+    return w;
+}
+
+// Lays out q and, where it has to be, G in PLANES planes.
+template <typename T, int PLANES>
+hipError_t pack_grad(const F8Grad& p, const GradPlan& pl, const GradWs& w, hipStream_t st) {
+    const T* g = static_cast<const T*>(p.g);
+    bf16_t* to = static_cast<bf16_t*>(w.g);
+    const PackF8Turned q{p.q.q, p.q.ld, p.depth, p.cols, p.q.scale, p.q.block_rows == 1 ? 0 : 7,
+                         static_cast<bf16_t*>(w.q), pl.depth};
+    if (!pl.pack_g) return launch_pack(q, PackNothing(), st);
+    if (p.transposed)
+        return launch_pack(q, PackTurned<T, bf16_t, PLANES>{g, p.ldg, p.depth, p.rows, nullptr, nullptr, to, pl.depth}, st);
+    if constexpr (PLANES > 1)
+        return launch_pack(q, PackPlanes<T, PLANES>{g, p.ldg, p.rows, p.depth, to, pl.depth}, st);
+    else
+        return launch_pack(q, bytes_job(p.g, p.ldg * 2, p.rows, p.depth * 2, w.g, pl.depth * 2), st);
+}
+
+}  // namespace
+
+std::string f8_gemm_plan(const F8Gemm& p) {
+    if (p.m == 0 || p.n == 0) return "none";
+    if (p.k == 0) return "bias";
+    const GemmPlan pl = plan_gemm(p);
+    if (pl.stream != 0) return "stream rows " + std::to_string(pl.stream) + (in_words(p) && pl.stream <= 32 ? " words" : "");
+    if (pl.wide) return "wide " + plane_gemm_plan(p.m, p.n, pl.ld / 128, 1);
+    return tiles_name(pl.tiles) + (pl.pack_a ? " pack a" : "") + (pl.pack_b ? " pack b" : "");
+}
+
+std::string f8_grad_plan(const F8Grad& p) {
+    if (p.rows == 0 || p.cols == 0) return "none";
+    if (p.depth == 0) return "zero";
+    const GradPlan pl = plan_grad(p);
+    return plane_gemm_plan(p.rows, p.cols, pl.steps, pl.planes) + (pl.pack_g ? " pack grad_c" : "");
+}
+
+size_t f8_gemm_ws(const F8Gemm& p) { return carve_gemm(p, plan_gemm(p), nullptr).bytes; }
+
+hipError_t f8_gemm(const F8Gemm& p, void* ws, hipStream_t st) {
+    if (p.m == 0 || p.n == 0) return hipSuccess;
+    return by_type(p.type, [&](auto tag) { return gemm_typed<decltype(tag)>(p, ws, st); });
+}
+
+size_t f8_grad_ws(const F8Grad& p) { return carve_grad(p, plan_grad(p), nullptr).bytes; }
+
+hipError_t f8_grad(const F8Grad& p, void* ws, hipStream_t st) {
+    if (p.rows == 0 || p.cols == 0) return hipSuccess;
+    if (p.depth == 0) return plane_gemm_zero(p.type, p.out, p.rows, p.cols, st);
+    const GradPlan pl = plan_grad(p);
+    const GradWs w = carve_grad(p, pl, ws);
+    hipError_t e;
+    switch (p.type) {
+        case TG_BF16: e = pack_grad<bf16_t, 1>(p, pl, w, st); break;
+        case TG_F16: e = pack_grad<f16_t, 2>(p, pl, w, st); break;
+        default: e = pack_grad<float, 3>(p, pl, w, st);
+    }
+    if (e != hipSuccess) return e;
+    const PlaneGemm t{p.type, pl.planes, pl.pack_g ? w.g : p.g, w.q, pl.pack_g ? pl.depth * pl.planes * 2 : p.ldg * 2,
+                      pl.depth * 2, pl.steps, pl.tail, nullptr, p.out, p.rows, p.cols};
+    return plane_gemm(t, w.part, st);
+}
+
+}  // namespace tg

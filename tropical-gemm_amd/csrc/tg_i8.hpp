@@ -75,4 +75,26 @@ size_t i8_grad_ws(const I8Grad& p);
 hipError_t i8_grad(const I8Grad& p, void* ws, hipStream_t st);
 std::string i8_grad_plan(const I8Grad& p);
 
+// out (m x n, of type) = A B^T + bias in bf16, for operands laid out as tg_i8_tiles
+// takes them: rows of `steps` steps of 128 bytes (the last of `tail` that count);
+// a row of A is the sum of `planes` such rows (3: for f32 alone), one behind the
+// other.
+struct PlaneGemm {
+    int type, planes;
+    const void *a, *b;
+    int64_t lda, ldb;  // bytes
+    int64_t steps;
+    int tail;
+    const void* bias;  // of type, or null
+    void* out;
+    int64_t m, n;
+};
+// Bytes for partial sums; the time of it in us.
+size_t plane_gemm_ws(int64_t m, int64_t n, int64_t steps, int planes);
+double plane_gemm_time(int64_t m, int64_t n, int64_t steps, int planes);
+hipError_t plane_gemm(const PlaneGemm& p, void* part, hipStream_t st);
+std::string plane_gemm_plan(int64_t m, int64_t n, int64_t steps, int planes);
+// out = 0 (an empty sum).
+hipError_t plane_gemm_zero(int type, void* out, int64_t m, int64_t n, hipStream_t st);
+
 }  // namespace tg

@@ -518,6 +518,50 @@ std::string i8_grad_plan(const I8Grad& p) {
     return tiles_name(pl.tiles) + (pl.pack_g ? " pack grad_c" : "");
 }
 
+// Two planes go through the forms of one, one plane after the other.
+static TilePlan plan_planes(int64_t m, int64_t n, int64_t steps, int planes, double* time = nullptr) {
+    return planes == 2 ? plan_tiles(m, n, steps * 2, 1, time) : plan_tiles(m, n, steps, planes, time);
+}
+
+size_t plane_gemm_ws(int64_t m, int64_t n, int64_t steps, int planes) {
+    return m == 0 || n == 0 || steps == 0 ? 0 : part_bytes(plan_planes(m, n, steps, planes), m, n);
+}
+
+double plane_gemm_time(int64_t m, int64_t n, int64_t steps, int planes) {
+    double time = 0;
+    plan_planes(m, n, steps, planes, &time);
+    return time;
+}
+
+std::string plane_gemm_plan(int64_t m, int64_t n, int64_t steps, int planes) {
+    return tiles_name(plan_planes(m, n, steps, planes));
+}
+
+hipError_t plane_gemm(const PlaneGemm& p, void* part, hipStream_t st) {
+    TileArgs t{};
+    t.a = static_cast<const char*>(p.a);
+    t.b = static_cast<const char*>(p.b);
+    t.lda = p.lda;
+    t.ldb = p.ldb;
+    t.m = int(p.m);
+    t.n = int(p.n);
+    t.b_steps = int(p.steps);
+    t.plane = p.steps * 128;
+    t.tail = p.tail;
+    return by_type(p.type, [&](auto tag) {
+        using T = decltype(tag);
+        const TileStore<T> out{nullptr, nullptr, nullptr, static_cast<const T*>(p.bias), static_cast<T*>(p.out), p.n};
+        return launch_tiles<Mma::BF16>(t, plan_planes(p.m, p.n, p.steps, p.planes), out, part, st);
+    });
+}
+
+hipError_t plane_gemm_zero(int type, void* out, int64_t m, int64_t n, hipStream_t st) {
+    return by_type(type, [&](auto tag) {
+        using T = decltype(tag);
+        return launch_join<float>(nullptr, 0, m, n, TileStore<T>{nullptr, nullptr, nullptr, nullptr, static_cast<T*>(out), n}, st);
+    });
+}
+
 size_t i8_gemm_ws(const I8Gemm& p) { return carve_gemm(p, plan_gemm(p), nullptr).bytes; }
 
 hipError_t i8_gemm(const I8Gemm& p, void* ws, hipStream_t st) {

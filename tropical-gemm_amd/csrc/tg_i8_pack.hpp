@@ -87,7 +87,7 @@ __device__ __forceinline__ ScaleRange scale_range(float top, float low) {
 }
 
 // The range of all the scales.
-__global__ __launch_bounds__(1024) void tg_i8_scale_range(const float* __restrict__ scale, int64_t n,
+static __global__ __launch_bounds__(1024) void tg_i8_scale_range(const float* __restrict__ scale, int64_t n,
                                                           ScaleRange* __restrict__ out) {
     __shared__ float part[2][16];
     float top = 0.0f, low = __builtin_huge_valf();

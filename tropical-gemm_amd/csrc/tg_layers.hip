@@ -1,0 +1,305 @@
+// tg_layers.hip -- layer norm with dropout and the residual's addition in one
+// pass, and dropout by itself.  Both are bound by memory:
+// every input element is read once, every output written once, a row's values
+// stay in registers between its reductions and its output.
+#include "tg_layers_rows.hpp"
+
+namespace tg {
+namespace {
+
+constexpr float kHuge = __builtin_huge_valf();
+// Squares of numbers above 2^64 pass f32: a row whose sum of them is not finite
+// is summed again with its values times kShrink (the largest become 2^48).
+constexpr float kShrink = 0x1p-80f;
+
+// A row's threads: NT lanes, several rows in a workgroup where NT is below 256.
+// A thread holds VPT groups of eight neighbours, group g of thread t from
+// element (g * NT + t) * 8 on.
+template <int NT>
+constexpr int kRowsPerBlock = NT < 256 ? 256 / NT : 1;
+template <int NT>
+constexpr int kBlock = NT < 256 ? 256 : NT;
+
+// Sum over the NT threads of each row, in every one of them.  `slot`: not the
+// same twice in turn, so that one barrier is enough.
+template <int NT>
+__device__ __forceinline__ float row_sum(float x, int slot) {
+    x = wave_sum(x);
+    if constexpr (NT > 64) {
+        constexpr int W = NT / 64;
+        __shared__ float part[2][kRowsPerBlock<NT> * W];
+        const int wave = threadIdx.x / 64, first = wave / W * W;
+        if (threadIdx.x % 64 == 0) part[slot][wave] = x;
+        __syncthreads();
+        x = part[slot][first];
+#pragma unroll
+        for (int i = 1; i < W; ++i) x += part[slot][first + i];
+    }
+    return x;
+}
+
+template <typename T, typename W>
+struct NormArgs {
+    const T *x, *res;
+    int64_t ldx, ldr;
+    const W *w, *b;
+    float eps;
+    Dropout drop;
+    T *y, *h;
+    float *mean, *rstd;
+    int64_t first_row, rows, cols;  // first_row: of the launch, as dropout counts
+};
+
+// h = round(dropout(x) + residual); mean and variance of h in two sums of the
+// values in registers, which loses nothing where the mean is large beside the
+// deviations; y = (h - mean) * rstd * w + b.
+//
+// VPT > 0, rows of at least eight elements: all loads of a thread are issued
+// before the first is used; a group that would end past the row is moved back to
+// end with it, and what it shares with the group before it is counted once.
+// VPT 0: any length, read again for each sum.
+template <typename T, typename W, bool DROP, bool RES, int NT, int VPT>
+__global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> p) {
+    constexpr bool STREAM = DROP || RES;  // h is not x
+    const int t = threadIdx.x % NT;
+    const int64_t row = int64_t(blockIdx.x) * kRowsPerBlock<NT> + threadIdx.x / NT;
+    const bool live = row < p.rows;  // every thread reaches the barriers
+    const int64_t cols = p.cols;
+    const T* xr = p.x + row * p.ldx;
+    const T* rr = RES ? p.res + row * p.ldr : nullptr;
+    const Keep keep(p.drop);
+    const float inv_n = 1.0f / float(cols);
+
+    // n values of the stream from `at` on, as they are stored.
+    auto stream = [&](int64_t at, int n, float(&v)[8]) {
+        load_upto8(xr + at, n, v);
+        if constexpr (DROP) keep.apply(p.first_row + row, at, v);
+        if constexpr (RES) {
+            float r[8];
+            load_upto8(rr + at, n, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += r[i];
+        }
+        if constexpr (STREAM) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_f32(static_cast<T>(v[i]));
+        }
+    };
+    struct Stats {
+        float mean, rstd, shrink;  // of the values times shrink
+    };
+    // The row's statistics with its values times kShrink; every wave makes them all.
+    auto shrunk = [&] {
+        float s = 0.0f, ss = 0.0f, v[8];
+        auto each = [&](auto&& f) {
+            for (int64_t at = int64_t(threadIdx.x % 64) * 8; at < cols; at += 512) {
+                const int n = cols - at < 8 ? int(cols - at) : 8;
+                stream(at, n, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < n) f(v[i] * kShrink);
+            }
+        };
+        each([&](float a) { s += a; });
+        const float mean = wave_sum(s) * inv_n;
+        each([&](float a) { ss += (a - mean) * (a - mean); });
+        return Stats{mean, 1.0f / sqrtf(wave_sum(ss) * inv_n + p.eps * kShrink * kShrink), kShrink};
+    };
+    auto finish = [&](float mean, float ss) {
+        Stats s{mean, 1.0f / sqrtf(ss * inv_n + p.eps), 1.0f};
+        if (live && !(ss < kHuge)) s = shrunk();
+        if (live && t == 0) {
+            float m = s.mean / s.shrink;  // rounding may pass the largest number
+            if (fabsf(s.mean) < kHuge) m = fminf(fmaxf(m, -3.402823466e38f), 3.402823466e38f);
+            p.mean[row] = m;
+            p.rstd[row] = s.rstd * s.shrink;
+        }
+        return s;
+    };
+    auto out = [&](int64_t at, int n, const float(&v)[8], const float(&f)[8], const float(&b)[8], const Stats& s) {
+        float o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = (v[i] * s.shrink - s.mean) * s.rstd * f[i] + b[i];
+        store_upto8(p.y + row * cols + at, n, o);
+    };
+
+    if constexpr (VPT > 0) {
+        float v[VPT][8];
+        Eight<W> f[VPT], b[VPT];
+        auto start = [&](int g) { return int64_t(g * NT + t) * 8; };
+        auto from = [&](int g) { return start(g) <= cols - 8 ? start(g) : cols - 8; };
+        auto again = [&](int g) { return int(start(g) - from(g)); };  // of the group before it; 8 and more: all
+        float s = 0.0f;
+        if (live) {
+            Eight<T> a[VPT], r[VPT];
+#pragma unroll
+            for (int g = 0; g < VPT; ++g) {
+                a[g].load(xr + from(g));
+                if constexpr (RES) r[g].load(rr + from(g));
+            }
+#pragma unroll
+            for (int g = 0; g < VPT; ++g) {
+                f[g].load(p.w + from(g));
+                if (p.b != nullptr) b[g].load(p.b + from(g));
+            }
+#pragma unroll
+            for (int g = 0; g < VPT; ++g) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[g][i] = to_f32(a[g].v[i]);
+                if constexpr (DROP)
+                    if (again(g) < 8) keep.apply(p.first_row + row, from(g), v[g]);
+                if constexpr (RES) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[g][i] += to_f32(r[g].v[i]);
+                }
+                if constexpr (STREAM) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[g][i] = to_f32(static_cast<T>(v[g][i]));
+                    if (again(g) < 8) store8(p.h + row * cols + from(g), v[g]);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += i >= again(g) ? v[g][i] : 0.0f;
+            }
+        }
+        const float mean = row_sum<NT>(s, 0) * inv_n;
+        float ss = 0.0f;
+        if (live) {
+#pragma unroll
+            for (int g = 0; g < VPT; ++g)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss += i >= again(g) ? (v[g][i] - mean) * (v[g][i] - mean) : 0.0f;
+        }
+        ss = row_sum<NT>(ss, 1);
+        const Stats stats = finish(mean, ss);
+        if (live) {
+#pragma unroll
+            for (int g = 0; g < VPT; ++g) {
+                if (again(g) >= 8) continue;
+                float fv[8], bv[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    fv[i] = to_f32(f[g].v[i]);
+                    bv[i] = p.b != nullptr ? to_f32(b[g].v[i]) : 0.0f;
+                }
+                out(from(g), 8, v[g], fv, bv, stats);
+            }
+        }
+    } else {
+        float v[8];
+        auto each = [&](auto&& f) {
+            if (!live) return;
+            for (int64_t at = int64_t(t) * 8; at < cols; at += NT * 8) {
+                const int n = cols - at < 8 ? int(cols - at) : 8;
+                stream(at, n, v);
+                f(at, n);
+            }
+        };
+        float s = 0.0f, ss = 0.0f;
+        each([&](int64_t at, int n) {
+            if constexpr (STREAM) store_upto8(p.h + row * cols + at, n, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += i < n ? v[i] : 0.0f;
+        });
+        const float mean = row_sum<NT>(s, 0) * inv_n;
+        each([&](int64_t, int n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += i < n ? (v[i] - mean) * (v[i] - mean) : 0.0f;
+        });
+        ss = row_sum<NT>(ss, 1);
+        const Stats stats = finish(mean, ss);
+        each([&](int64_t at, int n) {
+            float f[8], b[8] = {};
+            load_upto8(p.w + at, n, f);
+            if (p.b != nullptr) load_upto8(p.b + at, n, b);
+            out(at, n, v, f, b, stats);
+        });
+    }
+}
+
+template <typename T, typename W, bool DROP, bool RES, int NT, int VPT>
+hipError_t launch_norm(const LayerNorm& q, hipStream_t st) {
+    constexpr int64_t kMost = int64_t(1) << 21;  // a launch's thread count stays below 2^32
+    for (int64_t r0 = 0; r0 < q.rows; r0 += kMost) {
+        const int64_t n = q.rows - r0 < kMost ? q.rows - r0 : kMost;
+        const NormArgs<T, W> p{static_cast<const T*>(q.x) + r0 * q.ldx,
+                               RES ? static_cast<const T*>(q.residual) + r0 * q.ldr : nullptr,
+                               q.ldx, q.ldr, static_cast<const W*>(q.weight), static_cast<const W*>(q.bias), q.eps,
+                               q.drop, static_cast<T*>(q.y) + r0 * q.cols,
+                               DROP || RES ? static_cast<T*>(q.h) + r0 * q.cols : nullptr,
+                               q.mean + r0, q.rstd + r0, r0, n, q.cols};
+        hipLaunchKernelGGL((tg_layer_norm_rows<T, W, DROP, RES, NT, VPT>), dim3(unsigned(ceil_div(n, kRowsPerBlock<NT>))),
+                           dim3(kBlock<NT>), 0, st, p);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+template <typename T, typename W, bool DROP, bool RES>
+hipError_t norm_form(const LayerNorm& p, hipStream_t st) {
+    const int64_t groups = ceil_div(p.cols, 8);
+    if (p.cols < 8) return launch_norm<T, W, DROP, RES, 64, 0>(p, st);
+    if (groups <= 64) return launch_norm<T, W, DROP, RES, 64, 1>(p, st);
+    if (groups <= 128) return launch_norm<T, W, DROP, RES, 64, 2>(p, st);
+    if (groups <= 256) return launch_norm<T, W, DROP, RES, 128, 2>(p, st);
+    if (groups <= 512) return launch_norm<T, W, DROP, RES, 256, 2>(p, st);
+    if (groups <= 1024) return launch_norm<T, W, DROP, RES, 512, 2>(p, st);
+    return launch_norm<T, W, DROP, RES, 1024, 0>(p, st);
+}
+
+// ---- dropout -----------------------------------------------------------------
+
+// y = round(dropout(x) + residual), eight elements a thread.
+template <typename T, bool DROP, bool RES>
+__global__ __launch_bounds__(256) void tg_dropout_rows(const T* x, int64_t ldx, const T* res, int64_t ldr,
+                                                       Dropout drop, T* y, int64_t rows, int64_t cols, int64_t groups) {
+    const Keep keep(drop);
+    const int64_t stride = int64_t(gridDim.x) * 256;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * groups; i += stride) {
+        const int64_t row = i / groups, at = (i - row * groups) * 8;
+        const int n = cols - at < 8 ? int(cols - at) : 8;
+        float v[8], r[8];
+        load_upto8(x + row * ldx + at, n, v);
+        if constexpr (RES) load_upto8(res + row * ldr + at, n, r);
+        if constexpr (DROP) keep.apply(row, at, v);
+        if constexpr (RES) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r[e];
+        }
+        store_upto8(y + row * cols + at, n, v);
+    }
+}
+
+}  // namespace
+
+hipError_t dropout_rows(const DropoutRows& p, hipStream_t st) {
+    if (p.rows == 0 || p.cols == 0) return hipSuccess;
+    const int64_t groups = ceil_div(p.cols, 8), blocks = ceil_div(p.rows * groups, 256);
+    return by_type(p.type, [&](auto tag) {
+        using T = decltype(tag);
+        return by_flag(p.drop.below > 0, [&](auto drop) {
+            return by_flag(p.residual != nullptr, [&](auto res) {
+                hipLaunchKernelGGL((tg_dropout_rows<T, decltype(drop)::value, decltype(res)::value>),
+                                   dim3(unsigned(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st,
+                                   static_cast<const T*>(p.x), p.ldx, static_cast<const T*>(p.residual), p.ldr, p.drop,
+                                   static_cast<T*>(p.y), p.rows, p.cols, groups);
+                return hipGetLastError();
+            });
+        });
+    });
+}
+
+hipError_t layer_norm(const LayerNorm& p, hipStream_t st) {
+    if (p.rows == 0 || p.cols == 0) return hipSuccess;
+    return by_type(p.type, [&](auto tag) {
+        using T = decltype(tag);
+        return by_flag(p.drop.below > 0, [&](auto drop) {
+            return by_flag(p.residual != nullptr, [&](auto res) {
+                constexpr bool DROP = decltype(drop)::value, RES = decltype(res)::value;
+                return p.weight_type == p.type ? norm_form<T, T, DROP, RES>(p, st) : norm_form<T, float, DROP, RES>(p, st);
+            });
+        });
+    });
+}
+
+}  // namespace tg

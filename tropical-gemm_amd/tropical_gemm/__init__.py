@@ -12,8 +12,10 @@ and the ``mod gpu`` functions of ``crates/tropical-gemm-python/src/lib.rs:1657-2
 * ``cuda_available()`` (lib.rs:2341-2344), true when a HIP device and the
   native library are present.
 
-``tropical_gemm.int8`` holds the operators of an 8-bit linear layer (no
-counterpart in the reference).
+``tropical_gemm.int8`` holds the operators of an 8-bit linear layer,
+``tropical_gemm.fp8`` those of one in 8-bit floating point with a scale for each
+block, and ``tropical_gemm.layers`` layer norm and dropout (no counterpart in the
+reference).
 
 The reference's numpy GPU functions hand row-major numpy data to its
 column-major API without the operand swap (lib.rs:1904-1907), which is wrong

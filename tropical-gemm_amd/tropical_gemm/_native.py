@@ -37,6 +37,8 @@ _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
+_u64 = ctypes.c_uint64
 SIGNATURES = {
     "tg_version": ([], _i32),
     "tg_status_string": ([_i32], ctypes.c_char_p),
@@ -100,6 +102,27 @@ SIGNATURES = {
     "tg_i8_backward_b_workspace_size": ([_i32, _vp, _i64, _i64, _i64, _i64], _sz),
     "tg_i8_backward_b": ([_i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz,
                           _vp], _i32),
+    "tg_f8_quantize": ([_i32, _i32, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp], _i32),
+    "tg_f8_dequantize": ([_i32, _i32, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp], _i32),
+    "tg_f8_gemm_workspace_size": ([_i32, _vp, _i64, _vp, _i64, _i64, _i64, _i64], _sz),
+    "tg_f8_gemm": ([_i32, _i32, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64,
+                    _i64, _i64, _vp, _sz, _vp], _i32),
+    "tg_f8_gemm_plan": ([_i32, _vp, _i64, _vp, _i64, _i64, _i64, _i64], ctypes.c_char_p),
+    "tg_f8_backward_plan": ([_i32, _i32, _vp, _i64, _i64, _i64, _i64], ctypes.c_char_p),
+    "tg_f8_backward_a_workspace_size": ([_i32, _vp, _i64, _i64, _i64, _i64], _sz),
+    "tg_f8_backward_a": ([_i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64,
+                          _vp, _sz, _vp], _i32),
+    "tg_f8_backward_b_workspace_size": ([_i32, _vp, _i64, _i64, _i64, _i64], _sz),
+    "tg_f8_backward_b": ([_i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64,
+                          _vp, _sz, _vp], _i32),
+    "tg_dropout": ([_i32, _i32, _vp, _i64, _vp, _i64, _f64, _u64, _vp, _u64, _vp, _i64, _i64, _vp],
+                   _i32),
+    "tg_layer_norm": ([_i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _f32, _f64, _u64, _vp, _u64,
+                       _vp, _vp, _vp, _vp, _i64, _i64, _vp], _i32),
+    "tg_layer_norm_backward_workspace_size": ([_i64, _i64], _sz),
+    "tg_layer_norm_backward": ([_i32, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64,
+                                _f64, _u64, _vp, _u64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz,
+                                _vp], _i32),
 }
 
 
