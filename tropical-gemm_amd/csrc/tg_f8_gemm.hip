@@ -115,14 +115,14 @@ hipError_t launch_form(F8TileArgs p, const TilePlan& pl, const TileStore<T>& out
         const auto kernel = &tg_f8_tiles<WM, WN, FM, FN, NB, PER_CU, T>;
         static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
         if (attr != hipSuccess) return attr;
-        hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, out);
+        hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, F8Store<T>{out.bias, out.c, out.n});
         return hipGetLastError();
     }
     const auto kernel = &tg_f8_tiles_slice<WM, WN, FM, FN, NB, PER_CU>;
     static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
     if (attr != hipSuccess) return attr;
     float* sums = static_cast<float*>(part);
-    hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, TilePartial<float>{sums, round_up(p.n, 8)});
+    hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, F8Partial{sums, round_up(p.n, 8)});
     const hipError_t e = hipGetLastError();
     return e != hipSuccess ? e : launch_join(sums, pl.slices, p.m, p.n, out, st);
 }
@@ -272,7 +272,8 @@ hipError_t gemm_typed(const F8Gemm& p, void* ws, hipStream_t st) {
         const hipError_t e = launch_pack(a, b, st);
         if (e != hipSuccess) return e;
     }
-    return launch_tiles(t, pl.tiles, out, w.part, st);
+    if constexpr (std::is_same<T, float>::value) return hipErrorInvalidValue;  // wide, above
+    else return launch_tiles(t, pl.tiles, out, w.part, st);
 }
 
 // ---- gradients -----------------------------------------------------------
