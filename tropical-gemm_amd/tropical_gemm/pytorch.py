@@ -23,7 +23,7 @@ from __future__ import annotations
 
 import torch
 
-from . import cuda_available, int8, ops
+from . import cuda_available, fp8, int8, layers, ops
 
 GPU_AVAILABLE = cuda_available()
 _DLPACK_AVAILABLE = True
@@ -339,6 +339,165 @@ def rms_norm_int8_linear_gpu(x: torch.Tensor, residual: torch.Tensor | None, nor
     return RmsNormInt8LinearGPU.apply(x, residual, norm_weight, weight, eps)
 
 
+# ---------------------------------------------------------------------------
+# Blocks in 8-bit floating point (no counterpart in the reference)
+# ---------------------------------------------------------------------------
+
+class Fp8LinearGPU(torch.autograd.Function):
+    """``y = x @ weight.T`` with both operands rounded to e4m3 numbers, one power of
+    two for each 1 x 128 activations and 128 x 128 weights.
+
+    The backward pass reads the 8-bit operands, which are all that is kept of them:
+    the gradients are those of the product of the rounded operands, passed through
+    the rounding unchanged.  They have no gradients of their own: differentiating
+    them is an error."""
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+        x, weight = _prep_int8("Fp8LinearGPU", x, weight)
+        q, scale = fp8.quantize(x)
+        qw, scale_w = fp8.quantize(weight, fp8.BLOCK)
+        ctx.save_for_backward(q, scale, qw, scale_w)
+        return fp8.matmul(q, scale, qw, scale_w, dtype=x.dtype)
+
+    @staticmethod
+    def backward(ctx, grad_y: torch.Tensor):
+        q, scale, qw, scale_w = ctx.saved_tensors
+        want_x, want_w = ctx.needs_input_grad
+        with torch.no_grad():
+            grad_y = grad_y.contiguous()
+            grads = (fp8.backward_a(grad_y, qw, scale_w) if want_x else None,
+                     fp8.backward_b(grad_y, q, scale) if want_w else None)
+        return _first_derivatives("Fp8LinearGPU", *grads)
+
+
+def _prep_rows(name: str, x: torch.Tensor, residual: torch.Tensor | None):
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} requires GPU tensors.")
+    return x.detach().contiguous(), None if residual is None else residual.detach().contiguous()
+
+
+def _save_seed(ctx, seed, p: float, offset: int, *tensors):
+    """Keeps what makes the mask; a seed on the GPU as a tensor, so that changing it
+    before the backward pass is an error."""
+    at = isinstance(seed, torch.Tensor)
+    ctx.save_for_backward(*tensors, *((seed,) if at else ()))
+    ctx.random = (p, None if at else seed, offset)
+
+
+def _saved_seed(ctx):
+    """(the other tensors, (p, seed, offset)) that _save_seed kept."""
+    p, seed, offset = ctx.random
+    saved = ctx.saved_tensors
+    return (saved[:-1], (p, saved[-1], offset)) if seed is None else (saved, (p, seed, offset))
+
+
+class DropoutGPU(torch.autograd.Function):
+    """``dropout(x) + residual``; nothing is kept for the backward pass but the
+    seed.  The gradients have no gradients of their own: differentiating them is
+    an error."""
+
+    @staticmethod
+    def forward(ctx, x, residual, p: float, seed, offset: int) -> torch.Tensor:
+        x, residual = _prep_rows("DropoutGPU", x, residual)
+        _save_seed(ctx, seed, p, offset)
+        return layers.dropout(x, p, seed, offset, residual)
+
+    @staticmethod
+    def backward(ctx, grad_y: torch.Tensor):
+        want_x, want_r = ctx.needs_input_grad[:2]
+        _, random = _saved_seed(ctx)
+        with torch.no_grad():
+            grad_x = layers.dropout(grad_y.contiguous(), *random) if want_x else None
+        (grad_x,) = _first_derivatives("DropoutGPU", grad_x)
+        return grad_x, grad_y if want_r else None, None, None, None
+
+
+class LayerNormGPU(torch.autograd.Function):
+    """``(y, h)`` of one step of a residual stream: ``h = dropout(x) + residual``,
+    ``y = layer_norm(h, weight, bias, eps)``.
+
+    Kept for the backward pass: h, its rows' statistics and the seed.  The gradients
+    have no gradients of their own: differentiating them is an error."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps: float, p: float, seed, offset: int):
+        x, residual = _prep_rows("LayerNormGPU", x, residual)
+        weight, bias = weight.detach().contiguous(), None if bias is None else bias.detach().contiguous()
+        y, h, mean, rstd = layers.layer_norm(x, weight, bias, residual, eps, p, seed, offset)
+        _save_seed(ctx, seed, p, offset, h, mean, rstd, weight)
+        ctx.set_materialize_grads(False)
+        # An output that shares no memory with an input.
+        return y, x.clone() if h is x else h
+
+    @staticmethod
+    def backward(ctx, grad_y, grad_h):
+        (h, mean, rstd, weight), (p, seed, offset) = _saved_seed(ctx)
+        want_x, want_r, want_w, want_b = ctx.needs_input_grad[:4]
+        with torch.no_grad():
+            grad_h = None if grad_h is None else grad_h.contiguous()
+            if grad_y is not None:
+                grads = layers.layer_norm_backward(grad_y.contiguous(), h, mean, rstd, weight, grad_h, p, seed, offset)
+            elif grad_h is not None:
+                grads = layers.dropout(grad_h, p, seed, offset), grad_h, None, None
+            else:
+                grads = None, None, None, None
+            grads = tuple(g if want else None for g, want in zip(grads, (want_x, want_r, want_w, want_b)))
+        return *_first_derivatives("LayerNormGPU", *grads), None, None, None, None
+
+
+def _seed_of(x: torch.Tensor, p: float, seed):
+    """The seed, drawn by torch's generator of x's device where none is given (in a
+    captured graph, each replay draws another)."""
+    if seed is None and p > 0:
+        return torch.randint(0, 2 ** 63 - 1, (1,), dtype=torch.int64, device=x.device)
+    return 0 if seed is None else seed
+
+
+def fp8_linear_gpu(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """``x @ weight.T`` in 8-bit floating point, with gradients (``Fp8LinearGPU``)."""
+    return Fp8LinearGPU.apply(x, weight)
+
+
+def dropout_gpu(x: torch.Tensor, p: float, residual: torch.Tensor | None = None, seed=None,
+                offset: int = 0) -> torch.Tensor:
+    """``dropout(x) + residual`` with gradients (``DropoutGPU``)."""
+    return DropoutGPU.apply(x, residual, p, _seed_of(x, p, seed), offset)
+
+
+def layer_norm_gpu(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                   eps: float = 1e-5) -> torch.Tensor:
+    """``layer_norm(x)`` with gradients (``LayerNormGPU``)."""
+    return _LayerNormOnlyGPU.apply(x, weight, bias, eps)
+
+
+def dropout_add_layer_norm_gpu(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor,
+                               bias: torch.Tensor | None = None, p: float = 0.0, eps: float = 1e-5, seed=None,
+                               offset: int = 0):
+    """``(layer_norm(h), h)`` of ``h = dropout(x) + residual``, with gradients
+    (``LayerNormGPU``)."""
+    return LayerNormGPU.apply(x, residual, weight, bias, eps, p, _seed_of(x, p, seed), offset)
+
+
+class _LayerNormOnlyGPU(torch.autograd.Function):
+    """``LayerNormGPU`` where the stream is x itself: y alone."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps: float):
+        x, _ = _prep_rows("LayerNormGPU", x, None)
+        weight, bias = weight.detach().contiguous(), None if bias is None else bias.detach().contiguous()
+        y, _, mean, rstd = layers.layer_norm(x, weight, bias, None, eps)
+        ctx.save_for_backward(x, mean, rstd, weight)
+        return y
+
+    @staticmethod
+    def backward(ctx, grad_y):
+        with torch.no_grad():
+            grad_x, _, grad_w, grad_b = layers.layer_norm_backward(grad_y.contiguous(), *ctx.saved_tensors)
+            grads = tuple(g if want else None for g, want in zip((grad_x, grad_w, grad_b), ctx.needs_input_grad))
+        return *_first_derivatives("LayerNormGPU", *grads), None
+
+
 __all__ = [
     "TropicalMaxPlusMatmulGPU",
     "TropicalMinPlusMatmulGPU",
@@ -356,6 +515,13 @@ __all__ = [
     "RmsNormInt8LinearGPU",
     "int8_linear_gpu",
     "rms_norm_int8_linear_gpu",
+    "Fp8LinearGPU",
+    "DropoutGPU",
+    "LayerNormGPU",
+    "fp8_linear_gpu",
+    "dropout_gpu",
+    "layer_norm_gpu",
+    "dropout_add_layer_norm_gpu",
     "GPU_AVAILABLE",
     "_DLPACK_AVAILABLE",
 ]
