@@ -139,7 +139,7 @@ def test_weight_type(name):
 def test_workspaces():
     lib = nat.load()
     need = lib.tg_layer_norm_backward_workspace_size(4, 8)
-    assert need == 4 * 2 * 8 * 4 and lib.tg_layer_norm_backward_workspace_size(-1, 8) == NONE
+    assert need == 2 * 8 * 4 and lib.tg_layer_norm_backward_workspace_size(-1, 8) == NONE
     assert _call("tg_layer_norm_backward", ws_bytes=need - 1) == nat.TG_ERR_INVALID_ARGUMENT
     assert "workspace too small" in nat.last_error()
     assert _call("tg_layer_norm_backward", ws=P + 16) == nat.TG_ERR_INVALID_ARGUMENT

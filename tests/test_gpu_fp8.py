@@ -237,13 +237,16 @@ def test_matmul_f16_in_range(m, n, k):
     assert (c.cpu().double() - want).norm() <= 3e-4 * want.norm()
 
 
-@pytest.mark.parametrize("form", ["tiles 256x256", "tiles 128x128", "tiles 64x64"])
+@pytest.mark.parametrize("form", ["tiles 256x256", "tiles 128x256", "tiles 128x128", "tiles 128x64 halves",
+                                  "tiles 64x64", "tiles 64x64 halves"])
 def test_every_tile(form):
     """Each tile form is the plan of some product, whole and with edges."""
     found = 0
     for m, n, k in [(8192, 8192, 128), (8192 - 5, 4096 + 3, 144), (1500, 1400, 256), (1111, 1500, 384),
                     (4096, 1024, 512), (300, 256, 512), (2048, 2048, 144), (700, 900, 272), (5000, 6000, 128),
-                    (4096, 4096, 2048), (4096 - 5, 4096 + 3, 1040), (8192, 4096, 1024), (2053, 4099, 4112)]:
+                    (4096, 4096, 2048), (4096 - 5, 4096 + 3, 1040), (8192, 4096, 1024), (2053, 4099, 4112),
+                    (100, 1000, 4096), (129, 1033, 4240), (250, 8192, 4096), (131, 8190, 8080), (2048, 4096, 2048),
+                    (2047, 4090, 2064), (3500, 6000, 1024), (2048, 2560, 4096), (2041, 2563, 4112)]:
         plan = nat.load().tg_f8_gemm_plan(1, 256, k, 256, k, m, n, k).decode()
         if plan.split(" slices")[0] != form:
             continue

@@ -33,13 +33,14 @@ struct Keep {
     __device__ __forceinline__ explicit Keep(const Dropout& d)
         : below(d.below), o0(uint32_t(d.offset)), o1(uint32_t(d.offset >> 32)), factor(d.factor) {
         const uint64_t seed = d.seed_at != nullptr ? *d.seed_at : d.seed;
-        k0 = uint32_t(seed);
-        k1 = uint32_t(seed >> 32);
+        k0 = __builtin_amdgcn_readfirstlane(uint32_t(seed));
+        k1 = __builtin_amdgcn_readfirstlane(uint32_t(seed >> 32));
     }
     // Bit i: element 8 * group + i of the row is kept.
     __device__ __forceinline__ uint32_t group(int64_t row, uint32_t group) const {
-        uint32_t c[4] = {group, uint32_t(row), o0, o1};
-        philox(c, k0, k1);
+        uint32_t c[4] = {group, uint32_t(row), o0, o1}, a = k0, b = k1;
+        asm volatile("" : "+s"(a), "+s"(b));  // or a loop keeps the keys of all rounds in registers
+        philox(c, a, b);
         uint32_t bits = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -56,11 +57,11 @@ struct Keep {
         if (shift != 0) bits = (bits | group(row, g + 1) << 8) >> shift;
         return bits;
     }
-    __device__ __forceinline__ void apply(int64_t row, int64_t at, float (&v)[8]) const {
-        const uint32_t bits = from(row, at);
+    __device__ __forceinline__ void apply(uint32_t bits, float (&v)[8]) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = (bits >> i & 1u) != 0 ? v[i] * factor : 0.0f;
     }
+    __device__ __forceinline__ void apply(int64_t row, int64_t at, float (&v)[8]) const { apply(from(row, at), v); }
 };
 
 }  // namespace tg

@@ -25,15 +25,26 @@ hipError_t by_type(int type, F&& f) {
 
 // ---- choice of a tile ----------------------------------------------------
 
-// A tile's sizes, workgroups per CU, and its time in us: `start` + `step` for each
-// block of the sum while every workgroup has a CU of its own, otherwise rounds of
-// `round` + `full` for each block.
+// A tile's sizes, workgroups per CU, halves of its waves that share the sum, and
+// its time in us: `start` + step for each block of the sum while every workgroup
+// has a CU of its own (`crowd` more as the last CUs fill), otherwise rounds of
+// `round` + full for each block.  Fitted to 132 products on MI355X (M 64 ... 8192,
+// N 1024 ... 8192, K 256 ... 8192): the tile with the least time so reckoned is 0.6%
+// slower than the best of them in the mean, 16% at most.  A last round that only
+// some CUs have with several workgroups takes most of a whole one's time.
+//
+// A block costs a CU 64 bytes a clock at most on their way into LDS: 0.23 us for
+// 128 x 128 outputs, 0.47 for 256 x 256, four times as many, where the matrix
+// instructions take 0.95; so the tiles are as large as they can be with all CUs at
+// work.
 struct TileTime {
-    int bm, bn, per_cu;
-    double start, step, round, full;
+    int bm, bn, per_cu, halves;
+    double start, step, crowd, round, full;
 };
 constexpr TileTime kTiles[] = {
-    {256, 256, 1, 7.0, 1.1, 7.0, 1.2}, {128, 128, 2, 4.0, 0.42, 3.0, 0.80}, {64, 64, 3, 2.8, 0.20, 1.0, 0.48},
+    {256, 256, 1, 1, 11.93, 0.946, 0.558, 10.31, 1.322}, {128, 256, 1, 1, 8.13, 0.491, 0.308, 6.00, 0.728},
+    {128, 128, 2, 1, 5.96, 0.345, 0.089, 3.72, 0.820},   {128, 64, 1, 2, 5.82, 0.205, 0.073, 3.63, 0.272},
+    {64, 64, 3, 1, 3.74, 0.248, 0.023, 1.51, 0.513},     {64, 64, 1, 2, 3.99, 0.197, 0.025, 2.03, 0.207},
 };
 constexpr int kTileForms = sizeof(kTiles) / sizeof(kTiles[0]);
 
@@ -43,9 +54,16 @@ struct TilePlan {
 };
 
 double tile_time(const TileTime& c, int64_t tiles, int64_t steps) {
-    if (tiles <= 256) return c.start + double(steps) * c.step;
-    const int64_t slots = 256 * int64_t(c.per_cu);
-    return 3 + double(ceil_div(tiles, slots)) * (c.round + double(steps) * c.full);
+    const double alone = c.step + (tiles > 128 ? c.crowd * double((tiles < 256 ? tiles : 256) - 128) / 128 : 0);
+    if (tiles <= 256) return c.start + double(steps) * alone;
+    const int64_t slots = 256 * int64_t(c.per_cu), whole = tiles / slots;
+    const double last = double(tiles - whole * slots) / double(slots), depth = last * c.per_cu;
+    double t = 3 + double(whole) * (c.round + double(steps) * c.full);
+    if (last > 0 && c.per_cu > 1)
+        t += c.round + double(steps) * (depth <= 1 ? alone : alone + (c.full - alone) * (0.6 + 0.4 * (depth - 1) / (c.per_cu - 1)));
+    else if (last > 0)
+        t += c.round + double(steps) * c.full * (0.75 + 0.25 * last);
+    return t;
 }
 
 TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps) {
@@ -54,16 +72,17 @@ TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps) {
     for (int f = 0; f < kTileForms; ++f) {
         const TileTime& c = kTiles[f];
         const int64_t tm = ceil_div(m, c.bm), tn = ceil_div(n, c.bn);
-        if (tm * tn >= int64_t(1) << 24) continue;  // a launch's thread count stays below 2^32
+        if (tm * tn >= int64_t(1) << 23) continue;  // a launch's thread count stays below 2^32
         for (int s = 1; s <= 32; s *= 2) {
-            const int64_t slice = ceil_div(steps, s);
+            const int64_t slice = ceil_div(steps, s), slices = ceil_div(steps, slice);
             if (s > 1 && (tm * tn * s > 512 || slice < 4)) break;
+            if (steps - (slices - 1) * slice < c.halves) continue;  // a step for each half
             double t = tile_time(c, tm * tn * s, slice);
             // Partial sums' way through memory and the launch that joins them.
             if (s > 1) t += 4.5 + double(s + 1) * double(m) * double(n) * 4 / 4e6;
             if (t < least) {
                 least = t;
-                best = {f, int(ceil_div(steps, slice)), tm, tn, slice, steps};
+                best = {f, int(slices), tm, tn, slice, steps};
             }
         }
     }
@@ -73,6 +92,7 @@ TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps) {
 std::string tiles_name(const TilePlan& pl) {
     const TileTime& c = kTiles[pl.form];
     std::string name = "tiles " + std::to_string(c.bm) + "x" + std::to_string(c.bn);
+    if (c.halves > 1) name += " halves";
     if (pl.slices > 1) name += " slices " + std::to_string(pl.slices);
     return name;
 }
@@ -107,22 +127,22 @@ hipError_t launch_join(const float* part, int slices, int64_t m, int64_t n, cons
     return hipGetLastError();
 }
 
-template <int WM, int WN, int FM, int FN, int NB, int PER_CU, typename T>
+template <int WM, int WN, int FM, int FN, int NB, int KS, int PER_CU, typename T>
 hipError_t launch_form(F8TileArgs p, const TilePlan& pl, const TileStore<T>& out, void* part, hipStream_t st) {
-    using Cfg = F8Tile<WM, WN, FM, FN, NB>;
+    using Cfg = F8Tile<WM, WN, FM, FN, NB, KS>;
     const dim3 grid(unsigned(pl.tiles_m * pl.tiles_n), unsigned(pl.slices));
     if (pl.slices == 1) {
-        const auto kernel = &tg_f8_tiles<WM, WN, FM, FN, NB, PER_CU, T>;
+        const auto kernel = &tg_f8_tiles<WM, WN, FM, FN, NB, KS, PER_CU, T>;
         static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
         if (attr != hipSuccess) return attr;
-        hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, F8Store<T>{out.bias, out.c, out.n});
+        hipLaunchKernelGGL(kernel, grid, dim3(Cfg::THREADS), Cfg::LDS, st, p, F8Store<T>{out.bias, out.c, out.n});
         return hipGetLastError();
     }
-    const auto kernel = &tg_f8_tiles_slice<WM, WN, FM, FN, NB, PER_CU>;
+    const auto kernel = &tg_f8_tiles_slice<WM, WN, FM, FN, NB, KS, PER_CU>;
     static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
     if (attr != hipSuccess) return attr;
     float* sums = static_cast<float*>(part);
-    hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, F8Partial{sums, round_up(p.n, 8)});
+    hipLaunchKernelGGL(kernel, grid, dim3(Cfg::THREADS), Cfg::LDS, st, p, F8Partial{sums, round_up(p.n, 8)});
     const hipError_t e = hipGetLastError();
     return e != hipSuccess ? e : launch_join(sums, pl.slices, p.m, p.n, out, st);
 }
@@ -134,9 +154,12 @@ hipError_t launch_tiles(F8TileArgs p, const TilePlan& pl, const TileStore<T>& ou
     p.slice = int(pl.slice);
     p.steps = int(pl.steps);
     switch (pl.form) {
-        case 0: return launch_form<2, 2, 4, 4, 2, 1>(p, pl, out, part, st);
-        case 1: return launch_form<2, 2, 2, 2, 2, 2>(p, pl, out, part, st);
-        default: return launch_form<2, 2, 1, 1, 3, 3>(p, pl, out, part, st);
+        case 0: return launch_form<2, 2, 4, 4, 2, 1, 1>(p, pl, out, part, st);
+        case 1: return launch_form<2, 2, 2, 4, 2, 1, 1>(p, pl, out, part, st);
+        case 2: return launch_form<2, 2, 2, 2, 2, 1, 2>(p, pl, out, part, st);
+        case 3: return launch_form<2, 1, 2, 2, 2, 2, 1>(p, pl, out, part, st);
+        case 4: return launch_form<2, 2, 1, 1, 3, 1, 3>(p, pl, out, part, st);
+        default: return launch_form<2, 2, 1, 1, 3, 2, 1>(p, pl, out, part, st);
     }
 }
 

@@ -75,12 +75,13 @@ struct F8TileArgs {
 // of LDS row L lies at place c ^ (L / 2 % 8): LDS serves lanes {0-3, 12-15, 20-27}
 // and {4-11, 16-19, 28-31} of each 32 at a time, and so they meet 16 different
 // places of the 256 bytes that two rows take.
-template <int WM, int WN, int FM, int FN, int NB>
+template <int WM, int WN, int FM, int FN, int NB, int KS = 1>
 struct F8Tile {
     static constexpr int BM = WM * FM * 32, BN = WN * FN * 32, WAVES = WM * WN, NT = WAVES * 64;
     static constexpr int LOADS_A = BM * 8 / NT, LOADS_B = BN * 8 / NT, LOADS = LOADS_A + LOADS_B + 2;
     static constexpr int AT_B = BM * 128, AT_SA = AT_B + BN * 128, AT_SB = AT_SA + BM * 4;
-    static constexpr int STAGE = AT_SB + WAVES * 256, LDS = NB * STAGE;
+    static constexpr int STAGE = AT_SB + WAVES * 256, LDS = KS * NB * STAGE;
+    static constexpr int THREADS = KS * NT, MERGE = KS > 1 ? WAVES * FM * FN * 4096 : 0;
     static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0 && BM % 64 == 0, "whole loads");
     static_assert(NB >= 2 && NB <= 4, "wait_for's cases");
     static_assert(128 % (FN * 32) == 0, "one scale of B for a wave");
@@ -110,7 +111,7 @@ struct F8Tile {
     // Sums steps [s0, s1), at least one, of tile (tm, tn) into acc.
     static __device__ __forceinline__ void run(const F8TileArgs& p, int tm, int tn, int s0, int s1, lds_t* lds,
                                                f32x16 (&acc)[FM][FN]) {
-        const int t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64);
+        const int t = threadIdx.x % NT, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64);
         const uint32_t lds0 = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>(lds)));
         const int wm = wave / WN, wn = wave % WN, li = lane % 32, hh = lane / 32;
         const char* a0 = reinterpret_cast<const char*>(p.a) + int64_t(tm) * BM * p.lda;
@@ -289,7 +290,7 @@ struct F8Tile {
     static __device__ __forceinline__ void run_pairs(const F8TileArgs& p, int tm, int tn, int s0, int s1, lds_t* lds,
                                                      f32x16 (&acc)[FM][FN]) {
         static_assert(NB == 2 && FM % 2 == 0 && FN % 2 == 0, "halves");
-        const int t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64);
+        const int t = threadIdx.x % NT, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64);
         const uint32_t lds0 = __builtin_amdgcn_readfirstlane(uint32_t(reinterpret_cast<uintptr_t>(lds)));
         const int wm = wave / WN, wn = wave % WN, li = lane % 32, hh = lane / 32;
         const char* a0 = reinterpret_cast<const char*>(p.a) + int64_t(tm) * BM * p.lda;
@@ -484,12 +485,11 @@ struct F8Tile {
         constexpr int SIZE = Out::SIZE, PER = 16 / SIZE;  // bytes of an output, outputs of a chunk
         constexpr int J = FN * 32 * SIZE > 256 ? FN / 2 : FN, COLS = J * 32, CH = COLS / PER;
         constexpr int ROWS = FM * 32, AT_ONCE = 64 / CH;  // rows that a wave stores at a time
-        static_assert(WAVES * ROWS * CH * 16 <= LDS, "the tile's outputs fit");
+        static_assert(MERGE + WAVES * ROWS * CH * 16 <= LDS, "the tile's outputs fit");
         const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, li = lane % 32, hh = lane / 32;
         const int m0 = tm * BM + wave / WN * ROWS, n0 = tn * BN + wave % WN * FN * 32;
-        u32x4* mine = reinterpret_cast<u32x4*>(smem) + wave * ROWS * CH;
+        u32x4* mine = reinterpret_cast<u32x4*>(smem + MERGE) + wave * ROWS * CH;
         auto place = [](int r, int c) { return r * CH + (c ^ (r / FM & (CH - 1))); };
-        __syncthreads();  // all have read their last fragments
 #pragma unroll
         for (int j0 = 0; j0 < FN; j0 += J) {
             // A lane has 16 * FN columns, of which J * 16 belong to this pass: the
@@ -517,15 +517,52 @@ struct F8Tile {
         }
     }
 
-    // The workgroup's tile over slice `y` of the sum, from there to `out`.
+    // The workgroup's tile over slice `y` of the sum, from there to `out`.  KS 2:
+    // the second half of the waves takes the second half of the slice's steps, at
+    // least two, from stages of its own, and hands its sums over in LDS: where there
+    // is a workgroup for each CU at most, waves that wait leave the matrix unit to
+    // the others.
     template <typename Out>
     static __device__ __forceinline__ void whole(const F8TileArgs& p, int y, char* smem, const Out& out) {
-        const int s0 = y * p.slice, s1 = s0 + p.slice < p.steps ? s0 + p.slice : p.steps;
+        int s0 = y * p.slice, s1 = s0 + p.slice < p.steps ? s0 + p.slice : p.steps;
         f32x16 acc[FM][FN] = {};
         int tm, tn;
         place(p, tm, tn);
-        if constexpr (PAIRS) run_pairs(p, tm, tn, s0, s1, (lds_t*)(smem), acc);
-        else run(p, tm, tn, s0, s1, (lds_t*)(smem), acc);
+        const int part = KS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
+        bool fewer = false;  // steps than the other half
+        if constexpr (KS > 1) {
+            static_assert(KS == 2, "halves");
+            const int half = (s1 - s0 + 1) / 2;
+            fewer = part != 0 && (s1 - s0) % 2 != 0;
+            if (part == 0) s1 = s0 + half;
+            else s0 += half;
+        }
+        lds_t* stages = (lds_t*)(smem) + part * NB * STAGE;
+        if constexpr (PAIRS) run_pairs(p, tm, tn, s0, s1, stages, acc);
+        else run(p, tm, tn, s0, s1, stages, acc);
+        if (fewer) {  // the barriers of the step that it lacks
+            __builtin_amdgcn_s_barrier();
+            if (PAIRS) __builtin_amdgcn_s_barrier();
+        }
+        __syncthreads();  // all have read their last fragments
+        if constexpr (KS > 1) {
+            f32x4* sums = reinterpret_cast<f32x4*>(smem) + threadIdx.x % NT / 64 * (FM * FN * 256) + threadIdx.x % 64;
+            if (part != 0) {
+#pragma unroll
+                for (int f = 0; f < FM * FN * 4; ++f) {
+                    const f32x16& a = acc[f / 4 / FN][f / 4 % FN];
+                    sums[f * 64] = f32x4{a[f % 4 * 4], a[f % 4 * 4 + 1], a[f % 4 * 4 + 2], a[f % 4 * 4 + 3]};
+                }
+            }
+            __syncthreads();
+            if (part != 0) return;
+#pragma unroll
+            for (int f = 0; f < FM * FN * 4; ++f) {
+                const f32x4 v = sums[f * 64];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[f / 4 / FN][f / 4 % FN][f % 4 * 4 + e] += v[e];
+            }
+        }
         outputs(p, tm, tn, smem, acc, out);
     }
 };
@@ -605,18 +642,18 @@ struct F8Partial {
     }
 };
 
-template <int WM, int WN, int FM, int FN, int NB, int PER_CU, typename T>
-__global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_f8_tiles(F8TileArgs p, F8Store<T> out) {
+template <int WM, int WN, int FM, int FN, int NB, int KS, int PER_CU, typename T>
+__global__ __launch_bounds__(WM* WN * 64 * KS, PER_CU) void tg_f8_tiles(F8TileArgs p, F8Store<T> out) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    F8Tile<WM, WN, FM, FN, NB>::whole(p, 0, smem, out);
+    F8Tile<WM, WN, FM, FN, NB, KS>::whole(p, 0, smem, out);
 }
 
 // Slice blockIdx.y of the sum: its sums to part + blockIdx.y * M * ld.
-template <int WM, int WN, int FM, int FN, int NB, int PER_CU>
-__global__ __launch_bounds__(WM* WN * 64, PER_CU) void tg_f8_tiles_slice(F8TileArgs p, F8Partial out) {
+template <int WM, int WN, int FM, int FN, int NB, int KS, int PER_CU>
+__global__ __launch_bounds__(WM* WN * 64 * KS, PER_CU) void tg_f8_tiles_slice(F8TileArgs p, F8Partial out) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     out.c += int64_t(blockIdx.y) * p.m * out.ld;
-    F8Tile<WM, WN, FM, FN, NB>::whole(p, int(blockIdx.y), smem, out);
+    F8Tile<WM, WN, FM, FN, NB, KS>::whole(p, int(blockIdx.y), smem, out);
 }
 
 }  // namespace tg

@@ -62,7 +62,8 @@ template <typename T, typename W, bool DROP, bool RES, int NT, int VPT>
 __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> p) {
     constexpr bool STREAM = DROP || RES;  // h is not x
     const int t = threadIdx.x % NT;
-    const int64_t row = int64_t(blockIdx.x) * kRowsPerBlock<NT> + threadIdx.x / NT;
+    const int64_t row = int64_t(blockIdx.x) * kRowsPerBlock<NT> +
+                        (kRowsPerBlock<NT> > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0);  // of the wave
     const bool live = row < p.rows;  // every thread reaches the barriers
     const int64_t cols = p.cols;
     const T* xr = p.x + row * p.ldx;

@@ -16,35 +16,55 @@ struct BackwardArgs {
     int64_t rows, cols;
 };
 
+enum class Form { PLAIN, TINY, WIDE };
+
+// Rows that a workgroup holds at a time: 512 threads are at work on short ones
+// too (bf16, 8192 x 1024: 30 us one row at a time, XX so).
+template <int NT>
+constexpr int kRowsAtOnce = NT < 512 ? 512 / NT : 1;
+
 // xh = (h - mean) * rstd, u = gy * w, gr = rstd * (u - mean(u) - xh * mean(u *
-// xh)) + gh, gx = dropout(gr); the workgroup adds gy * xh and gy of its rows
-// (blockIdx.x, + gridDim.x, ...) in that order in registers and writes those
-// sums of each column to its two rows of `part`.  A thread holds eight columns;
-// its weights stay in registers, and the next row is loaded before this one is
-// reduced.  A row longer than NT * 8 is shared by blockIdx.y: every workgroup
-// reduces all of it and stores its own columns.  A row's last group is moved
-// back to end with the row; TINY, rows below eight elements, is one group with a
-// bound.
-template <typename T, typename W, bool DROP, bool GH, int NT, bool TINY>
-__global__ __launch_bounds__(NT) void tg_layer_norm_backward_rows(BackwardArgs<T, W> p) {
-    constexpr int W64 = NT / 64;
-    __shared__ float red[2][2][W64];
+// xh)) + gh, gx = dropout(gr); each of the G parts of a workgroup adds gy * xh and
+// gy of its rows (blockIdx.x * G, + gridDim.x * G, ...) in that order in registers,
+// the parts' sums are added in their order, and each column's go to the
+// workgroup's two rows of `part`.  A thread holds eight columns; its weights stay
+// in registers, and the next row is loaded, and what it drops made, before this
+// one is reduced.  A row's last group is moved back to end with the row.  TINY, rows
+// below eight elements, is one group with a bound; WIDE, a row longer than NT * 8, is
+// shared by blockIdx.y: every workgroup reduces all of it and stores its own
+// columns.
+template <typename T, typename W, bool DROP, bool GH, int NT, Form FORM>
+__global__ __launch_bounds__(NT* kRowsAtOnce<NT>, 4) void tg_layer_norm_backward_rows(BackwardArgs<T, W> p) {
+    constexpr int W64 = NT / 64, G = kRowsAtOnce<NT>;
+    constexpr bool TINY = FORM == Form::TINY, WIDE = FORM == Form::WIDE;
+    __shared__ float red[2][2][G * W64];
     const int64_t rows = p.rows, cols = p.cols;
-    const int t = threadIdx.x, wave = t / 64;
-    const int64_t base = int64_t(blockIdx.y) * (NT * 8), start = base + int64_t(t) * 8;
-    const int64_t at = TINY ? 0 : start <= cols - 8 ? start : cols - 8;
-    const bool live = start < cols;
-    const int again = live ? int(start - at) : 8;  // elements of the group before this one
-    const int n = TINY ? int(cols) : 8;
+    const int t = threadIdx.x % NT, wave = threadIdx.x / 64;
+    const int group = G > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0, first = group * W64;
+    // Columns fit 32 bits, and a row is the same in all lanes: addresses are one of
+    // the wave's and one offset of the lane's.
+    const int n_cols = int(cols), base = WIDE ? int(blockIdx.y) * (NT * 8) : 0, start = base + t * 8;
+    const int at = TINY ? 0 : start <= n_cols - 8 ? start : n_cols - 8;
+    const bool live = start < n_cols;
+    const int again = live ? start - at : 8;  // elements of the group before this one
+    const int n = TINY ? n_cols : 8;
     const Keep keep(p.drop);
+    // `again` without what the compiler knows of it: eight comparisons made once
+    // and kept for all rows take more registers than there are.
+    auto fresh = [&] {
+        int a = again;
+        asm volatile("" : "+v"(a));
+        return a;
+    };
     // Stores the thread's group, without the columns before the workgroup's first.
     auto store = [&](auto* to, const float(&v)[8]) {
-        if (at >= base) {
-            store_upto8(to, n, v);
+        if (!TINY && (!WIDE || at >= base)) {
+            store8(to, v);
         } else {
+            const int a = fresh();
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (i >= again) to[i] = static_cast<std::remove_reference_t<decltype(*to)>>(v[i]);
+                if (i >= a && i < n) to[i] = static_cast<std::remove_reference_t<decltype(*to)>>(v[i]);
         }
     };
     auto load8_of = [&](const auto* from, auto& x) {
@@ -57,6 +77,7 @@ __global__ __launch_bounds__(NT) void tg_layer_norm_backward_rows(BackwardArgs<T
     struct Row {
         Eight<T> g, h, gh;
         float mean, rstd;
+        uint32_t kept;
     } x[2];
     auto load = [&](int64_t row, Row& r) {
         if (row >= rows) return;
@@ -65,16 +86,17 @@ __global__ __launch_bounds__(NT) void tg_layer_norm_backward_rows(BackwardArgs<T
         if constexpr (GH) load8_of(p.gh + row * p.ldgh + at, r.gh);
         r.mean = p.mean[row];
         r.rstd = p.rstd[row];
+        if constexpr (DROP) r.kept = keep.from(row, at);
     };
     // (h - mean) * rstd; h - mean may pass f32, half of it does not.
     auto normal = [](float h, float mean, float rstd) { return (h * 0.5f - mean * 0.5f) * (rstd * 2.0f); };
     const float inv_n = 1.0f / float(cols);
     auto finish = [&](int64_t row, const Row& r, int slot) {
         float su = 0.0f, dot = 0.0f, xh[8], u[8];
-        if (gridDim.y > 1) {  // the part of the row that other workgroups hold
-            for (int64_t c = int64_t(t) * 8; c < cols; c += NT * 8) {
+        if (WIDE) {  // the part of the row that other workgroups hold
+            for (int c = t * 8; c < n_cols; c += NT * 8) {
                 if (c >= base && c < base + NT * 8) continue;
-                const int left = cols - c < 8 ? int(cols - c) : 8;
+                const int left = n_cols - c < 8 ? n_cols - c : 8;
                 float a[8], b[8], d[8];
                 load_upto8(p.gy + row * p.ldg + c, left, a);
                 load_upto8(p.h + row * p.ldh + c, left, b);
@@ -87,13 +109,13 @@ __global__ __launch_bounds__(NT) void tg_layer_norm_backward_rows(BackwardArgs<T
                 }
             }
         }
+        const int own = fresh();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             xh[i] = normal(to_f32(r.h.v[i]), r.mean, r.rstd);
             u[i] = to_f32(r.g.v[i]) * to_f32(wv.v[i]);
-            const bool counts = i >= again && (!TINY || i < n);
-            su += counts ? u[i] : 0.0f;
-            dot += counts ? u[i] * xh[i] : 0.0f;
+            su += i >= own ? u[i] : 0.0f;
+            dot += i >= own ? u[i] * xh[i] : 0.0f;
         }
         su = wave_sum(su);
         dot = wave_sum(dot);
@@ -106,10 +128,11 @@ __global__ __launch_bounds__(NT) void tg_layer_norm_backward_rows(BackwardArgs<T
             su = dot = 0.0f;
 #pragma unroll
             for (int i = 0; i < W64; ++i) {
-                su += red[slot][0][i];
-                dot += red[slot][1][i];
+                su += red[slot][0][first + i];
+                dot += red[slot][1][first + i];
             }
         }
+        if (G > 1 && row >= rows) return;
         su *= inv_n;
         dot *= inv_n;
         float o[8];
@@ -124,17 +147,37 @@ __global__ __launch_bounds__(NT) void tg_layer_norm_backward_rows(BackwardArgs<T
         if (!live) return;
         store(p.gr + row * cols + at, o);
         if constexpr (DROP) {
-            keep.apply(row, at, o);
+            keep.apply(r.kept, o);
             store(p.gx + row * cols + at, o);
         }
     };
-    const int64_t stride = gridDim.x;
-    load(blockIdx.x, x[0]);
-    for (int64_t row = blockIdx.x; row < rows; row += 2 * stride) {
-        load(row + stride, x[1]);
-        finish(row, x[0], 0);
-        load(row + 2 * stride, x[0]);
-        if (row + stride < rows) finish(row + stride, x[1], 1);
+    // Every part of the workgroup reaches the barriers of its first part's rows.
+    const int64_t stride = int64_t(gridDim.x) * G, from = int64_t(blockIdx.x) * G;
+    load(from + group, x[0]);
+    for (int64_t row = from; row < rows; row += 2 * stride) {
+        load(row + stride + group, x[1]);
+        finish(row + group, x[0], 0);
+        load(row + 2 * stride + group, x[0]);
+        if (row + stride < rows) finish(row + stride + group, x[1], 1);
+    }
+    if constexpr (G > 1) {
+        __shared__ f32x4 sums[G][4][NT];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float* a = q < 2 ? acc_w + 4 * q : acc_b + 4 * (q - 2);
+            sums[group][q][t] = f32x4{a[0], a[1], a[2], a[3]};
+        }
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (int g = 1; g < G; ++g)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float* a = q < 2 ? acc_w + 4 * q : acc_b + 4 * (q - 2);
+                const f32x4 v = sums[g][q][t];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] += v[e];
+            }
     }
     if (live) {
         float* to = p.part + int64_t(blockIdx.x) * 2 * cols + at;
@@ -143,44 +186,52 @@ __global__ __launch_bounds__(NT) void tg_layer_norm_backward_rows(BackwardArgs<T
     }
 }
 
-// gw and gb: each column's sum over the parts, 64 slices of them, each in order
-// with four loads on their way, then the slices in order: the same bits in every
+// gw and gb: each column's sum over the parts, 32 slices of them, each in order
+// with eight loads on their way, then the slices in order: the same bits in every
 // run.  Columns from `cols` on are the bias's.
 template <typename W>
 __global__ __launch_bounds__(1024) void tg_layer_norm_sum_parts(const float* __restrict__ part, int64_t parts,
                                                                 W* __restrict__ gw, W* __restrict__ gb, int64_t cols) {
-    __shared__ float s[64][17];
-    const int c = threadIdx.x % 16, y = threadIdx.x / 16;
-    const int64_t col = int64_t(blockIdx.x) * 16 + c, wide = 2 * cols;
+    __shared__ float s[32][33];
+    const int c = threadIdx.x % 32, y = threadIdx.x / 32;
+    const int64_t col = int64_t(blockIdx.x) * 32 + c, wide = 2 * cols;
     float a = 0.0f;
     if (col < wide) {
         for (int64_t r = y; r < parts; r += 256) {
-            float v[4];
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = r + 64 * i < parts ? part[(r + 64 * i) * wide + col] : 0.0f;
+            for (int i = 0; i < 8; ++i) v[i] = r + 32 * i < parts ? part[(r + 32 * i) * wide + col] : 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a += v[i];
+            for (int i = 0; i < 8; ++i) a += v[i];
         }
     }
     s[y][c] = a;
     __syncthreads();
-    if (threadIdx.x < 16 && col < wide) {
+    if (threadIdx.x < 32 && col < wide) {
         a = s[0][c];
 #pragma unroll
-        for (int i = 1; i < 64; ++i) a += s[i][c];
+        for (int i = 1; i < 32; ++i) a += s[i][c];
         if (col < cols) gw[col] = static_cast<W>(a);
         else gb[col - cols] = static_cast<W>(a);
     }
 }
 
+// Threads of a row.
+int64_t row_threads(int64_t cols) {
+    for (int64_t n = 64; n < 1024; n *= 2)
+        if (cols <= n * 8) return n;
+    return 1024;
+}
+
 // Workgroups along the rows, each with its parts of the sums: as many as the GPU
 // holds at once.
 int64_t backward_parts(int64_t rows, int64_t cols) {
-    const int64_t most = cols > 4096 ? 256 : 512;
-    return rows < most ? rows : most;
+    const int64_t most = cols > 4096 ? 256 : 512, at_once = row_threads(cols) < 512 ? 512 / row_threads(cols) : 1;
+    const int64_t n = ceil_div(rows, at_once);
+    return n < most ? n : most;
 }
 
-template <typename T, typename W, int NT, bool TINY = false>
+template <typename T, typename W, int NT, Form FORM = Form::PLAIN>
 hipError_t launch_backward(const LayerNormBackward& q, float* part, hipStream_t st) {
     const int64_t parts = backward_parts(q.rows, q.cols);
     if (parts > 0) {
@@ -191,26 +242,28 @@ hipError_t launch_backward(const LayerNormBackward& q, float* part, hipStream_t 
                                    static_cast<T*>(q.grad_x), static_cast<T*>(q.grad_residual), part, q.rows, q.cols};
         const hipError_t e = by_flag(q.drop.below > 0, [&](auto drop) {
             return by_flag(q.grad_h != nullptr, [&](auto gh) {
-                hipLaunchKernelGGL((tg_layer_norm_backward_rows<T, W, decltype(drop)::value, decltype(gh)::value, NT, TINY>),
-                                   grid, dim3(NT), 0, st, p);
+                hipLaunchKernelGGL((tg_layer_norm_backward_rows<T, W, decltype(drop)::value, decltype(gh)::value, NT, FORM>),
+                                   grid, dim3(NT * kRowsAtOnce<NT>), 0, st, p);
                 return hipGetLastError();
             });
         });
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((tg_layer_norm_sum_parts<W>), dim3(unsigned(ceil_div(2 * q.cols, 16))), dim3(1024), 0, st, part,
+    hipLaunchKernelGGL((tg_layer_norm_sum_parts<W>), dim3(unsigned(ceil_div(2 * q.cols, 32))), dim3(1024), 0, st, part,
                        parts, static_cast<W*>(q.grad_weight), static_cast<W*>(q.grad_bias), q.cols);
     return hipGetLastError();
 }
 
 template <typename T, typename W>
 hipError_t backward_form(const LayerNormBackward& p, float* part, hipStream_t st) {
-    const int64_t groups = ceil_div(p.cols, 8);
-    if (p.cols < 8) return launch_backward<T, W, 64, true>(p, part, st);
-    if (groups <= 64) return launch_backward<T, W, 64>(p, part, st);
-    if (groups <= 128) return launch_backward<T, W, 128>(p, part, st);
-    if (groups <= 256) return launch_backward<T, W, 256>(p, part, st);
-    if (groups <= 512) return launch_backward<T, W, 512>(p, part, st);
+    if (p.cols < 8) return launch_backward<T, W, 64, Form::TINY>(p, part, st);
+    switch (row_threads(p.cols)) {
+        case 64: return launch_backward<T, W, 64>(p, part, st);
+        case 128: return launch_backward<T, W, 128>(p, part, st);
+        case 256: return launch_backward<T, W, 256>(p, part, st);
+        case 512: return launch_backward<T, W, 512>(p, part, st);
+    }
+    if (p.cols > 8192) return launch_backward<T, W, 1024, Form::WIDE>(p, part, st);
     return launch_backward<T, W, 1024>(p, part, st);
 }
 
