@@ -297,7 +297,8 @@ def test_scale_range(m):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (3, 130, 129), (65, 64, 128), (130, 70, 300), (64, 257, 16),
-                                   (300, 200, 1000), (513, 129, 260), (1000, 1030, 520)])
+                                   (300, 200, 1000), (513, 129, 260), (1000, 1030, 520), (9, 8, 8), (7, 300, 200),
+                                   (2100, 1500, 136), (700, 2300, 1100)])
 def test_gradients(dtype, m, n, k):
     _say("gradients", dtype, m, n, k)
     a, b = _e4m3(m + k, m, k), _e4m3(n + k, n, k)

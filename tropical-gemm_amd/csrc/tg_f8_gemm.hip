@@ -6,6 +6,7 @@
 #include "tg_f8_pack.hpp"
 #include "tg_f8_stream.hpp"
 #include "tg_f8_tiles.hpp"
+#include "tg_f8_turn.hpp"
 #include "tg_i8.hpp"
 
 namespace tg {
@@ -307,7 +308,31 @@ hipError_t gemm_typed(const F8Gemm& p, void* ws, hipStream_t st) {
 // add up to it (8 + 3 bits), in f32 as three (8 + 8 + 8): every product is exact,
 // and the sums are f32.
 
+// Time of tg_f8_turn in us, as plane_gemm_time gives it for the other way: a step
+// takes the vector unit as long for each of a CU's tiles, and a wait of its own.
+// Fitted to 232 gradients of each type (rows 64 ... 4096, columns 128 ... 2048, sums
+// 64 ... 2049; 9% off in the root mean square).  Chosen with it, about half of them
+// take one launch; the choices lose 0.1 us on the GPU in the mean (f32: 0.3).
+double turn_time(const F8Grad& p) {
+    const int64_t tiles = ceil_div(p.rows, 64) * ceil_div(p.cols, 64);
+    if (tiles >= int64_t(1) << 23 || !turn_fits(p.transposed, p.rows, p.cols, p.depth)) return 1e30;
+    // A CU holds `slots` tiles at a time; a last round takes at least one tile's time.
+    const int64_t slots = p.type == TG_BF16 ? 4 : 2, rest = tiles % (256 * slots);
+    const double last = rest > 256 ? double(rest) / 256 : rest > 0 ? 1 : 0;
+    const double per_cu = double(tiles / (256 * slots) * slots) + last, steps = double(ceil_div(p.depth, 64));
+    if (p.type == TG_FLOAT32) return 1.9 + 1.45 * per_cu + steps * (0.38 + 0.62 * per_cu);
+    if (p.type == TG_F16) return 2.1 + 0.86 * per_cu + steps * (0.37 + 0.50 * per_cu);
+    return 2.4 + 0.65 * per_cu + steps * (0.24 + 0.34 * per_cu);
+}
+
+// A launch that lays out rows: what it takes beside the bytes' way through memory,
+// in us; and what one launch may take more than two where the GPU waits for the
+// caller's thread.
+constexpr double kPackTime = 2.5;
+bool one_launch(double one, double two) { return one < two + (one < 12 ? 2 : 0); }
+
 struct GradPlan {
+    bool turn;  // one launch of tg_f8_turn
     bool pack_g;
     int planes, tail;
     int64_t depth, steps;  // of packed rows, in elements and in 128 bytes
@@ -320,6 +345,9 @@ GradPlan plan_grad(const F8Grad& p) {
     pl.depth = round_up(p.depth, 64);
     pl.steps = pl.depth / 64;
     pl.tail = pl.pack_g || p.depth % 64 == 0 ? 128 : int(p.depth % 64 * 2);
+    const int64_t size = p.type == TG_FLOAT32 ? 4 : 2;
+    const double bytes = double(pl.depth) * (3 * double(p.cols) + (pl.pack_g ? double(size + 2 * pl.planes) * double(p.rows) : 0));
+    pl.turn = one_launch(turn_time(p), plane_gemm_time(p.rows, p.cols, pl.steps, pl.planes) + kPackTime + bytes / 4e6);
     return pl;
 }
 
@@ -331,7 +359,7 @@ struct GradWs {
 GradWs carve_grad(const F8Grad& p, const GradPlan& pl, void* ws) {
     Carver c{static_cast<char*>(ws)};
     GradWs w{};
-    if (p.rows == 0 || p.cols == 0 || p.depth == 0) return w;
+    if (p.rows == 0 || p.cols == 0 || p.depth == 0 || pl.turn) return w;
     if (pl.pack_g) w.g = c.take(size_t(p.rows) * size_t(pl.depth) * size_t(pl.planes) * 2);
     w.q = c.take(size_t(p.cols) * size_t(pl.depth) * 2);
     w.part = c.take(plane_gemm_ws(p.rows, p.cols, pl.steps, pl.planes));
@@ -355,6 +383,19 @@ hipError_t pack_grad(const F8Grad& p, const GradPlan& pl, const GradWs& w, hipSt
         return launch_pack(q, bytes_job(p.g, p.ldg * 2, p.rows, p.depth * 2, w.g, pl.depth * 2), st);
 }
 
+template <typename T, bool TRANS>
+hipError_t launch_turn(const F8Grad& p, hipStream_t st) {
+    using Cfg = F8Turn<T, TRANS>;
+    const auto kernel = &tg_f8_turn<T, TRANS>;
+    static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+    if (attr != hipSuccess) return attr;
+    const F8TurnArgs args{p.g, p.ldg, p.q.q, p.q.ld, p.q.scale, p.q.block_rows == 1 ? 0 : 7, int(p.rows), int(p.cols),
+                          int(p.depth), int(ceil_div(p.rows, 64)), int(ceil_div(p.cols, 64))};
+    const TileStore<T> out{nullptr, nullptr, nullptr, nullptr, static_cast<T*>(p.out), p.cols};
+    hipLaunchKernelGGL(kernel, dim3(unsigned(args.tiles_m * args.tiles_n)), dim3(Cfg::NT), Cfg::LDS, st, args, out);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 std::string f8_gemm_plan(const F8Gemm& p) {
@@ -370,6 +411,7 @@ std::string f8_grad_plan(const F8Grad& p) {
     if (p.rows == 0 || p.cols == 0) return "none";
     if (p.depth == 0) return "zero";
     const GradPlan pl = plan_grad(p);
+    if (pl.turn) return "turn";
     return plane_gemm_plan(p.rows, p.cols, pl.steps, pl.planes) + (pl.pack_g ? " pack grad_c" : "");
 }
 
@@ -386,6 +428,11 @@ hipError_t f8_grad(const F8Grad& p, void* ws, hipStream_t st) {
     if (p.rows == 0 || p.cols == 0) return hipSuccess;
     if (p.depth == 0) return plane_gemm_zero(p.type, p.out, p.rows, p.cols, st);
     const GradPlan pl = plan_grad(p);
+    if (pl.turn)
+        return by_type(p.type, [&](auto tag) {
+            using T = decltype(tag);
+            return p.transposed ? launch_turn<T, true>(p, st) : launch_turn<T, false>(p, st);
+        });
     const GradWs w = carve_grad(p, pl, ws);
     hipError_t e;
     switch (p.type) {
