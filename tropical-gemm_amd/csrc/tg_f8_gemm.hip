@@ -311,8 +311,8 @@ hipError_t gemm_typed(const F8Gemm& p, void* ws, hipStream_t st) {
 // Time of tg_f8_turn in us, as plane_gemm_time gives it for the other way: a step
 // takes the vector unit as long for each of a CU's tiles, and a wait of its own.
 // Fitted to 232 gradients of each type (rows 64 ... 4096, columns 128 ... 2048, sums
-// 64 ... 2049; 9% off in the root mean square).  Chosen with it, about half of them
-// take one launch; the choices lose 0.1 us on the GPU in the mean (f32: 0.3).
+// 64 ... 2049; 6% off in the root mean square).  Chosen with it, about half of them
+// take one launch; the choices lose 0.1 us on the GPU in the mean (f32: 0.4).
 double turn_time(const F8Grad& p) {
     const int64_t tiles = ceil_div(p.rows, 64) * ceil_div(p.cols, 64);
     if (tiles >= int64_t(1) << 23 || !turn_fits(p.transposed, p.rows, p.cols, p.depth)) return 1e30;
@@ -320,9 +320,11 @@ double turn_time(const F8Grad& p) {
     const int64_t slots = p.type == TG_BF16 ? 4 : 2, rest = tiles % (256 * slots);
     const double last = rest > 256 ? double(rest) / 256 : rest > 0 ? 1 : 0;
     const double per_cu = double(tiles / (256 * slots) * slots) + last, steps = double(ceil_div(p.depth, 64));
-    if (p.type == TG_FLOAT32) return 1.9 + 1.45 * per_cu + steps * (0.38 + 0.62 * per_cu);
-    if (p.type == TG_F16) return 2.1 + 0.86 * per_cu + steps * (0.37 + 0.50 * per_cu);
-    return 2.4 + 0.65 * per_cu + steps * (0.24 + 0.34 * per_cu);
+    // Tiles at an edge take longer, and a round as long as they.
+    const double edge = p.cols % 64 != 0 || (p.transposed && p.rows % 64 != 0) ? 1 : 0;
+    if (p.type == TG_FLOAT32) return 1.9 + 1.46 * per_cu + steps * (0.33 + 0.61 * per_cu + 0.21 * edge);
+    if (p.type == TG_F16) return 2.1 + 0.86 * per_cu + steps * (0.32 + 0.50 * per_cu + 0.15 * edge);
+    return 2.4 + 0.66 * per_cu + steps * (0.21 + 0.32 * per_cu + 0.16 * edge);
 }
 
 // A launch that lays out rows: what it takes beside the bytes' way through memory,
