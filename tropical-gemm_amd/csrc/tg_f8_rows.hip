@@ -28,25 +28,26 @@ __device__ __forceinline__ int block_exponent(float top) {
     return e > kF8LeastExponent ? e : kF8LeastExponent;
 }
 
-// A workgroup takes 128 rows of one block of columns, a thread eight neighbours
-// of rows t / 16, t / 16 + 16, ...; all loads are issued before the first is
-// used.  A block that holds a NaN or an infinity becomes NaNs with scale 1, so
-// that products of it are NaN.
-template <typename T, int BR>
+// A workgroup takes ROWS rows of COLS columns (whole blocks), a thread eight
+// neighbours of eight rows; all loads are issued before the first is used.  A block
+// that holds a NaN or an infinity becomes NaNs with scale 1, so that products of it
+// are NaN.
+template <typename T, int BR, int COLS>
 __global__ __launch_bounds__(256) void tg_f8_blocks(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
                                                     uint8_t* __restrict__ scale, int64_t ld_scale, int64_t rows,
-                                                    int64_t cols, int64_t col_blocks) {
-    constexpr int P = kF8Block / 16;
-    __shared__ uint8_t exps[kF8Block];
+                                                    int64_t cols, int64_t strips) {
+    constexpr int P = 8, LANES = COLS / 8, STEP = 256 / LANES, ROWS = P * STEP, BLOCKS = COLS / kF8Block;
+    static_assert(BR == 1 || ROWS == BR, "whole blocks");
+    __shared__ uint8_t exps[BLOCKS][ROWS];
     __shared__ float tops[4];
-    const int t = threadIdx.x, r = t / 16;
-    const int64_t cb = blockIdx.x % col_blocks, r0 = blockIdx.x / col_blocks * kF8Block;
-    const int64_t at = cb * kF8Block + t % 16 * 8;
+    const int t = threadIdx.x, r = t / LANES, b = t % LANES / 16;
+    const int64_t strip = blockIdx.x % strips, r0 = blockIdx.x / strips * ROWS;
+    const int64_t at = strip * COLS + t % LANES * 8;
     const int left = cols - at < 8 ? int(cols - at) : 8;  // none where not positive
     float v[P][8];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int64_t row = r0 + r + 16 * i;
+        const int64_t row = r0 + r + STEP * i;
         if (row < rows) load_upto8(x + row * ldx + at, left, v[i]);
         else
 #pragma unroll
@@ -76,12 +77,12 @@ __global__ __launch_bounds__(256) void tg_f8_blocks(const T* __restrict__ x, int
     }
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int64_t row = r0 + r + 16 * i;
+        const int64_t row = r0 + r + STEP * i;
         const bool finite = top[i] < __builtin_huge_valf();
         const int e = finite ? block_exponent(top[i]) : 0;
         const float f = __builtin_bit_cast(float, uint32_t(127 - e) << 23);
-        if (BR == 1 && t % 16 == 0) exps[r + 16 * i] = uint8_t(e + 127);
-        if (BR != 1 && i == 0 && t == 0) scale[cb * ld_scale + blockIdx.x / col_blocks] = uint8_t(e + 127);
+        if (BR == 1 && t % 16 == 0) exps[b][r + STEP * i] = uint8_t(e + 127);
+        if (BR != 1 && i == 0 && t == 0) scale[strip * ld_scale + blockIdx.x / strips] = uint8_t(e + 127);
         u32x2 w;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -89,10 +90,29 @@ __global__ __launch_bounds__(256) void tg_f8_blocks(const T* __restrict__ x, int
         if (!finite) w = u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
         if (row < rows) store_f8_upto8(q + row * cols + at, left, w);
     }
-    if constexpr (BR == 1) {
+    if constexpr (BR == 1) {  // the scales of a column of blocks are neighbours
         __syncthreads();
-        if (t < kF8Block && r0 + t < rows) scale[cb * ld_scale + r0 + t] = exps[t];
+        const int64_t row = r0 + t % ROWS, cb = strip * BLOCKS + t / ROWS;
+        if (t < BLOCKS * ROWS && row < rows && cb * kF8Block < cols) scale[cb * ld_scale + row] = exps[t / ROWS][t % ROWS];
     }
+}
+
+constexpr int64_t kWide = 512;
+
+template <typename T, int BR, int COLS>
+hipError_t launch_blocks(const F8Quantize& p, hipStream_t st) {
+    constexpr int ROWS = 8 * 256 / (COLS / 8);
+    // A launch's thread count stays below 2^32.
+    const int64_t strips = ceil_div(p.cols, COLS), most = (int64_t(1) << 23) / strips * ROWS;
+    for (int64_t r0 = 0; r0 < p.rows; r0 += most) {
+        const int64_t n = p.rows - r0 < most ? p.rows - r0 : most;
+        hipLaunchKernelGGL((tg_f8_blocks<T, BR, COLS>), dim3(unsigned(ceil_div(n, ROWS) * strips)), dim3(256), 0, st,
+                           static_cast<const T*>(p.x) + r0 * p.ldx, p.ldx, p.q + r0 * p.cols, p.scale + r0 / BR,
+                           ceil_div(p.rows, BR), n, p.cols, strips);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // y = round(q * scale), eight elements a thread.
@@ -119,21 +139,10 @@ __global__ __launch_bounds__(256) void tg_f8_restore(const uint8_t* __restrict__
 
 hipError_t f8_quantize(const F8Quantize& p, hipStream_t st) {
     if (p.rows == 0 || p.cols == 0) return hipSuccess;
-    const int64_t col_blocks = ceil_div(p.cols, kF8Block);
-    // A launch's thread count stays below 2^32.
-    const int64_t most = (int64_t(1) << 23) / col_blocks * kF8Block, row_blocks = ceil_div(p.rows, p.block_rows);
     return by_type(p.type, [&](auto tag) {
         using T = decltype(tag);
-        for (int64_t r0 = 0; r0 < p.rows; r0 += most) {
-            const int64_t n = p.rows - r0 < most ? p.rows - r0 : most;
-            const auto kernel = p.block_rows == 1 ? &tg_f8_blocks<T, 1> : &tg_f8_blocks<T, kF8Block>;
-            hipLaunchKernelGGL(kernel, dim3(unsigned(ceil_div(n, kF8Block) * col_blocks)), dim3(256), 0, st,
-                               static_cast<const T*>(p.x) + r0 * p.ldx, p.ldx, p.q + r0 * p.cols,
-                               p.scale + r0 / p.block_rows, row_blocks, n, p.cols, col_blocks);
-            const hipError_t e = hipGetLastError();
-            if (e != hipSuccess) return e;
-        }
-        return hipSuccess;
+        if (p.block_rows != 1) return launch_blocks<T, kF8Block, kF8Block>(p, st);
+        return p.cols >= kWide ? launch_blocks<T, 1, 1024>(p, st) : launch_blocks<T, 1, kF8Block>(p, st);
     });
 }
 
