@@ -29,10 +29,11 @@ __device__ __forceinline__ int block_exponent(float top) {
 }
 
 // A workgroup takes ROWS rows of COLS columns (whole blocks), a thread eight
-// neighbours of eight rows; all loads are issued before the first is used.  A block
+// neighbours of eight rows; all loads are issued before the first is used.  SHORT:
+// rows below eight elements.  A block
 // that holds a NaN or an infinity becomes NaNs with scale 1, so that products of it
 // are NaN.
-template <typename T, int BR, int COLS>
+template <typename T, int BR, int COLS, bool SHORT>
 __global__ __launch_bounds__(256) void tg_f8_blocks(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
                                                     uint8_t* __restrict__ scale, int64_t ld_scale, int64_t rows,
                                                     int64_t cols, int64_t strips) {
@@ -44,14 +45,25 @@ __global__ __launch_bounds__(256) void tg_f8_blocks(const T* __restrict__ x, int
     const int64_t strip = blockIdx.x % strips, r0 = blockIdx.x / strips * ROWS;
     const int64_t at = strip * COLS + t % LANES * 8;
     const int left = cols - at < 8 ? int(cols - at) : 8;  // none where not positive
+    // A row's last group is loaded with the elements before it, which are shifted
+    // out, so that it is one load as any other; and stored as one with the bytes of
+    // the lane before it, where that is in the same wave.
+    const int64_t from = left < 8 ? cols - 8 : at;
+    const bool joined = t % (LANES < 64 ? LANES : 64) != 0, edge = (strip + 1) * COLS > cols;
     float v[P][8];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         const int64_t row = r0 + r + STEP * i;
-        if (row < rows) load_upto8(x + row * ldx + at, left, v[i]);
-        else
+        if (row < rows && left > 0) {
+            if constexpr (SHORT) load_part(x + row * ldx + at, left, v[i]);
+            else load8(x + row * ldx + from, v[i]);
+        } else
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+    }
+    if (!SHORT && left < 8 && left > 0) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) shift8(8 - left, v[i]);
     }
     float top[P];
 #pragma unroll
@@ -88,7 +100,21 @@ __global__ __launch_bounds__(256) void tg_f8_blocks(const T* __restrict__ x, int
         for (int h = 0; h < 2; ++h)
             w[h] = e4m3_pack(v[i][4 * h] * f, v[i][4 * h + 1] * f, v[i][4 * h + 2] * f, v[i][4 * h + 3] * f);
         if (!finite) w = u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
-        if (row < rows) store_f8_upto8(q + row * cols + at, left, w);
+        if (row >= rows) continue;  // the same in the row's lanes
+        if (SHORT || edge) {
+            const u32x2 before = {uint32_t(__shfl_up(w[0], 1)), uint32_t(__shfl_up(w[1], 1))};
+            if (!SHORT && left < 8 && joined) {
+                if (left > 0) {
+                    const int bits = left * 8;
+                    const uint64_t a = __builtin_bit_cast(uint64_t, before), b8 = __builtin_bit_cast(uint64_t, w);
+                    *reinterpret_cast<u32x2_any*>(q + row * cols + from) = __builtin_bit_cast(u32x2, a >> bits | b8 << (64 - bits));
+                }
+            } else {
+                store_f8_upto8(q + row * cols + at, left, w);
+            }
+        } else {
+            *reinterpret_cast<u32x2_any*>(q + row * cols + at) = w;
+        }
     }
     if constexpr (BR == 1) {  // the scales of a column of blocks are neighbours
         __syncthreads();
@@ -99,14 +125,14 @@ __global__ __launch_bounds__(256) void tg_f8_blocks(const T* __restrict__ x, int
 
 constexpr int64_t kWide = 512;
 
-template <typename T, int BR, int COLS>
+template <typename T, int BR, int COLS, bool SHORT = false>
 hipError_t launch_blocks(const F8Quantize& p, hipStream_t st) {
     constexpr int ROWS = 8 * 256 / (COLS / 8);
     // A launch's thread count stays below 2^32.
     const int64_t strips = ceil_div(p.cols, COLS), most = (int64_t(1) << 23) / strips * ROWS;
     for (int64_t r0 = 0; r0 < p.rows; r0 += most) {
         const int64_t n = p.rows - r0 < most ? p.rows - r0 : most;
-        hipLaunchKernelGGL((tg_f8_blocks<T, BR, COLS>), dim3(unsigned(ceil_div(n, ROWS) * strips)), dim3(256), 0, st,
+        hipLaunchKernelGGL((tg_f8_blocks<T, BR, COLS, SHORT>), dim3(unsigned(ceil_div(n, ROWS) * strips)), dim3(256), 0, st,
                            static_cast<const T*>(p.x) + r0 * p.ldx, p.ldx, p.q + r0 * p.cols, p.scale + r0 / BR,
                            ceil_div(p.rows, BR), n, p.cols, strips);
         const hipError_t e = hipGetLastError();
@@ -141,6 +167,8 @@ hipError_t f8_quantize(const F8Quantize& p, hipStream_t st) {
     if (p.rows == 0 || p.cols == 0) return hipSuccess;
     return by_type(p.type, [&](auto tag) {
         using T = decltype(tag);
+        if (p.cols < 8)
+            return p.block_rows != 1 ? launch_blocks<T, kF8Block, kF8Block, true>(p, st) : launch_blocks<T, 1, kF8Block, true>(p, st);
         if (p.block_rows != 1) return launch_blocks<T, kF8Block, kF8Block>(p, st);
         return p.cols >= kWide ? launch_blocks<T, 1, 1024>(p, st) : launch_blocks<T, 1, kF8Block>(p, st);
     });

@@ -26,6 +26,16 @@ __device__ __forceinline__ void e4m3_unpack(uint32_t w, float* v) {
     v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1];
 }
 
+// v without its first n (0 ... 7) elements, zeros behind.
+__device__ __forceinline__ void shift8(int n, float (&v)[8]) {
+#pragma unroll
+    for (int d = 4; d > 0; d >>= 1) {
+        const bool by = (n & d) != 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = by ? (i + d < 8 ? v[i + d] : 0.0f) : v[i];
+    }
+}
+
 // Eight of them from p, at any address: the first n, zeros behind.
 __device__ __forceinline__ u32x2 load_f8_upto8(const uint8_t* p, int n) {
     u32x2 w = {0, 0};
