@@ -250,24 +250,34 @@ hipError_t norm_form(const LayerNorm& p, hipStream_t st) {
 
 // ---- dropout -----------------------------------------------------------------
 
-// y = round(dropout(x) + residual), eight elements a thread.
+// y = round(dropout(x) + residual), eight elements a thread; a row's last group is
+// moved back to end with the row, and what it shares with the one before it is
+// written twice, with the same values (bf16, 8192 x 4095 with residual: 50.8 us with
+// bounds instead).  Rows below eight elements: one group with a bound.
 template <typename T, bool DROP, bool RES>
-__global__ __launch_bounds__(256) void tg_dropout_rows(const T* x, int64_t ldx, const T* res, int64_t ldr,
-                                                       Dropout drop, T* y, int64_t rows, int64_t cols, int64_t groups) {
+__global__ __launch_bounds__(256) void tg_dropout_rows(const T* __restrict__ x, int64_t ldx, const T* __restrict__ res,
+                                                       int64_t ldr, Dropout drop, T* __restrict__ y, int64_t rows,
+                                                       int64_t cols, int64_t groups) {
     const Keep keep(drop);
     const int64_t stride = int64_t(gridDim.x) * 256;
+    const bool tiny = cols < 8;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * groups; i += stride) {
-        const int64_t row = i / groups, at = (i - row * groups) * 8;
-        const int n = cols - at < 8 ? int(cols - at) : 8;
+        const int64_t row = i / groups, start = (i - row * groups) * 8;
+        const int64_t at = tiny || start <= cols - 8 ? start : cols - 8;
         float v[8], r[8];
-        load_upto8(x + row * ldx + at, n, v);
-        if constexpr (RES) load_upto8(res + row * ldr + at, n, r);
+        if (tiny) {
+            load_part(x + row * ldx, int(cols), v);
+            if constexpr (RES) load_part(res + row * ldr, int(cols), r);
+        } else {
+            load8(x + row * ldx + at, v);
+            if constexpr (RES) load8(res + row * ldr + at, r);
+        }
         if constexpr (DROP) keep.apply(row, at, v);
         if constexpr (RES) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += r[e];
         }
-        store_upto8(y + row * cols + at, n, v);
+        store_upto8(y + row * cols + at, tiny ? int(cols) : 8, v);
     }
 }
 
