@@ -243,7 +243,9 @@ hipError_t norm_form(const LayerNorm& p, hipStream_t st) {
     if (groups <= 64) return launch_norm<T, W, DROP, RES, 64, 1>(p, st);
     if (groups <= 128) return launch_norm<T, W, DROP, RES, 64, 2>(p, st);
     if (groups <= 256) return launch_norm<T, W, DROP, RES, 128, 2>(p, st);
+    if (groups <= 384) return launch_norm<T, W, DROP, RES, 128, 3>(p, st);
     if (groups <= 512) return launch_norm<T, W, DROP, RES, 256, 2>(p, st);
+    if (groups <= 768) return launch_norm<T, W, DROP, RES, 256, 3>(p, st);
     if (groups <= 1024) return launch_norm<T, W, DROP, RES, 512, 2>(p, st);
     return launch_norm<T, W, DROP, RES, 1024, 0>(p, st);
 }
