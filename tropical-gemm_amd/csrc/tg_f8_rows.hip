@@ -123,7 +123,10 @@ __global__ __launch_bounds__(256) void tg_f8_blocks(const T* __restrict__ x, int
     }
 }
 
-constexpr int64_t kWide = 512;
+// Columns of a workgroup: one block, or eight where 8-bit rows do not start at whole
+// words of eight bytes, so that fewer lines are written in two parts (bf16, 8192 x
+// 8192: 43 us as one, 45 as eight; 8192 x 4095: 34 and 27).
+bool wide_strips(int64_t cols) { return cols >= 512 && cols % 8 != 0; }
 
 template <typename T, int BR, int COLS, bool SHORT = false>
 hipError_t launch_blocks(const F8Quantize& p, hipStream_t st) {
@@ -170,7 +173,7 @@ hipError_t f8_quantize(const F8Quantize& p, hipStream_t st) {
         if (p.cols < 8)
             return p.block_rows != 1 ? launch_blocks<T, kF8Block, kF8Block, true>(p, st) : launch_blocks<T, 1, kF8Block, true>(p, st);
         if (p.block_rows != 1) return launch_blocks<T, kF8Block, kF8Block>(p, st);
-        return p.cols >= kWide ? launch_blocks<T, 1, 1024>(p, st) : launch_blocks<T, 1, kF8Block>(p, st);
+        return wide_strips(p.cols) ? launch_blocks<T, 1, 1024>(p, st) : launch_blocks<T, 1, kF8Block>(p, st);
     });
 }
 
