@@ -173,6 +173,16 @@ def test_plans():
     assert lib.tg_f8_backward_plan(1, 1, P, 7, 4, 8, 8).decode() == "invalid"
 
 
+@pytest.mark.parametrize("kind,m,n,k,expected", [
+    (1, 32, 4096, 8192, "stream rows 32 words"), (1, 32, 8192, 8192, "tiles"),
+    (1, 48, 8192, 4096, "stream rows 48 words"), (2, 49, 4096, 4096, "stream rows 64 words"),
+    (1, 64, 4096, 4112, "tiles"), (1, 48, 16384, 4095, "stream rows 48"), (1, 64, 8192, 8191, "stream rows 64"),
+    (1, 64, 8193, 8191, "tiles"), (0, 64, 16384, 8192, "stream rows 64 words"), (0, 65, 16384, 8192, "wide tiles")])
+def test_few_rows_read_the_weights_once(kind, m, n, k, expected):
+    plan = nat.load().tg_f8_gemm_plan(kind, P, k, P, k, m, n, k).decode()
+    assert plan == expected if "rows" in expected else plan.startswith(expected)
+
+
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 

@@ -62,6 +62,21 @@ def test_split_sums(form, sizes):
         _check(*s)
 
 
+@pytest.mark.parametrize("dtype,u", [(torch.bfloat16, 2.0 ** -8), (torch.float32, 2.0 ** -24)], ids=["bf16", "f32"])
+@pytest.mark.parametrize("m", [1, 16, 17, 33, 47, 48, 49, 64])
+def test_few_rows(m, dtype, u):
+    """Whole and part words, either side of the weights that the rows are given up at."""
+    for n, k in [(1, 128), (19, 127), (130, 1156), (1000, 4112), (2064, 8192), (4128, 4096), (300, 1)]:
+        print("[case]", m, n, k, flush=True)
+        a, sa = _operand(m + k, m, k, m)
+        b, sb = _operand(n + 7 * k, n, k, -(-n // 128))
+        c = fp8.matmul(a, sa, b, sb, dtype=dtype)
+        da, db = _exact(a, sa, 1), _exact(b, sb, 128)
+        want, size = torch.mm(da, db.t()), torch.mm(da.abs(), db.abs().t())
+        bound = ((k + 1) * 2.0 ** -23 + (2.0 ** -10 if dtype is torch.bfloat16 else 0)) * size
+        assert ((c.double() - want).abs() <= bound + u * (want.abs() + bound)).all()
+
+
 @pytest.mark.parametrize("m,n,k", [(300, 512, 129 * 16), (520, 777, 1600), (4096, 300, 256), (70, 4096, 144)])
 def test_steps_of_every_count(m, n, k):
     """One step, two, three and more of each form that these sizes take."""

@@ -184,14 +184,22 @@ struct Carver {
 
 // Rows of A that tg_f8_stream takes (in sixteens; 0: the tiles take the
 // product): B is read once and needs no layout, but every 16 rows of B read all
-// of A.
+// of A, so more rows than 16 only where B is small or would have to be laid out
+// first, which for f32 outputs it always has.  us, cold weights, tg_f8_stream and
+// the tiles, M x N x K:
+//     bf16   16 x  4096 x 4096    6.7  11.3     16 x 16384 x 4096   17.9  16.3
+//            32 x  4096 x 8192   12.8  14.1     32 x  8192 x 8192   23.3  20.4
+//            48 x  8192 x 4096   14.9  15.0     48 x  8192 x 8192   25.8  26.8
+//            64 x  4096 x 4096   10.3  13.2     64 x  4096 x 8192   16.6  15.0
+// unaligned  48 x 16384 x 8191   68.7  75.1     64 x 16384 x 8191   80.9  75.8
+//     f32    64 x  1024 x 4096    8.7  17.0     64 x 16384 x 8192   58.8   131
 int stream_rows(const F8Gemm& p) {
     // A launch's thread count stays below 2^32: 1024 threads for 16 columns.
     if (p.m > 64 || p.n > (int64_t(1) << 26) - 16) return 0;
-    if (p.m <= 16) return 16;
-    const bool ready = in_place(p.a, p.lda, p.k) && in_place(p.b, p.ldb, p.k);
-    if (p.m <= 32) return p.n <= 8192 || !ready ? 32 : 0;
-    return p.n <= 8192 && !ready ? int(round_up(p.m, 16)) : 0;
+    const int rows = int(round_up(p.m, 16));
+    if (rows <= 16 || p.type == TG_FLOAT32) return rows;
+    if (!in_place(p.a, p.lda, p.k) || !in_place(p.b, p.ldb, p.k)) return rows <= 48 || p.n <= 8192 ? rows : 0;
+    return double(p.n) * double(p.k) <= (rows <= 48 ? 1 << 25 : 1 << 24) ? rows : 0;
 }
 
 struct GemmPlan {
@@ -260,8 +268,8 @@ hipError_t stream_typed(const F8Gemm& p, int rows, const TileStore<T>& out, hipS
     switch (rows) {
         case 16: return words ? launch_stream<1, 16, true>(p, out, st) : launch_stream<1, 8, false>(p, out, st);
         case 32: return words ? launch_stream<2, 8, true>(p, out, st) : launch_stream<2, 8, false>(p, out, st);
-        case 48: return launch_stream<3, 8, false>(p, out, st);
-        default: return launch_stream<4, 8, false>(p, out, st);
+        case 48: return words ? launch_stream<3, 8, true>(p, out, st) : launch_stream<3, 8, false>(p, out, st);
+        default: return words ? launch_stream<4, 8, true>(p, out, st) : launch_stream<4, 8, false>(p, out, st);
     }
 }
 
@@ -404,7 +412,7 @@ std::string f8_gemm_plan(const F8Gemm& p) {
     if (p.m == 0 || p.n == 0) return "none";
     if (p.k == 0) return "bias";
     const GemmPlan pl = plan_gemm(p);
-    if (pl.stream != 0) return "stream rows " + std::to_string(pl.stream) + (in_words(p) && pl.stream <= 32 ? " words" : "");
+    if (pl.stream != 0) return "stream rows " + std::to_string(pl.stream) + (in_words(p) ? " words" : "");
     if (pl.wide) return "wide " + plane_gemm_plan(p.m, p.n, pl.ld / 128, 1);
     return tiles_name(pl.tiles) + (pl.pack_a ? " pack a" : "") + (pl.pack_b ? " pack b" : "");
 }
