@@ -25,8 +25,9 @@ __device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k
 }
 
 // 16 bits for each element: eight neighbours in a row share one counter, (column
-// / 8, row, offset), so that the generator stays below the time that memory
-// takes.
+// / 8, row, offset).  Ten rounds are 20 wide multiplications; with 32 bits an
+// element the generator's work would be twice as much.  A probability is then a
+// multiple of 2^-16.
 struct Keep {
     uint32_t below, k0, k1, o0, o1;
     float factor;

@@ -11,7 +11,7 @@ namespace tg {
 // dst[c][r] = src[r][c] times its scale, exact in bf16: four significant bits and
 // a power of two.  Rows of dst have `depth` (a multiple of 64, at least rows)
 // elements, zeros from r = rows on.  A workgroup takes 64 rows of one block of
-// columns; LDS as in PackTurned.
+// columns; LDS as in PackTurned.  4096 x 4096: 14 us (50 MB).
 struct PackF8Turned {
     static constexpr int COLS = kF8Block, GROUPS = COLS / 8, PASSES = GROUPS * 32 / 256;
     static constexpr int kLdsWords = COLS * 33;

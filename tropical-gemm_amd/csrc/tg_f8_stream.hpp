@@ -59,7 +59,8 @@ __device__ __forceinline__ void f8_block(const u32x4 (&fb)[2], const u32x4 (&fa)
 // W waves take the sum's blocks of 128 in turn and add their sums in LDS.  Bound
 // by reading B: a wave has 2 KiB of B on their way, and the waves of a CU
 // together cover HBM's latency.  Rows need no alignment: they go through
-// registers.  WORDS: rows start at multiples of four bytes.
+// registers.  WORDS: rows start at multiples of four bytes.  M = 1, 8192 x 8192: 13
+// us (67 MB, 5.2 TB/s; weights partly in the last cache).
 template <int R, int W, bool WORDS, typename T>
 __global__ __launch_bounds__(W * 64) void tg_f8_stream(F8StreamArgs p, TileStore<T> out) {
     typedef StreamUnit<WORDS> Unit;

@@ -27,7 +27,10 @@ struct F8TurnArgs {
 // along the sum lies there in rows of 128 bytes, chunk c of row r at c ^ (r % 8).
 // G in f16 or f32 becomes two or three bf16 planes that add up to it.  Loads run
 // two steps ahead in registers, LDS holds two steps.  Bound by the vector unit,
-// which makes each workgroup's operands anew.
+// which makes each workgroup's operands anew: 0.5 us for every 64 of the sum in bf16,
+// 0.8 in f16, 0.9 in f32.  GPU time of 300 x 512 (rows x columns of the gradient) here
+// and with operands laid out first, us: a sum of 64 bf16 3.5 and 6.1, f32 4.2 and 6.4;
+// of 513 7.8 and 8.2, 11.4 and 9.5; of 2049 20.1 and 14.8, 32.9 and 19.7.
 //
 // Values past the matrices' edges are not stored and may be anything; a line's
 // 16 bytes that would end past it are its last ones, shifted into place.  Terms
