@@ -270,6 +270,24 @@ def test_layer_norm_huge(dtype, cols):
     assert ((gx - want).abs() <= (2e-5 + U[dtype]) * size + 8 * LEAST[dtype]).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("cols", [1, 7, 64, 300, 1000, 2501, 3100, 5003, 9000])
+def test_layer_norm_of_equal_values(dtype, cols):
+    """y is the bias, to the bit.  The first mean is off by k steps of f32, k below
+    300; the deviations are k steps each, exactly, and so is their sum, k * cols < 2^24
+    of them; its mean is k (1 + 2^-23) steps, which added to the first mean rounds to
+    the value.  The variance left is below 300e * (300 steps)^2: nothing beside eps up
+    to 1000, and none where the sum passes f32 and the row is done again."""
+    values = [0.1, -77.7, 1000.0, 65504.0] + ([1e25, 3e38] if dtype is not torch.float16 else [])
+    x = torch.tensor(values).to(dtype)[:, None].expand(-1, cols).contiguous()
+    w, b = torch.randn(2, cols, generator=_gen(cols)).to(dtype).to(DEV)
+    y, _, mean, rstd = layers.layer_norm(x.to(DEV), w, b)
+    assert torch.equal(y, b.expand(len(values), -1))
+    assert torch.equal(mean.cpu(), x[:, 0].float())
+    for i in [0, 1, 2] + ([5] if dtype is not torch.float16 else []):
+        assert abs(rstd[i].item() * 1e-5 ** 0.5 - 1) < 1e-3
+
+
 def test_layer_norm_not_finite_rows_stay_apart():
     x = torch.randn(200, 100, generator=_gen(1))
     x[3, 5], x[7, 9] = float("nan"), float("inf")

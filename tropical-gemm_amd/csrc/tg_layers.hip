@@ -20,22 +20,28 @@ constexpr int kRowsPerBlock = NT < 256 ? 256 / NT : 1;
 template <int NT>
 constexpr int kBlock = NT < 256 ? 256 : NT;
 
-// Sum over the NT threads of each row, in every one of them.  `slot`: not the
-// same twice in turn, so that one barrier is enough.
-template <int NT>
-__device__ __forceinline__ float row_sum(float x, int slot) {
-    x = wave_sum(x);
+// Sums of N numbers over the NT threads of each row, in every one of them.  Called
+// once for each N, so that one barrier is enough.
+template <int NT, int N>
+__device__ __forceinline__ void row_sums(float (&x)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = wave_sum(x[k]);
     if constexpr (NT > 64) {
         constexpr int W = NT / 64;
-        __shared__ float part[2][kRowsPerBlock<NT> * W];
+        __shared__ float part[N][kRowsPerBlock<NT> * W];
         const int wave = threadIdx.x / 64, first = wave / W * W;
-        if (threadIdx.x % 64 == 0) part[slot][wave] = x;
-        __syncthreads();
-        x = part[slot][first];
+        if (threadIdx.x % 64 == 0) {
 #pragma unroll
-        for (int i = 1; i < W; ++i) x += part[slot][first + i];
+            for (int k = 0; k < N; ++k) part[k][wave] = x[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            x[k] = part[k][first];
+#pragma unroll
+            for (int i = 1; i < W; ++i) x[k] += part[k][first + i];
+        }
     }
-    return x;
 }
 
 template <typename T, typename W>
@@ -52,16 +58,20 @@ struct NormArgs {
 
 // h = round(dropout(x) + residual); mean and variance of h in two sums of the
 // values in registers, which loses nothing where the mean is large beside the
-// deviations; y = (h - mean) * rstd * w + b.
+// deviations; y = (h - mean) * rstd * w + b.  With the deviations' squares go the
+// deviations themselves, whose mean is what rounding took from the mean: where that
+// is one step of f32, equal values of 1000 would come out as 0.02 (eps 1e-5) and not
+// as 0.
 //
 // VPT > 0, rows of at least eight elements: all loads of a thread are issued
 // before the first is used; a group that would end past the row is moved back to
 // end with it, and what it shares with the group before it is counted once.
 // VPT 0: any length, read again for each sum.
 //
-// bf16, 8192 x 8192 with dropout and residual: 102 us (537 MB, 5.3 TB/s), 8192 x 4096
-// with residual only 44 (268 MB, 6.0 TB/s); one row of 4096: 3.2 us, the loads'
-// latency, two reductions and the launch.
+// bf16, 8192 x 8192 with dropout and residual: 99 us (537 MB, 5.4 TB/s; 105 where
+// the rows whose sums pass f32 are stored with the others, which takes 82 registers
+// and not 58), 8192 x 4096 with residual only 44 (268 MB, 6.0 TB/s); one row of 4096:
+// 3.2 us, the loads' latency, two reductions and the launch.
 template <typename T, typename W, bool DROP, bool RES, int NT, int VPT>
 __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> p) {
     constexpr bool STREAM = DROP || RES;  // h is not x
@@ -90,42 +100,70 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> 
             for (int i = 0; i < 8; ++i) v[i] = to_f32(static_cast<T>(v[i]));
         }
     };
-    struct Stats {
-        float mean, rstd, shrink;  // of the values times shrink
+    auto keep_stats = [&](float mean, float rstd) {
+        if (t == 0) {
+            p.mean[row] = mean;
+            p.rstd[row] = rstd;
+        }
     };
-    // The row's statistics with its values times kShrink; every wave makes them all.
+    auto out = [&](int64_t at, int n, const float(&v)[8], const float(&f)[8], const float(&b)[8], float shrink,
+                   float mean, float rstd) {
+        float o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = (v[i] * shrink - mean) * rstd * f[i] + b[i];
+        store_upto8(p.y + row * cols + at, n, o);
+    };
+    // The row's statistics and outputs with its values times kShrink, from memory
+    // again; every wave makes all the sums.  The mean is corrected by the mean of the
+    // deviations from it, so that equal values have none; where the deviations
+    // themselves need no shrinking, eps counts beside them.
     auto shrunk = [&] {
-        float s = 0.0f, ss = 0.0f, v[8];
-        auto each = [&](auto&& f) {
+        float mean = 0.0f, var = 0.0f, v[8];
+#pragma unroll 1
+        for (int pass = 0; pass < 3; ++pass) {
+            float sum = 0.0f;
             for (int64_t at = int64_t(threadIdx.x % 64) * 8; at < cols; at += 512) {
                 const int n = cols - at < 8 ? int(cols - at) : 8;
                 stream(at, n, v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (i < n) f(v[i] * kShrink);
+                for (int i = 0; i < 8; ++i) {
+                    const float d = i < n ? v[i] * kShrink - mean : 0.0f;
+                    sum += pass < 2 ? d : d * d;
+                }
             }
-        };
-        each([&](float a) { s += a; });
-        const float mean = wave_sum(s) * inv_n;
-        each([&](float a) { ss += (a - mean) * (a - mean); });
-        return Stats{mean, 1.0f / sqrtf(wave_sum(ss) * inv_n + p.eps * kShrink * kShrink), kShrink};
-    };
-    auto finish = [&](float mean, float ss) {
-        Stats s{mean, 1.0f / sqrtf(ss * inv_n + p.eps), 1.0f};
-        if (live && !(ss < kHuge)) s = shrunk();
-        if (live && t == 0) {
-            float m = s.mean / s.shrink;  // rounding may pass the largest number
-            if (fabsf(s.mean) < kHuge) m = fminf(fmaxf(m, -3.402823466e38f), 3.402823466e38f);
-            p.mean[row] = m;
-            p.rstd[row] = s.rstd * s.shrink;
+            sum = wave_sum(sum) * inv_n;
+            if (pass < 2) mean += sum;
+            else var = sum;
         }
-        return s;
+        float whole = mean / kShrink;  // rounding may pass the largest number
+        if (fabsf(mean) < kHuge) whole = fminf(fmaxf(whole, -3.402823466e38f), 3.402823466e38f);
+        const bool small = var < 0x1p-100f;
+        const float shrink = small ? 1.0f : kShrink;
+        const float rstd = 1.0f / sqrtf(small ? var / kShrink / kShrink + p.eps : var);
+        keep_stats(whole, rstd * shrink);
+        for (int64_t at = int64_t(t) * 8; at < cols; at += NT * 8) {
+            const int n = cols - at < 8 ? int(cols - at) : 8;
+            float f[8], b[8] = {};
+            stream(at, n, v);
+            load_upto8(p.w + at, n, f);
+            if (p.b != nullptr) load_upto8(p.b + at, n, b);
+            out(at, n, v, f, b, shrink, small ? whole : mean, rstd);
+        }
     };
-    auto out = [&](int64_t at, int n, const float(&v)[8], const float(&f)[8], const float(&b)[8], const Stats& s) {
-        float o[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = (v[i] * s.shrink - s.mean) * s.rstd * f[i] + b[i];
-        store_upto8(p.y + row * cols + at, n, o);
+    // Mean and rstd from the sums of the deviations from `near` and of their squares;
+    // false: the row's outputs need nothing more.
+    auto finish = [&](float near, const float(&sums)[2], float& mean, float& rstd) {
+        if (!live) return false;
+        const float off = sums[0] * inv_n, left = sums[1] - sums[0] * off;
+        const float ss = left < 0.0f ? 0.0f : left;  // a NaN stays one
+        if (!(ss < kHuge)) {
+            shrunk();
+            return false;
+        }
+        mean = near + off;
+        rstd = 1.0f / sqrtf(ss * inv_n + p.eps);
+        keep_stats(mean, rstd);
+        return true;
     };
 
     if constexpr (VPT > 0) {
@@ -134,7 +172,7 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> 
         auto start = [&](int g) { return int64_t(g * NT + t) * 8; };
         auto from = [&](int g) { return start(g) <= cols - 8 ? start(g) : cols - 8; };
         auto again = [&](int g) { return int(start(g) - from(g)); };  // of the group before it; 8 and more: all
-        float s = 0.0f;
+        float s[1] = {};
         if (live) {
             Eight<T> a[VPT], r[VPT];
 #pragma unroll
@@ -163,31 +201,35 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> 
                     if (again(g) < 8) store8(p.h + row * cols + from(g), v[g]);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s += i >= again(g) ? v[g][i] : 0.0f;
+                for (int i = 0; i < 8; ++i) s[0] += i >= again(g) ? v[g][i] : 0.0f;
             }
         }
-        const float mean = row_sum<NT>(s, 0) * inv_n;
-        float ss = 0.0f;
+        row_sums<NT>(s);
+        const float near = s[0] * inv_n;
+        float ss[2] = {};
         if (live) {
 #pragma unroll
             for (int g = 0; g < VPT; ++g)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ss += i >= again(g) ? (v[g][i] - mean) * (v[g][i] - mean) : 0.0f;
-        }
-        ss = row_sum<NT>(ss, 1);
-        const Stats stats = finish(mean, ss);
-        if (live) {
-#pragma unroll
-            for (int g = 0; g < VPT; ++g) {
-                if (again(g) >= 8) continue;
-                float fv[8], bv[8];
-#pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    fv[i] = to_f32(f[g].v[i]);
-                    bv[i] = p.b != nullptr ? to_f32(b[g].v[i]) : 0.0f;
+                    const float d = i >= again(g) ? v[g][i] - near : 0.0f;
+                    ss[0] += d;
+                    ss[1] += d * d;
                 }
-                out(from(g), 8, v[g], fv, bv, stats);
+        }
+        row_sums<NT>(ss);
+        float mean, rstd;
+        if (!finish(near, ss, mean, rstd)) return;
+#pragma unroll
+        for (int g = 0; g < VPT; ++g) {
+            if (again(g) >= 8) continue;
+            float fv[8], bv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                fv[i] = to_f32(f[g].v[i]);
+                bv[i] = p.b != nullptr ? to_f32(b[g].v[i]) : 0.0f;
             }
+            out(from(g), 8, v[g], fv, bv, 1.0f, mean, rstd);
         }
     } else {
         float v[8];
@@ -199,24 +241,30 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> 
                 f(at, n);
             }
         };
-        float s = 0.0f, ss = 0.0f;
+        float s[1] = {}, ss[2] = {};
         each([&](int64_t at, int n) {
             if constexpr (STREAM) store_upto8(p.h + row * cols + at, n, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += i < n ? v[i] : 0.0f;
+            for (int i = 0; i < 8; ++i) s[0] += i < n ? v[i] : 0.0f;
         });
-        const float mean = row_sum<NT>(s, 0) * inv_n;
+        row_sums<NT>(s);
+        const float near = s[0] * inv_n;
         each([&](int64_t, int n) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss += i < n ? (v[i] - mean) * (v[i] - mean) : 0.0f;
+            for (int i = 0; i < 8; ++i) {
+                const float d = i < n ? v[i] - near : 0.0f;
+                ss[0] += d;
+                ss[1] += d * d;
+            }
         });
-        ss = row_sum<NT>(ss, 1);
-        const Stats stats = finish(mean, ss);
+        row_sums<NT>(ss);
+        float mean, rstd;
+        if (!finish(near, ss, mean, rstd)) return;
         each([&](int64_t at, int n) {
             float f[8], b[8] = {};
             load_upto8(p.w + at, n, f);
             if (p.b != nullptr) load_upto8(p.b + at, n, b);
-            out(at, n, v, f, b, stats);
+            out(at, n, v, f, b, 1.0f, mean, rstd);
         });
     }
 }
