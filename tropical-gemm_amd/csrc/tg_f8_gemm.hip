@@ -1,6 +1,8 @@
 // tg_f8_gemm.hip -- launches of the products in 8-bit floating point: rows times
 // rows with a power of two for each block, and the two gradients, which read one
 // 8-bit operand.
+#include <atomic>
+
 #include "../../include/tropical_gemm_hip.h"
 #include "tg_f8.hpp"
 #include "tg_f8_pack.hpp"
@@ -102,9 +104,19 @@ size_t part_bytes(const TilePlan& pl, int64_t m, int64_t n) {
     return pl.slices > 1 ? size_t(pl.slices) * size_t(m) * size_t(round_up(n, 8)) * 4 : 0;
 }
 
+// Lets a kernel have `bytes` of LDS on the current device; `done` keeps for which it
+// was asked before.
 template <typename K>
-hipError_t allow_lds(K* kernel, int bytes) {
-    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+hipError_t allow_lds(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int device = 0;
+    const hipError_t found = hipGetDevice(&device);
+    if (found != hipSuccess) return found;
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if ((done.load(std::memory_order_relaxed) & bit) != 0) return hipSuccess;
+    const hipError_t e =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 unsigned stride_grid(int64_t items) {
@@ -134,13 +146,15 @@ hipError_t launch_form(F8TileArgs p, const TilePlan& pl, const TileStore<T>& out
     const dim3 grid(unsigned(pl.tiles_m * pl.tiles_n), unsigned(pl.slices));
     if (pl.slices == 1) {
         const auto kernel = &tg_f8_tiles<WM, WN, FM, FN, NB, KS, PER_CU, T>;
-        static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+        static std::atomic<uint64_t> allowed{0};
+        const hipError_t attr = allow_lds(kernel, Cfg::LDS, allowed);
         if (attr != hipSuccess) return attr;
         hipLaunchKernelGGL(kernel, grid, dim3(Cfg::THREADS), Cfg::LDS, st, p, F8Store<T>{out.bias, out.c, out.n});
         return hipGetLastError();
     }
     const auto kernel = &tg_f8_tiles_slice<WM, WN, FM, FN, NB, KS, PER_CU>;
-    static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+    static std::atomic<uint64_t> allowed{0};
+    const hipError_t attr = allow_lds(kernel, Cfg::LDS, allowed);
     if (attr != hipSuccess) return attr;
     float* sums = static_cast<float*>(part);
     hipLaunchKernelGGL(kernel, grid, dim3(Cfg::THREADS), Cfg::LDS, st, p, F8Partial{sums, round_up(p.n, 8)});
@@ -397,7 +411,8 @@ template <typename T, bool TRANS>
 hipError_t launch_turn(const F8Grad& p, hipStream_t st) {
     using Cfg = F8Turn<T, TRANS>;
     const auto kernel = &tg_f8_turn<T, TRANS>;
-    static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+    static std::atomic<uint64_t> allowed{0};
+    const hipError_t attr = allow_lds(kernel, Cfg::LDS, allowed);
     if (attr != hipSuccess) return attr;
     const F8TurnArgs args{p.g, p.ldg, p.q.q, p.q.ld, p.q.scale, p.q.block_rows == 1 ? 0 : 7, int(p.rows), int(p.cols),
                           int(p.depth), int(ceil_div(p.rows, 64)), int(ceil_div(p.cols, 64))};

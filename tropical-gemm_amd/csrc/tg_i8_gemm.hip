@@ -1,6 +1,7 @@
 // tg_i8_gemm.hip -- launches of the 8-bit layer's products: rows times rows in
 // 8-bit integers with scales, and the two gradients, which read one 8-bit
 // operand.
+#include <atomic>
 #include <cstdio>
 
 #include "../../include/tropical_gemm_hip.h"
@@ -104,9 +105,19 @@ size_t part_bytes(const TilePlan& pl, int64_t m, int64_t n) {
     return pl.slices > 1 ? size_t(pl.slices) * size_t(m) * size_t(round_up(n, 8)) * 4 : 0;
 }
 
+// Lets a kernel have `bytes` of LDS on the current device; `done` keeps for which it
+// was asked before.
 template <typename K>
-hipError_t allow_lds(K* kernel, int bytes) {
-    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+hipError_t allow_lds(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int device = 0;
+    const hipError_t found = hipGetDevice(&device);
+    if (found != hipSuccess) return found;
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if ((done.load(std::memory_order_relaxed) & bit) != 0) return hipSuccess;
+    const hipError_t e =
+        hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 unsigned stride_grid(int64_t items) {
@@ -138,13 +149,15 @@ hipError_t launch_form(TileArgs p, const TilePlan& pl, const TileStore<T>& out, 
     const dim3 grid(unsigned(pl.tiles_m * pl.tiles_n), unsigned(pl.slices));
     if (pl.slices == 1) {
         const auto kernel = &tg_i8_tiles<KIND, WM, WN, FM, FN, NB, P, PER_CU, T>;
-        static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+        static std::atomic<uint64_t> allowed{0};
+        const hipError_t attr = allow_lds(kernel, Cfg::LDS, allowed);
         if (attr != hipSuccess) return attr;
         hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, out);
         return hipGetLastError();
     }
     const auto kernel = &tg_i8_tiles_slice<KIND, WM, WN, FM, FN, NB, P, PER_CU>;
-    static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+    static std::atomic<uint64_t> allowed{0};
+    const hipError_t attr = allow_lds(kernel, Cfg::LDS, allowed);
     if (attr != hipSuccess) return attr;
     auto* sums = static_cast<typename Cfg::Value*>(part);
     hipLaunchKernelGGL(kernel, grid, dim3(Cfg::NT), Cfg::LDS, st, p, TilePartial<typename Cfg::Value>{sums, round_up(p.n, 8)});
@@ -407,7 +420,8 @@ template <typename T, bool TRANS>
 hipError_t launch_turn(const I8Grad& p, const TileStore<T>& out, hipStream_t st) {
     using Cfg = Turn<T, TRANS>;
     const auto kernel = &tg_i8_turn<T, TRANS>;
-    static const hipError_t attr = allow_lds(kernel, Cfg::LDS);
+    static std::atomic<uint64_t> allowed{0};
+    const hipError_t attr = allow_lds(kernel, Cfg::LDS, allowed);
     if (attr != hipSuccess) return attr;
     const TurnArgs args{p.g, p.ldg, p.q, p.ldq, p.scale, int(p.rows), int(p.cols), int(p.depth),
                         int(ceil_div(p.rows, 64)), int(ceil_div(p.cols, 64))};
