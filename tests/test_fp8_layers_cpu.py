@@ -159,6 +159,21 @@ def test_workspaces():
     assert lib.tg_f8_backward_b_workspace_size(1, P, 8, -1, 1, 1) == NONE
 
 
+def test_sizes_of_refused_calls():
+    """What a call would refuse has no workspace size: SIZE_MAX, without a sum that overflows."""
+    lib = nat.load()
+    most = 2 ** 31 - 1
+    for m, n, k in [(most + 1, 4, 8), (4, 2 ** 62, 8), (4, 4, 2 ** 20 + 1), (2 ** 62, 2 ** 62, 8)]:
+        assert lib.tg_f8_gemm_workspace_size(1, P, k, P, k, m, n, k) == NONE
+    assert lib.tg_f8_gemm_workspace_size(7, P, 8, P, 8, 4, 4, 8) == NONE
+    for size in (lib.tg_f8_backward_a_workspace_size, lib.tg_f8_backward_b_workspace_size):
+        assert size(7, P, 8, 4, 8, 8) == NONE and size(1, P, 8, 2 ** 62, 2 ** 62, 8) == NONE
+    assert lib.tg_f8_backward_a_workspace_size(1, P, 2 ** 21, 4, 2 ** 21, 8) == NONE
+    assert lib.tg_f8_backward_b_workspace_size(1, P, 8, 2 ** 21, 8, 8) == NONE
+    assert lib.tg_layer_norm_backward_workspace_size(2 ** 62, 8) == NONE
+    assert lib.tg_layer_norm_backward_workspace_size(4, 2 ** 24 + 1) == NONE
+
+
 def test_plans():
     lib = nat.load()
     plan = lambda kind, a, lda, b, ldb, m, n, k: lib.tg_f8_gemm_plan(kind, a, lda, b, ldb, m, n, k).decode()

@@ -18,6 +18,12 @@ int check_scale(const char* name, const tg::F8Scale& s) {
                     ": 0 to 2^22 and 0 to 2^40 are supported");
 }
 
+// What the size functions answer for: the calls refuse the rest.
+bool sizes_fit(int type, int64_t m, int64_t n, int64_t k, int64_t sum) {
+    auto dim = [](int64_t d) { return d >= 0 && d <= 0x7fffffffLL; };
+    return (type == TG_FLOAT32 || type == TG_BF16 || type == TG_F16) && dim(m) && dim(n) && dim(k) && sum <= kMostSum;
+}
+
 int check_block_rows(int64_t n) {
     if (n == 1 || n == tg::kF8Block) return TG_OK;
     return bad_argument("block_rows is " + std::to_string(n) + ": 1 or 128 is needed");
@@ -107,7 +113,7 @@ int tg_f8_dequantize(int device, tg_float type, const uint8_t* q, int64_t ldq, c
 size_t tg_f8_gemm_workspace_size(tg_float type, const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
                                  int64_t m, int64_t n, int64_t k) {
     const tg::F8Gemm p{type, a, lda, {}, b, ldb, {}, nullptr, nullptr, m, n, k};
-    return m < 0 || n < 0 || k < 0 || k > kMostSum ? size_t(-1) : tg::f8_gemm_ws(p);
+    return sizes_fit(type, m, n, k, k) ? tg::f8_gemm_ws(p) : size_t(-1);
 }
 
 int tg_f8_gemm(int device, tg_float type, const uint8_t* a, int64_t lda, const uint8_t* a_scale, int64_t a_scale_row,
@@ -144,8 +150,8 @@ const char* tg_f8_backward_plan(tg_float type, int want_a, const void* grad_c, i
 
 size_t tg_f8_backward_a_workspace_size(tg_float type, const void* grad_c, int64_t ldg, int64_t m, int64_t n,
                                        int64_t k) {
-    return m < 0 || n < 0 || k < 0 ? size_t(-1)
-                                   : tg::f8_grad_ws(grad_a(type, grad_c, ldg, nullptr, k, {}, nullptr, m, n, k));
+    if (!sizes_fit(type, m, n, k, n)) return size_t(-1);
+    return tg::f8_grad_ws(grad_a(type, grad_c, ldg, nullptr, k, {}, nullptr, m, n, k));
 }
 
 int tg_f8_backward_a(int device, tg_float type, const void* grad_c, int64_t ldg, const uint8_t* b, int64_t ldb,
@@ -159,8 +165,8 @@ int tg_f8_backward_a(int device, tg_float type, const void* grad_c, int64_t ldg,
 
 size_t tg_f8_backward_b_workspace_size(tg_float type, const void* grad_c, int64_t ldg, int64_t m, int64_t n,
                                        int64_t k) {
-    return m < 0 || n < 0 || k < 0 ? size_t(-1)
-                                   : tg::f8_grad_ws(grad_b(type, grad_c, ldg, nullptr, k, {}, nullptr, m, n, k));
+    if (!sizes_fit(type, m, n, k, m)) return size_t(-1);
+    return tg::f8_grad_ws(grad_b(type, grad_c, ldg, nullptr, k, {}, nullptr, m, n, k));
 }
 
 int tg_f8_backward_b(int device, tg_float type, const void* grad_c, int64_t ldg, const uint8_t* a, int64_t lda,

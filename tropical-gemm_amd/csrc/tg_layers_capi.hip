@@ -74,7 +74,7 @@ int tg_layer_norm(int device, tg_float type, tg_float weight_type, const void* x
 }
 
 size_t tg_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
-    return rows < 0 || cols < 0 || cols > kMostCols ? size_t(-1) : tg::layer_norm_backward_ws(rows, cols);
+    return rows < 0 || rows > 0x7fffffffLL || cols < 0 || cols > kMostCols ? size_t(-1) : tg::layer_norm_backward_ws(rows, cols);
 }
 
 int tg_layer_norm_backward(int device, tg_float type, tg_float weight_type, const void* grad_y, int64_t ldg,

@@ -36,6 +36,7 @@ _vp = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
+SIZE_MAX = _sz(-1).value  # the layers' size functions: no call of these sizes
 _f32 = ctypes.c_float
 _f64 = ctypes.c_double
 _u64 = ctypes.c_uint64

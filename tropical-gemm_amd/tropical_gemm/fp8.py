@@ -32,6 +32,11 @@ BLOCK = 128
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
+def _bytes(size: int) -> int:
+    """A size function's answer; what it has none for is refused by the call."""
+    return 0 if size == nat.SIZE_MAX else size
+
+
 def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
@@ -104,7 +109,7 @@ def matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: tor
     c = _matrix(m, n, dtype, dev)
     lib = nat.load()
     pa, pb = a.data_ptr(), b.data_ptr()
-    nbytes = lib.tg_f8_gemm_workspace_size(kind, pa, lda, pb, ldb, m, n, k) if k <= 1 << 20 else 0
+    nbytes = _bytes(lib.tg_f8_gemm_workspace_size(kind, pa, lda, pb, ldb, m, n, k))
     ws = _workspace(nbytes, dev)
     nat.check(lib.tg_f8_gemm(dev.index, kind, pa, lda, a_scale.data_ptr(), a_row, a_col, pb, ldb, b_scale.data_ptr(),
                              b_row, b_col, _ptr(bias), c.data_ptr(), m, n, k, _ptr(ws), nbytes, _stream(dev)))
@@ -126,7 +131,7 @@ def _backward(which: str, grad_c: torch.Tensor, q: torch.Tensor, scale: torch.Te
     size, run = ((lib.tg_f8_backward_a_workspace_size, lib.tg_f8_backward_a) if which == "a" else
                  (lib.tg_f8_backward_b_workspace_size, lib.tg_f8_backward_b))
     kind = _FLOAT[grad_c.dtype]
-    nbytes = size(kind, grad_c.data_ptr(), ldg, m, n, k) if depth <= 1 << 20 else 0
+    nbytes = _bytes(size(kind, grad_c.data_ptr(), ldg, m, n, k))
     ws = _workspace(nbytes, dev)
     nat.check(run(dev.index, kind, grad_c.data_ptr(), ldg, q.data_ptr(), ldq, scale.data_ptr(), row, col,
                   out.data_ptr(), m, n, k, _ptr(ws), nbytes, _stream(dev)))

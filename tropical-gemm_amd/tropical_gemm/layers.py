@@ -27,6 +27,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as nat
+from .fp8 import _bytes
 from .int8 import _F32, _FLOAT, _elsewhere, _matrix, _rows, _same_shape, _vector, _workspace
 from .ops import _ptr, _stream
 
@@ -134,7 +135,7 @@ def layer_norm_backward(grad_y: torch.Tensor, h: torch.Tensor, mean: torch.Tenso
     grad_weight = torch.empty(cols, dtype=weight.dtype, device=dev)
     grad_bias = torch.empty(cols, dtype=weight.dtype, device=dev)
     lib = nat.load()
-    nbytes = lib.tg_layer_norm_backward_workspace_size(rows, cols) if cols <= 1 << 24 else 0
+    nbytes = _bytes(lib.tg_layer_norm_backward_workspace_size(rows, cols))
     ws = _workspace(nbytes, dev)
     nat.check(lib.tg_layer_norm_backward(
         dev.index, _FLOAT[h.dtype], _FLOAT[weight.dtype], grad_y.data_ptr(), ldg, h.data_ptr(), ldh, mean.data_ptr(),
