@@ -83,9 +83,9 @@ struct F8Tile {
     static constexpr int STAGE = AT_SB + WAVES * 256, LDS = KS * NB * STAGE;
     static constexpr int THREADS = KS * NT, MERGE = KS > 1 ? WAVES * FM * FN * 4096 : 0;
     static_assert(BM * 8 % NT == 0 && BN * 8 % NT == 0 && BM % 64 == 0, "whole loads");
-    static_assert(NB >= 2 && NB <= 4, "wait_for's cases");
     static_assert(128 % (FN * 32) == 0, "one scale of B for a wave");
     static constexpr bool PAIRS = FM % 2 == 0 && FN % 2 == 0 && NB == 2;
+    static_assert(PAIRS || (NB == 3 && FM * FN == 1), "run's forms");
 
     static __device__ __forceinline__ int key(int L) { return L >> 1 & 7; }
     // Matrix rows (from the tile's first) of LDS rows.
@@ -108,7 +108,8 @@ struct F8Tile {
         tn = id / height;
     }
 
-    // Sums steps [s0, s1), at least one, of tile (tm, tn) into acc.
+    // Sums steps [s0, s1), at least one, of tile (tm, tn) into acc, of one fragment
+    // each of A and B a wave.
     static __device__ __forceinline__ void run(const F8TileArgs& p, int tm, int tn, int s0, int s1, lds_t* lds,
                                                f32x16 (&acc)[FM][FN]) {
         const int t = threadIdx.x % NT, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64);
@@ -170,8 +171,7 @@ struct F8Tile {
         };
         // Waits until all but the newest `steps` steps' loads have landed.
         auto wait_for = [&](int steps) {
-            if (NB > 3 && steps >= 2) tile_wait<(NB > 3 ? 2 : 0) * LOADS>();
-            else if (NB > 2 && steps >= 1) tile_wait<(NB > 2 ? 1 : 0) * LOADS>();
+            if (steps >= 1) tile_wait<LOADS>();
             else tile_wait<0>();
         };
 
@@ -200,29 +200,19 @@ struct F8Tile {
 #pragma unroll
             for (int i = 0; i < FM; ++i) sa[0][i] = sa[1][i];
         };
-        // Multiplies the fragments of half h.  Between the products go the next
-        // half's reads (from the stage at `from`) and a later step's loads.
+        // Multiplies the fragments of half h.  Behind the product go the next half's
+        // reads (from the stage at `from`) and a later step's loads.
         auto products = [&](int h, auto reads, auto scales, auto loads, int from) {
-            constexpr int SLOTS = FM * FN, FOR_READS = SLOTS > 4 ? SLOTS - 2 : SLOTS;
+            acc[0][0] = f8_mma32(f8_operand(xb[h][0][0], xb[h][0][1]), f8_operand(xa[h][0][0], xa[h][0][1]), acc[0][0], sb[0],
+                                 sa[0][0]);
+            if constexpr (decltype(scales)::value) read_scales(from);
+            if constexpr (decltype(reads)::value) {
 #pragma unroll
-            for (int s = 0; s < SLOTS; ++s) {
-                const int i = s / FN, j = s % FN;
-                acc[i][j] = f8_mma32(f8_operand(xb[h][j][0], xb[h][j][1]), f8_operand(xa[h][i][0], xa[h][i][1]), acc[i][j],
-                                     sb[0], sa[0][i]);
-                if (SLOTS > 1) __builtin_amdgcn_sched_barrier(0);
-                if constexpr (decltype(scales)::value)
-                    if (s == 0) read_scales(from);
-                if constexpr (decltype(reads)::value) {
+                for (int r = 0; r < READS; ++r) read(r, h ^ 1, from);
+            }
+            if constexpr (decltype(loads)::value) {
 #pragma unroll
-                    for (int r = 0; r < READS; ++r)
-                        if (r * FOR_READS / READS == s) read(r, h ^ 1, from);
-                }
-                if constexpr (decltype(loads)::value) {
-#pragma unroll
-                    for (int l = 0; l < LOADS; ++l)
-                        if (l * SLOTS / LOADS == s) load(l);
-                }
-                if (SLOTS > 1) __builtin_amdgcn_sched_barrier(0);
+                for (int l = 0; l < LOADS; ++l) load(l);
             }
         };
         // Clears the chunks that lie past the sum's end.
