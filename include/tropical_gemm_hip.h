@@ -425,7 +425,8 @@ int tg_i8_backward_b(int device, tg_float type, const void* grad_c, int64_t ldg,
  * scale_col]: any order in memory (scale_row at most 2^22); the products are
  * fastest where those of a column of blocks are neighbours, as tg_f8_quantize
  * writes them.  No counterpart in the reference.  Conventions as for the 8-bit
- * layer above. */
+ * layer above; size functions give SIZE_MAX for sizes and types that the call
+ * refuses. */
 
 /* top = the block's largest magnitude, e = the least integer with top <= 448 *
  * 2^e, at least -100: scale = 2^e, q = x * 2^-e rounded to e4m3 (nearest, ties
