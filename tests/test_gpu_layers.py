@@ -288,6 +288,13 @@ def test_layer_norm_of_equal_values(dtype, cols):
         assert abs(rstd[i].item() * 1e-5 ** 0.5 - 1) < 1e-3
 
 
+def test_layer_norm_of_no_columns():
+    w = torch.ones(0, device=DEV)
+    y, h, mean, rstd = layers.layer_norm(torch.ones(4, 0, device=DEV), w, w)
+    assert y.shape == h.shape == (4, 0) and torch.isnan(mean).all() and torch.isnan(rstd).all()
+    assert [tuple(g.shape) for g in layers.layer_norm_backward(y, h, mean, rstd, w)] == [(4, 0), (4, 0), (0,), (0,)]
+
+
 def test_layer_norm_not_finite_rows_stay_apart():
     x = torch.randn(200, 100, generator=_gen(1))
     x[3, 5], x[7, 9] = float("nan"), float("inf")

@@ -102,6 +102,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     y = _matrix(rows, cols, x.dtype, dev)
     mean = torch.empty(rows, dtype=torch.float32, device=dev)
     rstd = torch.empty(rows, dtype=torch.float32, device=dev)
+    if cols == 0:  # rows without a mean
+        mean.fill_(float("nan"))
+        rstd.fill_(float("nan"))
     nat.check(nat.load().tg_layer_norm(
         dev.index, _FLOAT[x.dtype], _FLOAT[weight.dtype], x.data_ptr(), ldx, _ptr(residual), ldr, weight.data_ptr(),
         _ptr(bias), eps, p, seed, seed_at, offset, y.data_ptr(), None if h is x else h.data_ptr(), mean.data_ptr(),
