@@ -70,6 +70,7 @@ double tile_time(const TileTime& c, int64_t tiles, int64_t steps) {
 }
 
 TilePlan plan_tiles(int64_t m, int64_t n, int64_t steps) {
+    if (m <= 0 || n <= 0 || steps <= 0) return {0, 1, 0, 0, 1, 0};  // no tile, no slice of the sum
     TilePlan best = {0, 1, ceil_div(m, 256), ceil_div(n, 256), steps, steps};
     double least = 1e30;
     for (int f = 0; f < kTileForms; ++f) {
