@@ -514,8 +514,8 @@ int tg_dropout(int device, tg_float type, const void* x, int64_t ldx, const void
  * for x and may be NULL); mean and rstd = (variance + eps)^-1/2 of each row of h
  * in f32; y = (h - mean) * rstd * weight + bias.  weight and bias (NULL: none)
  * are of weight_type, which is type or f32.  The variance is of deviations from
- * the mean; deviations and sums may pass f32.  cols is at most 2^24; of rows
- * without elements nothing is written. */
+ * the mean; deviations and sums may pass f32, and their squares lie below it.  cols
+ * is at most 2^24; of rows without elements nothing is written. */
 int tg_layer_norm(int device, tg_float type, tg_float weight_type, const void* x, int64_t ldx,
                   const void* residual, int64_t ldr, const void* weight, const void* bias,
                   float eps, double p, uint64_t seed, const uint64_t* seed_at, uint64_t offset,

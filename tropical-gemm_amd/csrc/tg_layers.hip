@@ -9,8 +9,13 @@ namespace {
 
 constexpr float kHuge = __builtin_huge_valf();
 // Squares of numbers above 2^64 pass f32: a row whose sum of them is not finite
-// is summed again with its values times kShrink (the largest become 2^48).
+// is summed again with its values times kShrink (the largest become 2^48).  Those of
+// numbers below 2^-63 lose bits or all of themselves: a row whose variance and eps
+// together are below kFaint, and its mean below kFaintMean, is summed again with its
+// values times kGrow (the least become 2^-49).  With a larger mean such a row's
+// values are all equal, a step of f32 there being above the root of kFaint.
 constexpr float kShrink = 0x1p-80f;
+constexpr float kGrow = 0x1p100f, kFaint = 0x1p-100f, kFaintMean = 0x1p-10f;
 
 // A row's threads: NT lanes, several rows in a workgroup where NT is below 256.
 // A thread holds VPT groups of eight neighbours, group g of thread t from
@@ -75,8 +80,8 @@ struct NormArgs {
 // VPT 0: any length, read again for each sum.
 //
 // bf16, 8192 x 8192 with dropout and residual: 99 us (537 MB, 5.4 TB/s; 105 where
-// the rows whose sums pass f32 are stored with the others, which takes 82 registers
-// and not 58), 8192 x 4096 with residual only 44 (268 MB, 6.0 TB/s); one row of 4096:
+// the rows whose sums pass f32 were stored with the others, which took 82 registers;
+// 62 now), 8192 x 4096 with residual only 44 (268 MB, 6.0 TB/s); one row of 4096:
 // 3.2 us, the loads' latency, two reductions and the launch.
 template <typename T, typename W, bool DROP, bool RES, int NT, int VPT>
 __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> p) {
@@ -112,18 +117,18 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> 
             p.rstd[row] = rstd;
         }
     };
-    auto out = [&](int64_t at, int n, const float(&v)[8], const float(&f)[8], const float(&b)[8], float shrink,
+    auto out = [&](int64_t at, int n, const float(&v)[8], const float(&f)[8], const float(&b)[8], float scale,
                    float mean, float rstd) {
         float o[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = (v[i] * shrink - mean) * rstd * f[i] + b[i];
+        for (int i = 0; i < 8; ++i) o[i] = (v[i] * scale - mean) * rstd * f[i] + b[i];
         store_upto8(p.y + row * cols + at, n, o);
     };
-    // The row's statistics and outputs with its values times kShrink, from memory
-    // again; every wave makes all the sums.  The mean is corrected as in the other
-    // rows, so that equal values have no deviations; where the deviations themselves
-    // need no shrinking, eps counts beside them.
-    auto shrunk = [&] {
+    // The row's statistics and outputs with its values times `scale`, kShrink or
+    // kGrow, from memory again; every wave makes all the sums.  The mean is corrected
+    // as in the other rows, so that equal values have no deviations; where the
+    // deviations themselves need no shrinking, they are taken as they are.
+    auto again_times = [&](float scale) {
         float mean = 0.0f, var = 0.0f, v[8];
 #pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
@@ -133,7 +138,7 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> 
                 stream(at, n, v);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float d = i < n ? v[i] * kShrink - mean : 0.0f;
+                    const float d = i < n ? v[i] * scale - mean : 0.0f;
                     sum += d;
                     squares += d * d;
                 }
@@ -142,19 +147,20 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> 
             var = wave_sum(squares) * inv_n;
             if (pass == 0 || (pass == 1 && mean * mean >= var)) mean += sum;
         }
-        float whole = mean / kShrink;  // rounding may pass the largest number
+        const float back = scale == kGrow ? 1.0f / kGrow : 1.0f / kShrink;
+        float whole = mean * back;  // rounding may pass the largest number
         if (fabsf(mean) < kHuge) whole = fminf(fmaxf(whole, -3.402823466e38f), 3.402823466e38f);
-        const bool small = var < 0x1p-100f;
-        const float shrink = small ? 1.0f : kShrink;
-        const float rstd = 1.0f / sqrtf(small ? var / kShrink / kShrink + p.eps : var);
-        keep_stats(whole, rstd * shrink);
+        const bool small = scale == kShrink && var < 0x1p-100f;
+        const float use = small ? 1.0f : scale;
+        const float rstd = 1.0f / sqrtf(small ? var * back * back + p.eps : var + p.eps * use * use);
+        keep_stats(whole, rstd * use);
         for (int64_t at = int64_t(t) * 8; at < cols; at += NT * 8) {
             const int n = cols - at < 8 ? int(cols - at) : 8;
             float f[8], b[8] = {};
             stream(at, n, v);
             load_upto8(p.w + at, n, f);
             if (p.b != nullptr) load_upto8(p.b + at, n, b);
-            out(at, n, v, f, b, shrink, small ? whole : mean, rstd);
+            out(at, n, v, f, b, use, small ? whole : mean, rstd);
         }
     };
     // Mean and rstd from the sums of the deviations from `near` and of their squares;
@@ -163,8 +169,9 @@ __global__ __launch_bounds__(kBlock<NT>) void tg_layer_norm_rows(NormArgs<T, W> 
         if (!live) return false;
         const float off = sums[0] * inv_n, left = sums[1] - sums[0] * off;
         const float ss = left < 0.0f ? 0.0f : left;  // a NaN stays one
-        if (!(ss < kHuge)) {
-            shrunk();
+        const bool faint = ss * inv_n + p.eps < kFaint && fabsf(near) < kFaintMean;
+        if (!(ss < kHuge) || faint) {
+            again_times(faint ? kGrow : kShrink);
             return false;
         }
         mean = near * near >= ss * inv_n ? near + off : near;
