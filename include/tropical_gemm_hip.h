@@ -529,7 +529,9 @@ int tg_layer_norm(int device, tg_float type, tg_float weight_type, const void* x
  *   grad_weight = sum_i grad_y * xh, grad_bias = sum_i grad_y   (of weight_type).
  * grad_h, the gradient that reaches h from elsewhere, may be NULL.  grad_x is
  * made of grad_residual before its rounding.  Sums are made in a fixed order:
- * equal calls give equal bits. */
+ * equal calls give equal bits.  The workspace holds two f32 for each column and
+ * part of the rows, at most 512 parts (256 above 4096 columns).  Above 8192 columns
+ * every 8192 of them read the whole row for its sums. */
 size_t tg_layer_norm_backward_workspace_size(int64_t rows, int64_t cols);
 int tg_layer_norm_backward(int device, tg_float type, tg_float weight_type, const void* grad_y,
                            int64_t ldg, const void* h, int64_t ldh, const float* mean,

@@ -200,8 +200,9 @@ struct Carver {
 // Rows of A that tg_f8_stream takes (in sixteens; 0: the tiles take the
 // product): B is read once and needs no layout, but every 16 rows of B read all
 // of A, so more rows than 16 only where B is small or would have to be laid out
-// first, which for f32 outputs it always has.  us, cold weights, tg_f8_stream and
-// the tiles, M x N x K:
+// first, which for f32 outputs it always has.  Up to 16 rows always, though for many
+// columns the tiles take a tenth less.  us, cold weights, tg_f8_stream and the tiles,
+// M x N x K:
 //     bf16   16 x  4096 x 4096    6.7  11.3     16 x 16384 x 4096   17.9  16.3
 //            32 x  4096 x 8192   12.8  14.1     32 x  8192 x 8192   23.3  20.4
 //            48 x  8192 x 4096   14.9  15.0     48 x  8192 x 8192   25.8  26.8

@@ -32,8 +32,8 @@ __device__ __forceinline__ int block_exponent(float top) {
 // neighbours of eight rows; all loads are issued before the first is used.  SHORT:
 // rows below eight elements.  A block
 // that holds a NaN or an infinity becomes NaNs with scale 1, so that products of it
-// are NaN.  bf16, 8192 x 8192 in blocks of a row: 43 us (201 MB, 4.7 TB/s); f32, 5003
-// x 4099 in square blocks: 25 us (103 MB).
+// are NaN.  bf16, 8192 x 8192 in blocks of a row: 41 to 43 us (201 MB, 4.7 to 4.9
+// TB/s); f32, 5003 x 4099 in square blocks: 22 to 25 us (103 MB).
 template <typename T, int BR, int COLS, bool SHORT>
 __global__ __launch_bounds__(256) void tg_f8_blocks(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
                                                     uint8_t* __restrict__ scale, int64_t ld_scale, int64_t rows,
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void tg_f8_blocks(const T* __restrict__ x, int
 
 // Columns of a workgroup: one block, or eight where 8-bit rows do not start at whole
 // words of eight bytes, so that fewer lines are written in two parts (bf16, 8192 x
-// 8192: 43 us as one, 45 as eight; 8192 x 4095: 34 and 27).
+// 8192: 43 us as one, 45 as eight; 8192 x 4095: 34 and 26).
 bool wide_strips(int64_t cols) { return cols >= 512 && cols % 8 != 0; }
 
 template <typename T, int BR, int COLS, bool SHORT = false>

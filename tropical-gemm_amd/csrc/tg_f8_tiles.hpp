@@ -279,7 +279,7 @@ struct F8Tile {
     // for one step: the second half's of a new step are read where the old ones have
     // been used for the last time.
     //
-    // 8192^3 in 256 x 256 tiles, bf16: 395 to 415 us (2.7 P operations/s) with the
+    // 8192^3 in 256 x 256 tiles, bf16: 395 to 419 us (2.6 to 2.8 P/s) with the
     // matrix unit busy 71% of the cycles and the clock at 1.88 GHz under the load; of
     // zeros 290 us, and the instructions alone, on random registers, 3.7 P/s: power is
     // the bound, and where in a step loads and reads go makes no difference any more.

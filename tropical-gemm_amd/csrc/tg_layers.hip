@@ -77,7 +77,8 @@ struct NormArgs {
 // VPT > 0, rows of at least eight elements: all loads of a thread are issued
 // before the first is used; a group that would end past the row is moved back to
 // end with it, and what it shares with the group before it is counted once.
-// VPT 0: any length, read again for each sum.
+// VPT 0: any length, read again for each sum (bf16, 4096 x 12288 with dropout and
+// residual: 125 us, 403 MB if read once).
 //
 // bf16, 8192 x 8192 with dropout and residual: 99 us (537 MB, 5.4 TB/s; 105 where
 // the rows whose sums pass f32 were stored with the others, which took 82 registers;
