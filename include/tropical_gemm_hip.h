@@ -9,7 +9,9 @@
  * asynchronous on the given HIP stream (NULL = the device's null stream);
  * callers that need the reference's blocking behaviour call
  * tg_stream_synchronize() afterwards (the reference synchronises after every
- * launch, crates/tropical-gemm-cuda/src/kernels.rs:65).
+ * launch, crates/tropical-gemm-cuda/src/kernels.rs:65).  A call works on the
+ * device it names, whichever is the thread's current one, and leaves that as it
+ * was.
  *
  * Semantics (bit-exact with the reference CPU path; a NaN product replaces
  * the running value and the next product replaces a NaN, as the CPU's

@@ -78,7 +78,7 @@ bool valid_layout(int l) { return l == TG_ROW_MAJOR || l == TG_COL_MAJOR; }
 
 // Device handling: the ordinal is validated against the device count (the
 // reference answers an out-of-range ordinal with DimensionMismatch,
-// crates/tropical-gemm-cuda/src/lib.rs:81-87) and made current.
+// crates/tropical-gemm-cuda/src/lib.rs:81-87) and made current for the call.
 std::once_flag g_count_once;
 int g_device_count = -1;
 hipError_t g_count_err = hipSuccess;
@@ -95,7 +95,8 @@ int device_count_cached(int* out) {
     return TG_OK;
 }
 
-int select_device(int device) {
+// *before: the device to go back to (left alone where it is the same).
+int select_device(int device, int* before) {
     int n = 0;
     int rc = device_count_cached(&n);
     if (rc != TG_OK) return rc;
@@ -106,7 +107,9 @@ int select_device(int device) {
                                                    " HIP device(s) found)");
     int cur = -1;
     TG_HIP(hipGetDevice(&cur));
-    if (cur != device) TG_HIP(hipSetDevice(device));
+    if (cur == device) return TG_OK;
+    TG_HIP(hipSetDevice(device));
+    *before = cur;
     return TG_OK;
 }
 
@@ -1488,8 +1491,8 @@ int gemm_impl(int device, tg_semiring sr, tg_dtype dt, tg_layout layout, const v
     // A workspace the split-K partials cannot use (none, or misaligned when
     // no B^T staging is needed) runs the product unsplit.
     if (ws_given && (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0)) ws_bytes = 0;
-    rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     if (batch == 0 || m == 0 || n == 0) return TG_OK;
     hipStream_t st = as_stream(stream);
 
@@ -1990,8 +1993,8 @@ int backward_impl(int device, tg_dtype dt, tg_layout layout, bool want_a, const 
             return fail(TG_ERR_DIMENSION_MISMATCH, "gradient stride smaller than one matrix");
         if (s_c < 0 || s_other < 0) return fail(TG_ERR_DIMENSION_MISMATCH, "negative stride");
     }
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     if (batch == 0 || out_elems == 0) return TG_OK;
     if (!strided) {
         s_c = m * n;
@@ -2030,7 +2033,11 @@ namespace tg {
 
 int host_fail(int status, const std::string& msg) { return fail(status, msg); }
 int host_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
-int host_select_device(int device) { return select_device(device); }
+
+OnDevice::OnDevice(int device) : status_(select_device(device, &before_)) {}
+OnDevice::~OnDevice() {
+    if (before_ >= 0) (void)hipSetDevice(before_);
+}
 
 }  // namespace tg
 
@@ -2060,12 +2067,12 @@ int tg_device_count(int* count) {
 }
 
 int tg_context_init(int device) {
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     TG_HIP(hipFree(nullptr));  // forces runtime/context initialisation
     if (device < kScratchMaxDevices) {  // tg_gemm_noalloc's workspace address
         void* unused = nullptr;
-        rc = scratch_address(device, &unused);
+        const int rc = scratch_address(device, &unused);
         if (rc != TG_OK) return rc;
     }
     return TG_OK;
@@ -2073,8 +2080,8 @@ int tg_context_init(int device) {
 
 int tg_device_name(int device, char* buf, size_t len) {
     if (buf == nullptr || len == 0) return fail(TG_ERR_INVALID_ARGUMENT, "buffer is NULL");
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     hipDeviceProp_t prop;
     TG_HIP(hipGetDeviceProperties(&prop, device));
     std::snprintf(buf, len, "HIP Device %d (%s, %s)", device, prop.name, prop.gcnArchName);
@@ -2084,8 +2091,8 @@ int tg_device_name(int device, char* buf, size_t len) {
 int tg_malloc(int device, void** ptr, size_t bytes) {
     if (ptr == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "ptr is NULL");
     *ptr = nullptr;
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     if (bytes == 0) return TG_OK;
     TG_HIP(hipMalloc(ptr, bytes));
     return TG_OK;
@@ -2093,8 +2100,8 @@ int tg_malloc(int device, void** ptr, size_t bytes) {
 
 int tg_free(int device, void* ptr) {
     if (ptr == nullptr) return TG_OK;
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     TG_HIP(hipFree(ptr));
     return TG_OK;
 }
@@ -2102,8 +2109,8 @@ int tg_free(int device, void* ptr) {
 int tg_memcpy_htod(int device, void* dst, const void* src, size_t bytes) {
     if (bytes == 0) return TG_OK;
     if (dst == nullptr || src == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "NULL pointer");
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     TG_HIP(hipMemcpy(dst, src, bytes, hipMemcpyHostToDevice));
     return TG_OK;
 }
@@ -2111,8 +2118,8 @@ int tg_memcpy_htod(int device, void* dst, const void* src, size_t bytes) {
 int tg_memcpy_dtoh(int device, void* dst, const void* src, size_t bytes) {
     if (bytes == 0) return TG_OK;
     if (dst == nullptr || src == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "NULL pointer");
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     TG_HIP(hipMemcpy(dst, src, bytes, hipMemcpyDeviceToHost));
     return TG_OK;
 }
@@ -2120,8 +2127,8 @@ int tg_memcpy_dtoh(int device, void* dst, const void* src, size_t bytes) {
 int tg_memcpy_dtod(int device, void* dst, const void* src, size_t bytes, void* stream) {
     if (bytes == 0) return TG_OK;
     if (dst == nullptr || src == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "NULL pointer");
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     TG_HIP(hipMemcpyAsync(dst, src, bytes, hipMemcpyDeviceToDevice, as_stream(stream)));
     return TG_OK;
 }
@@ -2129,21 +2136,21 @@ int tg_memcpy_dtod(int device, void* dst, const void* src, size_t bytes, void* s
 int tg_memset_zero(int device, void* ptr, size_t bytes, void* stream) {
     if (bytes == 0) return TG_OK;
     if (ptr == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "ptr is NULL");
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     return launch_fill_zero(ptr, bytes, as_stream(stream));
 }
 
 int tg_synchronize(int device) {
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     TG_HIP(hipDeviceSynchronize());
     return TG_OK;
 }
 
 int tg_stream_synchronize(int device, void* stream) {
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     TG_HIP(hipStreamSynchronize(as_stream(stream)));
     return TG_OK;
 }
@@ -2198,8 +2205,8 @@ int tg_gemm_small(int device, tg_semiring semiring, tg_dtype dtype, tg_layout la
     tg::SmallForm form;
     const Small kernel = choose_small(semiring, dtype, p, &form);
     if (kernel == Small::NONE) return TG_OK;
-    rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     hipStream_t st = as_stream(stream);
     if (kernel == Small::KRESG) {
         rc = run_gemm_kresg(semiring == TG_MAXPLUS ? tg::SR_MAXPLUS : tg::SR_MINPLUS, p, st);
@@ -2251,8 +2258,8 @@ int tg_gemm_noalloc(int device, tg_semiring semiring, tg_dtype dtype, tg_layout 
                     "tg_gemm_noalloc: this problem needs " + std::to_string(need) +
                         " bytes of workspace, above the fixed " + std::to_string(kScratchBytes) +
                         "-byte scratch; use tg_gemm or tg_gemm_ws");
-    rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     if (empty) return TG_OK;
     void* ws = nullptr;
     rc = scratch_address(device, &ws);
@@ -2417,8 +2424,8 @@ int tg_transpose(int device, tg_dtype dtype, const void* src, void* dst, int64_t
     const int64_t elems = rows * cols;
     if (batch > 0 && elems > 0 && (src == nullptr || dst == nullptr))
         return fail(TG_ERR_INVALID_ARGUMENT, "src or dst is NULL");
-    int rc = select_device(device);
-    if (rc != TG_OK) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     if (batch == 0 || elems == 0) return TG_OK;
     hipStream_t st = as_stream(stream);
     auto run = [&](auto tag) {

@@ -80,7 +80,8 @@ int check_ws(size_t need, const void* ws, size_t bytes) {
 }
 
 int on_device(int device, const char* what, hipError_t (*run)(const void*), const void* arg) {
-    if (int rc = tg::host_select_device(device)) return rc;
+    const tg::OnDevice on(device);
+    if (on.status() != TG_OK) return on.status();
     const hipError_t e = run(arg);
     return e == hipSuccess ? int(TG_OK) : tg::host_hip_fail(e, what);
 }
