@@ -450,9 +450,10 @@ int tg_f8_dequantize(int device, tg_float type, const uint8_t* q, int64_t ldq, c
  * 2^20; k == 0 gives the bias (or zero).  Sums are f32.  For f32 outputs every
  * product is exact (scales of 2^-100 to 2^111); for bf16 and f16 the matrix
  * instructions add groups of eight neighbouring products first and drop of them
- * what lies 2^-13 below the largest: at most 2^-10 of the sum of the products'
- * magnitudes, which is more than f16's own rounding, and 1.5e-5 of the result in
- * the mean of normal values.  Where large products cancel, nothing bounds it by the
+ * what lies 2^-13 below the largest, as it would be with e4m3's numbers below 2^-6
+ * (which have fewer bits) taken as 2^-6, zeros aside: at most 2^-10 of the sum of
+ * the products' magnitudes so taken, which is more than f16's own rounding, and
+ * 1.5e-5 of the result in the mean of normal values.  Where large products cancel, nothing bounds it by the
  * result: take f32 outputs there (of many rows in about twice the time). */
 size_t tg_f8_gemm_workspace_size(tg_float type, const uint8_t* a, int64_t lda, const uint8_t* b,
                                  int64_t ldb, int64_t m, int64_t n, int64_t k);

@@ -93,10 +93,11 @@ def matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: tor
     one row for each output and scales for 128 x 128, ``bias`` of ``dtype``.
 
     For 16-bit outputs the matrix instructions add eight neighbouring products at a
-    time and drop of them what lies 2**-13 below the largest: up to 2**-10 of the sum
-    of the products' magnitudes (more than float16's own rounding), 1.5e-5 of the
-    result in the mean of normal values.  Where large products cancel, nothing bounds
-    that by the result.  float32 outputs are made of exact products (scales of 2**-100
+    time and drop of them what lies 2**-13 below the largest, as it would be with
+    operands that are not zero taken as 2**-6 at least (before their scales): up to
+    2**-10 of the sum of the products' magnitudes so taken (more than float16's own
+    rounding), 1.5e-5 of the result in the mean of normal values.  Where large
+    products cancel, nothing bounds that by the result.  float32 outputs are made of exact products (scales of 2**-100
     to 2**111) and sums of f32; those of many rows take about twice the time."""
     dev = a.device
     lda = _rows("a", a, _E4M3)
